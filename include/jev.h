@@ -291,6 +291,112 @@ enum { JEV_MATMUL_AUTO = 0, JEV_MATMUL_FLOAT = 1, JEV_MATMUL_INTEGER = 2 };
 int jev_set_matmul_strategy(int strategy);
 int jev_get_matmul_strategy(void);
 
+/* ---- A paged KV cache held in 8 bits, for many requests at once ---- */
+
+/* No counterpart in the reference, whose KvCache belongs to one conversation.
+ * A jev_pages is a pool of pages in HBM that requests share: a request is a row
+ * of a page table on the device, and grows by whole pages.  K and V take one
+ * byte an element.  Sixteen consecutive positions of a request are a block;
+ * per layer, KV head and block K has one scale and V another:
+ *
+ *   scale = max |x| / 127 (fp32) over the block's values,  code = x / scale
+ *   rounded to the nearest whole number (a half to the even one),  value read =
+ *   code * scale.
+ *
+ * Tokens added to a block that is begun raise its scale where they need a
+ * larger one; the codes it holds are then rounded to it.  A block that a
+ * request is cut back into keeps its scale.  A value that is not finite makes
+ * its block read as NaN until the block is begun anew.
+ *
+ * A step is: jev_pages_plan_device once, then per layer jev_pages_store_device
+ * and jev_pages_attend_device (jev_forward_pages: a whole model step).  Every
+ * call only enqueues on the handle's stream and allocates nothing, so a step
+ * can be captured into a HIP graph and replayed with other lengths in the same
+ * arrays; the lengths and tables stay on the device.  The stream
+ * (jev_pages_stream) orders itself with the device's null stream; a caller on
+ * another stream orders the two with events.  A handle's calls share its
+ * workspaces: one thread at a time, and no two of its graphs at once.  Pointers
+ * are device pointers of the handle's device; floats may have any 4-byte
+ * alignment (16 bytes: vector accesses, the same bits).  */
+typedef struct jev_pages jev_pages;
+typedef struct jev_pages_config {
+    int32_t n_pages;      /* of the pool; n_pages * page_tokens < 2^31          */
+    int32_t page_tokens;  /* 16, 32, 64, 128 or 256                             */
+    int32_t max_requests; /* rows of the page table, at most 4096               */
+    int32_t max_context;  /* tokens of one request, at most 2^24                */
+    int32_t max_tokens;   /* tokens of one plan, at most 2^22                   */
+    int32_t rope_half;    /* rotated pairs: 0 (2i, 2i + 1) as the model's Rope,
+                             1 (i, i + rope_dim / 2)                            */
+} jev_pages_config;
+
+/* Of `model` only the geometry (n_layers, n_heads, n_kv_heads, head_dim 64 or
+ * 128) and the rope_*, yarn_* and attention_temperature_scale fields are read,
+ * with jev_create's meaning (rope_dim 0: no rotation); frequencies, angles and
+ * rotations are in 64 bits here, rounded to fp32 once. */
+int jev_pages_create(const jev_config *model, const jev_pages_config *cfg, int device, jev_pages **out);
+void jev_pages_destroy(jev_pages *p);
+
+/* A step's bookkeeping on the device.  Batch row b < n_requests names request
+ * request[b], keeps its first past[b] tokens (past NULL: all it has) and adds
+ * fresh[b].  Pages past the kept tokens are given back; then the missing pages
+ * are taken, the lowest-numbered free one first, in batch order.  The batch's
+ * new tokens are its rows 0 .. total - 1 in the other calls, request after
+ * request; n_tokens >= total is how many rows their arrays have, and rows past
+ * the total are neither read nor written there.  past = fresh = 0 releases a
+ * request.  Optional outputs (NULL: not wanted), int32 on the device:
+ *   table    [n_requests][ceil(max_context / page_tokens)] page of each
+ *            page_tokens tokens, -1 past the request's last
+ *   slot     [n_tokens] page * page_tokens + offset    position [n_tokens]
+ *   row      [n_tokens] b           (these three -1 past the total)
+ *   start    [n_requests + 1] row of each request's first token, then the total
+ * A plan that does not fit changes nothing, plans no tokens (-1 and 0 in the
+ * outputs) and makes the calls after it do nothing; jev_pages_sync returns why:
+ * JEV_EINVAL (a request out of range or named twice, a kept length past what it
+ * has, a context past max_context, more than n_tokens) or JEV_ENOMEM (pages). */
+int jev_pages_plan_device(jev_pages *p, const int32_t *request, const int32_t *past, const int32_t *fresh,
+                          int32_t n_requests, int32_t n_tokens, int32_t *table, int32_t *slot, int32_t *position,
+                          int32_t *row, int32_t *start);
+
+/* The planned tokens' queries rotated into q_out [n_tokens][n_heads * head_dim]
+ * (q_out may be q where q_ld is that width), their keys rotated and stored,
+ * their values stored, in one layer.  Rows of q are q_ld floats apart, of k and
+ * v kv_ld.  q and q_out, or k and v, may be NULL. */
+int jev_pages_store_device(jev_pages *p, int32_t layer, const float *q, int64_t q_ld, const float *k, const float *v,
+                           int64_t kv_ld, float *q_out);
+
+/* out = softmax(q . K / sqrt(head_dim)) . V of every planned token over its
+ * request's stored tokens up to and with itself; query head h reads KV head
+ * h / (n_heads / n_kv_heads).  q and out are [n_tokens][n_heads * head_dim] and
+ * must not overlap.  A token's result has the same bits whatever else is in the
+ * batch as long as its request adds few tokens: fresh * heads per KV head <= 16. */
+int jev_pages_attend_device(jev_pages *p, int32_t layer, const float *q, float *out);
+
+/* k, v [n][n_kv_heads][head_dim] = the values stored at n slots of a layer
+ * (zeros for a slot outside the pool). */
+int jev_pages_read_device(jev_pages *p, int32_t layer, const int32_t *slot, int32_t n, float *k, float *v);
+
+/* Releases n requests (a host array): a plan that keeps nothing and adds
+ * nothing, waited for. */
+int jev_pages_release(jev_pages *p, const int32_t *request, int32_t n);
+
+/* Waits for the handle's stream; JEV_OK, or why the last plan was refused. */
+int jev_pages_sync(jev_pages *p);
+/* The handle's HIP stream (hipStream_t). */
+void *jev_pages_stream(jev_pages *p);
+
+/* A model step over the pages instead of the context's own cache: request
+ * request[b] keeps past[b] tokens (past NULL: all it has) and appends its
+ * fresh[b] >= 1 of `tokens` (n_tokens, request after request).  mode
+ * JEV_OUT_NONE, JEV_OUT_SELECTED (out: n_requests x n_rows) or JEV_OUT_FULL
+ * (n_requests x vocab), at each request's last token.  All arrays are host
+ * arrays, as in jev_forward; the call returns when the step is done.  `p` must
+ * have been created for this model on the same device, with rope_half 0.  The
+ * context's cache is left alone.  After an error or a cancel the requests'
+ * lengths may be those of the step: name `past` in the next one. */
+int jev_forward_pages(jev_ctx *ctx, jev_pages *p, const int32_t *request, const int32_t *past, const int32_t *fresh,
+                      int32_t n_requests, const int32_t *tokens, int32_t n_tokens, int mode, const int32_t *rows,
+                      int32_t n_rows, float *out, size_t out_len);
+
 /* ---- Test hooks (no managed counterpart) ---- */
 
 /* The Rope ctor's tables (Rope.cs:33-106): the n = rope_dim / 2 pair

@@ -404,4 +404,98 @@ hipError_t launch_kv_split(const float *src, uint16_t *dst, int heads_total, int
 hipError_t launch_kv_copy(const float *src, float *dst, int heads_total, int old_cap, int new_cap, int len, int hd,
                           hipStream_t s);
 
+// ---------------------------------------------------------------- 8-bit paged KV cache
+//
+// Many requests share one pool of pages of `page` tokens.  Sixteen consecutive
+// positions of a request are a block; per layer, page, KV head and block the
+// pool holds 16 x hd codes of K, as many of V, and their two scales: a value
+// is (byte - 128) * scale.  Both orders are the matrix cores' operands as a
+// wave loads them, 16 bytes a lane:
+//   K  [hd / 64][16 tokens][64 dims]: lane 16 g + r of a load reads dims 64 j +
+//      16 g .. + 15 of one token, two A fragments of v_mfma_f32_16x16x32_f16
+//   V  [hd dims][16 tokens]: lane 16 g + n reads the sixteen tokens of dim n of
+//      a slab of 16, the A fragments of V^T
+constexpr int kPageBlock = 16;         // tokens that share a scale
+constexpr int kPagesMaxRequests = 4096; // a plan's prefix sums live in LDS
+constexpr int kPagesTileRows = 16;     // (token, head) rows of a KV head in one attention tile
+
+// Keys per workgroup of a tile whose rows are one request's whole batch: a
+// function of the request's own length alone, so that its result does not
+// depend on the other requests.
+__host__ __device__ inline int pages_part_keys(int len) { return len <= 4096 ? 256 : len <= 32768 ? 512 : 1024; }
+
+struct PagesPlanHead {
+    int32_t status;  // JEV_OK, JEV_EINVAL or JEV_ENOMEM; not OK: everything below is zero
+    int32_t n_tokens;
+    int32_t n_units; // blocks that the batch's tokens go to
+    int32_t n_items; // workgroups of attention per KV head, 16-row tiles
+    int32_t n_wide;  // the same, wide tiles
+    int32_t n_parts; // partial results of split tiles
+    int32_t n_requests;
+    int32_t pad;
+};
+struct PagesRequest { // one batch row
+    int32_t id, past, len, start; // start: its first token's row in the batch
+    int32_t part0, n_parts;       // partial results of its tile, when split (n_parts > 1)
+};
+struct PagesItem {
+    int32_t b, row0, key0, key1, part; // part >= 0: where its partial result goes
+};
+struct Pages {
+    // geometry
+    int n_layers = 0, n_heads = 0, n_kv = 0, hd = 0, group = 1;
+    int page = 16, sub = 1;                 // tokens and blocks of a page
+    int n_pages = 0, max_requests = 0, max_context = 0, max_tokens = 0, width = 0; // width: pages of a table row
+    int half = 0, rope_half = 0;            // rotated pairs; 0: (2i, 2i + 1), 1: (i, i + half)
+    int orig_ctx = 0;
+    float temp_scale = 0.f, scale = 0.f;    // attention temperature; softmax scale
+    double mscale = 1.0;
+    // pool
+    uint8_t *k = nullptr, *v = nullptr;     // [layer][page][kv head][block][16 * hd]
+    float2 *ks = nullptr;                   // [layer][page][kv head][block] (K scale, V scale)
+    // state
+    int32_t *table = nullptr;               // [request][width]
+    int32_t *length = nullptr;              // [request] tokens; their pages are the table row's first
+    uint32_t *used = nullptr;               // a bit per page; past n_pages: set
+    int32_t *n_free = nullptr;
+    // the last plan
+    PagesPlanHead *head = nullptr;
+    PagesRequest *req = nullptr;            // [n_requests]
+    int32_t *fresh_pages = nullptr;         // pages taken, by rank
+    int32_t *prefix = nullptr;              // [4][max_requests + 1]: tokens, units, items, wide items before a batch row
+    int2 *unit = nullptr;                   // (batch row, block)
+    PagesItem *item = nullptr, *wide = nullptr;
+    double2 *angle = nullptr;               // [max_tokens][half] (cos, sin) * mscale
+    const double *freqs = nullptr;
+    float *part = nullptr;                  // [n_parts][kv head][16][hd + 2]
+    int max_units = 0, max_items = 0, max_wide = 0, max_parts = 0;
+    __host__ __device__ size_t n_blocks() const { return (size_t)n_pages * n_kv * sub; } // of a layer
+};
+struct PagesPlanArgs {
+    const int32_t *request = nullptr, *past = nullptr, *fresh = nullptr; // past may be null: keep everything
+    int n_requests = 0, n_tokens = 0;
+    int wide = 0; // requests of more rows than a 16-row tile go to the wide list
+    int32_t *table = nullptr, *slot = nullptr, *position = nullptr, *row = nullptr, *start = nullptr; // outputs, or null
+};
+hipError_t launch_pages_plan(const Pages &p, const PagesPlanArgs &a, hipStream_t s);
+struct PagesStoreArgs {
+    int layer = 0;
+    const float *q = nullptr, *k = nullptr, *v = nullptr; // q, or k and v, may be null
+    int64_t q_ld = 0, kv_ld = 0;
+    int nin = 1;            // K-split partials of the inputs, in_stride floats apart
+    size_t in_stride = 0;
+    float *q_out = nullptr;
+    int n_requests = 0, n_tokens = 0; // of the plan
+};
+hipError_t launch_pages_store(const Pages &p, const PagesStoreArgs &a, hipStream_t s);
+struct PagesAttendArgs {
+    int layer = 0;
+    const float *q = nullptr; // [n_tokens][n_heads * hd]
+    float *out = nullptr;     // the same
+    int n_requests = 0, n_tokens = 0, wide = 0; // of the plan
+};
+hipError_t launch_pages_attend(const Pages &p, const PagesAttendArgs &a, hipStream_t s);
+// k, v [n][n_kv][hd] = the values at slots; zeros for slots outside the pool.
+hipError_t launch_pages_read(const Pages &p, int layer, const int32_t *slot, int n, float *k, float *v, hipStream_t s);
+
 } // namespace jev

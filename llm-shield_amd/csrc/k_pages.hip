@@ -1,0 +1,925 @@
+// The 8-bit paged KV cache (Pages in jev_internal.h): a step's plan from the
+// requests' lengths, rotary positions with the store, attention, reading back.
+#include "../../include/jev.h"
+#include "jev_dev.h"
+
+namespace jev {
+
+namespace {
+
+constexpr int kPlanThreads = 1024;
+
+// Sum over the workgroup; every thread gets it.  `ws`: a 64-bit word per wave.
+template <int NT>
+__device__ __forceinline__ long long block_sum(long long v, long long *ws)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0;
+    for (int w = 0; w < NT / 64; w++) v += ws[w];
+    return v;
+}
+
+// Exclusive prefix sum over the workgroup's threads.  `ws`: a word per wave.
+template <int NT>
+__device__ __forceinline__ int block_scan(int v, int *ws)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(x, o, 64);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) ws[wave] = x;
+    __syncthreads();
+    int before = 0;
+    for (int w = 0; w < NT / 64; w++) before += w < wave ? ws[w] : 0;
+    return before + x - v;
+}
+
+// The last index b with prefix[b] <= i (prefix ascending, prefix[0] = 0, i < prefix[n]).
+__device__ __forceinline__ int find(const int *prefix, int n, int i)
+{
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (prefix[m] <= i) lo = m;
+        else hi = m;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ int div_up(int a, int b) { return (a + b - 1) / b; }
+
+// Where a batch row's counts come from: blocks its new tokens touch, 16-row
+// tiles of a KV head and their parts.
+struct Counts {
+    int units, items, wide, parts, n_parts;
+};
+__device__ __forceinline__ Counts counts(const Pages &p, int past, int fresh, int wide)
+{
+    Counts c = {0, 0, 0, 0, 1};
+    if (fresh <= 0) return c;
+    const int len = past + fresh, rows = fresh * p.group;
+    c.units = (len - 1) / kPageBlock - past / kPageBlock + 1;
+    const int tiles = div_up(rows, kPagesTileRows), most = div_up(p.group, kPagesTileRows);
+    if (tiles <= most) {
+        c.n_parts = div_up(len, pages_part_keys(len));
+        c.parts = c.n_parts > 1 ? tiles * c.n_parts : 0;
+    }
+    c.items = tiles * c.n_parts;
+    return c;
+}
+
+// The lists that follow from a valid plan, by `n` threads of which this is
+// number `i0`: the blocks to store, the attention's workgroups, the angles, and
+// what the caller asked for.  px: tokens, units and items before each batch row
+// (`stride` apart), R + 1 entries each.
+__device__ __forceinline__ void plan_lists(const Pages &p, const PagesPlanArgs &a, const PagesPlanHead &h, const int *px,
+                                           int stride, int i0, int n)
+{
+    const int R = h.n_requests;
+    const int *start = px, *unit0 = px + stride, *item0 = px + 2 * stride;
+    for (int u = i0; u < h.n_units; u += n) {
+        const int b = find(unit0, R, u);
+        p.unit[u] = make_int2(b, p.req[b].past / kPageBlock + u - unit0[b]);
+    }
+    for (int i = i0; i < h.n_items; i += n) {
+        const int b = find(item0, R, i), k = i - item0[b];
+        const PagesRequest r = p.req[b];
+        const int tiles = (item0[b + 1] - item0[b]) / r.n_parts, t = k % tiles, part = k / tiles;
+        const int keys = r.n_parts > 1 ? pages_part_keys(r.len) : r.len;
+        PagesItem it;
+        it.b = b;
+        it.row0 = t * kPagesTileRows;
+        it.key0 = part * keys;
+        it.key1 = min(r.len, it.key0 + keys);
+        it.part = r.n_parts > 1 ? r.part0 + k : -1;
+        p.item[i] = it;
+    }
+    // Angles in 64 bits: a far position times a frequency keeps its fraction.
+    // Once a plan, not once a layer and head: the library's 64-bit sine and
+    // cosine are ~150 instructions.
+    for (int64_t i = i0; i < (int64_t)h.n_tokens * p.half; i += n) {
+        const int t = (int)(i / p.half), j = (int)(i % p.half), b = find(start, R, t);
+        double sn, cs;
+        sincos((double)(p.req[b].past + t - start[b]) * p.freqs[j], &sn, &cs);
+        p.angle[i] = make_double2(cs * p.mscale, sn * p.mscale);
+    }
+    if (a.slot || a.position || a.row)
+        for (int t = i0; t < a.n_tokens; t += n) {
+            int b = -1, pos = -1, slot = -1;
+            if (t < h.n_tokens) {
+                b = find(start, R, t);
+                const PagesRequest r = p.req[b];
+                pos = r.past + t - start[b];
+                slot = p.table[(size_t)r.id * p.width + pos / p.page] * p.page + pos % p.page;
+            }
+            if (a.slot) a.slot[t] = slot;
+            if (a.position) a.position[t] = pos;
+            if (a.row) a.row[t] = b;
+        }
+    if (a.start)
+        for (int b = i0; b <= a.n_requests; b += n) a.start[b] = R > 0 ? start[b] : 0;
+    if (a.table)
+        for (int64_t i = i0; i < (int64_t)a.n_requests * p.width; i += n) {
+            const int b = (int)(i / p.width), j = (int)(i % p.width);
+            int page = -1;
+            if (b < R && j < div_up(p.req[b].len, p.page)) page = p.table[(size_t)p.req[b].id * p.width + j];
+            a.table[i] = page;
+        }
+}
+
+} // namespace
+
+// A step's bookkeeping in one workgroup: pages given back and taken, prefix
+// sums, and with LISTS everything that follows from them (many tokens: a
+// launch of its own, over the whole GPU).  Checks first: a plan that does not
+// fit changes nothing and plans no tokens.  Bounded by latency: a few trips to
+// memory, each of which every thread makes at once.
+template <bool LISTS>
+__global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(Pages p, PagesPlanArgs a)
+{
+    constexpr int NT = kPlanThreads, C = kPagesMaxRequests / NT;
+    __shared__ int px[3 * (kPagesMaxRequests + 1)];
+    __shared__ unsigned seen[kPagesMaxRequests / 32];
+    __shared__ long long ws64[NT / 64];
+    __shared__ int ws[NT / 64];
+    __shared__ int bad;
+    const int tid = threadIdx.x, R = a.n_requests, per = div_up(R, NT);
+    constexpr int S = kPagesMaxRequests + 1;
+    int *start = px, *need0 = px + S, *gone0 = px + 2 * S;
+    for (int i = tid; i < kPagesMaxRequests / 32; i += NT) seen[i] = 0;
+    if (tid == 0) bad = 0;
+    __syncthreads();
+
+    // the requests of this thread: b = tid * per + i
+    int id[C], past[C], fresh[C], keep[C], need[C], own[C];
+    long long tokens = 0, more = 0, gone = 0;
+#pragma unroll
+    for (int i = 0; i < C; i++) {
+        const int b = tid * per + i;
+        id[i] = past[i] = fresh[i] = keep[i] = need[i] = own[i] = 0;
+        if (i >= per || b >= R) continue;
+        id[i] = a.request[b];
+        fresh[i] = a.fresh[b];
+        bool ok = id[i] >= 0 && id[i] < p.max_requests;
+        if (ok) ok = !(atomicOr(&seen[id[i] >> 5], 1u << (id[i] & 31)) >> (id[i] & 31) & 1u);
+        if (ok) {
+            const int len = p.length[id[i]];
+            past[i] = a.past ? a.past[b] : len;
+            ok = past[i] >= 0 && past[i] <= len && fresh[i] >= 0 && fresh[i] <= p.max_context - past[i];
+        }
+        if (!ok) {
+            bad = 1;
+            continue;
+        }
+        own[i] = div_up(p.length[id[i]], p.page);
+        keep[i] = div_up(past[i], p.page);
+        need[i] = div_up(past[i] + fresh[i], p.page);
+        tokens += fresh[i];
+        more += need[i] - keep[i];
+        gone += own[i] - keep[i];
+    }
+    // 64-bit sums first: past them everything fits 32 bits
+    tokens = block_sum<NT>(tokens, ws64);
+    more = block_sum<NT>(more, ws64);
+    gone = block_sum<NT>(gone, ws64);
+    const int n_free = *p.n_free;
+    const int status = bad || tokens > a.n_tokens ? JEV_EINVAL : more > n_free + gone ? JEV_ENOMEM : JEV_OK;
+    if (status != JEV_OK) {
+        PagesPlanHead h = {status, 0, 0, 0, 0, 0, 0, 0};
+        if (tid == 0) *p.head = h;
+        if (LISTS) plan_lists(p, a, h, px, S, tid, NT);
+        return;
+    }
+
+    // exclusive sums over the batch of the tokens, the pages taken and given back
+    int s0 = 0, s1 = 0, s2 = 0;
+#pragma unroll
+    for (int i = 0; i < C; i++) {
+        s0 += fresh[i];
+        s1 += need[i] - keep[i];
+        s2 += own[i] - keep[i];
+    }
+    s0 = block_scan<NT>(s0, ws);
+    s1 = block_scan<NT>(s1, ws);
+    s2 = block_scan<NT>(s2, ws);
+#pragma unroll
+    for (int i = 0; i < C; i++) {
+        const int b = tid * per + i;
+        if (i >= per || b >= R) continue;
+        start[b] = s0;
+        need0[b] = s1;
+        gone0[b] = s2;
+        s0 += fresh[i];
+        s1 += need[i] - keep[i];
+        s2 += own[i] - keep[i];
+        PagesRequest r = {id[i], past[i], past[i] + fresh[i], start[b], 0, 1};
+        p.req[b] = r;
+    }
+    if (tid == 0) {
+        start[R] = (int)tokens;
+        need0[R] = (int)more;
+        gone0[R] = (int)gone;
+    }
+    __syncthreads();
+
+    for (int k = tid; k < (int)gone; k += NT) {
+        const int b = find(gone0, R, k);
+        const int page = p.table[(size_t)p.req[b].id * p.width + div_up(p.req[b].past, p.page) + k - gone0[b]];
+        atomicAnd(&p.used[page >> 5], ~(1u << (page & 31)));
+    }
+    __syncthreads(); // every page is back before the free ones are counted
+    if (more > 0) {
+        const int words = div_up(p.n_pages, 32), per_w = div_up(words, NT);
+        const int w0 = min(words, tid * per_w), w1 = min(words, w0 + per_w);
+        // past the first-level cache, which the atomics went around
+        auto word = [&](int w) { return __hip_atomic_load(&p.used[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+        int n = 0;
+        for (int w = w0; w < w1; w++) n += __popc(~word(w));
+        int rank = block_scan<NT>(n, ws);
+        for (int w = w0; w < w1 && rank < (int)more; w++) {
+            uint32_t u = word(w);
+            for (; ~u && rank < (int)more; rank++) {
+                const int bit = __ffs(~u) - 1;
+                u |= 1u << bit;
+                p.fresh_pages[rank] = 32 * w + bit;
+            }
+            __hip_atomic_store(&p.used[w], u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        for (int k = tid; k < (int)more; k += NT) {
+            const int b = find(need0, R, k);
+            p.table[(size_t)p.req[b].id * p.width + div_up(p.req[b].past, p.page) + k - need0[b]] = p.fresh_pages[k];
+        }
+    }
+    __syncthreads(); // need0 and gone0 are done with
+
+    // the lists' prefix sums take their place
+    int *unit0 = px + S, *item0 = px + 2 * S;
+    int u0 = 0, i0 = 0, g0 = 0;
+    Counts c[C];
+#pragma unroll
+    for (int i = 0; i < C; i++) {
+        c[i] = counts(p, past[i], fresh[i], a.wide);
+        u0 += c[i].units;
+        i0 += c[i].items;
+        g0 += c[i].parts;
+    }
+    const int nu = u0, ni = i0, ng = g0;
+    u0 = block_scan<NT>(u0, ws);
+    i0 = block_scan<NT>(i0, ws);
+    g0 = block_scan<NT>(g0, ws);
+    const bool last = tid == NT - 1;
+    PagesPlanHead h = {JEV_OK, (int)tokens, u0 + nu, i0 + ni, 0, g0 + ng, R, 0};
+    __shared__ PagesPlanHead all;
+    if (last) {
+        all = h;
+        *p.head = h;
+        unit0[R] = h.n_units;
+        item0[R] = h.n_items;
+        *p.n_free = n_free + (int)(gone - more);
+    }
+#pragma unroll
+    for (int i = 0; i < C; i++) {
+        const int b = tid * per + i;
+        if (i >= per || b >= R) continue;
+        unit0[b] = u0;
+        item0[b] = i0;
+        p.req[b].part0 = g0;
+        p.req[b].n_parts = c[i].n_parts;
+        u0 += c[i].units;
+        i0 += c[i].items;
+        g0 += c[i].parts;
+        p.length[id[i]] = past[i] + fresh[i];
+    }
+    __syncthreads();
+    if (LISTS) plan_lists(p, a, all, px, S, tid, NT);
+    else
+        for (int i = tid; i < 3 * S; i += NT)
+            if (i % S <= R) p.prefix[i] = px[i];
+}
+
+__global__ __launch_bounds__(256) void pages_lists_kernel(Pages p, PagesPlanArgs a)
+{
+    constexpr int S = kPagesMaxRequests + 1;
+    __shared__ int px[3 * S];
+    const PagesPlanHead h = *p.head;
+    if (h.n_requests > 0)
+        for (int j = 0; j < 3; j++)
+            for (int i = threadIdx.x; i <= h.n_requests; i += 256) px[j * S + i] = p.prefix[j * S + i];
+    __syncthreads();
+    plan_lists(p, a, h, px, S, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+}
+
+hipError_t launch_pages_plan(const Pages &p, const PagesPlanArgs &a, hipStream_t s)
+{
+    if (a.n_requests < 0 || a.n_requests > p.max_requests || a.n_tokens < 0 || a.n_tokens > p.max_tokens)
+        return hipErrorInvalidValue;
+    // what the lists write, in words; an angle counts for several
+    const double work = (double)a.n_tokens * (4 + 8.0 * p.half) + (a.table ? (double)a.n_requests * p.width : 0.0);
+    if (work <= 16384) {
+        hipLaunchKernelGGL(pages_plan_kernel<true>, dim3(1), dim3(kPlanThreads), 0, s, p, a);
+    } else {
+        hipLaunchKernelGGL(pages_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0, s, p, a);
+        const int wgs = (int)fmin(1024.0, ceil(work / 2048));
+        hipLaunchKernelGGL(pages_lists_kernel, dim3(wgs), dim3(256), 0, s, p, a);
+    }
+    return hipGetLastError();
+}
+
+// ------------------------------------------------------------ rotary positions and the store
+
+namespace {
+
+// The eight (HD 128) or four (HD 64) elements of a head's row that thread j of
+// its sixteen holds: NP rotation pairs (p, i.e. their two elements), consecutive
+// pairs; past the rotated part of the head a pair is two neighbours.
+template <int HD>
+struct RowPairs {
+    static constexpr int NP = HD / 32;
+    int e0[NP], e1[NP];
+    __device__ __forceinline__ RowPairs(const Pages &p, int j)
+    {
+#pragma unroll
+        for (int i = 0; i < NP; i++) {
+            const int q = NP * j + i;
+            const bool half = p.rope_half && q < p.half;
+            e0[i] = half ? q : 2 * q;
+            e1[i] = half ? q + p.half : 2 * q + 1;
+        }
+    }
+};
+
+template <int HD, bool VEC>
+__device__ __forceinline__ void load_pairs(const RowPairs<HD> &e, const float *x, float2 (&v)[HD / 32])
+{
+    constexpr int NP = HD / 32;
+    if constexpr (VEC) {
+        // the pairs are either neighbours throughout or two runs of NP floats
+        float r[2 * NP];
+        const bool split = e.e1[0] != e.e0[0] + 1;
+        const float *b = x + (split ? e.e1[0] : e.e0[0] + NP);
+        if constexpr (NP == 4) {
+            const float4 lo = *(const float4 *)(x + e.e0[0]), hi = *(const float4 *)b;
+            r[0] = lo.x, r[1] = lo.y, r[2] = lo.z, r[3] = lo.w, r[4] = hi.x, r[5] = hi.y, r[6] = hi.z, r[7] = hi.w;
+        } else {
+            const float2 lo = *(const float2 *)(x + e.e0[0]), hi = *(const float2 *)b;
+            r[0] = lo.x, r[1] = lo.y, r[2] = hi.x, r[3] = hi.y;
+        }
+#pragma unroll
+        for (int i = 0; i < NP; i++) v[i] = split ? make_float2(r[i], r[NP + i]) : make_float2(r[2 * i], r[2 * i + 1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NP; i++) v[i] = make_float2(x[e.e0[i]], x[e.e1[i]]);
+    }
+}
+
+template <int HD, bool VEC>
+__device__ __forceinline__ void store_pairs(const RowPairs<HD> &e, float *x, const float2 (&v)[HD / 32])
+{
+    constexpr int NP = HD / 32;
+    if constexpr (VEC) {
+        float r[2 * NP];
+        const bool split = e.e1[0] != e.e0[0] + 1;
+#pragma unroll
+        for (int i = 0; i < 2 * NP; i++) {
+            const float near = i & 1 ? v[i / 2].y : v[i / 2].x, apart = i < NP ? v[i % NP].x : v[i % NP].y;
+            r[i] = split ? apart : near;
+        }
+        float *b = x + (split ? e.e1[0] : e.e0[0] + NP);
+        if constexpr (NP == 4) {
+            *(float4 *)(x + e.e0[0]) = make_float4(r[0], r[1], r[2], r[3]);
+            *(float4 *)b = make_float4(r[4], r[5], r[6], r[7]);
+        } else {
+            *(float2 *)(x + e.e0[0]) = make_float2(r[0], r[1]);
+            *(float2 *)b = make_float2(r[2], r[3]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NP; i++) {
+            x[e.e0[i]] = v[i].x;
+            x[e.e1[i]] = v[i].y;
+        }
+    }
+}
+
+// x / by in 64 bits, rounded to the nearest whole number, a half to the even
+// one, as the byte q + 128; `inv` = 1 / by.  The product is within 2^-51 of the
+// quotient, and two fp32 numbers' quotient (or one times a code) is further
+// than that from a half unless it is one: then x - q by is exactly half of by.
+__device__ __forceinline__ uint32_t code_of(double x, double by, double inv)
+{
+    double q = rint(x * inv);
+    const double rest = fma(-q, by, x);
+    if (fabs(rest) * 2.0 == by && ((int)q & 1)) q += rest > 0.0 ? 1.0 : -1.0;
+    return (uint32_t)(int)(fmin(fmax(q, -127.0), 127.0) + 128.0);
+}
+
+// Byte of dim d of token t in a block's K and V codes.
+template <int HD>
+__device__ __forceinline__ int k_at(int t, int d) { return (d >> 6) * 1024 + t * 64 + (d & 63); }
+template <int HD>
+__device__ __forceinline__ int v_at(int t, int d) { return d * 16 + t; }
+
+} // namespace
+
+// One workgroup per block that the batch touches and KV head: the block's new
+// tokens' queries (of the head's group) rotated, their keys rotated and stored,
+// their values stored.  Sixteen threads hold a token's row.  Products of the
+// rotation are 64-bit and round to fp32 once, so a stored code does not depend
+// on how they are formed.  A block's scale only grows while the block fills;
+// codes it already holds are then rounded to the new one.  Bounded by memory:
+// 4 B in per element, 1 B (K, V) or 4 B (q) out.
+template <int HD, bool VEC>
+__global__ __launch_bounds__(256) void pages_store_kernel(Pages p, PagesStoreArgs a)
+{
+    constexpr int NP = HD / 32, BYTES = kPageBlock * HD;
+    __shared__ __align__(16) uint8_t code[2][BYTES];
+    __shared__ unsigned most[2];
+    const int tid = threadIdx.x, j = tid & 15, h = blockIdx.y;
+    if ((int)blockIdx.x >= p.head->n_units) return;
+    const int2 un = p.unit[blockIdx.x];
+    const PagesRequest r = p.req[un.x];
+    const int pos0 = max(r.past, un.y * kPageBlock), pos1 = min(r.len, (un.y + 1) * kPageBlock);
+    const int n = pos1 - pos0, row0 = r.start + pos0 - r.past, off = pos0 & (kPageBlock - 1);
+    const bool kv = a.k != nullptr;
+    const int lead = kv ? 2 : 0, rows = n * (lead + (a.q ? p.group : 0));
+    const RowPairs<HD> e(p, j);
+
+    // where the block lies
+    const int page = p.table[(size_t)r.id * p.width + un.y / p.sub];
+    const size_t block = ((size_t)page * p.n_kv + h) * p.sub + un.y % p.sub + (size_t)a.layer * p.n_blocks();
+    const bool begun = kv && off > 0;
+    float2 s_old = make_float2(0.f, 0.f);
+    if (kv) {
+        if (tid < 2) most[tid] = 0;
+        if (begun) s_old = p.ks[block];
+        if (tid < 2 * BYTES / 16) {
+            const bool v = tid >= BYTES / 16;
+            const int i = v ? tid - BYTES / 16 : tid;
+            uint4 w = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+            if (begun) w = ((const uint4 *)((v ? p.v : p.k) + block * BYTES))[i];
+            ((uint4 *)code[v])[i] = w;
+        }
+        __syncthreads();
+    }
+
+    float2 x[2][NP]; // the K and V rows of this thread: two rows at most
+#pragma unroll 1
+    for (int base = 0; base < rows; base += 32) {
+#pragma unroll
+        for (int it = 0; it < 2; it++) {
+            const int i = base + 16 * it + (tid >> 4);
+            if (i >= rows) continue;
+            const int t = i % n, which = i / n - lead; // -2: K, -1: V, else a query head of the group
+            const int row = row0 + t;
+            const float *src = which == -2 ? a.k + row * a.kv_ld + h * HD
+                               : which == -1 ? a.v + row * a.kv_ld + h * HD
+                                             : a.q + row * a.q_ld + (size_t)(h * p.group + which) * HD;
+            float2 y[NP];
+            load_pairs<HD, VEC>(e, src, y);
+            for (int z = 1; z < a.nin; z++) {
+                float2 w[NP];
+                load_pairs<HD, VEC>(e, src + z * a.in_stride, w);
+#pragma unroll
+                for (int c = 0; c < NP; c++) y[c] = make_float2(y[c].x + w[c].x, y[c].y + w[c].y);
+            }
+            if (which != -1) {
+                double f = 1.0;
+                const int pos = pos0 + t;
+                if (which >= 0 && p.orig_ctx > 0 && p.temp_scale != 0.f && pos >= p.orig_ctx)
+                    f = 1.0 + (double)p.temp_scale * log(1.0 + (double)(pos / p.orig_ctx));
+#pragma unroll
+                for (int c = 0; c < NP; c++) {
+                    double u = y[c].x, v = y[c].y;
+                    const int q = NP * j + c;
+                    if (q < p.half) {
+                        const double2 g = p.angle[(size_t)row * p.half + q];
+                        const double m0 = u * g.x, m1 = v * g.y, m2 = u * g.y, m3 = v * g.x;
+                        u = m0 - m1;
+                        v = m2 + m3;
+                    }
+                    y[c] = make_float2((float)(u * f), (float)(v * f));
+                }
+            }
+            if (which >= 0) {
+                store_pairs<HD, VEC>(e, a.q_out + ((size_t)row * p.n_heads + h * p.group + which) * HD, y);
+            } else {
+                unsigned m = 0; // a value that is not finite has the largest bits
+#pragma unroll
+                for (int c = 0; c < NP; c++) {
+                    x[it][c] = y[c];
+                    m = max(m, max(__float_as_uint(fabsf(y[c].x)), __float_as_uint(fabsf(y[c].y))));
+                }
+                atomicMax(&most[which + 2], m);
+            }
+        }
+        if (!kv) continue;
+        if (base > 0) continue;
+        __syncthreads(); // K and V rows are all in the first round
+    }
+    if (!kv) return;
+
+    float s[2];
+    double by[2], inv[2];
+#pragma unroll
+    for (int v = 0; v < 2; v++) {
+        const float old = v ? s_old.y : s_old.x;
+        const float now = most[v] >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float(most[v]) / 127.0f;
+        s[v] = now > old || now != now ? now : old; // NaN stays
+        by[v] = (double)s[v];
+        inv[v] = s[v] > 0.f ? 1.0 / by[v] : 0.0;
+    }
+    if (begun && tid < 2 * BYTES / 16) {
+        const bool v = tid >= BYTES / 16;
+        const float old = v ? s_old.y : s_old.x;
+        if (s[v] != old) { // also where either is NaN
+            uint32_t *w = (uint32_t *)code[v] + 4 * (v ? tid - BYTES / 16 : tid);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint32_t y = 0;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const int q = (int)((w[i] >> (8 * c)) & 255u) - 128;
+                    y |= (s[v] > 0.f ? code_of((double)q * (double)old, by[v], inv[v]) : 128u) << (8 * c);
+                }
+                w[i] = y;
+            }
+        }
+        // places from the first new token on held nothing, or what a shorter
+        // keep gave up: the new tokens' codes come over them below, the rest
+        // is past the request's end
+    }
+    __syncthreads();
+#pragma unroll
+    for (int it = 0; it < 2; it++) {
+        const int i = 16 * it + (tid >> 4);
+        if (i >= 2 * n) continue;
+        const int v = i / n, t = off + i % n;
+#pragma unroll
+        for (int c = 0; c < NP; c++) {
+            const bool zero = !(s[v] > 0.f);
+            const uint32_t q0 = zero ? 128u : code_of((double)x[it][c].x, by[v], inv[v]);
+            const uint32_t q1 = zero ? 128u : code_of((double)x[it][c].y, by[v], inv[v]);
+            const int a0 = v ? v_at<HD>(t, e.e0[c]) : k_at<HD>(t, e.e0[c]), a1 = v ? v_at<HD>(t, e.e1[c]) : k_at<HD>(t, e.e1[c]);
+            code[v][a0] = (uint8_t)q0;
+            code[v][a1] = (uint8_t)q1;
+        }
+    }
+    __syncthreads();
+    if (tid < 2 * BYTES / 16) {
+        const bool v = tid >= BYTES / 16;
+        const int i = v ? tid - BYTES / 16 : tid;
+        ((uint4 *)((v ? p.v : p.k) + block * BYTES))[i] = ((const uint4 *)code[v])[i];
+    }
+    if (tid == 0) p.ks[block] = make_float2(s[0], s[1]);
+}
+
+hipError_t launch_pages_store(const Pages &p, const PagesStoreArgs &a, hipStream_t s)
+{
+    const int units = a.n_tokens / kPageBlock + 2 * (a.n_requests < a.n_tokens ? a.n_requests : a.n_tokens);
+    if (units == 0) return hipSuccess;
+    const int np = p.hd / 32;
+    auto vec = [&](const void *x, int64_t ld) { return !x || ((uintptr_t)x % (4 * np) == 0 && ld % np == 0); };
+    // a thread's pairs in vector accesses: rows that start aligned, and no
+    // thread with pairs on both sides of the rotated part's end
+    const bool v = vec(a.q, a.q_ld) && vec(a.k, a.kv_ld) && vec(a.v, a.kv_ld) && vec(a.q_out, 0) && a.in_stride % np == 0 &&
+                   (!p.rope_half || p.half % np == 0);
+    const dim3 grid(units, p.n_kv);
+    if (p.hd == 128 && v) hipLaunchKernelGGL((pages_store_kernel<128, true>), grid, dim3(256), 0, s, p, a);
+    else if (p.hd == 128) hipLaunchKernelGGL((pages_store_kernel<128, false>), grid, dim3(256), 0, s, p, a);
+    else if (v) hipLaunchKernelGGL((pages_store_kernel<64, true>), grid, dim3(256), 0, s, p, a);
+    else hipLaunchKernelGGL((pages_store_kernel<64, false>), grid, dim3(256), 0, s, p, a);
+    return hipGetLastError();
+}
+
+// ------------------------------------------------------------ attention
+
+// Sixteen (token, head) rows of a request and KV head over keys [key0, key1) of
+// its pages; the four waves take blocks of 64 keys in turn and merge at the
+// end.  S^T = K Q^T: with the rows of the K operand (token i, block b) dealt so
+// that a lane's sixteen scores are the sixteen tokens of ONE block, the
+// accumulators are the P^T operand of O^T += V^T P^T as they stand -- no
+// exchange between lanes -- and a lane has one K and one V scale per 64 keys.
+// Codes are exact in fp16; q and p enter as fp16 pairs (hi + lo), ~22 bits, so
+// each product is two matrix instructions.  q is first scaled to below 2^14 by
+// a power of two per row, p by the V scale relative to the largest one so far
+// (a power of two, `ev`), so that neither leaves fp16's range.  Softmax
+// statistics, scores and outputs are fp32.
+// Single tokens are bound by HBM: 2 hd bytes a key and KV head.
+template <int HD>
+__global__ __launch_bounds__(256, 2) void pages_attend_kernel(Pages p, PagesAttendArgs a)
+{
+    constexpr int NJ = HD / 64, NS = HD / 16, BYTES = kPageBlock * HD, LDO = HD + 4;
+    __shared__ float lo[4][kPagesTileRows][LDO];
+    __shared__ float lm[4][kPagesTileRows], ll[4][kPagesTileRows];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, n = lane & 15, h = blockIdx.y;
+    const int n_items = p.head->n_items;
+    const uint8_t *kbase = p.k + (size_t)a.layer * p.n_blocks() * BYTES;
+    const uint8_t *vbase = p.v + (size_t)a.layer * p.n_blocks() * BYTES;
+    const float2 *sbase = p.ks + (size_t)a.layer * p.n_blocks();
+
+    for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
+        const PagesItem it = p.item[item];
+        const PagesRequest r = p.req[it.b];
+        const int32_t *table = p.table + (size_t)r.id * p.width;
+        const int n_rows = (r.len - r.past) * p.group, row = it.row0 + n;
+        const bool live = row < n_rows;
+        const int token = live ? row / p.group : 0, head = h * p.group + (live ? row % p.group : 0);
+        const int limit = live ? r.past + token : -1; // last visible key
+        const size_t qrow = ((size_t)(r.start + token) * p.n_heads + head) * HD;
+        // the tile's last visible key, and the first row's: blocks below it need no mask
+        const int top = r.past + min(n_rows - 1, it.row0 + kPagesTileRows - 1) / p.group;
+        const int key1 = min(it.key1, top + 1);
+        const bool full = it.row0 + kPagesTileRows <= n_rows;
+        const int clear = full ? r.past + it.row0 / p.group : -1;
+
+        // Q^T fragments: dims 64 j + 16 g + 8 c .. + 7 of row n
+        half8_t qh[2 * NJ], ql[2 * NJ];
+        float qs;
+        {
+            float x[2 * NJ][8];
+            float m = 0.f;
+#pragma unroll
+            for (int c = 0; c < 2 * NJ; c++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    x[c][i] = a.q[qrow + 64 * (c >> 1) + 16 * g + 8 * (c & 1) + i];
+                    m = fmaxf(m, fabsf(x[c][i]));
+                }
+            m = fmaxf(m, __shfl_xor(m, 16, 64));
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
+            // m * 2^(14 - e) in [2^13, 2^14); rows of zeros and rows with infinities stay as they are
+            const int ex = m > 0.f && m < INFINITY ? 14 - (ilogbf(m) + 1) : 0;
+            const int e1 = ex / 2, e2 = ex - e1; // in two steps: neither factor leaves fp32's range
+            const float f1 = ldexpf(1.f, e1), f2 = ldexpf(1.f, e2);
+            qs = ldexpf(ldexpf(p.scale * 1.44269504088896341f, -e1), -e2);
+#pragma unroll
+            for (int c = 0; c < 2 * NJ; c++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float y = x[c][i] * f1 * f2;
+                    const _Float16 hi = (_Float16)y;
+                    qh[c][i] = hi;
+                    ql[c][i] = (_Float16)(y - (float)hi);
+                }
+        }
+
+        floatx4 o[NS];
+#pragma unroll
+        for (int s = 0; s < NS; s++) o[s] = floatx4{0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.f;
+        int ev = -200; // outputs are held times 2^(10 - ev)
+
+        const int last = (r.len - 1) / kPageBlock; // blocks past it are read as this one, and masked
+        auto block_of = [&](int b) {
+            const int c = min(b, last);
+            return ((size_t)table[c / p.sub] * p.n_kv + h) * p.sub + c % p.sub;
+        };
+        for (int kb = it.key0 / 64 + wave; kb * 64 < key1; kb += 4) {
+            const size_t bk = block_of(4 * kb + (n >> 2)), bv = block_of(4 * kb + g);
+            uint4 kr[4][NJ], vr[NS];
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int j = 0; j < NJ; j++)
+                    kr[t][j] = *(const uint4 *)(kbase + bk * BYTES + j * 1024 + (4 * t + (n & 3)) * 64 + 16 * g);
+            const float2 sc = sbase[bv];
+#pragma unroll
+            for (int s = 0; s < NS; s++) vr[s] = *(const uint4 *)(vbase + bv * BYTES + (16 * s + n) * 16);
+
+            const _Float16 bias = (_Float16)1152.f;
+            auto frag = [&](uint32_t w0, uint32_t w1) {
+                uint4 u;
+                bytes_to_f16(w0, bias, u.x, u.y);
+                bytes_to_f16(w1, bias, u.z, u.w);
+                return __builtin_bit_cast(half8_t, u);
+            };
+            float sv[4][4];
+            const float ks = sc.x * qs;
+            float mx = -INFINITY;
+            const bool masked = kb * 64 + 63 > clear;
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < NJ; j++) {
+                    const half8_t k0 = frag(kr[t][j].x, kr[t][j].y), k1 = frag(kr[t][j].z, kr[t][j].w);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh[2 * j], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh[2 * j + 1], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql[2 * j], acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql[2 * j + 1], acc, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float x = acc[i] * ks;
+                    if (masked && kb * 64 + 16 * g + 4 * t + i > limit) x = -INFINITY;
+                    sv[t][i] = x;
+                    mx = fmaxf(mx, x);
+                }
+            }
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn;
+            float alpha = exp2f(m - mu);
+            l = l * alpha;
+            // the largest V scale of the four blocks sets the power of two
+            float vm = sc.y;
+            vm = fmaxf(vm, __shfl_xor(vm, 16, 64));
+            vm = fmaxf(vm, __shfl_xor(vm, 32, 64));
+            if (vm > 0.f && vm < INFINITY) {
+                const int en = max(ev, ilogbf(vm));
+                alpha = ldexpf(alpha, max(ev - en, -400));
+                ev = en;
+            }
+            const float vs = ldexpf(sc.y, 10 - ev);
+            float w[4][4];
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float e = exp2f(sv[t][i] - mu);
+                    l += e;
+                    w[t][i] = masked && kb * 64 + 16 * g + 4 * t + i > limit ? 0.f : e * vs;
+                }
+            m = mn;
+            half8_t ph[2], pl[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float x = w[2 * j + (i >> 2)][i & 3];
+                    const _Float16 hi = (_Float16)x;
+                    ph[j][i] = hi;
+                    pl[j][i] = (_Float16)(x - (float)hi);
+                }
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                const half8_t v0 = frag(vr[s].x, vr[s].y), v1 = frag(vr[s].z, vr[s].w);
+                floatx4 acc = o[s] * alpha;
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[0], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[1], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[0], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[1], acc, 0, 0, 0);
+                o[s] = acc;
+            }
+        }
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+
+        // the four waves' results, in wave order
+        const float up = ldexpf(1.f, max(ev, -149));
+#pragma unroll
+        for (int s = 0; s < NS; s++) *(floatx4 *)&lo[wave][n][16 * s + 4 * g] = o[s] * 0x1p-10f * up;
+        if (g == 0) {
+            lm[wave][n] = m;
+            ll[wave][n] = l;
+        }
+        __syncthreads();
+        for (int i = tid; i < kPagesTileRows * (HD / 4); i += 256) {
+            const int c = i / (HD / 4), d = 4 * (i % (HD / 4)), rr = it.row0 + c;
+            if (rr >= n_rows) continue;
+            float mm = lm[0][c];
+#pragma unroll
+            for (int w = 1; w < 4; w++) mm = fmaxf(mm, lm[w][c]);
+            const float mu = mm == -INFINITY ? 0.f : mm;
+            float sum = 0.f;
+            floatx4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float f = exp2f(lm[w][c] - mu);
+                sum += ll[w][c] * f;
+                x += *(const floatx4 *)&lo[w][c][d] * f;
+            }
+            if (it.part < 0) {
+                const int tk = rr / p.group, hd = h * p.group + rr % p.group;
+                float *dst = a.out + ((size_t)(r.start + tk) * p.n_heads + hd) * HD + d;
+                const float inv = 1.f / sum;
+#pragma unroll
+                for (int k = 0; k < 4; k++) dst[k] = x[k] * inv;
+            } else {
+                float *dst = p.part + (((size_t)it.part * p.n_kv + h) * kPagesTileRows + c) * (HD + 4);
+                *(floatx4 *)(dst + d) = x;
+                if (d == 0) {
+                    dst[HD] = mm;
+                    dst[HD + 1] = sum;
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// The parts of split tiles, per batch row and head: sixteen threads hold the
+// head's dims (HD / 16 each), the sixteen groups take every sixteenth part and
+// are summed in group order.
+template <int HD>
+__global__ __launch_bounds__(256) void pages_merge_kernel(Pages p, PagesAttendArgs a)
+{
+    constexpr int ND = HD / 16, LD = HD + 4;
+    __shared__ float lo[16][HD];
+    __shared__ float ll[16], wm[4];
+    const int tid = threadIdx.x, b = blockIdx.x, head = blockIdx.y, h = head / p.group;
+    if (b >= p.head->n_requests) return;
+    const PagesRequest r = p.req[b];
+    if (r.n_parts <= 1) return;
+    const int tiles = div_up((r.len - r.past) * p.group, kPagesTileRows);
+    for (int t = 0; t < r.len - r.past; t++) {
+        const int row = t * p.group + head % p.group, tile = row / kPagesTileRows, c = row % kPagesTileRows;
+        // part k of the row
+        auto at = [&](int k) { return p.part + (((size_t)(r.part0 + k * tiles + tile) * p.n_kv + h) * kPagesTileRows + c) * LD; };
+        float m = -INFINITY;
+        for (int k = tid; k < r.n_parts; k += 256) m = fmaxf(m, at(k)[HD]);
+        m = warp_max(m);
+        __syncthreads();
+        if ((tid & 63) == 0) wm[tid >> 6] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
+        if (m == -INFINITY) m = 0.f;
+        const int grp = tid >> 4, j = tid & 15;
+        float x[ND] = {}, sum = 0.f;
+        for (int k = grp; k < r.n_parts; k += 16) {
+            const float *src = at(k);
+            const float f = exp2f(src[HD] - m);
+            sum += src[HD + 1] * f;
+#pragma unroll
+            for (int i = 0; i < ND; i++) x[i] += src[ND * j + i] * f;
+        }
+#pragma unroll
+        for (int i = 0; i < ND; i++) lo[grp][ND * j + i] = x[i];
+        if (j == 0) ll[grp] = sum;
+        __syncthreads();
+        if (tid < HD) {
+            float y = 0.f, z = 0.f;
+            for (int k = 0; k < 16; k++) {
+                y += lo[k][tid];
+                z += ll[k];
+            }
+            a.out[((size_t)(r.start + t) * p.n_heads + head) * HD + tid] = y / z;
+        }
+    }
+}
+
+hipError_t launch_pages_attend(const Pages &p, const PagesAttendArgs &a, hipStream_t s)
+{
+    if (a.n_tokens == 0 || a.n_requests == 0) return hipSuccess;
+    const int64_t most = (int64_t)p.max_parts + (int64_t)a.n_tokens * p.group / kPagesTileRows + a.n_requests;
+    const int wgs = (int)(most < 2048 ? most : 2048);
+    const dim3 grid(wgs, p.n_kv);
+    if (p.hd == 128) hipLaunchKernelGGL(pages_attend_kernel<128>, grid, dim3(256), 0, s, p, a);
+    else hipLaunchKernelGGL(pages_attend_kernel<64>, grid, dim3(256), 0, s, p, a);
+    if (p.max_context > pages_part_keys(1)) {
+        const dim3 mg(a.n_requests, p.n_heads);
+        if (p.hd == 128) hipLaunchKernelGGL(pages_merge_kernel<128>, mg, dim3(256), 0, s, p, a);
+        else hipLaunchKernelGGL(pages_merge_kernel<64>, mg, dim3(256), 0, s, p, a);
+    }
+    return hipGetLastError();
+}
+
+// ------------------------------------------------------------ reading back
+
+// Sixteen threads hold a (slot, KV head) row of K and V.
+template <int HD>
+__global__ __launch_bounds__(256) void pages_read_kernel(Pages p, int layer, const int32_t *slot, int n, float *k, float *v)
+{
+    constexpr int ND = HD / 16, BYTES = kPageBlock * HD;
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;
+    const int j = threadIdx.x & 15;
+    if (i >= (int64_t)n * p.n_kv) return;
+    const int h = (int)(i % p.n_kv), sl = slot[i / p.n_kv];
+    float kk[ND] = {}, vv[ND] = {};
+    if (sl >= 0 && sl / p.page < p.n_pages) {
+        const int t = sl % kPageBlock;
+        const size_t b = ((size_t)(sl / p.page) * p.n_kv + h) * p.sub + sl % p.page / kPageBlock + (size_t)layer * p.n_blocks();
+        const float2 s = p.ks[b];
+#pragma unroll
+        for (int c = 0; c < ND; c++) {
+            kk[c] = (float)((int)p.k[b * BYTES + k_at<HD>(t, ND * j + c)] - 128) * s.x;
+            vv[c] = (float)((int)p.v[b * BYTES + v_at<HD>(t, ND * j + c)] - 128) * s.y;
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < ND; c++) {
+        k[i * HD + ND * j + c] = kk[c];
+        v[i * HD + ND * j + c] = vv[c];
+    }
+}
+
+hipError_t launch_pages_read(const Pages &p, int layer, const int32_t *slot, int n, float *k, float *v, hipStream_t s)
+{
+    if (n <= 0) return hipSuccess;
+    const dim3 grid((unsigned)(((int64_t)n * p.n_kv * 16 + 255) / 256));
+    if (p.hd == 128) hipLaunchKernelGGL(pages_read_kernel<128>, grid, dim3(256), 0, s, p, layer, slot, n, k, v);
+    else hipLaunchKernelGGL(pages_read_kernel<64>, grid, dim3(256), 0, s, p, layer, slot, n, k, v);
+    return hipGetLastError();
+}
+
+} // namespace jev

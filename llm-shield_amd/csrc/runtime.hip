@@ -806,6 +806,12 @@ int throttle_group(const jev_ctx *c, int T)
     return (int)std::max(1.0, std::min(k, (double)std::max(1, f.n_layers / 2)));
 }
 
+// A step over a paged cache (jev_forward_pages).
+struct PagedStep {
+    const Pages *pages = nullptr;
+    PagesPlanArgs args;
+};
+
 // `call` (optional) is the cancellable call this pass belongs to: its cancel
 // flag is checked before every layer; with `throttle` the host also waits,
 // before each group of throttle_group layers, until the device has finished
@@ -814,8 +820,11 @@ int throttle_group(const jev_ctx *c, int T)
 // With `cap` (a causal call of jev_capture) every tap is recorded as the pass
 // produces it; the one-token pass then runs RoPE before the decode attention
 // instead of inside it, so the rotated queries exist in memory.
+// With `paged` the tokens' keys and values go to, and are attended from, its
+// pages (planned for these tokens) instead of the context's cache.
 int enqueue_forward(jev_ctx *c, const Plan &p, int mode, int n_rows, float *dout, const int32_t *dpos = nullptr,
-                    const CallScope *call = nullptr, bool throttle = false, Capture *cap = nullptr)
+                    const CallScope *call = nullptr, bool throttle = false, Capture *cap = nullptr,
+                    const PagedStep *paged = nullptr)
 {
 #define CAP_TRY(expr)                                                                                           \
     do {                                                                                                        \
@@ -928,13 +937,38 @@ int enqueue_forward(jev_ctx *c, const Plan &p, int mode, int n_rows, float *dout
         // one token, or rows of one token that see none of each other's keys:
         // RoPE and the KV store run inside the decode attention kernel
         const bool rows_fused = p.single_rows && p.rows_independent && !cap;
-        if ((T != 1 && !rows_fused) || cap) HIP_TRY(launch_rope_store(ra, s));
+        if (!paged && ((T != 1 && !rows_fused) || cap)) HIP_TRY(launch_rope_store(ra, s));
         CAP_TRY(cap_add(c, cap, layer_tap(l, "q_rope"), c->q.p, T, qdim));
         CAP_TRY(cap_kv(c, cap, layer_tap(l, "k_rope"), kc, p.start, T));
         CAP_TRY(cap_kv(c, cap, layer_tap(l, "v"), vc, p.start, T));
         DecodeChunks dchunks;
 
-        if (T == 1) {
+        if (paged) {
+            PagesStoreArgs sa;
+            sa.layer = l;
+            sa.q = ra.q_in;
+            sa.k = ra.k_in;
+            sa.v = ra.v_in;
+            sa.q_ld = sa.kv_ld = ldqkv;
+            sa.nin = ra.nin;
+            sa.in_stride = ra.in_stride;
+            sa.q_out = c->q.p;
+            sa.n_requests = paged->args.n_requests;
+            sa.n_tokens = T;
+            HIP_TRY(launch_pages_store(*paged->pages, sa, s));
+            PagesAttendArgs pa;
+            pa.layer = l;
+            pa.q = c->q.p;
+            pa.out = T == 1 ? c->x32.p : c->y.p; // the projections in y are stored by now
+            pa.n_requests = sa.n_requests;
+            pa.n_tokens = T;
+            pa.wide = paged->args.wide;
+            HIP_TRY(launch_pages_attend(*paged->pages, pa, s));
+            if (T > 1) {
+                HIP_TRY(launch_split(c->y.p, T, qdim, c->xt.p, s));
+                if (L.o.type == kQ5_1) HIP_TRY(launch_block_sums(c->xt.p, T, qdim, c->xsum.p, s));
+            }
+        } else if (T == 1) {
             DecodeAttnArgs da;
             da.T = 1;
             da.n_heads = f.n_heads;
@@ -1057,8 +1091,8 @@ int enqueue_forward(jev_ctx *c, const Plan &p, int mode, int n_rows, float *dout
         }
         {
             const QWeight *wo[1] = {&L.o};
-            const bool combined = T == 1 && dchunks.max_chunks > kCombineChunks;
-            if (combined) {
+            const bool many = dchunks.max_chunks > kCombineChunks, combined = T == 1 && (paged || many);
+            if (many) {
                 ProfScope pc(c, JEV_PROF_DECODE_ATTN, 0.0, 0.0, true);
                 HIP_TRY(launch_attn_combine_one(dchunks, f.n_heads, c->x32.p, pc.a, pc.z, s));
             }
@@ -2519,6 +2553,410 @@ int jev_matmul_q(int type, const void *wbytes, int64_t rows, int64_t cols, const
     free_weight(w);
     if (e != hipSuccess) return fail(JEV_EDEVICE, "matmul: %s", hipGetErrorString(e));
     return JEV_OK;
+}
+
+// ---------------------------------------------------------------- paged 8-bit KV cache
+
+} // extern "C"
+
+struct jev_pages {
+    Pages p;
+    jev_config cfg{};
+    int device = 0;
+    hipStream_t stream = nullptr;
+    std::vector<void *> blocks; // owning allocations
+    PagesPlanArgs plan;         // the last plan's batch (its arrays are the caller's: not read again)
+    int32_t *ids = nullptr;     // jev_pages_release: [max_requests] requests, then as many zeros
+};
+
+namespace {
+
+// rope_table in 64 bits.
+double rope_table64(const jev_config &c, std::vector<double> &freqs)
+{
+    const int half = c.rope_dim / 2;
+    freqs.assign(half, 0.0);
+    const double factor = c.rope_scale_factor, base = c.rope_freq_base, dims = c.rope_dim;
+    for (int i = 0; i < half; i++) freqs[i] = pow(base, -2.0 * i / dims);
+    if (!(c.rope_scaling_yarn && c.rope_original_context > 0 && c.yarn_ext_factor != 0.0f && factor > 1.0)) {
+        for (double &f : freqs) f /= factor;
+        return c.rope_attn_factor;
+    }
+    double low = 3.402823466e+38, high = dims / 2 - 1;
+    if (c.yarn_beta_fast != 0.0f || c.yarn_beta_slow != 0.0f) {
+        auto corr = [&](double rot) { return dims * log(c.rope_original_context / (rot * 2 * M_PI)) / (2 * log(base)); };
+        low = fmax(0.0, floor(corr(c.yarn_beta_fast)));
+        high = fmin(dims / 2 - 1, ceil(corr(c.yarn_beta_slow)));
+    }
+    for (int i = 0; i < half; i++) {
+        const double ramp = fmin(1.0, fmax(0.0, (i - low) / fmax(0.001, high - low)));
+        const double mix = (1.0 - ramp) * c.yarn_ext_factor;
+        freqs[i] = freqs[i] / factor * (1.0 - mix) + freqs[i] * mix;
+    }
+    auto ms = [](double scale, double m) { return scale <= 1.0 ? 1.0 : 0.1 * m * log(scale) + 1.0; };
+    const double m = c.yarn_mscale != 0.0f ? c.yarn_mscale : 1.0;
+    const double ratio = c.yarn_mscale_all_dim != 0.0f ? ms(factor, m) / ms(factor, c.yarn_mscale_all_dim) : ms(factor, 1.0);
+    return ratio * c.rope_attn_factor;
+}
+
+template <typename T>
+int pages_alloc(jev_pages *h, T *&out, size_t n)
+{
+    void *b = nullptr;
+    const size_t bytes = std::max<size_t>(n, 1) * sizeof(T);
+    const hipError_t e = hipMalloc(&b, bytes);
+    if (e != hipSuccess) {
+        (void)hipGetLastError();
+        return fail(JEV_ENOMEM, "hipMalloc(%zu) for a paged cache failed: %s", bytes, hipGetErrorString(e));
+    }
+    h->blocks.push_back(b);
+    out = (T *)b;
+    HIP_TRY(hipMemsetAsync(b, 0, bytes, h->stream));
+    return JEV_OK;
+}
+
+int check_pages(jev_pages *h)
+{
+    if (!h) return fail(JEV_EINVAL, "null paged cache");
+    HIP_TRY(hipSetDevice(h->device));
+    return JEV_OK;
+}
+
+int check_pages_layer(jev_pages *h, int layer)
+{
+    const int rc = check_pages(h);
+    if (rc) return rc;
+    if (layer < 0 || layer >= h->p.n_layers) return fail(JEV_EINVAL, "layer %d of %d", layer, h->p.n_layers);
+    return JEV_OK;
+}
+
+int pages_plan(jev_pages *h, const PagesPlanArgs &a, hipStream_t s)
+{
+    if (a.n_requests < 0 || a.n_requests > h->p.max_requests)
+        return fail(JEV_EINVAL, "%d requests: the cache was made for %d", a.n_requests, h->p.max_requests);
+    if (a.n_tokens < 0 || a.n_tokens > h->p.max_tokens)
+        return fail(JEV_EINVAL, "%d tokens: the cache was made for plans of %d", a.n_tokens, h->p.max_tokens);
+    if (a.n_requests > 0 && (!a.request || !a.fresh)) return fail(JEV_EINVAL, "request and fresh must not be null");
+    h->plan = a;
+    HIP_TRY(launch_pages_plan(h->p, h->plan, s));
+    return JEV_OK;
+}
+
+int pages_status(jev_pages *h, hipStream_t s)
+{
+    PagesPlanHead head;
+    HIP_TRY(hipMemcpyAsync(&head, h->p.head, sizeof head, hipMemcpyDeviceToHost, s));
+    HIP_TRY(hipStreamSynchronize(s));
+    if (head.status == JEV_EINVAL)
+        return fail(JEV_EINVAL, "the plan was refused: a request out of range or named twice, a kept length past what a "
+                                "request has, a context past %d tokens, or more than %d new tokens",
+                    h->p.max_context, h->plan.n_tokens);
+    if (head.status == JEV_ENOMEM)
+        return fail(JEV_ENOMEM, "the plan was refused: it needs more pages than are free of the pool's %d", h->p.n_pages);
+    return JEV_OK;
+}
+
+} // namespace
+
+extern "C" {
+
+int jev_pages_create(const jev_config *model, const jev_pages_config *cfg, int device, jev_pages **out)
+{
+    if (!out) return fail(JEV_EINVAL, "out is null");
+    *out = nullptr;
+    if (!model || !cfg) return fail(JEV_EINVAL, "null argument");
+    const jev_config &f = *model;
+    const jev_pages_config &g = *cfg;
+    if (f.n_layers <= 0 || f.n_heads <= 0 || f.n_kv_heads <= 0) return fail(JEV_EINVAL, "model dimensions must be positive");
+    if (f.n_heads % f.n_kv_heads != 0)
+        return fail(JEV_EDATA, "%d attention heads do not divide into %d KV heads.", f.n_heads, f.n_kv_heads);
+    if (f.n_heads > 1024) return fail(JEV_EINVAL, "%d heads: at most 1024", f.n_heads);
+    if (f.head_dim != 64 && f.head_dim != 128)
+        return fail(JEV_EINVAL, "head_dim %d: the paged cache is built for 64- and 128-wide heads", f.head_dim);
+    if (f.rope_dim < 0 || f.rope_dim > f.head_dim || f.rope_dim % 2 != 0)
+        return fail(JEV_EINVAL, "rope_dim %d must be even and at most head_dim", f.rope_dim);
+    if (f.rope_dim > 0 && (!(f.rope_freq_base > 0.f) || !(f.rope_scale_factor > 0.f)))
+        return fail(JEV_EINVAL, "the rotary base and scale factor must be positive");
+    if (g.page_tokens < kPageBlock || g.page_tokens > 256 || (g.page_tokens & (g.page_tokens - 1)))
+        return fail(JEV_EINVAL, "page_tokens %d must be 16, 32, 64, 128 or 256", g.page_tokens);
+    if (g.n_pages <= 0 || (int64_t)g.n_pages * g.page_tokens > INT32_MAX)
+        return fail(JEV_EINVAL, "%d pages of %d tokens: slots must be positive and fit 31 bits", g.n_pages, g.page_tokens);
+    if (g.max_requests <= 0 || g.max_requests > kPagesMaxRequests)
+        return fail(JEV_EINVAL, "max_requests %d must be in [1, %d]", g.max_requests, kPagesMaxRequests);
+    if (g.max_context <= 0 || g.max_context > 1 << 24) return fail(JEV_EINVAL, "max_context %d must be in [1, 2^24]", g.max_context);
+    if (g.max_tokens <= 0 || g.max_tokens > 1 << 22) return fail(JEV_EINVAL, "max_tokens %d must be in [1, 2^22]", g.max_tokens);
+    if (g.rope_half != 0 && g.rope_half != 1) return fail(JEV_EINVAL, "rope_half must be 0 or 1");
+    int ndev = 0;
+    hipError_t e = hipGetDeviceCount(&ndev);
+    if (e != hipSuccess || ndev == 0) return fail(JEV_EDEVICE, "no HIP device: %s", hipGetErrorString(e));
+    if (device < 0 || device >= ndev) return fail(JEV_EINVAL, "device %d of %d", device, ndev);
+    HIP_TRY(hipSetDevice(device));
+
+    jev_pages *h = new jev_pages;
+    h->cfg = f;
+    h->device = device;
+    e = hipStreamCreate(&h->stream);
+    if (e != hipSuccess) {
+        delete h;
+        return fail(JEV_EDEVICE, "stream: %s", hipGetErrorString(e));
+    }
+    Pages &p = h->p;
+    p.n_layers = f.n_layers;
+    p.n_heads = f.n_heads;
+    p.n_kv = f.n_kv_heads;
+    p.hd = f.head_dim;
+    p.group = f.n_heads / f.n_kv_heads;
+    p.page = g.page_tokens;
+    p.sub = g.page_tokens / kPageBlock;
+    p.n_pages = g.n_pages;
+    p.max_requests = g.max_requests;
+    p.max_context = g.max_context;
+    p.max_tokens = g.max_tokens;
+    p.width = (g.max_context + g.page_tokens - 1) / g.page_tokens;
+    p.half = f.rope_dim / 2;
+    p.rope_half = g.rope_half;
+    p.orig_ctx = f.rope_original_context;
+    p.temp_scale = f.attention_temperature_scale;
+    p.scale = 1.0f / sqrtf((float)f.head_dim);
+    std::vector<double> freqs;
+    p.mscale = rope_table64(f, freqs);
+
+    // a tile's parts hold pages_part_keys() keys, the smallest where contexts are short
+    const size_t R = p.max_requests, T = p.max_tokens, pool = (size_t)p.n_pages * p.page;
+    const size_t split = (p.group + kPagesTileRows - 1) / kPagesTileRows; // tiles of a request that is split
+    p.max_parts = (int)(split * (pool / pages_part_keys(1) + R));
+    p.max_items = (int)(p.max_parts + T * p.group / kPagesTileRows + (split + 1) * R);
+    p.max_units = (int)(T / kPageBlock + 2 * R);
+    const size_t codes = p.n_blocks() * p.n_layers * kPageBlock * p.hd;
+    const int words = (p.n_pages + 31) / 32;
+    double *dfreqs = nullptr;
+    int rc = pages_alloc(h, p.k, codes);
+    if (!rc) rc = pages_alloc(h, p.v, codes);
+    if (!rc) rc = pages_alloc(h, p.ks, p.n_blocks() * p.n_layers);
+    if (!rc) rc = pages_alloc(h, p.table, R * p.width);
+    if (!rc) rc = pages_alloc(h, p.length, R);
+    if (!rc) rc = pages_alloc(h, p.used, words);
+    if (!rc) rc = pages_alloc(h, p.n_free, 1);
+    if (!rc) rc = pages_alloc(h, p.head, 1);
+    if (!rc) rc = pages_alloc(h, p.req, R);
+    if (!rc) rc = pages_alloc(h, p.fresh_pages, p.n_pages);
+    if (!rc) rc = pages_alloc(h, p.prefix, 4 * (size_t)(kPagesMaxRequests + 1));
+    if (!rc) rc = pages_alloc(h, p.unit, p.max_units);
+    if (!rc) rc = pages_alloc(h, p.item, p.max_items);
+    if (!rc) rc = pages_alloc(h, p.angle, T * p.half);
+    if (!rc) rc = pages_alloc(h, dfreqs, freqs.size());
+    if (!rc) rc = pages_alloc(h, h->ids, 2 * R);
+    if (!rc) rc = pages_alloc(h, p.part, (size_t)p.max_parts * p.n_kv * kPagesTileRows * (p.hd + 4));
+    if (!rc) {
+        p.freqs = dfreqs;
+        std::vector<uint32_t> used(words, 0);
+        if (p.n_pages % 32) used.back() = ~0u << (p.n_pages % 32); // bits past the pool are never free
+        e = hipStreamSynchronize(h->stream);
+        if (e == hipSuccess && !freqs.empty()) e = hipMemcpy(dfreqs, freqs.data(), freqs.size() * sizeof(double), hipMemcpyHostToDevice);
+        if (e == hipSuccess) e = hipMemcpy(p.used, used.data(), used.size() * sizeof(uint32_t), hipMemcpyHostToDevice);
+        if (e == hipSuccess) e = hipMemcpy(p.n_free, &p.n_pages, sizeof(int32_t), hipMemcpyHostToDevice);
+        if (e != hipSuccess) rc = fail(JEV_EDEVICE, "paged cache: %s", hipGetErrorString(e));
+    }
+    if (rc) {
+        std::string msg = g_error;
+        jev_pages_destroy(h);
+        return fail(rc, "%s", msg.c_str());
+    }
+    *out = h;
+    return JEV_OK;
+}
+
+void jev_pages_destroy(jev_pages *h)
+{
+    if (!h) return;
+    (void)hipSetDevice(h->device);
+    (void)hipStreamSynchronize(h->stream);
+    for (void *b : h->blocks) (void)hipFree(b);
+    (void)hipStreamDestroy(h->stream);
+    delete h;
+}
+
+int jev_pages_plan_device(jev_pages *h, const int32_t *request, const int32_t *past, const int32_t *fresh,
+                          int32_t n_requests, int32_t n_tokens, int32_t *table, int32_t *slot, int32_t *position,
+                          int32_t *row, int32_t *start)
+{
+    const int rc = check_pages(h);
+    if (rc) return rc;
+    PagesPlanArgs a;
+    a.request = request;
+    a.past = past;
+    a.fresh = fresh;
+    a.n_requests = n_requests;
+    a.n_tokens = n_tokens;
+    a.table = table;
+    a.slot = slot;
+    a.position = position;
+    a.row = row;
+    a.start = start;
+    return pages_plan(h, a, h->stream);
+}
+
+int jev_pages_store_device(jev_pages *h, int32_t layer, const float *q, int64_t q_ld, const float *k, const float *v,
+                           int64_t kv_ld, float *q_out)
+{
+    const int rc = check_pages_layer(h, layer);
+    if (rc) return rc;
+    const int64_t qdim = (int64_t)h->p.n_heads * h->p.hd, kvdim = (int64_t)h->p.n_kv * h->p.hd;
+    if (!q != !q_out || !k != !v || (!q && !k))
+        return fail(JEV_EINVAL, "q and q_out, or k and v, come together, and one of the two at least");
+    if (q && q_ld < qdim) return fail(JEV_EINVAL, "q_ld %lld is less than a row of %lld", (long long)q_ld, (long long)qdim);
+    if (k && kv_ld < kvdim) return fail(JEV_EINVAL, "kv_ld %lld is less than a row of %lld", (long long)kv_ld, (long long)kvdim);
+    if (q && q == q_out && q_ld != qdim) return fail(JEV_EINVAL, "rotating in place needs q_ld %lld", (long long)qdim);
+    PagesStoreArgs a;
+    a.layer = layer;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.q_ld = q_ld;
+    a.kv_ld = kv_ld;
+    a.q_out = q_out;
+    a.n_requests = h->plan.n_requests;
+    a.n_tokens = h->plan.n_tokens;
+    HIP_TRY(launch_pages_store(h->p, a, h->stream));
+    return JEV_OK;
+}
+
+int jev_pages_attend_device(jev_pages *h, int32_t layer, const float *q, float *out)
+{
+    const int rc = check_pages_layer(h, layer);
+    if (rc) return rc;
+    if (!q || !out || q == out) return fail(JEV_EINVAL, "q and out must not be null, nor the same array");
+    PagesAttendArgs a;
+    a.layer = layer;
+    a.q = q;
+    a.out = out;
+    a.n_requests = h->plan.n_requests;
+    a.n_tokens = h->plan.n_tokens;
+    a.wide = h->plan.wide;
+    HIP_TRY(launch_pages_attend(h->p, a, h->stream));
+    return JEV_OK;
+}
+
+int jev_pages_read_device(jev_pages *h, int32_t layer, const int32_t *slot, int32_t n, float *k, float *v)
+{
+    const int rc = check_pages_layer(h, layer);
+    if (rc) return rc;
+    if (n < 0 || (n > 0 && (!slot || !k || !v))) return fail(JEV_EINVAL, "bad arguments");
+    HIP_TRY(launch_pages_read(h->p, layer, slot, n, k, v, h->stream));
+    return JEV_OK;
+}
+
+int jev_pages_release(jev_pages *h, const int32_t *request, int32_t n)
+{
+    int rc = check_pages(h);
+    if (rc) return rc;
+    if (n < 0 || n > h->p.max_requests || (n > 0 && !request))
+        return fail(JEV_EINVAL, "a release needs 0 to %d requests", h->p.max_requests);
+    if (n > 0) HIP_TRY(hipMemcpyAsync(h->ids, request, n * sizeof(int32_t), hipMemcpyHostToDevice, h->stream));
+    PagesPlanArgs a;
+    a.request = h->ids;
+    a.past = a.fresh = h->ids + h->p.max_requests;
+    a.n_requests = n;
+    rc = pages_plan(h, a, h->stream);
+    return rc ? rc : pages_status(h, h->stream);
+}
+
+int jev_pages_sync(jev_pages *h)
+{
+    const int rc = check_pages(h);
+    return rc ? rc : pages_status(h, h->stream);
+}
+
+void *jev_pages_stream(jev_pages *h) { return h ? (void *)h->stream : nullptr; }
+
+int jev_forward_pages(jev_ctx *c, jev_pages *h, const int32_t *request, const int32_t *past, const int32_t *fresh,
+                      int32_t n_requests, const int32_t *tokens, int32_t n_tokens, int mode, const int32_t *rows,
+                      int32_t n_rows, float *out, size_t out_len)
+{
+    int rc = check_ready(c);
+    if (rc) return rc;
+    if (!h) return fail(JEV_EINVAL, "null paged cache");
+    const jev_config &f = c->cfg, &g = h->cfg;
+    const Pages &pg = h->p;
+    if (h->device != c->device) return fail(JEV_EINVAL, "the paged cache is on device %d, the model on %d", h->device, c->device);
+    if (g.n_layers != f.n_layers || g.n_heads != f.n_heads || g.n_kv_heads != f.n_kv_heads || g.head_dim != f.head_dim)
+        return fail(JEV_EINVAL, "the paged cache was made for another model's geometry");
+    if (pg.rope_half || g.rope_dim != f.rope_dim || g.rope_freq_base != f.rope_freq_base ||
+        g.rope_scale_factor != f.rope_scale_factor || g.rope_scaling_yarn != f.rope_scaling_yarn ||
+        g.rope_original_context != f.rope_original_context || g.yarn_beta_fast != f.yarn_beta_fast ||
+        g.yarn_beta_slow != f.yarn_beta_slow || g.yarn_ext_factor != f.yarn_ext_factor || g.yarn_mscale != f.yarn_mscale ||
+        g.yarn_mscale_all_dim != f.yarn_mscale_all_dim || g.rope_attn_factor != f.rope_attn_factor ||
+        g.attention_temperature_scale != f.attention_temperature_scale)
+        return fail(JEV_EINVAL, "the paged cache rotates positions otherwise than the model");
+    if (!request || !fresh || !tokens || n_requests <= 0 || n_requests > pg.max_requests || n_tokens <= 0 || n_tokens > pg.max_tokens)
+        return fail(JEV_EINVAL, "a step needs 1 to %d requests and 1 to %d tokens", pg.max_requests, pg.max_tokens);
+    if (mode != JEV_OUT_NONE && mode != JEV_OUT_SELECTED && mode != JEV_OUT_FULL)
+        return fail(JEV_EINVAL, "output mode %d: a step over pages returns nothing, selected rows or full rows", mode);
+    if (mode == JEV_OUT_SELECTED) {
+        if (!rows || n_rows <= 0) return fail(JEV_EINVAL, "selected-rows mode needs rows");
+        for (int i = 0; i < n_rows; i++)
+            if (rows[i] < 0 || rows[i] >= c->table().rows)
+                return fail(JEV_EINVAL, "vocabulary row %d is outside the %d-row head", rows[i], c->table().rows);
+    }
+    std::vector<int32_t> ids(request, request + n_requests), last(n_requests);
+    std::sort(ids.begin(), ids.end());
+    if (ids.front() < 0 || ids.back() >= pg.max_requests || std::adjacent_find(ids.begin(), ids.end()) != ids.end())
+        return fail(JEV_EINVAL, "requests must be distinct and in [0, %d)", pg.max_requests);
+    int64_t total = 0;
+    for (int b = 0; b < n_requests; b++) {
+        if (fresh[b] < 1 || (past && past[b] < 0)) return fail(JEV_EINVAL, "request %d: a negative past or no new token", request[b]);
+        total += fresh[b];
+        last[b] = (int32_t)(total - 1);
+    }
+    if (total != n_tokens) return fail(JEV_EINVAL, "the requests add %lld tokens, and %d came", (long long)total, n_tokens);
+    for (int t = 0; t < n_tokens; t++)
+        if (tokens[t] < 0 || tokens[t] >= c->embd.rows)
+            return fail(JEV_EINVAL, "Token id %d is outside the %d-entry embedding table.", tokens[t], c->embd.rows);
+    const size_t nf = out_floats(c, mode, n_requests, n_rows);
+    if (nf > 0 && (!out || out_len < nf)) return fail(JEV_EINVAL, "the output needs %zu floats", nf);
+
+    Plan p;
+    p.T = n_tokens;
+    p.n_out = n_requests;
+    rc = ensure_workspace(c, n_tokens, n_requests, mode, 1);
+    if (rc) return rc;
+    // tokens, request, past, fresh, last rows, vocabulary rows
+    std::vector<int32_t> &H = c->host_ints;
+    H.assign(tokens, tokens + n_tokens);
+    const size_t o_req = H.size();
+    H.insert(H.end(), request, request + n_requests);
+    const size_t o_past = H.size();
+    if (past) H.insert(H.end(), past, past + n_requests);
+    const size_t o_fresh = H.size();
+    H.insert(H.end(), fresh, fresh + n_requests);
+    const size_t o_out = H.size();
+    H.insert(H.end(), last.begin(), last.end());
+    const size_t o_rows = H.size();
+    if (mode == JEV_OUT_SELECTED) H.insert(H.end(), rows, rows + n_rows);
+    HIP_TRY(grow(c, c->ints, H.size()));
+    if (mode == JEV_OUT_SELECTED) HIP_TRY(grow(c, c->logits, nf));
+    HIP_TRY(hipStreamSynchronize(h->stream)); // what the handle's own calls do comes first
+    // from pageable memory: the copy has read H when it returns
+    HIP_TRY(hipMemcpyAsync(c->ints.p, H.data(), H.size() * sizeof(int32_t), hipMemcpyHostToDevice, c->stream));
+    const int32_t *base = c->ints.p;
+    p.d_tokens = base;
+    p.d_out = base + o_out;
+    p.d_rows = mode == JEV_OUT_SELECTED ? base + o_rows : nullptr;
+    PagedStep step;
+    step.pages = &pg;
+    step.args.request = base + o_req;
+    step.args.past = past ? base + o_past : nullptr;
+    step.args.fresh = base + o_fresh;
+    step.args.n_requests = n_requests;
+    step.args.n_tokens = n_tokens;
+    CallScope call(c);
+    rc = pages_plan(h, step.args, c->stream);
+    step.args = h->plan;
+    if (!rc) rc = enqueue_forward(c, p, mode, n_rows, c->logits.p, nullptr, &call, true, nullptr, &step);
+    if (!rc) rc = copy_out(c, out, c->logits.p, nf);
+    else (void)hipStreamSynchronize(c->stream);
+    if (!rc && call.cancelled()) rc = fail(JEV_ECANCELED, "the forward pass was cancelled");
+    return rc ? rc : pages_status(h, c->stream);
 }
 
 } // extern "C"

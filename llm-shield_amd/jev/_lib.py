@@ -54,6 +54,14 @@ class Layout(ctypes.Structure):
     ]
 
 
+class PagesConfig(ctypes.Structure):
+    """jev_pages_config."""
+    _fields_ = [
+        ("n_pages", c_int32), ("page_tokens", c_int32), ("max_requests", c_int32), ("max_context", c_int32),
+        ("max_tokens", c_int32), ("rope_half", c_int32),
+    ]
+
+
 # jev_sink: IActivationSink.Observe (MinistralModel.cs:787-790)
 SINK = ctypes.CFUNCTYPE(None, c_void_p, c_char_p, POINTER(c_float), c_int32, c_int32)
 
@@ -131,6 +139,17 @@ def lib():
         "jev_matmul_device_noalloc": (c_int, [c_void_p, c_void_p, c_int32, c_void_p]),
         "jev_weight_sync": (c_int, [c_void_p]),
         "jev_weight_stream": (c_void_p, [c_void_p]),
+        "jev_pages_create": (c_int, [POINTER(Config), POINTER(PagesConfig), c_int, POINTER(c_void_p)]),
+        "jev_pages_destroy": (None, [c_void_p]),
+        "jev_pages_plan_device": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32] + [c_void_p] * 5),
+        "jev_pages_store_device": (c_int, [c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
+        "jev_pages_attend_device": (c_int, [c_void_p, c_int32, c_void_p, c_void_p]),
+        "jev_pages_read_device": (c_int, [c_void_p, c_int32, c_void_p, c_int32, c_void_p, c_void_p]),
+        "jev_pages_release": (c_int, [c_void_p, I32P, c_int32]),
+        "jev_pages_sync": (c_int, [c_void_p]),
+        "jev_pages_stream": (c_void_p, [c_void_p]),
+        "jev_forward_pages": (c_int, [c_void_p, c_void_p, I32P, I32P, I32P, c_int32, I32P, c_int32, c_int, I32P, c_int32,
+                                      F32P, c_size_t]),
         "jev_rope_table": (c_int, [POINTER(Config), F32P, c_int32, F32P]),
         "jev_dequantize": (c_int, [c_int, c_void_p, c_size_t, F32P, c_int64]),
         "jev_matmul_q": (c_int, [c_int, c_void_p, c_int64, c_int64, F32P, c_int32, F32P]),
@@ -163,4 +182,6 @@ EXPORTED = [
     "jev_set_matmul_strategy", "jev_get_matmul_strategy", "jev_quantize_activations", "jev_rope_table",
     "jev_matmul_device_noalloc", "jev_capture", "jev_weight_stream", "jev_kv_snapshot_device",
     "jev_kv_restore_device", "jev_snapshot_length", "jev_snapshot_read", "jev_snapshot_destroy",
+    "jev_pages_create", "jev_pages_destroy", "jev_pages_plan_device", "jev_pages_store_device", "jev_pages_attend_device",
+    "jev_pages_read_device", "jev_pages_release", "jev_pages_sync", "jev_pages_stream", "jev_forward_pages",
 ]

@@ -378,6 +378,26 @@ class MinistralModel:
         flat = self.forward_layout(tokens, lay, L.OUT_SELECTED, r).reshape(len(counts), len(r))
         return [flat[i].copy() for i in range(len(counts))]
 
+    def forward_pages(self, pages, requests, request_tokens, past=None, vocab_rows=None, outputs: bool = True):
+        """A step over a paged cache (KvPages): requests[b] keeps past[b] tokens (past None: all it
+        has) and appends request_tokens[b].  Returns each request's last-token logits (of
+        vocab_rows, or the whole vocabulary), or None without `outputs`.  The context's own
+        cache is left alone."""
+        ids, counts = _i32(requests), _i32([len(t) for t in request_tokens])
+        kept = _i32(past) if past is not None else None
+        if len(ids) != len(counts) or (kept is not None and len(kept) != len(ids)):
+            raise L.ArgumentError(L.JEV_EINVAL, "requests, request_tokens and past must have one entry per request")
+        tok = np.concatenate([_i32(t) for t in request_tokens]) if len(counts) else _i32([])
+        r = _i32(vocab_rows) if vocab_rows is not None else None
+        mode = L.OUT_NONE if not outputs else L.OUT_FULL if r is None else L.OUT_SELECTED
+        width = 0 if not outputs else self.config.vocab if r is None else len(r)
+        out = np.empty(max(1, len(ids) * width), np.float32)
+        L.check(self._lib.jev_forward_pages(self._h, pages.handle, _ptr(ids, ctypes.c_int32), _ptr(kept, ctypes.c_int32),
+                                            _ptr(counts, ctypes.c_int32), len(ids), _ptr(tok, ctypes.c_int32), len(tok), mode,
+                                            _ptr(r, ctypes.c_int32), 0 if r is None else len(r), _ptr(out, ctypes.c_float),
+                                            out.size))
+        return out.reshape(len(ids), width) if outputs else None
+
     def decode_greedy(self, first: int, steps: int) -> np.ndarray:
         """Greedy decode: ForwardAsync([next]) + ArgMax per step (Benchmark.cs:411-422)."""
         out = np.empty(steps, np.int32)

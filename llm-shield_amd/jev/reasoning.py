@@ -171,3 +171,47 @@ def batched_greedy(model, prompts: Sequence[Sequence[int]], max_new_tokens: int,
             results[i] = toks
         model.reset_kv_cache()
     return results
+
+
+def paged_greedy(model, pages, prompts: Sequence[Sequence[int]], max_new_tokens: int, stop_tokens: Sequence[int] = ()) -> List[List[int]]:
+    """Every prompt's greedy continuation over a paged cache (KvPages), as batched_greedy's results.
+
+    A prompt starts as soon as a request of the cache, the plan's rows and the pages for its
+    whole continuation are free, beside the ones already decoding: a step is the new prompts'
+    tokens and one token of every running request.  The requests of `pages` are released at
+    the end; what they held before is dropped."""
+    if max_new_tokens < 1:
+        raise L.ArgumentError(L.JEV_EINVAL, "max_new_tokens must be at least 1.")
+    if any(len(p) == 0 for p in prompts):
+        raise L.ArgumentError(L.JEV_EINVAL, "Every row needs at least one token.")
+    need = [-(-(len(p) + max_new_tokens - 1) // pages.page_tokens) for p in prompts]
+    for p, n in zip(prompts, need):
+        if len(p) + max_new_tokens - 1 > pages.max_context or len(p) > pages.max_tokens or n > pages.n_pages:
+            raise L.ArgumentError(L.JEV_EINVAL, f"a prompt of {len(p)} tokens and its continuation do not fit the paged cache.")
+    stops = set(int(t) for t in stop_tokens)
+    out: List[List[int]] = [[] for _ in prompts]
+    pages.release(range(pages.max_requests))
+    idle, free, waiting = list(range(pages.max_requests))[::-1], pages.n_pages, list(range(len(prompts)))[::-1]
+    running = {}  # prompt -> (request, tokens it holds, tokens to feed)
+    while waiting or running:
+        rows = len(running)
+        while waiting and idle and need[waiting[-1]] <= free and rows + len(prompts[waiting[-1]]) <= pages.max_tokens:
+            i = waiting.pop()
+            rows += len(prompts[i])
+            free -= need[i]
+            running[i] = (idle.pop(), 0, list(prompts[i]))
+        order = list(running)
+        logits = model.forward_pages(pages, [running[i][0] for i in order], [running[i][2] for i in order],
+                                     past=[running[i][1] for i in order])
+        for i, row in zip(order, logits):
+            request, held, fed = running[i]
+            token = _argmax(row)
+            out[i].append(token)
+            if token in stops or len(out[i]) == max_new_tokens:
+                pages.release([request])
+                idle.append(request)
+                free += need[i]
+                del running[i]
+            else:
+                running[i] = (request, held + len(fed), [token])
+    return out
