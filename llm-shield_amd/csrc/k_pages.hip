@@ -432,15 +432,17 @@ __device__ __forceinline__ int v_at(int t, int d) { return d * 16 + t; }
 
 // One workgroup per block that the batch touches and KV head: the block's new
 // tokens' queries (of the head's group) rotated, their keys rotated and stored,
-// their values stored.  Sixteen threads hold a token's row.  Products of the
-// rotation are 64-bit and round to fp32 once, so a stored code does not depend
-// on how they are formed.  A block's scale only grows while the block fills;
-// codes it already holds are then rounded to the new one.  Bounded by memory:
-// 4 B in per element, 1 B (K, V) or 4 B (q) out.
+// their values stored.  Sixteen threads hold a token's row, and keep to one
+// token, so its angles are loaded once for all rows; with fewer tokens in the
+// block its rows are dealt over the idle sixteens.  Products of the rotation
+// are 64-bit and round to fp32 once, so a stored code does not depend on how
+// they are formed.  A block's scale only grows while the block fills; codes it
+// already holds are then rounded to the new one.  Bounded by memory: 4 B in per
+// element, 1 B (K, V) or 4 B (q) out.
 template <int HD, bool VEC>
 __global__ __launch_bounds__(256) void pages_store_kernel(Pages p, PagesStoreArgs a)
 {
-    constexpr int NP = HD / 32, BYTES = kPageBlock * HD;
+    constexpr int NP = HD / 32, BYTES = kPageBlock * HD, RING = 2;
     __shared__ __align__(16) uint8_t code[2][BYTES];
     __shared__ unsigned most[2];
     const int tid = threadIdx.x, j = tid & 15, h = blockIdx.y;
@@ -450,8 +452,12 @@ __global__ __launch_bounds__(256) void pages_store_kernel(Pages p, PagesStoreArg
     const int pos0 = max(r.past, un.y * kPageBlock), pos1 = min(r.len, (un.y + 1) * kPageBlock);
     const int n = pos1 - pos0, row0 = r.start + pos0 - r.past, off = pos0 & (kPageBlock - 1);
     const bool kv = a.k != nullptr;
-    const int lead = kv ? 2 : 0, rows = n * (lead + (a.q ? p.group : 0));
     const RowPairs<HD> e(p, j);
+
+    // this thread's token, and its rows: K (-2), V (-1), then the group's queries
+    const int nt = n > 8 ? 16 : n > 4 ? 8 : n > 2 ? 4 : n, step = 16 / nt; // (nt: 1, 2, 4, 8, 16)
+    const int t = (tid >> 4) % nt, row = row0 + t, first = (kv ? -2 : 0) + (tid >> 4) / nt, end = t < n && a.q ? p.group : 0;
+    const bool mine = t < n;
 
     // where the block lies
     const int page = p.table[(size_t)r.id * p.width + un.y / p.sub];
@@ -468,64 +474,77 @@ __global__ __launch_bounds__(256) void pages_store_kernel(Pages p, PagesStoreArg
             if (begun) w = ((const uint4 *)((v ? p.v : p.k) + block * BYTES))[i];
             ((uint4 *)code[v])[i] = w;
         }
-        __syncthreads();
     }
+    double2 g[NP];
+#pragma unroll
+    for (int c = 0; c < NP; c++) {
+        const int q = NP * j + c;
+        g[c] = mine && q < p.half ? p.angle[(size_t)row * p.half + q] : make_double2(0.0, 0.0);
+    }
+    auto load = [&](int which, float2 (&y)[NP]) {
+        const float *src = which == -2 ? a.k + row * a.kv_ld + h * HD
+                           : which == -1 ? a.v + row * a.kv_ld + h * HD
+                                         : a.q + row * a.q_ld + (size_t)(h * p.group + which) * HD;
+        load_pairs<HD, VEC>(e, src, y);
+        for (int z = 1; z < a.nin; z++) {
+            float2 w[NP];
+            load_pairs<HD, VEC>(e, src + z * a.in_stride, w);
+#pragma unroll
+            for (int c = 0; c < NP; c++) y[c] = make_float2(y[c].x + w[c].x, y[c].y + w[c].y);
+        }
+    };
+    auto rotate = [&](double f, float2 (&y)[NP]) {
+#pragma unroll
+        for (int c = 0; c < NP; c++) {
+            const double u = y[c].x, v = y[c].y;
+            const double m0 = u * g[c].x, m1 = v * g[c].y, m2 = u * g[c].y, m3 = v * g[c].x;
+            const bool turned = NP * j + c < p.half;
+            y[c] = make_float2((float)((turned ? m0 - m1 : u) * f), (float)((turned ? m2 + m3 : v) * f));
+        }
+    };
 
-    float2 x[2][NP]; // the K and V rows of this thread: two rows at most
-#pragma unroll 1
-    for (int base = 0; base < rows; base += 32) {
+    float2 x[2][NP]; // this thread's rows of K and V
+    int w = first;
+    if (kv) {
+        __syncthreads(); // `most` is zero
+#pragma unroll
+        for (int it = 0; it < 2; it++)
+            if (mine && w + it * step < 0) load(w + it * step, x[it]);
 #pragma unroll
         for (int it = 0; it < 2; it++) {
-            const int i = base + 16 * it + (tid >> 4);
-            if (i >= rows) continue;
-            const int t = i % n, which = i / n - lead; // -2: K, -1: V, else a query head of the group
-            const int row = row0 + t;
-            const float *src = which == -2 ? a.k + row * a.kv_ld + h * HD
-                               : which == -1 ? a.v + row * a.kv_ld + h * HD
-                                             : a.q + row * a.q_ld + (size_t)(h * p.group + which) * HD;
-            float2 y[NP];
-            load_pairs<HD, VEC>(e, src, y);
-            for (int z = 1; z < a.nin; z++) {
-                float2 w[NP];
-                load_pairs<HD, VEC>(e, src + z * a.in_stride, w);
+            const int which = w + it * step;
+            if (!mine || which >= 0) continue;
+            if (which == -2) rotate(1.0, x[it]);
+            unsigned m = 0; // a value that is not finite has the largest bits
 #pragma unroll
-                for (int c = 0; c < NP; c++) y[c] = make_float2(y[c].x + w[c].x, y[c].y + w[c].y);
-            }
-            if (which != -1) {
-                double f = 1.0;
-                const int pos = pos0 + t;
-                if (which >= 0 && p.orig_ctx > 0 && p.temp_scale != 0.f && pos >= p.orig_ctx)
-                    f = 1.0 + (double)p.temp_scale * log(1.0 + (double)(pos / p.orig_ctx));
-#pragma unroll
-                for (int c = 0; c < NP; c++) {
-                    double u = y[c].x, v = y[c].y;
-                    const int q = NP * j + c;
-                    if (q < p.half) {
-                        const double2 g = p.angle[(size_t)row * p.half + q];
-                        const double m0 = u * g.x, m1 = v * g.y, m2 = u * g.y, m3 = v * g.x;
-                        u = m0 - m1;
-                        v = m2 + m3;
-                    }
-                    y[c] = make_float2((float)(u * f), (float)(v * f));
-                }
-            }
-            if (which >= 0) {
-                store_pairs<HD, VEC>(e, a.q_out + ((size_t)row * p.n_heads + h * p.group + which) * HD, y);
-            } else {
-                unsigned m = 0; // a value that is not finite has the largest bits
-#pragma unroll
-                for (int c = 0; c < NP; c++) {
-                    x[it][c] = y[c];
-                    m = max(m, max(__float_as_uint(fabsf(y[c].x)), __float_as_uint(fabsf(y[c].y))));
-                }
-                atomicMax(&most[which + 2], m);
-            }
+            for (int c = 0; c < NP; c++)
+                m = max(m, max(__float_as_uint(fabsf(x[it][c].x)), __float_as_uint(fabsf(x[it][c].y))));
+            for (int o = 1; o < 16; o <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
+            if (j == 0) atomicMax(&most[which + 2], m);
         }
-        if (!kv) continue;
-        if (base > 0) continue;
-        __syncthreads(); // K and V rows are all in the first round
+        while (w < 0) w += step;
+    }
+    if (end) {
+        double f = 1.0;
+        const int pos = pos0 + t;
+        if (p.orig_ctx > 0 && p.temp_scale != 0.f && pos >= p.orig_ctx)
+            f = 1.0 + (double)p.temp_scale * log(1.0 + (double)(pos / p.orig_ctx));
+        // RING rows in flight
+        for (; w < end; w += RING * step) {
+            float2 y[RING][NP];
+#pragma unroll
+            for (int i = 0; i < RING; i++)
+                if (w + i * step < end) load(w + i * step, y[i]);
+#pragma unroll
+            for (int i = 0; i < RING; i++)
+                if (w + i * step < end) {
+                    rotate(f, y[i]);
+                    store_pairs<HD, VEC>(e, a.q_out + ((size_t)row * p.n_heads + h * p.group + w + i * step) * HD, y[i]);
+                }
+        }
     }
     if (!kv) return;
+    __syncthreads(); // `most` and the old codes are whole
 
     float s[2];
     double by[2], inv[2];
@@ -539,38 +558,39 @@ __global__ __launch_bounds__(256) void pages_store_kernel(Pages p, PagesStoreArg
     }
     if (begun && tid < 2 * BYTES / 16) {
         const bool v = tid >= BYTES / 16;
-        const float old = v ? s_old.y : s_old.x;
-        if (s[v] != old) { // also where either is NaN
-            uint32_t *w = (uint32_t *)code[v] + 4 * (v ? tid - BYTES / 16 : tid);
+        const float old = v ? s_old.y : s_old.x, now = v ? s[1] : s[0];
+        const double d = v ? by[1] : by[0], id = v ? inv[1] : inv[0];
+        if (now != old) { // also where either is NaN
+            uint32_t *word = (uint32_t *)code[v] + 4 * (v ? tid - BYTES / 16 : tid);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 uint32_t y = 0;
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    const int q = (int)((w[i] >> (8 * c)) & 255u) - 128;
-                    y |= (s[v] > 0.f ? code_of((double)q * (double)old, by[v], inv[v]) : 128u) << (8 * c);
+                    const int q = (int)((word[i] >> (8 * c)) & 255u) - 128;
+                    y |= (now > 0.f ? code_of((double)q * (double)old, d, id) : 128u) << (8 * c);
                 }
-                w[i] = y;
+                word[i] = y;
             }
         }
-        // places from the first new token on held nothing, or what a shorter
-        // keep gave up: the new tokens' codes come over them below, the rest
-        // is past the request's end
     }
+    // places from the first new token on held nothing, or what the request was
+    // cut back from: the new codes come over them, the rest is past its end
     __syncthreads();
 #pragma unroll
     for (int it = 0; it < 2; it++) {
-        const int i = 16 * it + (tid >> 4);
-        if (i >= 2 * n) continue;
-        const int v = i / n, t = off + i % n;
+        const int which = first + it * step;
+        if (!mine || which >= 0) continue;
+        const bool v = which == -1;
+        const double d = v ? by[1] : by[0], id = v ? inv[1] : inv[0];
+        const bool zero = !(d > 0.0);
+        const int tk = off + t;
 #pragma unroll
         for (int c = 0; c < NP; c++) {
-            const bool zero = !(s[v] > 0.f);
-            const uint32_t q0 = zero ? 128u : code_of((double)x[it][c].x, by[v], inv[v]);
-            const uint32_t q1 = zero ? 128u : code_of((double)x[it][c].y, by[v], inv[v]);
-            const int a0 = v ? v_at<HD>(t, e.e0[c]) : k_at<HD>(t, e.e0[c]), a1 = v ? v_at<HD>(t, e.e1[c]) : k_at<HD>(t, e.e1[c]);
-            code[v][a0] = (uint8_t)q0;
-            code[v][a1] = (uint8_t)q1;
+            const uint32_t q0 = zero ? 128u : code_of((double)x[it][c].x, d, id);
+            const uint32_t q1 = zero ? 128u : code_of((double)x[it][c].y, d, id);
+            code[v][v ? v_at<HD>(tk, e.e0[c]) : k_at<HD>(tk, e.e0[c])] = (uint8_t)q0;
+            code[v][v ? v_at<HD>(tk, e.e1[c]) : k_at<HD>(tk, e.e1[c])] = (uint8_t)q1;
         }
     }
     __syncthreads();
@@ -886,37 +906,57 @@ hipError_t launch_pages_attend(const Pages &p, const PagesAttendArgs &a, hipStre
 
 // ------------------------------------------------------------ reading back
 
-// Sixteen threads hold a (slot, KV head) row of K and V.
+// Sixteen slots and one KV head to a workgroup.  K rows lie in runs of 64
+// dims.  V lies dim by dim, so its bytes are read with the tokens along the
+// lanes (neighbouring slots: one 64-byte run per load) and turned in LDS.
 template <int HD>
 __global__ __launch_bounds__(256) void pages_read_kernel(Pages p, int layer, const int32_t *slot, int n, float *k, float *v)
 {
-    constexpr int ND = HD / 16, BYTES = kPageBlock * HD;
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;
-    const int j = threadIdx.x & 15;
-    if (i >= (int64_t)n * p.n_kv) return;
-    const int h = (int)(i % p.n_kv), sl = slot[i / p.n_kv];
-    float kk[ND] = {}, vv[ND] = {};
-    if (sl >= 0 && sl / p.page < p.n_pages) {
-        const int t = sl % kPageBlock;
-        const size_t b = ((size_t)(sl / p.page) * p.n_kv + h) * p.sub + sl % p.page / kPageBlock + (size_t)layer * p.n_blocks();
-        const float2 s = p.ks[b];
-#pragma unroll
-        for (int c = 0; c < ND; c++) {
-            kk[c] = (float)((int)p.k[b * BYTES + k_at<HD>(t, ND * j + c)] - 128) * s.x;
-            vv[c] = (float)((int)p.v[b * BYTES + v_at<HD>(t, ND * j + c)] - 128) * s.y;
+    constexpr int ND = HD / 16, BYTES = kPageBlock * HD, LD = HD + 4;
+    __shared__ __align__(16) float lv[16][LD];
+    const int tid = threadIdx.x, h = blockIdx.y, first = blockIdx.x * 16;
+    struct Place {
+        size_t block;
+        int token;
+        float2 s;
+    };
+    auto place = [&](int i) { // of the workgroup's slot i
+        Place r = {0, 0, make_float2(0.f, 0.f)};
+        const int sl = first + i < n ? slot[first + i] : -1;
+        if (sl >= 0 && sl / p.page < p.n_pages) {
+            r.token = sl % kPageBlock;
+            r.block = ((size_t)(sl / p.page) * p.n_kv + h) * p.sub + sl % p.page / kPageBlock + (size_t)layer * p.n_blocks();
+            r.s = p.ks[r.block];
         }
-    }
+        return r; // elsewhere the pool's first block with scales of zero
+    };
+    {
+        const Place r = place(tid & 15);
+        const uint8_t *src = p.v + r.block * BYTES + r.token;
+        uint8_t c[ND];
 #pragma unroll
-    for (int c = 0; c < ND; c++) {
-        k[i * HD + ND * j + c] = kk[c];
-        v[i * HD + ND * j + c] = vv[c];
+        for (int i = 0; i < ND; i++) c[i] = src[(i * 16 + (tid >> 4)) * 16];
+#pragma unroll
+        for (int i = 0; i < ND; i++) lv[tid & 15][i * 16 + (tid >> 4)] = (float)((int)c[i] - 128) * r.s.y;
     }
+    const int i = tid >> 4, j = tid & 15;
+    const Place r = place(i);
+    uint32_t w[ND / 4];
+#pragma unroll
+    for (int c = 0; c < ND / 4; c++) w[c] = *(const uint32_t *)(p.k + r.block * BYTES + k_at<HD>(r.token, ND * j + 4 * c));
+    __syncthreads();
+    if (first + i >= n) return;
+    const size_t to = ((size_t)(first + i) * p.n_kv + h) * HD + ND * j;
+#pragma unroll
+    for (int c = 0; c < ND; c++) k[to + c] = (float)((int)((w[c / 4] >> (8 * (c % 4))) & 255u) - 128) * r.s.x;
+#pragma unroll
+    for (int c = 0; c < ND; c++) v[to + c] = lv[i][ND * j + c];
 }
 
 hipError_t launch_pages_read(const Pages &p, int layer, const int32_t *slot, int n, float *k, float *v, hipStream_t s)
 {
     if (n <= 0) return hipSuccess;
-    const dim3 grid((unsigned)(((int64_t)n * p.n_kv * 16 + 255) / 256));
+    const dim3 grid((n + 15) / 16, p.n_kv);
     if (p.hd == 128) hipLaunchKernelGGL(pages_read_kernel<128>, grid, dim3(256), 0, s, p, layer, slot, n, k, v);
     else hipLaunchKernelGGL(pages_read_kernel<64>, grid, dim3(256), 0, s, p, layer, slot, n, k, v);
     return hipGetLastError();
