@@ -418,6 +418,12 @@ hipError_t launch_kv_copy(const float *src, float *dst, int heads_total, int old
 constexpr int kPageBlock = 16;         // tokens that share a scale
 constexpr int kPagesMaxRequests = 4096; // a plan's prefix sums live in LDS
 constexpr int kPagesTileRows = 16;     // (token, head) rows of a KV head in one attention tile
+constexpr int kPagesWideRows = 128;    // the same in a wide tile, for requests that add many tokens
+// Wide tiles are split over their keys when there are few: into at most this
+// many workgroups over all KV heads (two fit a compute unit: one round), none of
+// less than kPagesWideKeys keys.
+constexpr int kPagesWideWgs = 512, kPagesWideKeys = 512;
+__host__ __device__ inline int pages_wide_target(int n_kv) { return n_kv < kPagesWideWgs ? kPagesWideWgs / n_kv : 1; }
 
 // Keys per workgroup of a tile whose rows are one request's whole batch: a
 // function of the request's own length alone, so that its result does not
@@ -430,13 +436,14 @@ struct PagesPlanHead {
     int32_t n_units; // blocks that the batch's tokens go to
     int32_t n_items; // workgroups of attention per KV head, 16-row tiles
     int32_t n_wide;  // the same, wide tiles
-    int32_t n_parts; // partial results of split tiles
+    int32_t n_parts, n_wide_parts; // partial results of split tiles
     int32_t n_requests;
     int32_t pad;
 };
 struct PagesRequest { // one batch row
     int32_t id, past, len, start; // start: its first token's row in the batch
-    int32_t part0, n_parts;       // partial results of its tile, when split (n_parts > 1)
+    int32_t part0, n_parts;       // partial results of its tiles, when split (n_parts > 1)
+    int32_t wide;                 // its tiles are wide ones
 };
 struct PagesItem {
     int32_t b, row0, key0, key1, part; // part >= 0: where its partial result goes
@@ -467,8 +474,10 @@ struct Pages {
     PagesItem *item = nullptr, *wide = nullptr;
     double2 *angle = nullptr;               // [max_tokens][half] (cos, sin) * mscale
     const double *freqs = nullptr;
-    float *part = nullptr;                  // [n_parts][kv head][16][hd + 2]
-    int max_units = 0, max_items = 0, max_wide = 0, max_parts = 0;
+    float *part = nullptr;                  // [n_parts][kv head][16][hd + 4]: output, max, sum
+    float *wide_part = nullptr;             // [n_wide_parts][kv head][128][hd + 4]
+    int2 *wide_owner = nullptr;             // [n_wide_parts] batch row, place among its request's
+    int max_units = 0, max_items = 0, max_wide = 0, max_parts = 0, max_wide_parts = 0;
     __host__ __device__ size_t n_blocks() const { return (size_t)n_pages * n_kv * sub; } // of a layer
 };
 struct PagesPlanArgs {

@@ -56,35 +56,44 @@ __device__ __forceinline__ int find(const int *prefix, int n, int i)
 
 __device__ __forceinline__ int div_up(int a, int b) { return (a + b - 1) / b; }
 
-// Where a batch row's counts come from: blocks its new tokens touch, 16-row
-// tiles of a KV head and their parts.
+// What a batch row adds to the lists: blocks its new tokens touch; 16-row or
+// wide tiles of a KV head, times their parts; partial results.
 struct Counts {
-    int units, items, wide, parts, n_parts;
+    int units, items, wides, parts, wide_parts, n_parts, wide;
 };
-__device__ __forceinline__ Counts counts(const Pages &p, int past, int fresh, int wide)
+__device__ __forceinline__ bool is_wide(const Pages &p, int fresh, int wide)
 {
-    Counts c = {0, 0, 0, 0, 1};
+    return wide && div_up(fresh * p.group, kPagesTileRows) > div_up(p.group, kPagesTileRows);
+}
+__device__ __forceinline__ Counts counts(const Pages &p, int past, int fresh, int wide, int wide_keys)
+{
+    Counts c = {0, 0, 0, 0, 0, 1, 0};
     if (fresh <= 0) return c;
     const int len = past + fresh, rows = fresh * p.group;
     c.units = (len - 1) / kPageBlock - past / kPageBlock + 1;
-    const int tiles = div_up(rows, kPagesTileRows), most = div_up(p.group, kPagesTileRows);
-    if (tiles <= most) {
-        c.n_parts = div_up(len, pages_part_keys(len));
-        c.parts = c.n_parts > 1 ? tiles * c.n_parts : 0;
+    if (is_wide(p, fresh, wide)) {
+        c.wide = 1;
+        c.n_parts = div_up(len, wide_keys);
+        c.wides = div_up(rows, kPagesWideRows) * c.n_parts;
+        c.wide_parts = c.n_parts > 1 ? c.wides : 0;
+        return c;
     }
+    const int tiles = div_up(rows, kPagesTileRows);
+    if (tiles <= div_up(p.group, kPagesTileRows)) c.n_parts = div_up(len, pages_part_keys(len));
     c.items = tiles * c.n_parts;
+    c.parts = c.n_parts > 1 ? c.items : 0;
     return c;
 }
 
 // The lists that follow from a valid plan, by `n` threads of which this is
 // number `i0`: the blocks to store, the attention's workgroups, the angles, and
-// what the caller asked for.  px: tokens, units and items before each batch row
-// (`stride` apart), R + 1 entries each.
+// what the caller asked for.  px: tokens, units, items and wide items before
+// each batch row (`stride` apart), R + 1 entries each.
 __device__ __forceinline__ void plan_lists(const Pages &p, const PagesPlanArgs &a, const PagesPlanHead &h, const int *px,
                                            int stride, int i0, int n)
 {
     const int R = h.n_requests;
-    const int *start = px, *unit0 = px + stride, *item0 = px + 2 * stride;
+    const int *start = px, *unit0 = px + stride, *item0 = px + 2 * stride, *wide0 = px + 3 * stride;
     for (int u = i0; u < h.n_units; u += n) {
         const int b = find(unit0, R, u);
         p.unit[u] = make_int2(b, p.req[b].past / kPageBlock + u - unit0[b]);
@@ -101,6 +110,20 @@ __device__ __forceinline__ void plan_lists(const Pages &p, const PagesPlanArgs &
         it.key1 = min(r.len, it.key0 + keys);
         it.part = r.n_parts > 1 ? r.part0 + k : -1;
         p.item[i] = it;
+    }
+    for (int i = i0; i < h.n_wide; i += n) {
+        const int b = find(wide0, R, i), k = i - wide0[b];
+        const PagesRequest r = p.req[b];
+        const int tiles = (wide0[b + 1] - wide0[b]) / r.n_parts, part = k % r.n_parts;
+        const int keys = (div_up(r.len, r.n_parts) + 63) & ~63; // parts of a length, in whole blocks of 64
+        PagesItem it;
+        it.b = b;
+        it.row0 = (tiles - 1 - k / r.n_parts) * kPagesWideRows; // the longest first
+        it.key0 = part * keys;
+        it.key1 = min(r.len, it.key0 + keys);
+        it.part = r.n_parts > 1 ? r.part0 + k : -1;
+        p.wide[i] = it;
+        if (it.part >= 0) p.wide_owner[it.part] = make_int2(b, k);
     }
     // Angles in 64 bits: a far position times a frequency keeps its fraction.
     // Once a plan, not once a layer and head: the library's 64-bit sine and
@@ -146,7 +169,7 @@ template <bool LISTS>
 __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(Pages p, PagesPlanArgs a)
 {
     constexpr int NT = kPlanThreads, C = kPagesMaxRequests / NT;
-    __shared__ int px[3 * (kPagesMaxRequests + 1)];
+    __shared__ int px[4 * (kPagesMaxRequests + 1)];
     __shared__ unsigned seen[kPagesMaxRequests / 32];
     __shared__ long long ws64[NT / 64];
     __shared__ int ws[NT / 64];
@@ -193,7 +216,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(Pages p, Pages
     const int n_free = *p.n_free;
     const int status = bad || tokens > a.n_tokens ? JEV_EINVAL : more > n_free + gone ? JEV_ENOMEM : JEV_OK;
     if (status != JEV_OK) {
-        PagesPlanHead h = {status, 0, 0, 0, 0, 0, 0, 0};
+        PagesPlanHead h = {status, 0, 0, 0, 0, 0, 0, 0, 0};
         if (tid == 0) *p.head = h;
         if (LISTS) plan_lists(p, a, h, px, S, tid, NT);
         return;
@@ -220,7 +243,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(Pages p, Pages
         s0 += fresh[i];
         s1 += need[i] - keep[i];
         s2 += own[i] - keep[i];
-        PagesRequest r = {id[i], past[i], past[i] + fresh[i], start[b], 0, 1};
+        PagesRequest r = {id[i], past[i], past[i] + fresh[i], start[b], 0, 1, 0};
         p.req[b] = r;
     }
     if (tid == 0) {
@@ -262,57 +285,84 @@ __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(Pages p, Pages
     __syncthreads(); // need0 and gone0 are done with
 
     // the lists' prefix sums take their place
-    int *unit0 = px + S, *item0 = px + 2 * S;
-    int u0 = 0, i0 = 0, g0 = 0;
+    int *unit0 = px + S, *item0 = px + 2 * S, *wide0 = px + 3 * S;
+    int wide_keys = kPagesWideKeys;
+    if (a.wide) {
+        long long keys = 0, tiles = 0;
+#pragma unroll
+        for (int i = 0; i < C; i++)
+            if (is_wide(p, fresh[i], 1)) {
+                const int n = div_up(fresh[i] * p.group, kPagesWideRows);
+                tiles += n;
+                keys += (long long)n * (past[i] + fresh[i]);
+            }
+        keys = block_sum<NT>(keys, ws64);
+        tiles = block_sum<NT>(tiles, ws64);
+        // a tile's last part may be short: with keys / room of them each there are
+        // at most room + tiles parts, one round; many tiles split only where one
+        // is twice as long as their mean
+        const long long target = pages_wide_target(p.n_kv), room = max(target - tiles, (target + 1) / 2);
+        wide_keys = (int)max((long long)wide_keys, (keys + room - 1) / room);
+    }
+    int n0[5] = {0, 0, 0, 0, 0}; // units, items, wide items, parts, wide parts
     Counts c[C];
 #pragma unroll
     for (int i = 0; i < C; i++) {
-        c[i] = counts(p, past[i], fresh[i], a.wide);
-        u0 += c[i].units;
-        i0 += c[i].items;
-        g0 += c[i].parts;
+        c[i] = counts(p, past[i], fresh[i], a.wide, wide_keys);
+        n0[0] += c[i].units;
+        n0[1] += c[i].items;
+        n0[2] += c[i].wides;
+        n0[3] += c[i].parts;
+        n0[4] += c[i].wide_parts;
     }
-    const int nu = u0, ni = i0, ng = g0;
-    u0 = block_scan<NT>(u0, ws);
-    i0 = block_scan<NT>(i0, ws);
-    g0 = block_scan<NT>(g0, ws);
-    const bool last = tid == NT - 1;
-    PagesPlanHead h = {JEV_OK, (int)tokens, u0 + nu, i0 + ni, 0, g0 + ng, R, 0};
+    int all_n[5];
+#pragma unroll
+    for (int i = 0; i < 5; i++) {
+        const int v = n0[i];
+        n0[i] = (i == 2 || i == 4) && !a.wide ? 0 : block_scan<NT>(v, ws);
+        all_n[i] = n0[i] + v;
+    }
     __shared__ PagesPlanHead all;
-    if (last) {
+    if (tid == NT - 1) {
+        PagesPlanHead h = {JEV_OK, (int)tokens, all_n[0], all_n[1], all_n[2], all_n[3], all_n[4], R, 0};
         all = h;
         *p.head = h;
         unit0[R] = h.n_units;
         item0[R] = h.n_items;
+        wide0[R] = h.n_wide;
         *p.n_free = n_free + (int)(gone - more);
     }
 #pragma unroll
     for (int i = 0; i < C; i++) {
         const int b = tid * per + i;
         if (i >= per || b >= R) continue;
-        unit0[b] = u0;
-        item0[b] = i0;
-        p.req[b].part0 = g0;
+        unit0[b] = n0[0];
+        item0[b] = n0[1];
+        wide0[b] = n0[2];
+        p.req[b].part0 = c[i].wide ? n0[4] : n0[3];
         p.req[b].n_parts = c[i].n_parts;
-        u0 += c[i].units;
-        i0 += c[i].items;
-        g0 += c[i].parts;
+        p.req[b].wide = c[i].wide;
+        n0[0] += c[i].units;
+        n0[1] += c[i].items;
+        n0[2] += c[i].wides;
+        n0[3] += c[i].parts;
+        n0[4] += c[i].wide_parts;
         p.length[id[i]] = past[i] + fresh[i];
     }
     __syncthreads();
     if (LISTS) plan_lists(p, a, all, px, S, tid, NT);
     else
-        for (int i = tid; i < 3 * S; i += NT)
+        for (int i = tid; i < 4 * S; i += NT)
             if (i % S <= R) p.prefix[i] = px[i];
 }
 
 __global__ __launch_bounds__(256) void pages_lists_kernel(Pages p, PagesPlanArgs a)
 {
     constexpr int S = kPagesMaxRequests + 1;
-    __shared__ int px[3 * S];
+    __shared__ int px[4 * S];
     const PagesPlanHead h = *p.head;
     if (h.n_requests > 0)
-        for (int j = 0; j < 3; j++)
+        for (int j = 0; j < 4; j++)
             for (int i = threadIdx.x; i <= h.n_requests; i += 256) px[j * S + i] = p.prefix[j * S + i];
     __syncthreads();
     plan_lists(p, a, h, px, S, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
@@ -651,16 +701,15 @@ __global__ __launch_bounds__(256, 2) void pages_attend_kernel(Pages p, PagesAtte
         const PagesItem it = p.item[item];
         const PagesRequest r = p.req[it.b];
         const int32_t *table = p.table + (size_t)r.id * p.width;
-        const int n_rows = (r.len - r.past) * p.group, row = it.row0 + n;
-        const bool live = row < n_rows;
-        const int token = live ? row / p.group : 0, head = h * p.group + (live ? row % p.group : 0);
-        const int limit = live ? r.past + token : -1; // last visible key
+        // lanes past the request's rows repeat its last one
+        const int n_rows = (r.len - r.past) * p.group, row = min(it.row0 + n, n_rows - 1);
+        const int token = row / p.group, head = h * p.group + row % p.group;
+        const int limit = r.past + token; // last visible key
         const size_t qrow = ((size_t)(r.start + token) * p.n_heads + head) * HD;
         // the tile's last visible key, and the first row's: blocks below it need no mask
         const int top = r.past + min(n_rows - 1, it.row0 + kPagesTileRows - 1) / p.group;
         const int key1 = min(it.key1, top + 1);
-        const bool full = it.row0 + kPagesTileRows <= n_rows;
-        const int clear = full ? r.past + it.row0 / p.group : -1;
+        const int clear = r.past + it.row0 / p.group;
 
         // Q^T fragments: dims 64 j + 16 g + 8 c .. + 7 of row n
         half8_t qh[2 * NJ], ql[2 * NJ];
@@ -838,6 +887,262 @@ __global__ __launch_bounds__(256, 2) void pages_attend_kernel(Pages p, PagesAtte
     }
 }
 
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+// 128 (token, head) rows of a request and KV head, 32 to a wave, over its keys
+// in blocks of 64: as above, with K and V turned into fp16 fragments in LDS once
+// for the four waves (double buffered: the next block's codes are in flight
+// during a block's products and written as it ends).  v_mfma_f32_32x32x16_f16:
+// S^T is two tiles of 32 keys, their rows dealt so that a lane's sixteen scores
+// are one block's tokens in order, which is again the P^T operand.  The V scale
+// enters through the exponent (one fused multiply-add and one exp2 a score), and
+// the maximum moves only when a score passes it by 2^6, so most blocks rescale
+// nothing.  Bound by the matrix cores at two instructions a product, with the
+// exponentials and fp16 pairs of ~9 vector instructions a score beside them.
+template <int HD>
+__global__ __launch_bounds__(256, 2) void pages_attend_wide_kernel(Pages p, PagesAttendArgs a)
+{
+    constexpr int NC = HD / 16, ND = HD / 32, NL = HD / 64, BYTES = kPageBlock * HD, LD = HD + 4;
+    __shared__ __align__(16) uint4 kf[2][2 * NC * 64], vf[2][4 * ND * 64];
+    __shared__ __align__(16) float2 sc[2][4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int hh = lane >> 5, n = lane & 31, h = blockIdx.x % p.n_kv, item = blockIdx.x / p.n_kv;
+    if (item >= p.head->n_wide) return;
+    const PagesItem it = p.wide[item];
+    const PagesRequest r = p.req[it.b];
+    const int32_t *table = p.table + (size_t)r.id * p.width;
+    const uint8_t *kbase = p.k + (size_t)a.layer * p.n_blocks() * BYTES;
+    const uint8_t *vbase = p.v + (size_t)a.layer * p.n_blocks() * BYTES;
+    const float2 *sbase = p.ks + (size_t)a.layer * p.n_blocks();
+
+    const int n_rows = (r.len - r.past) * p.group, wrow = it.row0 + 32 * wave;
+    const bool active = wrow < n_rows;
+    const int row = min(wrow + n, n_rows - 1), token = row / p.group, head = h * p.group + row % p.group;
+    const int limit = r.past + token; // last visible key
+    const int key1 = min(it.key1, r.past + min(n_rows - 1, it.row0 + kPagesWideRows - 1) / p.group + 1);
+    // keys below `clear` are seen by every row of the wave, keys past `wtop` by none
+    const int clear = r.past + min(wrow, n_rows - 1) / p.group, wtop = active ? r.past + min(n_rows - 1, wrow + 31) / p.group : -1;
+    const int last = (r.len - 1) / kPageBlock;
+
+    // a wave stages one of a block's four 16-token blocks
+    auto block_of = [&](int kb) {
+        const int c = min(4 * kb + wave, last);
+        return ((size_t)table[c / p.sub] * p.n_kv + h) * p.sub + c % p.sub;
+    };
+    uint4 kr[NL], vr[NL];
+    float2 sr;
+    auto fetch = [&](size_t b) {
+#pragma unroll
+        for (int i = 0; i < NL; i++) kr[i] = ((const uint4 *)(kbase + b * BYTES))[64 * i + lane];
+#pragma unroll
+        for (int i = 0; i < NL; i++) vr[i] = ((const uint4 *)(vbase + b * BYTES))[64 * i + lane];
+        sr = sbase[b];
+    };
+    auto frag = [&](uint32_t w0, uint32_t w1) {
+        uint4 u;
+        bytes_to_f16(w0, (_Float16)1152.f, u.x, u.y);
+        bytes_to_f16(w1, (_Float16)1152.f, u.z, u.w);
+        return u;
+    };
+    auto put = [&](int buf) {
+        // K: sixteen dims of token lane / 4, chunk 4 i + lane % 4; its row of the tile
+        const int tk = lane >> 2, m = 8 * (tk >> 2) + 4 * (wave & 1) + (tk & 3);
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            uint4 *to = kf[buf] + ((wave >> 1) * NC + 4 * i + (lane & 3)) * 64 + m;
+            to[0] = frag(kr[i].x, kr[i].y);
+            to[32] = frag(kr[i].z, kr[i].w);
+        }
+        // V: sixteen tokens of dim 64 i + lane
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            uint4 *to = vf[buf] + ((2 * i + hh) * 4 + (wave >> 1) * 2) * 64 + 32 * (wave & 1) + n;
+            to[0] = frag(vr[i].x, vr[i].y);
+            to[64] = frag(vr[i].z, vr[i].w);
+        }
+        if (lane == 0) sc[buf][wave] = sr;
+    };
+
+    int kb = it.key0 / 64;
+    const bool any = kb * 64 < key1;
+    size_t next = block_of(kb);
+    if (any) fetch(next);
+    next = block_of(kb + 1);
+
+    // Q^T fragments: dims 16 c + 8 hh .. + 7 of row n
+    half8_t qh[NC], ql[NC];
+    float qs;
+    {
+        const float *src = a.q + ((size_t)(r.start + token) * p.n_heads + head) * HD + 8 * hh;
+        float m = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(src[16 * c + i]));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        const int ex = m > 0.f && m < INFINITY ? 14 - (ilogbf(m) + 1) : 0;
+        const int e1 = ex / 2, e2 = ex - e1; // in two steps: neither factor leaves fp32's range
+        const float f1 = ldexpf(1.f, e1), f2 = ldexpf(1.f, e2);
+        qs = ldexpf(ldexpf(p.scale * 1.44269504088896341f, -e1), -e2);
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float y = src[16 * c + i] * f1 * f2;
+                const _Float16 hi = (_Float16)y;
+                qh[c][i] = hi;
+                ql[c][i] = (_Float16)(y - (float)hi);
+            }
+    }
+
+    floatx16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++) o[d] = floatx16{};
+    float m = -INFINITY, l = 0.f;
+    int ev = -200; // outputs are held times 2^(8 - ev)
+    if (any) put(0);
+    __syncthreads();
+
+    for (int buf = 0; kb * 64 < key1; kb++, buf ^= 1) {
+        const bool more = (kb + 1) * 64 < key1;
+        if (more) {
+            fetch(next);
+            next = block_of(kb + 2);
+        }
+        if (kb * 64 <= wtop) {
+            floatx16 s[2] = {floatx16{}, floatx16{}};
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    const half8_t k = __builtin_bit_cast(half8_t, kf[buf][(t * NC + c) * 64 + lane]);
+                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[c], s[t], 0, 0, 0);
+                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[c], s[t], 0, 0, 0);
+                }
+            const float2 s0 = sc[buf][hh], s1 = sc[buf][2 + hh];
+            const float ks[2] = {s0.x * qs, s1.x * qs}, vs[2] = {s0.y, s1.y};
+            const bool masked = kb * 64 + 63 > clear;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                float y = -INFINITY;
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        y = fmaxf(y, kb * 64 + 32 * t + 16 * hh + i > limit ? -INFINITY : s[t][i]);
+                    // (a block with nothing visible: no product of infinity and a zero scale)
+                    y = y == -INFINITY ? y : y * ks[t];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) y = fmaxf(y, s[t][i]);
+                    y = y * ks[t];
+                }
+                mx = fmaxf(mx, y);
+            }
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            float vm = fmaxf(vs[0], vs[1]);
+            vm = fmaxf(vm, __shfl_xor(vm, 32, 64));
+            const int en = vm > 0.f && vm < INFINITY ? max(ev, ilogbf(vm)) : ev;
+            if (__any(mx > m + 6.f || en > ev)) {
+                const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2f(m - mn);
+                l *= f;
+                const float g = ldexpf(f, max(ev - en, -400));
+#pragma unroll
+                for (int d = 0; d < ND; d++) o[d] *= g;
+                m = mn;
+                ev = en;
+            }
+            const float mu = m == -INFINITY ? 0.f : m;
+            half8_t ph[2][2], pl[2][2];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                // w = 2^(score - m + 8) times the V scale over 2^ev; a block of zeros has codes of zero
+                float lv = vs[t] == 0.f ? 0.f : fmaxf(__builtin_amdgcn_logf(ldexpf(vs[t], -ev)), -60.f);
+                if (vs[t] != vs[t]) lv = vs[t];
+                const float c = lv + 8.f - mu;
+                float w[16], sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    w[i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], ks[t], c));
+                    if (masked && kb * 64 + 32 * t + 16 * hh + i > limit) w[i] = 0.f;
+                    sum += w[i];
+                }
+                l += sum == 0.f ? 0.f : sum * __builtin_amdgcn_exp2f(-8.f - lv);
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) split2_rtz(w[2 * i], w[2 * i + 1], hi[i], lo[i]);
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    ph[t][j] = __builtin_bit_cast(half8_t, make_uint4(hi[4 * j], hi[4 * j + 1], hi[4 * j + 2], hi[4 * j + 3]));
+                    pl[t][j] = __builtin_bit_cast(half8_t, make_uint4(lo[4 * j], lo[4 * j + 1], lo[4 * j + 2], lo[4 * j + 3]));
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int d = 0; d < ND; d++) {
+                        const half8_t v = __builtin_bit_cast(half8_t, vf[buf][((d * 2 + t) * 2 + j) * 64 + lane]);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[t][j], o[d], 0, 0, 0);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[t][j], o[d], 0, 0, 0);
+                    }
+        }
+        if (more) put(buf ^ 1);
+        __syncthreads();
+    }
+    if (!active || wrow + n >= n_rows) return;
+    l += __shfl_xor(l, 32, 64);
+    const float up = ldexpf(1.f, max(ev, -149));
+    float *dst;
+    float f = 0x1p-8f;
+    if (it.part < 0) {
+        dst = a.out + ((size_t)(r.start + token) * p.n_heads + head) * HD;
+        f /= l;
+    } else {
+        dst = p.wide_part + (((size_t)it.part * p.n_kv + h) * kPagesWideRows + 32 * wave + n) * LD;
+        if (hh == 0) {
+            dst[HD] = m;
+            dst[HD + 1] = l;
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) dst[32 * d + 8 * (i >> 2) + 4 * hh + (i & 3)] = o[d][i] * f * up;
+}
+
+// The parts of split wide tiles: a workgroup takes sixteen rows, sixteen
+// threads a row.
+template <int HD>
+__global__ __launch_bounds__(256) void pages_merge_wide_kernel(Pages p, PagesAttendArgs a)
+{
+    constexpr int N = HD / 16, LD = HD + 4;
+    if ((int)blockIdx.x >= p.head->n_wide_parts) return;
+    const int2 own = p.wide_owner[blockIdx.x];
+    const PagesRequest r = p.req[own.x];
+    if (own.y % r.n_parts) return; // a tile's first part stands for it
+    const int n_rows = (r.len - r.past) * p.group, tiles = div_up(n_rows, kPagesWideRows);
+    const int h = blockIdx.y, c = 16 * blockIdx.z + (threadIdx.x >> 4), j = threadIdx.x & 15;
+    const int row = (tiles - 1 - own.y / r.n_parts) * kPagesWideRows + c;
+    if (row >= n_rows) return;
+    auto at = [&](int k) { return p.wide_part + (((size_t)(blockIdx.x + k) * p.n_kv + h) * kPagesWideRows + c) * LD; };
+    float m = -INFINITY;
+    for (int k = 0; k < r.n_parts; k++) m = fmaxf(m, at(k)[HD]);
+    if (m == -INFINITY) m = 0.f;
+    float x[N] = {}, sum = 0.f;
+    for (int k = 0; k < r.n_parts; k++) {
+        const float *src = at(k);
+        const float f = exp2f(src[HD] - m);
+        sum += src[HD + 1] * f;
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] += src[N * j + i] * f;
+    }
+    float *dst = a.out + ((size_t)(r.start + row / p.group) * p.n_heads + h * p.group + row % p.group) * HD + N * j;
+#pragma unroll
+    for (int i = 0; i < N; i++) dst[i] = x[i] / sum;
+}
+
 // The parts of split tiles, per batch row and head: sixteen threads hold the
 // head's dims (HD / 16 each), the sixteen groups take every sixteenth part and
 // are summed in group order.
@@ -850,7 +1155,7 @@ __global__ __launch_bounds__(256) void pages_merge_kernel(Pages p, PagesAttendAr
     const int tid = threadIdx.x, b = blockIdx.x, head = blockIdx.y, h = head / p.group;
     if (b >= p.head->n_requests) return;
     const PagesRequest r = p.req[b];
-    if (r.n_parts <= 1) return;
+    if (r.n_parts <= 1 || r.wide) return;
     const int tiles = div_up((r.len - r.past) * p.group, kPagesTileRows);
     for (int t = 0; t < r.len - r.past; t++) {
         const int row = t * p.group + head % p.group, tile = row / kPagesTileRows, c = row % kPagesTileRows;
@@ -900,6 +1205,16 @@ hipError_t launch_pages_attend(const Pages &p, const PagesAttendArgs &a, hipStre
         const dim3 mg(a.n_requests, p.n_heads);
         if (p.hd == 128) hipLaunchKernelGGL(pages_merge_kernel<128>, mg, dim3(256), 0, s, p, a);
         else hipLaunchKernelGGL(pages_merge_kernel<64>, mg, dim3(256), 0, s, p, a);
+    }
+    if (a.wide) {
+        const int64_t tiles = (int64_t)a.n_tokens * p.group / kPagesWideRows + a.n_requests + pages_wide_target(p.n_kv);
+        const dim3 wg((unsigned)(tiles * p.n_kv)), mg(p.max_wide_parts, p.n_kv, kPagesWideRows / 16);
+        if (p.hd == 128) hipLaunchKernelGGL(pages_attend_wide_kernel<128>, wg, dim3(256), 0, s, p, a);
+        else hipLaunchKernelGGL(pages_attend_wide_kernel<64>, wg, dim3(256), 0, s, p, a);
+        if (p.max_context > kPagesWideKeys) {
+            if (p.hd == 128) hipLaunchKernelGGL(pages_merge_wide_kernel<128>, mg, dim3(256), 0, s, p, a);
+            else hipLaunchKernelGGL(pages_merge_wide_kernel<64>, mg, dim3(256), 0, s, p, a);
+        }
     }
     return hipGetLastError();
 }

@@ -2638,6 +2638,9 @@ int pages_plan(jev_pages *h, const PagesPlanArgs &a, hipStream_t s)
         return fail(JEV_EINVAL, "%d tokens: the cache was made for plans of %d", a.n_tokens, h->p.max_tokens);
     if (a.n_requests > 0 && (!a.request || !a.fresh)) return fail(JEV_EINVAL, "request and fresh must not be null");
     h->plan = a;
+    // as many tokens as requests: 16-row tiles serve whatever there is, and the
+    // wide tiles' launches are saved
+    h->plan.wide = a.n_tokens > a.n_requests;
     HIP_TRY(launch_pages_plan(h->p, h->plan, s));
     return JEV_OK;
 }
@@ -2685,6 +2688,8 @@ int jev_pages_create(const jev_config *model, const jev_pages_config *cfg, int d
         return fail(JEV_EINVAL, "max_requests %d must be in [1, %d]", g.max_requests, kPagesMaxRequests);
     if (g.max_context <= 0 || g.max_context > 1 << 24) return fail(JEV_EINVAL, "max_context %d must be in [1, 2^24]", g.max_context);
     if (g.max_tokens <= 0 || g.max_tokens > 1 << 22) return fail(JEV_EINVAL, "max_tokens %d must be in [1, 2^22]", g.max_tokens);
+    if ((int64_t)g.max_tokens * (f.n_heads / f.n_kv_heads) > 1 << 28)
+        return fail(JEV_EINVAL, "max_tokens %d times %d heads to a KV head is more than 2^28", g.max_tokens, f.n_heads / f.n_kv_heads);
     if (g.rope_half != 0 && g.rope_half != 1) return fail(JEV_EINVAL, "rope_half must be 0 or 1");
     int ndev = 0;
     hipError_t e = hipGetDeviceCount(&ndev);
@@ -2727,6 +2732,13 @@ int jev_pages_create(const jev_config *model, const jev_pages_config *cfg, int d
     p.max_parts = (int)(split * (pool / pages_part_keys(1) + R));
     p.max_items = (int)(p.max_parts + T * p.group / kPagesTileRows + (split + 1) * R);
     p.max_units = (int)(T / kPageBlock + 2 * R);
+    // tiles x parts <= tiles x (keys / keys of a part + 1), and a part is at least the sum over
+    // tiles of keys / target; a split tile has more keys than a part
+    const size_t target = pages_wide_target(p.n_kv);
+    p.max_wide = (int)(T * p.group / kPagesWideRows + R + target);
+    p.max_wide_parts = g.max_context <= kPagesWideKeys
+                           ? 0
+                           : (int)std::min(2 * target, (T * p.group / kPagesWideRows + R) * ((size_t)g.max_context / kPagesWideKeys + 1));
     const size_t codes = p.n_blocks() * p.n_layers * kPageBlock * p.hd;
     const int words = (p.n_pages + 31) / 32;
     double *dfreqs = nullptr;
@@ -2743,6 +2755,9 @@ int jev_pages_create(const jev_config *model, const jev_pages_config *cfg, int d
     if (!rc) rc = pages_alloc(h, p.prefix, 4 * (size_t)(kPagesMaxRequests + 1));
     if (!rc) rc = pages_alloc(h, p.unit, p.max_units);
     if (!rc) rc = pages_alloc(h, p.item, p.max_items);
+    if (!rc) rc = pages_alloc(h, p.wide, p.max_wide);
+    if (!rc) rc = pages_alloc(h, p.wide_owner, p.max_wide_parts);
+    if (!rc) rc = pages_alloc(h, p.wide_part, (size_t)p.max_wide_parts * p.n_kv * kPagesWideRows * (p.hd + 4));
     if (!rc) rc = pages_alloc(h, p.angle, T * p.half);
     if (!rc) rc = pages_alloc(h, dfreqs, freqs.size());
     if (!rc) rc = pages_alloc(h, h->ids, 2 * R);
