@@ -451,7 +451,7 @@ struct PagesItem {
 struct Pages {
     // geometry
     int n_layers = 0, n_heads = 0, n_kv = 0, hd = 0, group = 1;
-    int page = 16, sub = 1;                 // tokens and blocks of a page
+    int page = 16, sub = 1, sub_shift = 0;  // tokens and blocks of a page (powers of two)
     int n_pages = 0, max_requests = 0, max_context = 0, max_tokens = 0, width = 0; // width: pages of a table row
     int half = 0, rope_half = 0;            // rotated pairs; 0: (2i, 2i + 1), 1: (i, i + half)
     int orig_ctx = 0;

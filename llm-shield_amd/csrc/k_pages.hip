@@ -889,6 +889,17 @@ __global__ __launch_bounds__(256, 2) void pages_attend_kernel(Pages p, PagesAtte
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 
+// split2_rtz with the remainders as mixed-precision multiply-adds: four
+// instructions for the two values instead of six (the compiler converts first).
+__device__ __forceinline__ void split2_mix(float x0, float x1, uint32_t &hi, uint32_t &lo)
+{
+    float r0, r1;
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x0, x1));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(hi), "v"(x0));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(hi), "v"(x1));
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r0, r1));
+}
+
 // 128 (token, head) rows of a request and KV head, 32 to a wave, over its keys
 // in blocks of 64: as above, with K and V turned into fp16 fragments in LDS once
 // for the four waves (double buffered: the next block's codes are in flight
@@ -924,19 +935,25 @@ __global__ __launch_bounds__(256, 2) void pages_attend_wide_kernel(Pages p, Page
     const int clear = r.past + min(wrow, n_rows - 1) / p.group, wtop = active ? r.past + min(n_rows - 1, wrow + 31) / p.group : -1;
     const int last = (r.len - 1) / kPageBlock;
 
-    // a wave stages one of a block's four 16-token blocks
-    auto block_of = [&](int kb) {
-        const int c = min(4 * kb + wave, last);
-        return ((size_t)table[c / p.sub] * p.n_kv + h) * p.sub + c % p.sub;
+    // A wave stages one of a block's four 16-token blocks.  Buffer loads: their
+    // bases are the wave's, so no vector registers hold addresses, and its page and
+    // scales do not become scalar loads, which were waited for where they were
+    // issued, at the top of every block.
+    const rsrc_t rt = make_rsrc(table, 4 * p.width);
+    auto page_of = [&](int kb) {
+        return __builtin_amdgcn_raw_buffer_load_b32(rt, 0, 4 * (min(4 * kb + wave, last) >> p.sub_shift), 0);
     };
     uint4 kr[NL], vr[NL];
     float2 sr;
-    auto fetch = [&](size_t b) {
+    auto fetch = [&](int kb, int page) {
+        const int c = min(4 * kb + wave, last) & (p.sub - 1);
+        const size_t b = (((size_t)__builtin_amdgcn_readfirstlane(page) * p.n_kv + h) << p.sub_shift) + c;
+        const rsrc_t rk = make_rsrc(kbase + b * BYTES, BYTES), rv = make_rsrc(vbase + b * BYTES, BYTES), rs = make_rsrc(sbase + b, 8);
 #pragma unroll
-        for (int i = 0; i < NL; i++) kr[i] = ((const uint4 *)(kbase + b * BYTES))[64 * i + lane];
+        for (int i = 0; i < NL; i++) kr[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rk, 16 * lane, 1024 * i, 0));
 #pragma unroll
-        for (int i = 0; i < NL; i++) vr[i] = ((const uint4 *)(vbase + b * BYTES))[64 * i + lane];
-        sr = sbase[b];
+        for (int i = 0; i < NL; i++) vr[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rv, 16 * lane, 1024 * i, 0));
+        sr = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rs, 0, 0, 0));
     };
     auto frag = [&](uint32_t w0, uint32_t w1) {
         uint4 u;
@@ -965,9 +982,9 @@ __global__ __launch_bounds__(256, 2) void pages_attend_wide_kernel(Pages p, Page
 
     int kb = it.key0 / 64;
     const bool any = kb * 64 < key1;
-    size_t next = block_of(kb);
-    if (any) fetch(next);
-    next = block_of(kb + 1);
+    int next = page_of(kb);
+    if (any) fetch(kb, next);
+    next = page_of(kb + 1);
 
     // Q^T fragments: dims 16 c + 8 hh .. + 7 of row n
     half8_t qh[NC], ql[NC];
@@ -999,15 +1016,15 @@ __global__ __launch_bounds__(256, 2) void pages_attend_wide_kernel(Pages p, Page
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = floatx16{};
     float m = -INFINITY, l = 0.f;
-    int ev = -200; // outputs are held times 2^(8 - ev)
+    int ev = -200; // outputs are held times 2^(9 - ev); V scales are below 2^ev
     if (any) put(0);
     __syncthreads();
 
     for (int buf = 0; kb * 64 < key1; kb++, buf ^= 1) {
         const bool more = (kb + 1) * 64 < key1;
         if (more) {
-            fetch(next);
-            next = block_of(kb + 2);
+            fetch(kb + 1, next);
+            next = page_of(kb + 2);
         }
         if (kb * 64 <= wtop) {
             floatx16 s[2] = {floatx16{}, floatx16{}};
@@ -1020,29 +1037,34 @@ __global__ __launch_bounds__(256, 2) void pages_attend_wide_kernel(Pages p, Page
                     s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[c], s[t], 0, 0, 0);
                 }
             const float2 s0 = sc[buf][hh], s1 = sc[buf][2 + hh];
-            const float ks[2] = {s0.x * qs, s1.x * qs}, vs[2] = {s0.y, s1.y};
-            const bool masked = kb * 64 + 63 > clear;
+            float ks[2] = {s0.x * qs, s1.x * qs}, vs[2] = {s0.y, s1.y};
+#pragma unroll
+            for (int t = 0; t < 2; t++) ks[t] = ks[t] < 1e-37f ? 1e-37f : ks[t]; // a scale of zero has codes of zero
+            if (kb * 64 + 63 > clear) {
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    const int left = limit - (kb * 64 + 32 * t + 16 * hh); // last visible token of the lane's block
+                    if (left < 0) { // none: whatever its scales are
+                        ks[t] = 1.f;
+                        vs[t] = 0.f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (i > left) s[t][i] = -INFINITY;
+                }
+            }
             float mx = -INFINITY;
 #pragma unroll
             for (int t = 0; t < 2; t++) {
                 float y = -INFINITY;
-                if (masked) {
 #pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        y = fmaxf(y, kb * 64 + 32 * t + 16 * hh + i > limit ? -INFINITY : s[t][i]);
-                    // (a block with nothing visible: no product of infinity and a zero scale)
-                    y = y == -INFINITY ? y : y * ks[t];
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; i++) y = fmaxf(y, s[t][i]);
-                    y = y * ks[t];
-                }
-                mx = fmaxf(mx, y);
+                for (int i = 0; i < 16; i++) y = fmaxf(y, s[t][i]);
+                mx = fmaxf(mx, y * ks[t]);
             }
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
             float vm = fmaxf(vs[0], vs[1]);
             vm = fmaxf(vm, __shfl_xor(vm, 32, 64));
-            const int en = vm > 0.f && vm < INFINITY ? max(ev, ilogbf(vm)) : ev;
+            const int en = vm > 0.f && vm < INFINITY ? max(ev, __builtin_amdgcn_frexp_expf(vm)) : ev;
             if (__any(mx > m + 6.f || en > ev)) {
                 const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2f(m - mn);
                 l *= f;
@@ -1053,40 +1075,34 @@ __global__ __launch_bounds__(256, 2) void pages_attend_wide_kernel(Pages p, Page
                 ev = en;
             }
             const float mu = m == -INFINITY ? 0.f : m;
-            half8_t ph[2][2], pl[2][2];
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                // w = 2^(score - m + 8) times the V scale over 2^ev; a block of zeros has codes of zero
+                // w = 2^(score - m + 9) times the V scale over 2^ev; a scale of zero has codes of zero
                 float lv = vs[t] == 0.f ? 0.f : fmaxf(__builtin_amdgcn_logf(ldexpf(vs[t], -ev)), -60.f);
                 if (vs[t] != vs[t]) lv = vs[t];
-                const float c = lv + 8.f - mu;
+                const float c = lv + 9.f - mu;
                 float w[16], sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     w[i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], ks[t], c));
-                    if (masked && kb * 64 + 32 * t + 16 * hh + i > limit) w[i] = 0.f;
                     sum += w[i];
                 }
-                l += sum == 0.f ? 0.f : sum * __builtin_amdgcn_exp2f(-8.f - lv);
+                l += sum * __builtin_amdgcn_exp2f(-9.f - lv);
                 uint32_t hi[8], lo[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) split2_rtz(w[2 * i], w[2 * i + 1], hi[i], lo[i]);
+                for (int i = 0; i < 8; i++) split2_mix(w[2 * i], w[2 * i + 1], hi[i], lo[i]);
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    ph[t][j] = __builtin_bit_cast(half8_t, make_uint4(hi[4 * j], hi[4 * j + 1], hi[4 * j + 2], hi[4 * j + 3]));
-                    pl[t][j] = __builtin_bit_cast(half8_t, make_uint4(lo[4 * j], lo[4 * j + 1], lo[4 * j + 2], lo[4 * j + 3]));
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int j = 0; j < 2; j++)
+                    const half8_t ph = __builtin_bit_cast(half8_t, make_uint4(hi[4 * j], hi[4 * j + 1], hi[4 * j + 2], hi[4 * j + 3]));
+                    const half8_t pl = __builtin_bit_cast(half8_t, make_uint4(lo[4 * j], lo[4 * j + 1], lo[4 * j + 2], lo[4 * j + 3]));
 #pragma unroll
                     for (int d = 0; d < ND; d++) {
                         const half8_t v = __builtin_bit_cast(half8_t, vf[buf][((d * 2 + t) * 2 + j) * 64 + lane]);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[t][j], o[d], 0, 0, 0);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[t][j], o[d], 0, 0, 0);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[d], 0, 0, 0);
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[d], 0, 0, 0);
                     }
+                }
+            }
         }
         if (more) put(buf ^ 1);
         __syncthreads();
@@ -1095,7 +1111,7 @@ __global__ __launch_bounds__(256, 2) void pages_attend_wide_kernel(Pages p, Page
     l += __shfl_xor(l, 32, 64);
     const float up = ldexpf(1.f, max(ev, -149));
     float *dst;
-    float f = 0x1p-8f;
+    float f = 0x1p-9f;
     if (it.part < 0) {
         dst = a.out + ((size_t)(r.start + token) * p.n_heads + head) * HD;
         f /= l;

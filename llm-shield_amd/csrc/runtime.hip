@@ -2713,6 +2713,7 @@ int jev_pages_create(const jev_config *model, const jev_pages_config *cfg, int d
     p.group = f.n_heads / f.n_kv_heads;
     p.page = g.page_tokens;
     p.sub = g.page_tokens / kPageBlock;
+    while (1 << p.sub_shift < p.sub) p.sub_shift++;
     p.n_pages = g.n_pages;
     p.max_requests = g.max_requests;
     p.max_context = g.max_context;
