@@ -672,17 +672,63 @@ hipError_t launch_pages_store(const Pages &p, const PagesStoreArgs &a, hipStream
 
 // ------------------------------------------------------------ attention
 
+namespace {
+
+// split2_rtz with the remainders as mixed-precision multiply-adds: four
+// instructions for the two values instead of six (the compiler converts first).
+__device__ __forceinline__ void split2_mix(float x0, float x1, uint32_t &hi, uint32_t &lo)
+{
+    float r0, r1;
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x0, x1));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(hi), "v"(x0));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(hi), "v"(x1));
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r0, r1));
+}
+
+// Sixteen codes (two words each) as fp16: exact.
+__device__ __forceinline__ uint4 codes_f16(uint32_t w0, uint32_t w1)
+{
+    uint4 u;
+    bytes_to_f16(w0, (_Float16)1152.f, u.x, u.y);
+    bytes_to_f16(w1, (_Float16)1152.f, u.z, u.w);
+    return u;
+}
+
+// A query row as fp16 pairs: scaled by a power of two so that its largest
+// element m lies in [2^13, 2^14); rows of zeros and rows with infinities stay as
+// they are.  `qs` undoes it in the scores, times the softmax scale for exponents
+// of two; f1 f2 is the factor, in two steps that stay inside fp32's range.
+struct QueryScale {
+    float f1, f2, qs;
+    __device__ __forceinline__ QueryScale(float m, float scale)
+    {
+        const int ex = m > 0.f && m < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(m) : 0;
+        const int e1 = ex / 2, e2 = ex - e1;
+        f1 = ldexpf(1.f, e1), f2 = ldexpf(1.f, e2);
+        qs = ldexpf(ldexpf(scale * 1.44269504088896341f, -e1), -e2);
+    }
+    __device__ __forceinline__ void split(float x, _Float16 &hi, _Float16 &lo) const
+    {
+        const float y = x * f1 * f2;
+        hi = (_Float16)y;
+        lo = (_Float16)(y - (float)hi);
+    }
+};
+
+} // namespace
+
 // Sixteen (token, head) rows of a request and KV head over keys [key0, key1) of
-// its pages; the four waves take blocks of 64 keys in turn and merge at the
+// its pages; the four waves take 64 keys (four blocks) in turn and merge at the
 // end.  S^T = K Q^T: with the rows of the K operand (token i, block b) dealt so
 // that a lane's sixteen scores are the sixteen tokens of ONE block, the
 // accumulators are the P^T operand of O^T += V^T P^T as they stand -- no
 // exchange between lanes -- and a lane has one K and one V scale per 64 keys.
 // Codes are exact in fp16; q and p enter as fp16 pairs (hi + lo), ~22 bits, so
-// each product is two matrix instructions.  q is first scaled to below 2^14 by
-// a power of two per row, p by the V scale relative to the largest one so far
-// (a power of two, `ev`), so that neither leaves fp16's range.  Softmax
-// statistics, scores and outputs are fp32.
+// each product is two matrix instructions.  p carries the V scale, relative to a
+// power of two (2^ev) above the largest so far, through its exponent: one fused
+// multiply-add and one exp2 a score; the maximum moves only when a score passes
+// it by 2^6.  Statistics, scores and outputs are fp32.  The next 64 keys' K is in
+// flight during the softmax and V^T P^T, their V during the next scores.
 // Single tokens are bound by HBM: 2 hd bytes a key and KV head.
 template <int HD>
 __global__ __launch_bounds__(256, 2) void pages_attend_kernel(Pages p, PagesAttendArgs a)
@@ -691,13 +737,13 @@ __global__ __launch_bounds__(256, 2) void pages_attend_kernel(Pages p, PagesAtte
     __shared__ float lo[4][kPagesTileRows][LDO];
     __shared__ float lm[4][kPagesTileRows], ll[4][kPagesTileRows];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int g = lane >> 4, n = lane & 15, h = blockIdx.y;
-    const int n_items = p.head->n_items;
+    const int g = lane >> 4, n = lane & 15, h = blockIdx.x % p.n_kv;
+    const int n_items = p.head->n_items, stride = gridDim.x / p.n_kv;
     const uint8_t *kbase = p.k + (size_t)a.layer * p.n_blocks() * BYTES;
     const uint8_t *vbase = p.v + (size_t)a.layer * p.n_blocks() * BYTES;
     const float2 *sbase = p.ks + (size_t)a.layer * p.n_blocks();
 
-    for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
+    for (int item = blockIdx.x / p.n_kv; item < n_items; item += stride) {
         const PagesItem it = p.item[item];
         const PagesRequest r = p.req[it.b];
         const int32_t *table = p.table + (size_t)r.id * p.width;
@@ -705,40 +751,66 @@ __global__ __launch_bounds__(256, 2) void pages_attend_kernel(Pages p, PagesAtte
         const int n_rows = (r.len - r.past) * p.group, row = min(it.row0 + n, n_rows - 1);
         const int token = row / p.group, head = h * p.group + row % p.group;
         const int limit = r.past + token; // last visible key
-        const size_t qrow = ((size_t)(r.start + token) * p.n_heads + head) * HD;
-        // the tile's last visible key, and the first row's: blocks below it need no mask
+        // the tile's last visible key; keys up to `clear` are seen by every row
         const int top = r.past + min(n_rows - 1, it.row0 + kPagesTileRows - 1) / p.group;
-        const int key1 = min(it.key1, top + 1);
-        const int clear = r.past + it.row0 / p.group;
+        const int key1 = min(it.key1, top + 1), clear = r.past + it.row0 / p.group;
+        const int last = (r.len - 1) / kPageBlock; // blocks past it are read as this one, and masked
+
+        // a lane reads K of block n / 4 of the four, V of block g
+        auto page_of = [&](int kb, int i) { return table[min(4 * kb + i, last) >> p.sub_shift]; };
+        auto block_of = [&](int kb, int i, int page) {
+            return (((size_t)page * p.n_kv + h) << p.sub_shift) + (min(4 * kb + i, last) & (p.sub - 1));
+        };
+        uint4 kr[4][NJ], vr[NS];
+        float2 sc;
+        auto fetch_k = [&](int kb, int page) {
+            const uint8_t *src = kbase + block_of(kb, n >> 2, page) * BYTES + (n & 3) * 64 + 16 * g;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int j = 0; j < NJ; j++) kr[t][j] = *(const uint4 *)(src + j * 1024 + 256 * t);
+        };
+        auto fetch_v = [&](int kb, int page) {
+            const size_t b = block_of(kb, g, page);
+            const uint8_t *src = vbase + b * BYTES + 16 * n;
+            sc = sbase[b];
+#pragma unroll
+            for (int s = 0; s < NS; s++) vr[s] = *(const uint4 *)(src + 256 * s);
+        };
+        int kb = it.key0 / 64 + wave;
+        int pk = page_of(kb, n >> 2), pv = page_of(kb, g);
+        if (kb * 64 < key1) {
+            fetch_k(kb, pk);
+            fetch_v(kb, pv);
+        }
+        pk = page_of(kb + 4, n >> 2);
+        pv = page_of(kb + 4, g);
 
         // Q^T fragments: dims 64 j + 16 g + 8 c .. + 7 of row n
         half8_t qh[2 * NJ], ql[2 * NJ];
         float qs;
         {
-            float x[2 * NJ][8];
-            float m = 0.f;
+            const float *src = a.q + ((size_t)(r.start + token) * p.n_heads + head) * HD + 16 * g;
+            float x[2 * NJ][8], m = 0.f;
 #pragma unroll
             for (int c = 0; c < 2 * NJ; c++)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    x[c][i] = a.q[qrow + 64 * (c >> 1) + 16 * g + 8 * (c & 1) + i];
+                    x[c][i] = src[64 * (c >> 1) + 8 * (c & 1) + i];
                     m = fmaxf(m, fabsf(x[c][i]));
                 }
             m = fmaxf(m, __shfl_xor(m, 16, 64));
             m = fmaxf(m, __shfl_xor(m, 32, 64));
-            // m * 2^(14 - e) in [2^13, 2^14); rows of zeros and rows with infinities stay as they are
-            const int ex = m > 0.f && m < INFINITY ? 14 - (ilogbf(m) + 1) : 0;
-            const int e1 = ex / 2, e2 = ex - e1; // in two steps: neither factor leaves fp32's range
-            const float f1 = ldexpf(1.f, e1), f2 = ldexpf(1.f, e2);
-            qs = ldexpf(ldexpf(p.scale * 1.44269504088896341f, -e1), -e2);
+            const QueryScale s(m, p.scale);
+            qs = s.qs;
 #pragma unroll
             for (int c = 0; c < 2 * NJ; c++)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float y = x[c][i] * f1 * f2;
-                    const _Float16 hi = (_Float16)y;
+                    _Float16 hi, lw;
+                    s.split(x[c][i], hi, lw);
                     qh[c][i] = hi;
-                    ql[c][i] = (_Float16)(y - (float)hi);
+                    ql[c][i] = lw;
                 }
         }
 
@@ -746,99 +818,92 @@ __global__ __launch_bounds__(256, 2) void pages_attend_kernel(Pages p, PagesAtte
 #pragma unroll
         for (int s = 0; s < NS; s++) o[s] = floatx4{0.f, 0.f, 0.f, 0.f};
         float m = -INFINITY, l = 0.f;
-        int ev = -200; // outputs are held times 2^(10 - ev)
+        int ev = -200; // outputs are held times 2^(9 - ev); V scales are below 2^ev
 
-        const int last = (r.len - 1) / kPageBlock; // blocks past it are read as this one, and masked
-        auto block_of = [&](int b) {
-            const int c = min(b, last);
-            return ((size_t)table[c / p.sub] * p.n_kv + h) * p.sub + c % p.sub;
-        };
-        for (int kb = it.key0 / 64 + wave; kb * 64 < key1; kb += 4) {
-            const size_t bk = block_of(4 * kb + (n >> 2)), bv = block_of(4 * kb + g);
-            uint4 kr[4][NJ], vr[NS];
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int j = 0; j < NJ; j++)
-                    kr[t][j] = *(const uint4 *)(kbase + bk * BYTES + j * 1024 + (4 * t + (n & 3)) * 64 + 16 * g);
-            const float2 sc = sbase[bv];
-#pragma unroll
-            for (int s = 0; s < NS; s++) vr[s] = *(const uint4 *)(vbase + bv * BYTES + (16 * s + n) * 16);
-
-            const _Float16 bias = (_Float16)1152.f;
-            auto frag = [&](uint32_t w0, uint32_t w1) {
-                uint4 u;
-                bytes_to_f16(w0, bias, u.x, u.y);
-                bytes_to_f16(w1, bias, u.z, u.w);
-                return __builtin_bit_cast(half8_t, u);
-            };
-            float sv[4][4];
-            const float ks = sc.x * qs;
-            float mx = -INFINITY;
-            const bool masked = kb * 64 + 63 > clear;
+        for (; kb * 64 < key1; kb += 4) {
+            const bool more = (kb + 4) * 64 < key1;
+            floatx4 sv[4];
 #pragma unroll
             for (int t = 0; t < 4; t++) {
                 floatx4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int j = 0; j < NJ; j++) {
-                    const half8_t k0 = frag(kr[t][j].x, kr[t][j].y), k1 = frag(kr[t][j].z, kr[t][j].w);
+                    const half8_t k0 = __builtin_bit_cast(half8_t, codes_f16(kr[t][j].x, kr[t][j].y));
+                    const half8_t k1 = __builtin_bit_cast(half8_t, codes_f16(kr[t][j].z, kr[t][j].w));
                     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh[2 * j], acc, 0, 0, 0);
                     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh[2 * j + 1], acc, 0, 0, 0);
                     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql[2 * j], acc, 0, 0, 0);
                     acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql[2 * j + 1], acc, 0, 0, 0);
                 }
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    float x = acc[i] * ks;
-                    if (masked && kb * 64 + 16 * g + 4 * t + i > limit) x = -INFINITY;
-                    sv[t][i] = x;
-                    mx = fmaxf(mx, x);
+                sv[t] = acc;
+            }
+            if (more) fetch_k(kb + 4, pk);
+            // a scale of zero has codes of zero: any other does as well
+            float ks = sc.x * qs, vs = sc.y;
+            ks = ks < 1e-37f ? 1e-37f : ks;
+            if (kb * 64 + 63 > clear) {
+                const int left = limit - (kb * 64 + 16 * g); // last visible token of the lane's block
+                if (left < 0) { // none: whatever its scales are
+                    ks = 1.f;
+                    vs = 0.f;
                 }
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (4 * t + i > left) sv[t][i] = -INFINITY;
             }
-            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn;
-            float alpha = exp2f(m - mu);
-            l = l * alpha;
-            // the largest V scale of the four blocks sets the power of two
-            float vm = sc.y;
-            vm = fmaxf(vm, __shfl_xor(vm, 16, 64));
-            vm = fmaxf(vm, __shfl_xor(vm, 32, 64));
-            if (vm > 0.f && vm < INFINITY) {
-                const int en = max(ev, ilogbf(vm));
-                alpha = ldexpf(alpha, max(ev - en, -400));
-                ev = en;
-            }
-            const float vs = ldexpf(sc.y, 10 - ev);
-            float w[4][4];
+            float mx = -INFINITY, vm = vs;
 #pragma unroll
             for (int t = 0; t < 4; t++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float e = exp2f(sv[t][i] - mu);
-                    l += e;
-                    w[t][i] = masked && kb * 64 + 16 * g + 4 * t + i > limit ? 0.f : e * vs;
-                }
-            m = mn;
-            half8_t ph[2], pl[2];
+                for (int i = 0; i < 4; i++) mx = fmaxf(mx, sv[t][i]);
+            mx *= ks;
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            vm = fmaxf(vm, __shfl_xor(vm, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            vm = fmaxf(vm, __shfl_xor(vm, 32, 64));
+            const int en = vm > 0.f && vm < INFINITY ? max(ev, __builtin_amdgcn_frexp_expf(vm)) : ev;
+            if (__any(mx > m + 6.f || en > ev)) {
+                const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2f(m - mn);
+                l *= f;
+                const float up = ldexpf(f, max(ev - en, -400));
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+                for (int s = 0; s < NS; s++) o[s] *= up;
+                m = mn;
+                ev = en;
+            }
+            const float mu = m == -INFINITY ? 0.f : m;
+            float lv = vs == 0.f ? 0.f : fmaxf(__builtin_amdgcn_logf(ldexpf(vs, -ev)), -60.f);
+            if (vs != vs) lv = vs;
+            const float c = lv + 9.f - mu;
+            float w[16], sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float x = w[2 * j + (i >> 2)][i & 3];
-                    const _Float16 hi = (_Float16)x;
-                    ph[j][i] = hi;
-                    pl[j][i] = (_Float16)(x - (float)hi);
-                }
+            for (int i = 0; i < 16; i++) {
+                w[i] = __builtin_amdgcn_exp2f(fmaf(sv[i >> 2][i & 3], ks, c));
+                sum += w[i];
+            }
+            l += sum * __builtin_amdgcn_exp2f(-9.f - lv);
+            uint32_t hi[8], lw[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) split2_mix(w[2 * i], w[2 * i + 1], hi[i], lw[i]);
+            const half8_t ph0 = __builtin_bit_cast(half8_t, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+            const half8_t ph1 = __builtin_bit_cast(half8_t, make_uint4(hi[4], hi[5], hi[6], hi[7]));
+            const half8_t pl0 = __builtin_bit_cast(half8_t, make_uint4(lw[0], lw[1], lw[2], lw[3]));
+            const half8_t pl1 = __builtin_bit_cast(half8_t, make_uint4(lw[4], lw[5], lw[6], lw[7]));
 #pragma unroll
             for (int s = 0; s < NS; s++) {
-                const half8_t v0 = frag(vr[s].x, vr[s].y), v1 = frag(vr[s].z, vr[s].w);
-                floatx4 acc = o[s] * alpha;
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[0], acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[1], acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[0], acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[1], acc, 0, 0, 0);
-                o[s] = acc;
+                const half8_t v0 = __builtin_bit_cast(half8_t, codes_f16(vr[s].x, vr[s].y));
+                const half8_t v1 = __builtin_bit_cast(half8_t, codes_f16(vr[s].z, vr[s].w));
+                o[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph0, o[s], 0, 0, 0);
+                o[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph1, o[s], 0, 0, 0);
+                o[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl0, o[s], 0, 0, 0);
+                o[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl1, o[s], 0, 0, 0);
+            }
+            if (more) {
+                fetch_v(kb + 4, pv);
+                pk = page_of(kb + 8, n >> 2);
+                pv = page_of(kb + 8, g);
             }
         }
         l += __shfl_xor(l, 16, 64);
@@ -847,7 +912,7 @@ __global__ __launch_bounds__(256, 2) void pages_attend_kernel(Pages p, PagesAtte
         // the four waves' results, in wave order
         const float up = ldexpf(1.f, max(ev, -149));
 #pragma unroll
-        for (int s = 0; s < NS; s++) *(floatx4 *)&lo[wave][n][16 * s + 4 * g] = o[s] * 0x1p-10f * up;
+        for (int s = 0; s < NS; s++) *(floatx4 *)&lo[wave][n][16 * s + 4 * g] = o[s] * 0x1p-9f * up;
         if (g == 0) {
             lm[wave][n] = m;
             ll[wave][n] = l;
@@ -888,17 +953,6 @@ __global__ __launch_bounds__(256, 2) void pages_attend_kernel(Pages p, PagesAtte
 }
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
-
-// split2_rtz with the remainders as mixed-precision multiply-adds: four
-// instructions for the two values instead of six (the compiler converts first).
-__device__ __forceinline__ void split2_mix(float x0, float x1, uint32_t &hi, uint32_t &lo)
-{
-    float r0, r1;
-    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x0, x1));
-    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(hi), "v"(x0));
-    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(hi), "v"(x1));
-    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r0, r1));
-}
 
 // 128 (token, head) rows of a request and KV head, 32 to a wave, over its keys
 // in blocks of 64: as above, with K and V turned into fp16 fragments in LDS once
@@ -955,27 +1009,22 @@ __global__ __launch_bounds__(256, 2) void pages_attend_wide_kernel(Pages p, Page
         for (int i = 0; i < NL; i++) vr[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rv, 16 * lane, 1024 * i, 0));
         sr = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rs, 0, 0, 0));
     };
-    auto frag = [&](uint32_t w0, uint32_t w1) {
-        uint4 u;
-        bytes_to_f16(w0, (_Float16)1152.f, u.x, u.y);
-        bytes_to_f16(w1, (_Float16)1152.f, u.z, u.w);
-        return u;
-    };
     auto put = [&](int buf) {
-        // K: sixteen dims of token lane / 4, chunk 4 i + lane % 4; its row of the tile
-        const int tk = lane >> 2, m = 8 * (tk >> 2) + 4 * (wave & 1) + (tk & 3);
+        // K: sixteen dims of token lane / 4, chunk 4 i + lane % 4; its row of the
+        // tile, dealt by chunk so that neighbouring lanes' writes take all banks
+        const int tk = lane >> 2, m = (8 * (tk >> 2) + 4 * (wave & 1) + (tk & 3)) ^ ((lane & 3) << 1);
 #pragma unroll
         for (int i = 0; i < NL; i++) {
             uint4 *to = kf[buf] + ((wave >> 1) * NC + 4 * i + (lane & 3)) * 64 + m;
-            to[0] = frag(kr[i].x, kr[i].y);
-            to[32] = frag(kr[i].z, kr[i].w);
+            to[0] = codes_f16(kr[i].x, kr[i].y);
+            to[32] = codes_f16(kr[i].z, kr[i].w);
         }
         // V: sixteen tokens of dim 64 i + lane
 #pragma unroll
         for (int i = 0; i < NL; i++) {
             uint4 *to = vf[buf] + ((2 * i + hh) * 4 + (wave >> 1) * 2) * 64 + 32 * (wave & 1) + n;
-            to[0] = frag(vr[i].x, vr[i].y);
-            to[64] = frag(vr[i].z, vr[i].w);
+            to[0] = codes_f16(vr[i].x, vr[i].y);
+            to[64] = codes_f16(vr[i].z, vr[i].w);
         }
         if (lane == 0) sc[buf][wave] = sr;
     };
@@ -997,18 +1046,16 @@ __global__ __launch_bounds__(256, 2) void pages_attend_wide_kernel(Pages p, Page
 #pragma unroll
             for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(src[16 * c + i]));
         m = fmaxf(m, __shfl_xor(m, 32, 64));
-        const int ex = m > 0.f && m < INFINITY ? 14 - (ilogbf(m) + 1) : 0;
-        const int e1 = ex / 2, e2 = ex - e1; // in two steps: neither factor leaves fp32's range
-        const float f1 = ldexpf(1.f, e1), f2 = ldexpf(1.f, e2);
-        qs = ldexpf(ldexpf(p.scale * 1.44269504088896341f, -e1), -e2);
+        const QueryScale y(m, p.scale);
+        qs = y.qs;
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float y = src[16 * c + i] * f1 * f2;
-                const _Float16 hi = (_Float16)y;
+                _Float16 hi, lw;
+                y.split(src[16 * c + i], hi, lw);
                 qh[c][i] = hi;
-                ql[c][i] = (_Float16)(y - (float)hi);
+                ql[c][i] = lw;
             }
     }
 
@@ -1032,7 +1079,7 @@ __global__ __launch_bounds__(256, 2) void pages_attend_wide_kernel(Pages p, Page
             for (int c = 0; c < NC; c++)
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
-                    const half8_t k = __builtin_bit_cast(half8_t, kf[buf][(t * NC + c) * 64 + lane]);
+                    const half8_t k = __builtin_bit_cast(half8_t, kf[buf][(t * NC + c) * 64 + (lane ^ ((c & 3) << 1))]);
                     s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[c], s[t], 0, 0, 0);
                     s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[c], s[t], 0, 0, 0);
                 }
@@ -1214,7 +1261,7 @@ hipError_t launch_pages_attend(const Pages &p, const PagesAttendArgs &a, hipStre
     if (a.n_tokens == 0 || a.n_requests == 0) return hipSuccess;
     const int64_t most = (int64_t)p.max_parts + (int64_t)a.n_tokens * p.group / kPagesTileRows + a.n_requests;
     const int wgs = (int)(most < 2048 ? most : 2048);
-    const dim3 grid(wgs, p.n_kv);
+    const dim3 grid(wgs * p.n_kv);
     if (p.hd == 128) hipLaunchKernelGGL(pages_attend_kernel<128>, grid, dim3(256), 0, s, p, a);
     else hipLaunchKernelGGL(pages_attend_kernel<64>, grid, dim3(256), 0, s, p, a);
     if (p.max_context > pages_part_keys(1)) {
