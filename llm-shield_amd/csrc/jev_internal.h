@@ -476,7 +476,7 @@ struct Pages {
     const double *freqs = nullptr;
     float *part = nullptr;                  // [n_parts][kv head][16][hd + 4]: output, max, sum
     float *wide_part = nullptr;             // [n_wide_parts][kv head][128][hd + 4]
-    int2 *wide_owner = nullptr;             // [n_wide_parts] batch row, place among its request's
+    int32_t *tickets = nullptr, *wide_tickets = nullptr; // [parts][kv head] parts that have arrived, at a tile's first part
     int max_units = 0, max_items = 0, max_wide = 0, max_parts = 0, max_wide_parts = 0;
     __host__ __device__ size_t n_blocks() const { return (size_t)n_pages * n_kv * sub; } // of a layer
 };

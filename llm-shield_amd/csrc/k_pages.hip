@@ -123,7 +123,6 @@ __device__ __forceinline__ void plan_lists(const Pages &p, const PagesPlanArgs &
         it.key1 = min(r.len, it.key0 + keys);
         it.part = r.n_parts > 1 ? r.part0 + k : -1;
         p.wide[i] = it;
-        if (it.part >= 0) p.wide_owner[it.part] = make_int2(b, k);
     }
     // Angles in 64 bits: a far position times a frequency keeps its fraction.
     // Once a plan, not once a layer and head: the library's 64-bit sine and
@@ -715,6 +714,70 @@ struct QueryScale {
     }
 };
 
+// Partial results pass between workgroups inside a launch, which may run on
+// different dies with an L2 each: they are stored and read as agent-scope atomics
+// (written through, and read past, caches that other dies do not see), two floats
+// at a time.  A fence would write back the whole L2 of the die for every part
+// (measured: 64 rows of up to 12000 keys 1090 us instead of 104).
+__device__ __forceinline__ void store_shared(float *p, float x, float y)
+{
+    __hip_atomic_store((uint64_t *)p, (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load_shared(const float *p)
+{
+    const uint64_t v = __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+
+// True in the workgroup that is the last of `parts` to come here; its ticket is
+// left at zero for the next call.  Every thread's store_shared()s are complete
+// (acknowledged by memory) before its workgroup's arrival is counted, so the last
+// one's load_shared()s, issued after it has read the count, find them.
+__device__ __forceinline__ bool arrives_last(int32_t *ticket, int parts, int &shared)
+{
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const int before = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        shared = before == parts - 1;
+        if (shared) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    return shared;
+}
+
+// One row's parts (part k at at(k): HD outputs, maximum, sum) merged in their
+// order by sixteen threads.
+template <int HD, typename At>
+__device__ __forceinline__ void merge_parts(At at, int n_parts, float *dst, int j)
+{
+    constexpr int N = HD / 16;
+    float m = -INFINITY;
+    for (int k = j; k < n_parts; k += 16) m = fmaxf(m, load_shared(at(k) + HD).x);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if (m == -INFINITY) m = 0.f;
+    float x[N] = {}, sum = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < n_parts; k++) {
+        const float *src = at(k);
+        const float2 ml = load_shared(src + HD);
+        const float f = exp2f(ml.x - m);
+        sum += ml.y * f;
+#pragma unroll
+        for (int i = 0; i < N; i += 2) { // (a row's sixteen threads side by side)
+            const float2 y = load_shared(src + 16 * i + 2 * j);
+            x[i] += y.x * f;
+            x[i + 1] += y.y * f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        dst[16 * i + 2 * j] = x[i] / sum;
+        dst[16 * i + 2 * j + 1] = x[i + 1] / sum;
+    }
+}
+
 } // namespace
 
 // Sixteen (token, head) rows of a request and KV head over keys [key0, key1) of
@@ -731,19 +794,25 @@ struct QueryScale {
 // flight during the softmax and V^T P^T, their V during the next scores.
 // Single tokens are bound by HBM: 2 hd bytes a key and KV head.
 template <int HD>
-__global__ __launch_bounds__(256, 2) void pages_attend_kernel(Pages p, PagesAttendArgs a)
+struct TileLds {
+    float lo[4][kPagesTileRows][HD + 4];
+    float lm[4][kPagesTileRows], ll[4][kPagesTileRows];
+    int last;
+};
+template <int HD>
+__device__ __forceinline__ void attend_tiles(const Pages &p, const PagesAttendArgs &a, TileLds<HD> &lds, int first, int count)
 {
-    constexpr int NJ = HD / 64, NS = HD / 16, BYTES = kPageBlock * HD, LDO = HD + 4;
-    __shared__ float lo[4][kPagesTileRows][LDO];
-    __shared__ float lm[4][kPagesTileRows], ll[4][kPagesTileRows];
+    constexpr int NJ = HD / 64, NS = HD / 16, BYTES = kPageBlock * HD, LD = HD + 4;
+    auto &lo = lds.lo;
+    auto &lm = lds.lm, &ll = lds.ll;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int g = lane >> 4, n = lane & 15, h = blockIdx.x % p.n_kv;
-    const int n_items = p.head->n_items, stride = gridDim.x / p.n_kv;
+    const int g = lane >> 4, n = lane & 15, h = first % p.n_kv;
+    const int n_items = p.head->n_items, stride = count / p.n_kv;
     const uint8_t *kbase = p.k + (size_t)a.layer * p.n_blocks() * BYTES;
     const uint8_t *vbase = p.v + (size_t)a.layer * p.n_blocks() * BYTES;
     const float2 *sbase = p.ks + (size_t)a.layer * p.n_blocks();
 
-    for (int item = blockIdx.x / p.n_kv; item < n_items; item += stride) {
+    for (int item = first / p.n_kv; item < n_items; item += stride) {
         const PagesItem it = p.item[item];
         const PagesRequest r = p.req[it.b];
         const int32_t *table = p.table + (size_t)r.id * p.width;
@@ -940,13 +1009,22 @@ __global__ __launch_bounds__(256, 2) void pages_attend_kernel(Pages p, PagesAtte
 #pragma unroll
                 for (int k = 0; k < 4; k++) dst[k] = x[k] * inv;
             } else {
-                float *dst = p.part + (((size_t)it.part * p.n_kv + h) * kPagesTileRows + c) * (HD + 4);
-                *(floatx4 *)(dst + d) = x;
-                if (d == 0) {
-                    dst[HD] = mm;
-                    dst[HD + 1] = sum;
-                }
+                float *dst = p.part + (((size_t)it.part * p.n_kv + h) * kPagesTileRows + c) * LD;
+                store_shared(dst + d, x[0], x[1]);
+                store_shared(dst + d + 2, x[2], x[3]);
+                if (d == 0) store_shared(dst + HD, mm, sum);
             }
+        }
+        if (it.part >= 0) {
+            // the tile's last part to arrive merges them all, in their order
+            const int tiles = div_up(n_rows, kPagesTileRows), tile = it.row0 / kPagesTileRows;
+            if (arrives_last(p.tickets + (size_t)(r.part0 + tile) * p.n_kv + h, r.n_parts, lds.last))
+                for (int c = tid >> 4; c < min(kPagesTileRows, n_rows - it.row0); c += 16) {
+                    const int rr = it.row0 + c, tk = rr / p.group;
+                    merge_parts<HD>(
+                        [&](int k) { return p.part + (((size_t)(r.part0 + k * tiles + tile) * p.n_kv + h) * kPagesTileRows + c) * LD; },
+                        r.n_parts, a.out + ((size_t)(r.start + tk) * p.n_heads + h * p.group + rr % p.group) * HD, tid & 15);
+                }
         }
         __syncthreads();
     }
@@ -965,13 +1043,72 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 // nothing.  Bound by the matrix cores at two instructions a product, with the
 // exponentials and fp16 pairs of ~9 vector instructions a score beside them.
 template <int HD>
-__global__ __launch_bounds__(256, 2) void pages_attend_wide_kernel(Pages p, PagesAttendArgs a)
+struct WideLds {
+    union {
+        struct {
+            uint4 kf[2][2 * (HD / 16) * 64], vf[2][4 * (HD / 32) * 64];
+            float2 sc[2][4];
+        };
+        float rows[kPagesWideRows * (HD + 4)]; // a part: outputs, maximum, sum
+    };
+    int last;
+};
+
+// A wide tile's end: its outputs, or its part and, from its last part, theirs.
+template <int HD>
+__device__ __forceinline__ void wide_result(const Pages &p, const PagesAttendArgs &a, WideLds<HD> &lds, int item, int h,
+                                            const floatx16 (&o)[HD / 32], float up, float m, float l)
+{
+    constexpr int ND = HD / 32, LD = HD + 4;
+    // read again: nothing of them takes registers during the products
+    asm volatile("" : "+s"(item));
+    const PagesItem it = p.wide[item];
+    const PagesRequest r = p.req[it.b];
+    const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, n = lane & 31, wrow = 32 * (tid >> 6) + n;
+    const int n_rows = min(kPagesWideRows, (r.len - r.past) * p.group - it.row0); // of the tile
+    auto out_of = [&](int c) { // the tile's row c
+        const int row = it.row0 + c;
+        return a.out + ((size_t)(r.start + row / p.group) * p.n_heads + h * p.group + row % p.group) * HD;
+    };
+    if (it.part < 0) {
+        if (wrow >= n_rows) return;
+        float *dst = out_of(wrow);
+        const float f = 0x1p-9f / l;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) dst[32 * d + 8 * (i >> 2) + 4 * hh + (i & 3)] = o[d][i] * f * up;
+        return;
+    }
+    // through LDS, where the fragments were: whole runs of a row to a store
+    float *rows = lds.rows, *mine = rows + wrow * LD;
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            *(floatx4 *)(mine + 32 * d + 8 * i + 4 * hh) =
+                floatx4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]} * 0x1p-9f * up;
+    if (hh == 0) *(float2 *)(mine + HD) = make_float2(m, l);
+    __syncthreads();
+    float *part = p.wide_part + ((size_t)it.part * p.n_kv + h) * kPagesWideRows * LD;
+    for (int i = 2 * tid; i < n_rows * LD; i += 512)
+        if (i % LD < HD + 2) store_shared(part + i, rows[i], rows[i + 1]);
+    const int part0 = it.part - (it.part - r.part0) % r.n_parts; // of this tile
+    if (!arrives_last(p.wide_tickets + (size_t)part0 * p.n_kv + h, r.n_parts, lds.last)) return;
+    for (int c = tid >> 4; c < n_rows; c += 16)
+        merge_parts<HD>([&](int k) { return p.wide_part + (((size_t)(part0 + k) * p.n_kv + h) * kPagesWideRows + c) * LD; }, r.n_parts,
+                        out_of(c), tid & 15);
+}
+
+template <int HD>
+__device__ __forceinline__ void attend_wide(const Pages &p, const PagesAttendArgs &a, WideLds<HD> &lds, int first)
 {
     constexpr int NC = HD / 16, ND = HD / 32, NL = HD / 64, BYTES = kPageBlock * HD, LD = HD + 4;
-    __shared__ __align__(16) uint4 kf[2][2 * NC * 64], vf[2][4 * ND * 64];
-    __shared__ __align__(16) float2 sc[2][4];
+    auto &kf = lds.kf;
+    auto &vf = lds.vf;
+    auto &sc = lds.sc;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int hh = lane >> 5, n = lane & 31, h = blockIdx.x % p.n_kv, item = blockIdx.x / p.n_kv;
+    const int hh = lane >> 5, n = lane & 31, h = first % p.n_kv, item = first / p.n_kv;
     if (item >= p.head->n_wide) return;
     const PagesItem it = p.wide[item];
     const PagesRequest r = p.req[it.b];
@@ -1154,131 +1291,42 @@ __global__ __launch_bounds__(256, 2) void pages_attend_wide_kernel(Pages p, Page
         if (more) put(buf ^ 1);
         __syncthreads();
     }
-    if (!active || wrow + n >= n_rows) return;
     l += __shfl_xor(l, 32, 64);
     const float up = ldexpf(1.f, max(ev, -149));
-    float *dst;
-    float f = 0x1p-9f;
-    if (it.part < 0) {
-        dst = a.out + ((size_t)(r.start + token) * p.n_heads + head) * HD;
-        f /= l;
-    } else {
-        dst = p.wide_part + (((size_t)it.part * p.n_kv + h) * kPagesWideRows + 32 * wave + n) * LD;
-        if (hh == 0) {
-            dst[HD] = m;
-            dst[HD + 1] = l;
-        }
-    }
-#pragma unroll
-    for (int d = 0; d < ND; d++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) dst[32 * d + 8 * (i >> 2) + 4 * hh + (i & 3)] = o[d][i] * f * up;
+    wide_result<HD>(p, a, lds, item, h, o, up, m, l);
 }
 
-// The parts of split wide tiles: a workgroup takes sixteen rows, sixteen
-// threads a row.
-template <int HD>
-__global__ __launch_bounds__(256) void pages_merge_wide_kernel(Pages p, PagesAttendArgs a)
+// The attention of a plan in one launch: wide tiles first, then 16-row tiles,
+// `tiles` workgroups of which take turns.
+template <int HD, bool WIDE>
+__global__ __launch_bounds__(256, 2) void pages_attend_kernel(Pages p, PagesAttendArgs a, int wides, int tiles)
 {
-    constexpr int N = HD / 16, LD = HD + 4;
-    if ((int)blockIdx.x >= p.head->n_wide_parts) return;
-    const int2 own = p.wide_owner[blockIdx.x];
-    const PagesRequest r = p.req[own.x];
-    if (own.y % r.n_parts) return; // a tile's first part stands for it
-    const int n_rows = (r.len - r.past) * p.group, tiles = div_up(n_rows, kPagesWideRows);
-    const int h = blockIdx.y, c = 16 * blockIdx.z + (threadIdx.x >> 4), j = threadIdx.x & 15;
-    const int row = (tiles - 1 - own.y / r.n_parts) * kPagesWideRows + c;
-    if (row >= n_rows) return;
-    auto at = [&](int k) { return p.wide_part + (((size_t)(blockIdx.x + k) * p.n_kv + h) * kPagesWideRows + c) * LD; };
-    float m = -INFINITY;
-    for (int k = 0; k < r.n_parts; k++) m = fmaxf(m, at(k)[HD]);
-    if (m == -INFINITY) m = 0.f;
-    float x[N] = {}, sum = 0.f;
-    for (int k = 0; k < r.n_parts; k++) {
-        const float *src = at(k);
-        const float f = exp2f(src[HD] - m);
-        sum += src[HD + 1] * f;
-#pragma unroll
-        for (int i = 0; i < N; i++) x[i] += src[N * j + i] * f;
-    }
-    float *dst = a.out + ((size_t)(r.start + row / p.group) * p.n_heads + h * p.group + row % p.group) * HD + N * j;
-#pragma unroll
-    for (int i = 0; i < N; i++) dst[i] = x[i] / sum;
-}
-
-// The parts of split tiles, per batch row and head: sixteen threads hold the
-// head's dims (HD / 16 each), the sixteen groups take every sixteenth part and
-// are summed in group order.
-template <int HD>
-__global__ __launch_bounds__(256) void pages_merge_kernel(Pages p, PagesAttendArgs a)
-{
-    constexpr int ND = HD / 16, LD = HD + 4;
-    __shared__ float lo[16][HD];
-    __shared__ float ll[16], wm[4];
-    const int tid = threadIdx.x, b = blockIdx.x, head = blockIdx.y, h = head / p.group;
-    if (b >= p.head->n_requests) return;
-    const PagesRequest r = p.req[b];
-    if (r.n_parts <= 1 || r.wide) return;
-    const int tiles = div_up((r.len - r.past) * p.group, kPagesTileRows);
-    for (int t = 0; t < r.len - r.past; t++) {
-        const int row = t * p.group + head % p.group, tile = row / kPagesTileRows, c = row % kPagesTileRows;
-        // part k of the row
-        auto at = [&](int k) { return p.part + (((size_t)(r.part0 + k * tiles + tile) * p.n_kv + h) * kPagesTileRows + c) * LD; };
-        float m = -INFINITY;
-        for (int k = tid; k < r.n_parts; k += 256) m = fmaxf(m, at(k)[HD]);
-        m = warp_max(m);
-        __syncthreads();
-        if ((tid & 63) == 0) wm[tid >> 6] = m;
-        __syncthreads();
-        m = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
-        if (m == -INFINITY) m = 0.f;
-        const int grp = tid >> 4, j = tid & 15;
-        float x[ND] = {}, sum = 0.f;
-        for (int k = grp; k < r.n_parts; k += 16) {
-            const float *src = at(k);
-            const float f = exp2f(src[HD] - m);
-            sum += src[HD + 1] * f;
-#pragma unroll
-            for (int i = 0; i < ND; i++) x[i] += src[ND * j + i] * f;
-        }
-#pragma unroll
-        for (int i = 0; i < ND; i++) lo[grp][ND * j + i] = x[i];
-        if (j == 0) ll[grp] = sum;
-        __syncthreads();
-        if (tid < HD) {
-            float y = 0.f, z = 0.f;
-            for (int k = 0; k < 16; k++) {
-                y += lo[k][tid];
-                z += ll[k];
-            }
-            a.out[((size_t)(r.start + t) * p.n_heads + head) * HD + tid] = y / z;
+    union Lds {
+        TileLds<HD> tile;
+        WideLds<WIDE ? HD : 16> wide;
+    };
+    __shared__ __align__(16) char mem[sizeof(Lds)];
+    Lds &lds = *(Lds *)mem;
+    if constexpr (WIDE) {
+        if ((int)blockIdx.x < wides) {
+            attend_wide<HD>(p, a, *(WideLds<HD> *)mem, blockIdx.x);
+            return;
         }
     }
+    attend_tiles<HD>(p, a, lds.tile, (int)blockIdx.x - wides, tiles);
 }
 
 hipError_t launch_pages_attend(const Pages &p, const PagesAttendArgs &a, hipStream_t s)
 {
     if (a.n_tokens == 0 || a.n_requests == 0) return hipSuccess;
     const int64_t most = (int64_t)p.max_parts + (int64_t)a.n_tokens * p.group / kPagesTileRows + a.n_requests;
-    const int wgs = (int)(most < 2048 ? most : 2048);
-    const dim3 grid(wgs * p.n_kv);
-    if (p.hd == 128) hipLaunchKernelGGL(pages_attend_kernel<128>, grid, dim3(256), 0, s, p, a);
-    else hipLaunchKernelGGL(pages_attend_kernel<64>, grid, dim3(256), 0, s, p, a);
-    if (p.max_context > pages_part_keys(1)) {
-        const dim3 mg(a.n_requests, p.n_heads);
-        if (p.hd == 128) hipLaunchKernelGGL(pages_merge_kernel<128>, mg, dim3(256), 0, s, p, a);
-        else hipLaunchKernelGGL(pages_merge_kernel<64>, mg, dim3(256), 0, s, p, a);
-    }
-    if (a.wide) {
-        const int64_t tiles = (int64_t)a.n_tokens * p.group / kPagesWideRows + a.n_requests + pages_wide_target(p.n_kv);
-        const dim3 wg((unsigned)(tiles * p.n_kv)), mg(p.max_wide_parts, p.n_kv, kPagesWideRows / 16);
-        if (p.hd == 128) hipLaunchKernelGGL(pages_attend_wide_kernel<128>, wg, dim3(256), 0, s, p, a);
-        else hipLaunchKernelGGL(pages_attend_wide_kernel<64>, wg, dim3(256), 0, s, p, a);
-        if (p.max_context > kPagesWideKeys) {
-            if (p.hd == 128) hipLaunchKernelGGL(pages_merge_wide_kernel<128>, mg, dim3(256), 0, s, p, a);
-            else hipLaunchKernelGGL(pages_merge_wide_kernel<64>, mg, dim3(256), 0, s, p, a);
-        }
-    }
+    const int64_t most_wide = (int64_t)a.n_tokens * p.group / kPagesWideRows + a.n_requests + pages_wide_target(p.n_kv);
+    const int wides = a.wide ? (int)(most_wide * p.n_kv) : 0, tiles = (int)(most < 2048 ? most : 2048) * p.n_kv;
+    const dim3 grid(wides + tiles);
+    if (p.hd == 128 && a.wide) hipLaunchKernelGGL((pages_attend_kernel<128, true>), grid, dim3(256), 0, s, p, a, wides, tiles);
+    else if (p.hd == 128) hipLaunchKernelGGL((pages_attend_kernel<128, false>), grid, dim3(256), 0, s, p, a, wides, tiles);
+    else if (a.wide) hipLaunchKernelGGL((pages_attend_kernel<64, true>), grid, dim3(256), 0, s, p, a, wides, tiles);
+    else hipLaunchKernelGGL((pages_attend_kernel<64, false>), grid, dim3(256), 0, s, p, a, wides, tiles);
     return hipGetLastError();
 }
 

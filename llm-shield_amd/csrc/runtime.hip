@@ -2757,7 +2757,8 @@ int jev_pages_create(const jev_config *model, const jev_pages_config *cfg, int d
     if (!rc) rc = pages_alloc(h, p.unit, p.max_units);
     if (!rc) rc = pages_alloc(h, p.item, p.max_items);
     if (!rc) rc = pages_alloc(h, p.wide, p.max_wide);
-    if (!rc) rc = pages_alloc(h, p.wide_owner, p.max_wide_parts);
+    if (!rc) rc = pages_alloc(h, p.tickets, (size_t)p.max_parts * p.n_kv);
+    if (!rc) rc = pages_alloc(h, p.wide_tickets, (size_t)p.max_wide_parts * p.n_kv);
     if (!rc) rc = pages_alloc(h, p.wide_part, (size_t)p.max_wide_parts * p.n_kv * kPagesWideRows * (p.hd + 4));
     if (!rc) rc = pages_alloc(h, p.angle, T * p.half);
     if (!rc) rc = pages_alloc(h, dfreqs, freqs.size());
