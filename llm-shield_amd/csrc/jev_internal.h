@@ -425,10 +425,15 @@ constexpr int kPagesWideRows = 128;    // the same in a wide tile, for requests 
 constexpr int kPagesWideWgs = 512, kPagesWideKeys = 512;
 __host__ __device__ inline int pages_wide_target(int n_kv) { return n_kv < kPagesWideWgs ? kPagesWideWgs / n_kv : 1; }
 
-// Keys per workgroup of a tile whose rows are one request's whole batch: a
-// function of the request's own length alone, so that its result does not
-// depend on the other requests.
-__host__ __device__ inline int pages_part_keys(int len) { return len <= 4096 ? 256 : len <= 32768 ? 512 : 1024; }
+// Keys per workgroup of a 16-row tile: a function of the request's own length
+// alone, so that its result does not depend on the other requests.  Fewer keys
+// spread a lone request further, more save each part's start and end (us a pass,
+// 512 / 1024 / 2048 keys: one request of 4000 4.5 / 5.3 / 7.5, of 30000 11.5 / 11.0 /
+// 10.6; 64 of 500 to 12000 91 / 86 / 83, 128 of 2000 106 / 94 / 87).
+__host__ __device__ inline int pages_part_keys(int len)
+{
+    return len <= 16384 ? 1024 : len <= 131072 ? 2048 : (len / 64 + 63) & ~63; // at most 65 parts
+}
 
 struct PagesPlanHead {
     int32_t status;  // JEV_OK, JEV_EINVAL or JEV_ENOMEM; not OK: everything below is zero
@@ -445,8 +450,10 @@ struct PagesRequest { // one batch row
     int32_t part0, n_parts;       // partial results of its tiles, when split (n_parts > 1)
     int32_t wide;                 // its tiles are wide ones
 };
-struct PagesItem {
-    int32_t b, row0, key0, key1, part; // part >= 0: where its partial result goes
+struct PagesItem { // a workgroup's tile and keys, with its request's fields: one load away
+    int32_t row0, key0, key1, part; // part >= 0: where its partial result goes
+    int32_t id, past, len, start;
+    int32_t n_parts, part0, row1, pad; // row1: past the tile's last row (16-row tiles: the request's)
 };
 struct Pages {
     // geometry

@@ -103,12 +103,9 @@ __device__ __forceinline__ void plan_lists(const Pages &p, const PagesPlanArgs &
         const PagesRequest r = p.req[b];
         const int tiles = (item0[b + 1] - item0[b]) / r.n_parts, t = k % tiles, part = k / tiles;
         const int keys = r.n_parts > 1 ? pages_part_keys(r.len) : r.len;
-        PagesItem it;
-        it.b = b;
-        it.row0 = t * kPagesTileRows;
-        it.key0 = part * keys;
-        it.key1 = min(r.len, it.key0 + keys);
-        it.part = r.n_parts > 1 ? r.part0 + k : -1;
+        const int key0 = part * keys;
+        const PagesItem it = {t * kPagesTileRows, key0, min(r.len, key0 + keys), r.n_parts > 1 ? r.part0 + k : -1,
+                              r.id, r.past, r.len, r.start, r.n_parts, r.part0, (r.len - r.past) * p.group, 0};
         p.item[i] = it;
     }
     for (int i = i0; i < h.n_wide; i += n) {
@@ -116,12 +113,11 @@ __device__ __forceinline__ void plan_lists(const Pages &p, const PagesPlanArgs &
         const PagesRequest r = p.req[b];
         const int tiles = (wide0[b + 1] - wide0[b]) / r.n_parts, part = k % r.n_parts;
         const int keys = (div_up(r.len, r.n_parts) + 63) & ~63; // parts of a length, in whole blocks of 64
-        PagesItem it;
-        it.b = b;
-        it.row0 = (tiles - 1 - k / r.n_parts) * kPagesWideRows; // the longest first
-        it.key0 = part * keys;
-        it.key1 = min(r.len, it.key0 + keys);
-        it.part = r.n_parts > 1 ? r.part0 + k : -1;
+        // a request's tiles take like numbers of rows, whole waves' of 32; the longest come first
+        const int rows = (r.len - r.past) * p.group, per = (div_up(rows, tiles) + 31) & ~31;
+        const int key0 = part * keys, row0 = (tiles - 1 - k / r.n_parts) * per;
+        const PagesItem it = {row0, key0, min(r.len, key0 + keys), r.n_parts > 1 ? r.part0 + k : -1,
+                              r.id, r.past, r.len, r.start, r.n_parts, r.part0, min(rows, row0 + per), 0};
         p.wide[i] = it;
     }
     // Angles in 64 bits: a far position times a frequency keeps its fraction.
@@ -813,11 +809,10 @@ __device__ __forceinline__ void attend_tiles(const Pages &p, const PagesAttendAr
     const float2 *sbase = p.ks + (size_t)a.layer * p.n_blocks();
 
     for (int item = first / p.n_kv; item < n_items; item += stride) {
-        const PagesItem it = p.item[item];
-        const PagesRequest r = p.req[it.b];
+        const PagesItem it = p.item[item], &r = it;
         const int32_t *table = p.table + (size_t)r.id * p.width;
         // lanes past the request's rows repeat its last one
-        const int n_rows = (r.len - r.past) * p.group, row = min(it.row0 + n, n_rows - 1);
+        const int n_rows = it.row1, row = min(it.row0 + n, n_rows - 1);
         const int token = row / p.group, head = h * p.group + row % p.group;
         const int limit = r.past + token; // last visible key
         // the tile's last visible key; keys up to `clear` are seen by every row
@@ -1050,6 +1045,7 @@ struct WideLds {
             float2 sc[2][4];
         };
         float rows[kPagesWideRows * (HD + 4)]; // a part: outputs, maximum, sum
+        float factor[8][kPagesWideRows];
     };
     int last;
 };
@@ -1059,13 +1055,12 @@ template <int HD>
 __device__ __forceinline__ void wide_result(const Pages &p, const PagesAttendArgs &a, WideLds<HD> &lds, int item, int h,
                                             const floatx16 (&o)[HD / 32], float up, float m, float l)
 {
-    constexpr int ND = HD / 32, LD = HD + 4;
+    constexpr int ND = HD / 32, LD = HD + 4, kMost = 8;
     // read again: nothing of them takes registers during the products
     asm volatile("" : "+s"(item));
-    const PagesItem it = p.wide[item];
-    const PagesRequest r = p.req[it.b];
+    const PagesItem it = p.wide[item], &r = it;
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, n = lane & 31, wrow = 32 * (tid >> 6) + n;
-    const int n_rows = min(kPagesWideRows, (r.len - r.past) * p.group - it.row0); // of the tile
+    const int n_rows = it.row1 - it.row0; // of the tile
     auto out_of = [&](int c) { // the tile's row c
         const int row = it.row0 + c;
         return a.out + ((size_t)(r.start + row / p.group) * p.n_heads + h * p.group + row % p.group) * HD;
@@ -1095,9 +1090,49 @@ __device__ __forceinline__ void wide_result(const Pages &p, const PagesAttendArg
         if (i % LD < HD + 2) store_shared(part + i, rows[i], rows[i + 1]);
     const int part0 = it.part - (it.part - r.part0) % r.n_parts; // of this tile
     if (!arrives_last(p.wide_tickets + (size_t)part0 * p.n_kv + h, r.n_parts, lds.last)) return;
-    for (int c = tid >> 4; c < n_rows; c += 16)
-        merge_parts<HD>([&](int k) { return p.wide_part + (((size_t)(part0 + k) * p.n_kv + h) * kPagesWideRows + c) * LD; }, r.n_parts,
-                        out_of(c), tid & 15);
+    if (r.n_parts > kMost) {
+        for (int c = tid >> 4; c < n_rows; c += 16)
+            merge_parts<HD>([&](int k) { return p.wide_part + (((size_t)(part0 + k) * p.n_kv + h) * kPagesWideRows + c) * LD; }, r.n_parts,
+                            out_of(c), tid & 15);
+        return;
+    }
+    // few parts: every row's factors first, then no sum waits for them
+    const float *at = p.wide_part + ((size_t)part0 * p.n_kv + h) * kPagesWideRows * LD;
+    const size_t step = (size_t)p.n_kv * kPagesWideRows * LD;
+    if (tid < n_rows) {
+        float2 ml[kMost];
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kMost; k++)
+            if (k < r.n_parts) ml[k] = load_shared(at + k * step + tid * LD + HD);
+#pragma unroll
+        for (int k = 0; k < kMost; k++)
+            if (k < r.n_parts) top = fmaxf(top, ml[k].x);
+        if (top == -INFINITY) top = 0.f;
+#pragma unroll
+        for (int k = 0; k < kMost; k++)
+            if (k < r.n_parts) sum += ml[k].y * exp2f(ml[k].x - top);
+#pragma unroll
+        for (int k = 0; k < kMost; k++)
+            if (k < r.n_parts) lds.factor[k][tid] = exp2f(ml[k].x - top) / sum;
+    }
+    __syncthreads();
+    constexpr int TH = HD / 2, RT = 256 / TH; // threads of a row, rows at once
+    const int j = 2 * (tid % TH);
+#pragma unroll 4
+    for (int c = tid / TH; c < n_rows; c += RT) {
+        float x = 0.f, y = 0.f;
+#pragma unroll
+        for (int k = 0; k < kMost; k++)
+            if (k < r.n_parts) {
+                const float2 v = load_shared(at + k * step + c * LD + j);
+                x += v.x * lds.factor[k][c];
+                y += v.y * lds.factor[k][c];
+            }
+        float *dst = out_of(c) + j;
+        dst[0] = x;
+        dst[1] = y;
+    }
 }
 
 template <int HD>
@@ -1110,14 +1145,13 @@ __device__ __forceinline__ void attend_wide(const Pages &p, const PagesAttendArg
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hh = lane >> 5, n = lane & 31, h = first % p.n_kv, item = first / p.n_kv;
     if (item >= p.head->n_wide) return;
-    const PagesItem it = p.wide[item];
-    const PagesRequest r = p.req[it.b];
+    const PagesItem it = p.wide[item], &r = it;
     const int32_t *table = p.table + (size_t)r.id * p.width;
     const uint8_t *kbase = p.k + (size_t)a.layer * p.n_blocks() * BYTES;
     const uint8_t *vbase = p.v + (size_t)a.layer * p.n_blocks() * BYTES;
     const float2 *sbase = p.ks + (size_t)a.layer * p.n_blocks();
 
-    const int n_rows = (r.len - r.past) * p.group, wrow = it.row0 + 32 * wave;
+    const int n_rows = it.row1, wrow = it.row0 + 32 * wave;
     const bool active = wrow < n_rows;
     const int row = min(wrow + n, n_rows - 1), token = row / p.group, head = h * p.group + row % p.group;
     const int limit = r.past + token; // last visible key
