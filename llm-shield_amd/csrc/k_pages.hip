@@ -1156,8 +1156,7 @@ __device__ __forceinline__ void attend_wide(const Pages &p, const PagesAttendArg
     const int row = min(wrow + n, n_rows - 1), token = row / p.group, head = h * p.group + row % p.group;
     const int limit = r.past + token; // last visible key
     const int key1 = min(it.key1, r.past + min(n_rows - 1, it.row0 + kPagesWideRows - 1) / p.group + 1);
-    // keys below `clear` are seen by every row of the wave, keys past `wtop` by none
-    const int clear = r.past + min(wrow, n_rows - 1) / p.group, wtop = active ? r.past + min(n_rows - 1, wrow + 31) / p.group : -1;
+    const int clear = r.past + min(wrow, n_rows - 1) / p.group; // keys up to it are seen by every row of the wave
     const int last = (r.len - 1) / kPageBlock;
 
     // A wave stages one of a block's four 16-token blocks.  Buffer loads: their
@@ -1180,30 +1179,24 @@ __device__ __forceinline__ void attend_wide(const Pages &p, const PagesAttendArg
         for (int i = 0; i < NL; i++) vr[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rv, 16 * lane, 1024 * i, 0));
         sr = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rs, 0, 0, 0));
     };
-    auto put = [&](int buf) {
-        // K: sixteen dims of token lane / 4, chunk 4 i + lane % 4; its row of the
-        // tile, dealt by chunk so that neighbouring lanes' writes take all banks
-        const int tk = lane >> 2, m = (8 * (tk >> 2) + 4 * (wave & 1) + (tk & 3)) ^ ((lane & 3) << 1);
-#pragma unroll
-        for (int i = 0; i < NL; i++) {
-            uint4 *to = kf[buf] + ((wave >> 1) * NC + 4 * i + (lane & 3)) * 64 + m;
-            to[0] = codes_f16(kr[i].x, kr[i].y);
-            to[32] = codes_f16(kr[i].z, kr[i].w);
-        }
-        // V: sixteen tokens of dim 64 i + lane
-#pragma unroll
-        for (int i = 0; i < NL; i++) {
-            uint4 *to = vf[buf] + ((2 * i + hh) * 4 + (wave >> 1) * 2) * 64 + 32 * (wave & 1) + n;
-            to[0] = codes_f16(vr[i].x, vr[i].y);
-            to[64] = codes_f16(vr[i].z, vr[i].w);
-        }
-        if (lane == 0) sc[buf][wave] = sr;
+    // K: sixteen dims of token lane / 4, chunk 4 i + lane % 4; its row of the tile,
+    // dealt by chunk so that neighbouring lanes' writes take all banks.  V: sixteen
+    // tokens of dim 64 i + lane.  One of the 4 NL halves of these to a piece.
+    const int krow = (8 * (lane >> 4) + 4 * (wave & 1) + ((lane >> 2) & 3)) ^ ((lane & 3) << 1);
+    auto put = [&](int buf, int piece) {
+        const int i = piece >> 2, half = piece & 1;
+        if (piece & 2)
+            (vf[buf] + ((2 * i + hh) * 4 + (wave >> 1) * 2) * 64 + 32 * (wave & 1) + n)[64 * half] =
+                half ? codes_f16(vr[i].z, vr[i].w) : codes_f16(vr[i].x, vr[i].y);
+        else
+            (kf[buf] + ((wave >> 1) * NC + 4 * i + (lane & 3)) * 64 + krow)[32 * half] =
+                half ? codes_f16(kr[i].z, kr[i].w) : codes_f16(kr[i].x, kr[i].y);
+        if (piece == 0 && lane == 0) sc[buf][wave] = sr;
     };
 
     int kb = it.key0 / 64;
-    const bool any = kb * 64 < key1;
     int next = page_of(kb);
-    if (any) fetch(kb, next);
+    fetch(kb, next);
     next = page_of(kb + 1);
 
     // Q^T fragments: dims 16 c + 8 hh .. + 7 of row n
@@ -1235,94 +1228,123 @@ __device__ __forceinline__ void attend_wide(const Pages &p, const PagesAttendArg
     for (int d = 0; d < ND; d++) o[d] = floatx16{};
     float m = -INFINITY, l = 0.f;
     int ev = -200; // outputs are held times 2^(9 - ev); V scales are below 2^ev
-    if (any) put(0);
+#pragma unroll
+    for (int i = 0; i < 4 * NL; i++) put(0, i);
+    fetch(kb + 1, next); // (past the last block: the last again, which nobody reads)
+    next = page_of(kb + 2);
     __syncthreads();
 
+    if (!active) { // no rows of its own: it stages for the others
+        for (int buf = 0; kb * 64 < key1; kb++, buf ^= 1) {
+#pragma unroll
+            for (int i = 0; i < 4 * NL; i++) put(buf ^ 1, i);
+            fetch(kb + 2, next);
+            next = page_of(kb + 3);
+            __syncthreads();
+        }
+    }
     for (int buf = 0; kb * 64 < key1; kb++, buf ^= 1) {
-        const bool more = (kb + 1) * 64 < key1;
-        if (more) {
-            fetch(kb + 1, next);
-            next = page_of(kb + 2);
+        // the scores; beside their matrix instructions the next block's codes,
+        // here by now, become fragments, and the block after it is asked for
+        floatx16 s[2] = {floatx16{}, floatx16{}};
+        auto kfrag = [&](int t, int c) { return __builtin_bit_cast(half8_t, kf[buf][(t * NC + c) * 64 + (lane ^ ((c & 3) << 1))]); };
+        half8_t k0 = kfrag(0, 0), k1 = kfrag(1, 0);
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const half8_t n0 = kfrag(0, min(c + 1, NC - 1)), n1 = kfrag(1, min(c + 1, NC - 1));
+            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qh[c], s[0], 0, 0, 0);
+            s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qh[c], s[1], 0, 0, 0);
+            put(buf ^ 1, c);
+            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, ql[c], s[0], 0, 0, 0);
+            s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, ql[c], s[1], 0, 0, 0);
+            k0 = n0, k1 = n1;
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if (kb * 64 <= wtop) {
-            floatx16 s[2] = {floatx16{}, floatx16{}};
+        fetch(kb + 2, next);
+        next = page_of(kb + 3);
+        const float4 s01 = *(const float4 *)&sc[buf][0], s23 = *(const float4 *)&sc[buf][2];
+        const float vm = fmaxf(fmaxf(s01.y, s01.w), fmaxf(s23.y, s23.w));
+        const float2 s0 = hh ? make_float2(s01.z, s01.w) : make_float2(s01.x, s01.y);
+        const float2 s1 = hh ? make_float2(s23.z, s23.w) : make_float2(s23.x, s23.y);
+        float ks[2] = {s0.x * qs, s1.x * qs}, vs[2] = {s0.y, s1.y};
 #pragma unroll
-            for (int c = 0; c < NC; c++)
-#pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const half8_t k = __builtin_bit_cast(half8_t, kf[buf][(t * NC + c) * 64 + (lane ^ ((c & 3) << 1))]);
-                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[c], s[t], 0, 0, 0);
-                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[c], s[t], 0, 0, 0);
-                }
-            const float2 s0 = sc[buf][hh], s1 = sc[buf][2 + hh];
-            float ks[2] = {s0.x * qs, s1.x * qs}, vs[2] = {s0.y, s1.y};
-#pragma unroll
-            for (int t = 0; t < 2; t++) ks[t] = ks[t] < 1e-37f ? 1e-37f : ks[t]; // a scale of zero has codes of zero
-            if (kb * 64 + 63 > clear) {
-#pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const int left = limit - (kb * 64 + 32 * t + 16 * hh); // last visible token of the lane's block
-                    if (left < 0) { // none: whatever its scales are
-                        ks[t] = 1.f;
-                        vs[t] = 0.f;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        if (i > left) s[t][i] = -INFINITY;
-                }
-            }
-            float mx = -INFINITY;
+        for (int t = 0; t < 2; t++) ks[t] = ks[t] < 1e-37f ? 1e-37f : ks[t]; // a scale of zero has codes of zero
+        if (kb * 64 + 63 > clear) {
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                float y = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 16; i++) y = fmaxf(y, s[t][i]);
-                mx = fmaxf(mx, y * ks[t]);
-            }
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            float vm = fmaxf(vs[0], vs[1]);
-            vm = fmaxf(vm, __shfl_xor(vm, 32, 64));
-            const int en = vm > 0.f && vm < INFINITY ? max(ev, __builtin_amdgcn_frexp_expf(vm)) : ev;
-            if (__any(mx > m + 6.f || en > ev)) {
-                const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2f(m - mn);
-                l *= f;
-                const float g = ldexpf(f, max(ev - en, -400));
-#pragma unroll
-                for (int d = 0; d < ND; d++) o[d] *= g;
-                m = mn;
-                ev = en;
-            }
-            const float mu = m == -INFINITY ? 0.f : m;
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                // w = 2^(score - m + 9) times the V scale over 2^ev; a scale of zero has codes of zero
-                float lv = vs[t] == 0.f ? 0.f : fmaxf(__builtin_amdgcn_logf(ldexpf(vs[t], -ev)), -60.f);
-                if (vs[t] != vs[t]) lv = vs[t];
-                const float c = lv + 9.f - mu;
-                float w[16], sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    w[i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], ks[t], c));
-                    sum += w[i];
+                const int left = limit - (kb * 64 + 32 * t + 16 * hh); // last visible token of the lane's block
+                if (left < 0) { // none: whatever its scales are
+                    ks[t] = 1.f;
+                    vs[t] = 0.f;
                 }
-                l += sum * __builtin_amdgcn_exp2f(-9.f - lv);
-                uint32_t hi[8], lo[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) split2_mix(w[2 * i], w[2 * i + 1], hi[i], lo[i]);
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const half8_t ph = __builtin_bit_cast(half8_t, make_uint4(hi[4 * j], hi[4 * j + 1], hi[4 * j + 2], hi[4 * j + 3]));
-                    const half8_t pl = __builtin_bit_cast(half8_t, make_uint4(lo[4 * j], lo[4 * j + 1], lo[4 * j + 2], lo[4 * j + 3]));
-#pragma unroll
-                    for (int d = 0; d < ND; d++) {
-                        const half8_t v = __builtin_bit_cast(half8_t, vf[buf][((d * 2 + t) * 2 + j) * 64 + lane]);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[d], 0, 0, 0);
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[d], 0, 0, 0);
-                    }
-                }
+                for (int i = 0; i < 16; i++)
+                    if (i > left) s[t][i] = -INFINITY;
             }
         }
-        if (more) put(buf ^ 1);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            float y = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; i++) y = fmaxf(y, s[t][i]);
+            mx = fmaxf(mx, y * ks[t]);
+        }
+        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+        mx = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+        const int en = vm > 0.f && vm < INFINITY ? max(ev, __builtin_amdgcn_frexp_expf(vm)) : ev;
+        if (__any(mx > m + 6.f || en > ev)) {
+            const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2f(m - mn);
+            l *= f;
+            const float g = ldexpf(f, max(ev - en, -400));
+#pragma unroll
+            for (int d = 0; d < ND; d++) o[d] *= g;
+            m = mn;
+            ev = en;
+        }
+        const float mu = m == -INFINITY ? 0.f : m;
+        // w = 2^(score - m + 9) times the V scale over 2^ev; a scale of zero has codes of zero
+        float lv[2], sum[2] = {0.f, 0.f};
+        uint32_t hi[2][8], lw[2][8];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            lv[t] = vs[t] == 0.f ? 0.f : fmaxf(__builtin_amdgcn_logf(ldexpf(vs[t], -ev)), -60.f);
+            if (vs[t] != vs[t]) lv[t] = vs[t];
+        }
+        const float c0 = lv[0] + 9.f - mu, c1 = lv[1] + 9.f - mu;
+        auto weights = [&](int t, int i) { // of tokens 2 i and 2 i + 1 of the lane's block
+            const float x = __builtin_amdgcn_exp2f(fmaf(s[t][2 * i], ks[t], t ? c1 : c0));
+            const float y = __builtin_amdgcn_exp2f(fmaf(s[t][2 * i + 1], ks[t], t ? c1 : c0));
+            sum[t] += x;
+            sum[t] += y;
+            split2_mix(x, y, hi[t][i], lw[t][i]);
+        };
+        auto pfrag = [&](const uint32_t (&x)[8], int j) {
+            return __builtin_bit_cast(half8_t, make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]));
+        };
+        auto vfrag = [&](int t, int k) { // k = ND j + d
+            return __builtin_bit_cast(half8_t, vf[buf][(((k % ND) * 2 + t) * 2 + k / ND) * 64 + lane]);
+        };
+        half8_t v = vfrag(0, 0);
+#pragma unroll
+        for (int i = 0; i < 8; i++) weights(0, i);
+        __builtin_amdgcn_sched_barrier(0);
+        // the second tile's exponentials run beside the first's V^T P^T
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int k = 0; k < 2 * ND; k++) {
+                const half8_t ahead = t && k == 2 * ND - 1 ? v : vfrag(k == 2 * ND - 1 ? 1 : t, (k + 1) % (2 * ND));
+                o[k % ND] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pfrag(hi[t], k / ND), o[k % ND], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4 / ND; i++)
+                    if (!t) weights(1, 8 / ND / 2 * k + i);
+                o[k % ND] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pfrag(lw[t], k / ND), o[k % ND], 0, 0, 0);
+                v = ahead;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        l += sum[0] * __builtin_amdgcn_exp2f(-9.f - lv[0]);
+        l += sum[1] * __builtin_amdgcn_exp2f(-9.f - lv[1]);
         __syncthreads();
     }
     l += __shfl_xor(l, 32, 64);
