@@ -7,39 +7,38 @@ namespace jev {
 
 namespace {
 
-constexpr int kPlanThreads = 1024;
-
-// Sum over the workgroup; every thread gets it.  `ws`: a 64-bit word per wave.
-template <int NT>
-__device__ __forceinline__ long long block_sum(long long v, long long *ws)
-{
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0;
-    for (int w = 0; w < NT / 64; w++) v += ws[w];
-    return v;
-}
-
-// Exclusive prefix sum over the workgroup's threads.  `ws`: a word per wave.
-template <int NT>
-__device__ __forceinline__ int block_scan(int v, int *ws)
+// Exclusive prefix sums over the workgroup's threads of N values at once, in
+// place, and their totals.  `ws`: N words per wave.
+template <int NT, int N, typename T>
+__device__ __forceinline__ void block_scan(T (&v)[N], T (&total)[N], T *ws)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int x = v;
+    T x[N];
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o, 64);
-        if (lane >= o) x += y;
+    for (int i = 0; i < N; i++) x[i] = v[i];
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1)
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const T y = __shfl_up(x[i], o, 64);
+            if (lane >= o) x[i] += y;
+        }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; i++)
+        if (lane == 63) ws[wave * N + i] = x[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        T before = 0;
+        total[i] = 0;
+        for (int w = 0; w < NT / 64; w++) {
+            const T y = ws[w * N + i];
+            before += w < wave ? y : 0;
+            total[i] += y;
+        }
+        v[i] = before + x[i] - v[i];
     }
-    __syncthreads();
-    if (lane == 63) ws[wave] = x;
-    __syncthreads();
-    int before = 0;
-    for (int w = 0; w < NT / 64; w++) before += w < wave ? ws[w] : 0;
-    return before + x - v;
 }
 
 // The last index b with prefix[b] <= i (prefix ascending, prefix[0] = 0, i < prefix[n]).
@@ -123,8 +122,8 @@ __device__ __forceinline__ void plan_lists(const Pages &p, const PagesPlanArgs &
     // Angles in 64 bits: a far position times a frequency keeps its fraction.
     // Once a plan, not once a layer and head: the library's 64-bit sine and
     // cosine are ~150 instructions.
-    for (int64_t i = i0; i < (int64_t)h.n_tokens * p.half; i += n) {
-        const int t = (int)(i / p.half), j = (int)(i % p.half), b = find(start, R, t);
+    for (int i = i0; i < h.n_tokens * p.half; i += n) { // (at most 2^22 tokens x 64)
+        const int t = i / p.half, j = i - t * p.half, b = find(start, R, t);
         double sn, cs;
         sincos((double)(p.req[b].past + t - start[b]) * p.freqs[j], &sn, &cs);
         p.angle[i] = make_double2(cs * p.mscale, sn * p.mscale);
@@ -144,13 +143,22 @@ __device__ __forceinline__ void plan_lists(const Pages &p, const PagesPlanArgs &
         }
     if (a.start)
         for (int b = i0; b <= a.n_requests; b += n) a.start[b] = R > 0 ? start[b] : 0;
-    if (a.table)
-        for (int64_t i = i0; i < (int64_t)a.n_requests * p.width; i += n) {
-            const int b = (int)(i / p.width), j = (int)(i % p.width);
-            int page = -1;
-            if (b < R && j < div_up(p.req[b].len, p.page)) page = p.table[(size_t)p.req[b].id * p.width + j];
-            a.table[i] = page;
-        }
+    if (a.table) // a wave to a row, four rows' loads in flight
+        for (int b0 = i0 >> 6; b0 < a.n_requests; b0 += 4 * (n >> 6))
+            for (int j = i0 & 63; j < p.width; j += 64) {
+                int page[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const int b = b0 + u * (n >> 6);
+                    page[u] = -1;
+                    if (b < R && j < div_up(p.req[b].len, p.page)) page[u] = p.table[(size_t)p.req[b].id * p.width + j];
+                }
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const int b = b0 + u * (n >> 6);
+                    if (b < a.n_requests) a.table[(size_t)b * p.width + j] = page[u];
+                }
+            }
 }
 
 } // namespace
@@ -160,25 +168,24 @@ __device__ __forceinline__ void plan_lists(const Pages &p, const PagesPlanArgs &
 // launch of its own, over the whole GPU).  Checks first: a plan that does not
 // fit changes nothing and plans no tokens.  Bounded by latency: a few trips to
 // memory, each of which every thread makes at once.
-template <bool LISTS>
-__global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(Pages p, PagesPlanArgs a)
+template <int NT, bool LISTS>
+__global__ __launch_bounds__(NT) void pages_plan_kernel(Pages p, PagesPlanArgs a)
 {
-    constexpr int NT = kPlanThreads, C = kPagesMaxRequests / NT;
-    __shared__ int px[4 * (kPagesMaxRequests + 1)];
+    constexpr int C = NT == 256 ? 4 : 8, S = NT * C + 1; // requests of a thread; entries of a prefix sum
+    __shared__ int px[4 * S];
     __shared__ unsigned seen[kPagesMaxRequests / 32];
-    __shared__ long long ws64[NT / 64];
-    __shared__ int ws[NT / 64];
+    __shared__ long long ws[5 * NT / 64];
     __shared__ int bad;
     const int tid = threadIdx.x, R = a.n_requests, per = div_up(R, NT);
-    constexpr int S = kPagesMaxRequests + 1;
     int *start = px, *need0 = px + S, *gone0 = px + 2 * S;
     for (int i = tid; i < kPagesMaxRequests / 32; i += NT) seen[i] = 0;
     if (tid == 0) bad = 0;
+    const int n_free = *p.n_free;
     __syncthreads();
 
     // the requests of this thread: b = tid * per + i
     int id[C], past[C], fresh[C], keep[C], need[C], own[C];
-    long long tokens = 0, more = 0, gone = 0;
+    long long sum[3] = {0, 0, 0}, all_of[3]; // tokens, pages taken, pages given back: 64 bits before they are checked
 #pragma unroll
     for (int i = 0; i < C; i++) {
         const int b = tid * per + i;
@@ -200,15 +207,12 @@ __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(Pages p, Pages
         own[i] = div_up(p.length[id[i]], p.page);
         keep[i] = div_up(past[i], p.page);
         need[i] = div_up(past[i] + fresh[i], p.page);
-        tokens += fresh[i];
-        more += need[i] - keep[i];
-        gone += own[i] - keep[i];
+        sum[0] += fresh[i];
+        sum[1] += need[i] - keep[i];
+        sum[2] += own[i] - keep[i];
     }
-    // 64-bit sums first: past them everything fits 32 bits
-    tokens = block_sum<NT>(tokens, ws64);
-    more = block_sum<NT>(more, ws64);
-    gone = block_sum<NT>(gone, ws64);
-    const int n_free = *p.n_free;
+    block_scan<NT, 3>(sum, all_of, ws);
+    const long long tokens = all_of[0], more = all_of[1], gone = all_of[2];
     const int status = bad || tokens > a.n_tokens ? JEV_EINVAL : more > n_free + gone ? JEV_ENOMEM : JEV_OK;
     if (status != JEV_OK) {
         PagesPlanHead h = {status, 0, 0, 0, 0, 0, 0, 0, 0};
@@ -217,17 +221,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(Pages p, Pages
         return;
     }
 
-    // exclusive sums over the batch of the tokens, the pages taken and given back
-    int s0 = 0, s1 = 0, s2 = 0;
-#pragma unroll
-    for (int i = 0; i < C; i++) {
-        s0 += fresh[i];
-        s1 += need[i] - keep[i];
-        s2 += own[i] - keep[i];
-    }
-    s0 = block_scan<NT>(s0, ws);
-    s1 = block_scan<NT>(s1, ws);
-    s2 = block_scan<NT>(s2, ws);
+    int s0 = (int)sum[0], s1 = (int)sum[1], s2 = (int)sum[2];
 #pragma unroll
     for (int i = 0; i < C; i++) {
         const int b = tid * per + i;
@@ -261,7 +255,9 @@ __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(Pages p, Pages
         auto word = [&](int w) { return __hip_atomic_load(&p.used[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
         int n = 0;
         for (int w = w0; w < w1; w++) n += __popc(~word(w));
-        int rank = block_scan<NT>(n, ws);
+        int rank_of[1] = {n}, free_of[1];
+        block_scan<NT, 1>(rank_of, free_of, (int *)ws);
+        int rank = rank_of[0];
         for (int w = w0; w < w1 && rank < (int)more; w++) {
             uint32_t u = word(w);
             for (; ~u && rank < (int)more; rank++) {
@@ -283,16 +279,16 @@ __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(Pages p, Pages
     int *unit0 = px + S, *item0 = px + 2 * S, *wide0 = px + 3 * S;
     int wide_keys = kPagesWideKeys;
     if (a.wide) {
-        long long keys = 0, tiles = 0;
+        long long of[2] = {0, 0}, total[2]; // keys over the tiles, tiles
 #pragma unroll
         for (int i = 0; i < C; i++)
             if (is_wide(p, fresh[i], 1)) {
                 const int n = div_up(fresh[i] * p.group, kPagesWideRows);
-                tiles += n;
-                keys += (long long)n * (past[i] + fresh[i]);
+                of[0] += (long long)n * (past[i] + fresh[i]);
+                of[1] += n;
             }
-        keys = block_sum<NT>(keys, ws64);
-        tiles = block_sum<NT>(tiles, ws64);
+        block_scan<NT, 2>(of, total, ws);
+        const long long keys = total[0], tiles = total[1];
         // a tile's last part may be short: with keys / room of them each there are
         // at most room + tiles parts, one round; many tiles split only where one
         // is twice as long as their mean
@@ -311,14 +307,9 @@ __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(Pages p, Pages
         n0[4] += c[i].wide_parts;
     }
     int all_n[5];
-#pragma unroll
-    for (int i = 0; i < 5; i++) {
-        const int v = n0[i];
-        n0[i] = (i == 2 || i == 4) && !a.wide ? 0 : block_scan<NT>(v, ws);
-        all_n[i] = n0[i] + v;
-    }
+    block_scan<NT, 5>(n0, all_n, (int *)ws);
     __shared__ PagesPlanHead all;
-    if (tid == NT - 1) {
+    if (tid == 0) {
         PagesPlanHead h = {JEV_OK, (int)tokens, all_n[0], all_n[1], all_n[2], all_n[3], all_n[4], R, 0};
         all = h;
         *p.head = h;
@@ -347,8 +338,8 @@ __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(Pages p, Pages
     __syncthreads();
     if (LISTS) plan_lists(p, a, all, px, S, tid, NT);
     else
-        for (int i = tid; i < 4 * S; i += NT)
-            if (i % S <= R) p.prefix[i] = px[i];
+        for (int j = 0; j < 4; j++)
+            for (int i = tid; i <= R; i += NT) p.prefix[j * (kPagesMaxRequests + 1) + i] = px[j * S + i];
 }
 
 __global__ __launch_bounds__(256) void pages_lists_kernel(Pages p, PagesPlanArgs a)
@@ -369,13 +360,12 @@ hipError_t launch_pages_plan(const Pages &p, const PagesPlanArgs &a, hipStream_t
         return hipErrorInvalidValue;
     // what the lists write, in words; an angle counts for several
     const double work = (double)a.n_tokens * (4 + 8.0 * p.half) + (a.table ? (double)a.n_requests * p.width : 0.0);
-    if (work <= 16384) {
-        hipLaunchKernelGGL(pages_plan_kernel<true>, dim3(1), dim3(kPlanThreads), 0, s, p, a);
-    } else {
-        hipLaunchKernelGGL(pages_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0, s, p, a);
-        const int wgs = (int)fmin(1024.0, ceil(work / 2048));
-        hipLaunchKernelGGL(pages_lists_kernel, dim3(wgs), dim3(256), 0, s, p, a);
-    }
+    const bool lists = work <= 6144, small = a.n_requests <= 256; // a request to a thread, else up to eight
+    if (small && lists) hipLaunchKernelGGL((pages_plan_kernel<256, true>), dim3(1), dim3(256), 0, s, p, a);
+    else if (small) hipLaunchKernelGGL((pages_plan_kernel<256, false>), dim3(1), dim3(256), 0, s, p, a);
+    else if (lists) hipLaunchKernelGGL((pages_plan_kernel<512, true>), dim3(1), dim3(512), 0, s, p, a);
+    else hipLaunchKernelGGL((pages_plan_kernel<512, false>), dim3(1), dim3(512), 0, s, p, a);
+    if (!lists) hipLaunchKernelGGL(pages_lists_kernel, dim3((int)fmin(1024.0, ceil(work / 512))), dim3(256), 0, s, p, a);
     return hipGetLastError();
 }
 
