@@ -450,6 +450,9 @@ struct PagesRequest { // one batch row
     int32_t part0, n_parts;       // partial results of its tiles, when split (n_parts > 1)
     int32_t wide;                 // its tiles are wide ones
 };
+struct PagesUnit { // new tokens of one block: their first row and position, how many, page * blocks of a page + block
+    int32_t row, pos, n, block;
+};
 struct PagesItem { // a workgroup's tile and keys, with its request's fields: one load away
     int32_t row0, key0, key1, part; // part >= 0: where its partial result goes
     int32_t id, past, len, start;
@@ -477,7 +480,7 @@ struct Pages {
     PagesRequest *req = nullptr;            // [n_requests]
     int32_t *fresh_pages = nullptr;         // pages taken, by rank
     int32_t *prefix = nullptr;              // [4][max_requests + 1]: tokens, units, items, wide items before a batch row
-    int2 *unit = nullptr;                   // (batch row, block)
+    PagesUnit *unit = nullptr;
     PagesItem *item = nullptr, *wide = nullptr;
     double2 *angle = nullptr;               // [max_tokens][half] (cos, sin) * mscale
     const double *freqs = nullptr;

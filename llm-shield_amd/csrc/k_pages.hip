@@ -95,7 +95,12 @@ __device__ __forceinline__ void plan_lists(const Pages &p, const PagesPlanArgs &
     const int *start = px, *unit0 = px + stride, *item0 = px + 2 * stride, *wide0 = px + 3 * stride;
     for (int u = i0; u < h.n_units; u += n) {
         const int b = find(unit0, R, u);
-        p.unit[u] = make_int2(b, p.req[b].past / kPageBlock + u - unit0[b]);
+        const PagesRequest r = p.req[b];
+        const int block = r.past / kPageBlock + u - unit0[b], pos = max(r.past, block * kPageBlock);
+        const int page = p.table[(size_t)r.id * p.width + (block >> p.sub_shift)];
+        const PagesUnit un = {r.start + pos - r.past, pos, min(r.len, (block + 1) * kPageBlock) - pos,
+                              (page << p.sub_shift) + (block & (p.sub - 1))};
+        p.unit[u] = un;
     }
     for (int i = i0; i < h.n_items; i += n) {
         const int b = find(item0, R, i), k = i - item0[b];
@@ -481,11 +486,9 @@ __global__ __launch_bounds__(256) void pages_store_kernel(Pages p, PagesStoreArg
     __shared__ __align__(16) uint8_t code[2][BYTES];
     __shared__ unsigned most[2];
     const int tid = threadIdx.x, j = tid & 15, h = blockIdx.y;
-    if ((int)blockIdx.x >= p.head->n_units) return;
-    const int2 un = p.unit[blockIdx.x];
-    const PagesRequest r = p.req[un.x];
-    const int pos0 = max(r.past, un.y * kPageBlock), pos1 = min(r.len, (un.y + 1) * kPageBlock);
-    const int n = pos1 - pos0, row0 = r.start + pos0 - r.past, off = pos0 & (kPageBlock - 1);
+    const PagesUnit un = p.unit[blockIdx.x];
+    if ((int)blockIdx.x >= p.head->n_units) return; // (the unit's load does not wait for this)
+    const int pos0 = un.pos, n = un.n, row0 = un.row, off = pos0 & (kPageBlock - 1);
     const bool kv = a.k != nullptr;
     const RowPairs<HD> e(p, j);
 
@@ -495,8 +498,8 @@ __global__ __launch_bounds__(256) void pages_store_kernel(Pages p, PagesStoreArg
     const bool mine = t < n;
 
     // where the block lies
-    const int page = p.table[(size_t)r.id * p.width + un.y / p.sub];
-    const size_t block = ((size_t)page * p.n_kv + h) * p.sub + un.y % p.sub + (size_t)a.layer * p.n_blocks();
+    const size_t block = ((((size_t)(un.block >> p.sub_shift) * p.n_kv + h) << p.sub_shift) | (un.block & (p.sub - 1))) +
+                         (size_t)a.layer * p.n_blocks();
     const bool begun = kv && off > 0;
     float2 s_old = make_float2(0.f, 0.f);
     if (kv) {
