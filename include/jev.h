@@ -309,22 +309,26 @@ int jev_get_matmul_strategy(void);
  * its block read as NaN until the block is begun anew.
  *
  * A step is: jev_pages_plan_device once, then per layer jev_pages_store_device
- * and jev_pages_attend_device (jev_forward_pages: a whole model step).  Every
- * call only enqueues on the handle's stream and allocates nothing, so a step
- * can be captured into a HIP graph and replayed with other lengths in the same
- * arrays; the lengths and tables stay on the device.  The stream
- * (jev_pages_stream) orders itself with the device's null stream; a caller on
- * another stream orders the two with events.  A handle's calls share its
- * workspaces: one thread at a time, and no two of its graphs at once.  Pointers
- * are device pointers of the handle's device; floats may have any 4-byte
- * alignment (16 bytes: vector accesses, the same bits).  */
+ * and jev_pages_attend_device (jev_forward_pages: a whole model step).  The
+ * *_device calls only enqueue on the handle's stream and allocate nothing, so a
+ * step can be captured into a HIP graph and replayed with other lengths in the
+ * same arrays; the lengths and tables stay on the device.  Nothing checks that
+ * a planned token was stored before it is attended or read: it has whatever its
+ * page held.  The stream (jev_pages_stream) orders itself with the device's null
+ * stream; a caller on another stream orders the two with events.  A handle's
+ * calls share its workspaces: one thread at a time, and no two of its graphs at
+ * once.  Pointers are device pointers of the handle's device; floats may have
+ * any 4-byte alignment (the result bits are the same).  */
 typedef struct jev_pages jev_pages;
 typedef struct jev_pages_config {
-    int32_t n_pages;      /* of the pool; n_pages * page_tokens < 2^31          */
+    int32_t n_pages;      /* of the pool; n_pages * page_tokens < 2^31.  Their
+                             bytes: 2 x layers x KV heads x head_dim a token,
+                             and 8 x layers x KV heads a block                  */
     int32_t page_tokens;  /* 16, 32, 64, 128 or 256                             */
     int32_t max_requests; /* rows of the page table, at most 4096               */
     int32_t max_context;  /* tokens of one request, at most 2^24                */
-    int32_t max_tokens;   /* tokens of one plan, at most 2^22                   */
+    int32_t max_tokens;   /* tokens of one plan, at most 2^22, and times the
+                             query heads of a KV head at most 2^28              */
     int32_t rope_half;    /* rotated pairs: 0 (2i, 2i + 1) as the model's Rope,
                              1 (i, i + rope_dim / 2)                            */
 } jev_pages_config;
@@ -367,8 +371,9 @@ int jev_pages_store_device(jev_pages *p, int32_t layer, const float *q, int64_t 
 /* out = softmax(q . K / sqrt(head_dim)) . V of every planned token over its
  * request's stored tokens up to and with itself; query head h reads KV head
  * h / (n_heads / n_kv_heads).  q and out are [n_tokens][n_heads * head_dim] and
- * must not overlap.  A token's result has the same bits whatever else is in the
- * batch as long as its request adds few tokens: fresh * heads per KV head <= 16. */
+ * must not overlap; rows past the planned total stay as they were.  A token's
+ * result has the same bits whatever else is in the batch where its request adds
+ * one token, or few: fresh * heads per KV head <= 16. */
 int jev_pages_attend_device(jev_pages *p, int32_t layer, const float *q, float *out);
 
 /* k, v [n][n_kv_heads][head_dim] = the values stored at n slots of a layer

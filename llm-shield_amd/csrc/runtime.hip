@@ -14,7 +14,9 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <memory>
 #include <mutex>
+#include <new>
 #include <optional>
 #include <string>
 #include <thread>
@@ -2664,7 +2666,7 @@ int pages_status(jev_pages *h, hipStream_t s)
 extern "C" {
 
 int jev_pages_create(const jev_config *model, const jev_pages_config *cfg, int device, jev_pages **out)
-{
+try {
     if (!out) return fail(JEV_EINVAL, "out is null");
     *out = nullptr;
     if (!model || !cfg) return fail(JEV_EINVAL, "null argument");
@@ -2697,14 +2699,13 @@ int jev_pages_create(const jev_config *model, const jev_pages_config *cfg, int d
     if (device < 0 || device >= ndev) return fail(JEV_EINVAL, "device %d of %d", device, ndev);
     HIP_TRY(hipSetDevice(device));
 
-    jev_pages *h = new jev_pages;
+    std::unique_ptr<jev_pages, decltype(&jev_pages_destroy)> own(new jev_pages, jev_pages_destroy);
+    jev_pages *h = own.get();
     h->cfg = f;
     h->device = device;
+    h->blocks.reserve(32); // (an allocation is never lost to a failing push)
     e = hipStreamCreate(&h->stream);
-    if (e != hipSuccess) {
-        delete h;
-        return fail(JEV_EDEVICE, "stream: %s", hipGetErrorString(e));
-    }
+    if (e != hipSuccess) return fail(JEV_EDEVICE, "stream: %s", hipGetErrorString(e));
     Pages &p = h->p;
     p.n_layers = f.n_layers;
     p.n_heads = f.n_heads;
@@ -2774,22 +2775,19 @@ int jev_pages_create(const jev_config *model, const jev_pages_config *cfg, int d
         if (e == hipSuccess) e = hipMemcpy(p.n_free, &p.n_pages, sizeof(int32_t), hipMemcpyHostToDevice);
         if (e != hipSuccess) rc = fail(JEV_EDEVICE, "paged cache: %s", hipGetErrorString(e));
     }
-    if (rc) {
-        std::string msg = g_error;
-        jev_pages_destroy(h);
-        return fail(rc, "%s", msg.c_str());
-    }
-    *out = h;
-    return JEV_OK;
+    if (!rc) *out = own.release();
+    return rc;
+} catch (const std::bad_alloc &) {
+    return fail(JEV_ENOMEM, "no host memory for a paged cache");
 }
 
 void jev_pages_destroy(jev_pages *h)
 {
     if (!h) return;
     (void)hipSetDevice(h->device);
-    (void)hipStreamSynchronize(h->stream);
+    if (h->stream) (void)hipStreamSynchronize(h->stream);
     for (void *b : h->blocks) (void)hipFree(b);
-    (void)hipStreamDestroy(h->stream);
+    if (h->stream) (void)hipStreamDestroy(h->stream);
     delete h;
 }
 
@@ -2889,7 +2887,7 @@ void *jev_pages_stream(jev_pages *h) { return h ? (void *)h->stream : nullptr; }
 int jev_forward_pages(jev_ctx *c, jev_pages *h, const int32_t *request, const int32_t *past, const int32_t *fresh,
                       int32_t n_requests, const int32_t *tokens, int32_t n_tokens, int mode, const int32_t *rows,
                       int32_t n_rows, float *out, size_t out_len)
-{
+try {
     int rc = check_ready(c);
     if (rc) return rc;
     if (!h) return fail(JEV_EINVAL, "null paged cache");
@@ -2974,6 +2972,9 @@ int jev_forward_pages(jev_ctx *c, jev_pages *h, const int32_t *request, const in
     else (void)hipStreamSynchronize(c->stream);
     if (!rc && call.cancelled()) rc = fail(JEV_ECANCELED, "the forward pass was cancelled");
     return rc ? rc : pages_status(h, c->stream);
+} catch (const std::bad_alloc &) {
+    if (c) (void)hipStreamSynchronize(c->stream);
+    return fail(JEV_ENOMEM, "no host memory for a step over pages");
 }
 
 } // extern "C"

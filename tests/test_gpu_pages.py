@@ -412,6 +412,24 @@ def test_single_tokens_do_not_depend_on_the_batch(gpu, rs):
     np.testing.assert_array_equal(rig.attend(x[0])[800], together[3])
 
 
+@pytest.mark.parametrize("fresh", [1, 60])
+def test_parts_of_an_earlier_call_are_not_seen(gpu, rs, fresh):
+    """Split tiles' partial results, whose places every call uses again, with other queries each time."""
+    rig = Rig(cfg(8, 2, 128), 1300, 16, 3, 9100, 20000)
+    rig.fill(rs, [0, 1, 2], [9000, 3000, 1030])
+    rig.fill(rs, [0, 1, 2], [fresh] * 3)
+    q = [rs.randn(3 * fresh, 8, 128).astype(np.float32) * s for s in (1, 3, 0.1)]
+    first = [rig.attend(x) for x in q]
+    dq = [rig.dev(x) for x in q]
+    out = [rig.t.empty_like(dq[0]) for _ in range(60)]
+    rig.t.cuda.synchronize()
+    for i in range(60):
+        rig.p.attend_device(0, dq[i % 3].data_ptr(), out[i].data_ptr())
+    rig.p.sync()
+    for i in range(60):
+        np.testing.assert_array_equal(out[i].cpu().numpy(), first[i % 3])
+
+
 def test_two_caches_at_once(gpu, rs):
     """Handles have their own streams and workspaces."""
     rigs = [Rig(cfg(8, 2, 128), 200, 16, 4, 800) for _ in range(2)]

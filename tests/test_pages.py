@@ -17,7 +17,7 @@ from jev import _lib as L
     (dict(rope_scale_factor=0.0), {}), (dict(rope_scale_factor=float("nan")), {}),
     ({}, dict(page_tokens=8)), ({}, dict(page_tokens=48)), ({}, dict(page_tokens=512)), ({}, dict(n_pages=0)), ({}, dict(n_pages=1 << 27)),
     ({}, dict(max_requests=0)), ({}, dict(max_requests=4097)), ({}, dict(max_context=0)), ({}, dict(max_context=(1 << 24) + 1)),
-    ({}, dict(max_tokens=0)), ({}, dict(max_tokens=(1 << 22) + 1)), ({}, dict(rope_half=2))])
+    (dict(n_heads=1024, n_kv_heads=1), dict(max_tokens=(1 << 18) + 1)), ({}, dict(max_tokens=0)), ({}, dict(max_tokens=(1 << 22) + 1)), ({}, dict(rope_half=2))])
 def test_create_refuses_before_touching_a_device(model, kw):
     c = L.PagesConfig(**{**dict(n_pages=10, page_tokens=16, max_requests=2, max_context=100, max_tokens=100, rope_half=0), **kw})
     h = ctypes.c_void_p()
