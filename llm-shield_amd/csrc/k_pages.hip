@@ -7,6 +7,25 @@ namespace jev {
 
 namespace {
 
+// Kernels take what they need of a cache and a call (the layer's base in the
+// pointers) instead of all of it: a launch costs by its arguments' bytes (an empty
+// kernel's with 400 of them 3.8 us, with 16 2.8; the attention's call 3.5 -> 3.4),
+// and one or two launches are all there is to a small step's layer.
+struct PlanView {
+    int32_t *table, *length, *n_free, *fresh_pages, *prefix;
+    uint32_t *used;
+    PagesPlanHead *head;
+    PagesRequest *req;
+    PagesUnit *unit;
+    PagesItem *item, *wide;
+    double2 *angle;
+    const double *freqs;
+    double mscale;
+    int page, sub, sub_shift, n_pages, max_requests, max_context, width, half, group, n_kv;
+};
+template <typename T>
+T *layer_of(const Pages &p, T *base, int layer, size_t per_block) { return base + layer * p.n_blocks() * per_block; }
+
 // Exclusive prefix sums over the workgroup's threads of N values at once, in
 // place, and their totals.  `ws`: N words per wave.
 template <int NT, int N, typename T>
@@ -60,11 +79,11 @@ __device__ __forceinline__ int div_up(int a, int b) { return (a + b - 1) / b; }
 struct Counts {
     int units, items, wides, parts, wide_parts, n_parts, wide;
 };
-__device__ __forceinline__ bool is_wide(const Pages &p, int fresh, int wide)
+__device__ __forceinline__ bool is_wide(const PlanView &p, int fresh, int wide)
 {
     return wide && div_up(fresh * p.group, kPagesTileRows) > div_up(p.group, kPagesTileRows);
 }
-__device__ __forceinline__ Counts counts(const Pages &p, int past, int fresh, int wide, int wide_keys)
+__device__ __forceinline__ Counts counts(const PlanView &p, int past, int fresh, int wide, int wide_keys)
 {
     Counts c = {0, 0, 0, 0, 0, 1, 0};
     if (fresh <= 0) return c;
@@ -88,7 +107,7 @@ __device__ __forceinline__ Counts counts(const Pages &p, int past, int fresh, in
 // number `i0`: the blocks to store, the attention's workgroups, the angles, and
 // what the caller asked for.  px: tokens, units, items and wide items before
 // each batch row (`stride` apart), R + 1 entries each.
-__device__ __forceinline__ void plan_lists(const Pages &p, const PagesPlanArgs &a, const PagesPlanHead &h, const int *px,
+__device__ __forceinline__ void plan_lists(const PlanView &p, const PagesPlanArgs &a, const PagesPlanHead &h, const int *px,
                                            int stride, int i0, int n)
 {
     const int R = h.n_requests;
@@ -174,7 +193,7 @@ __device__ __forceinline__ void plan_lists(const Pages &p, const PagesPlanArgs &
 // fit changes nothing and plans no tokens.  Bounded by latency: a few trips to
 // memory, each of which every thread makes at once.
 template <int NT, bool LISTS>
-__global__ __launch_bounds__(NT) void pages_plan_kernel(Pages p, PagesPlanArgs a)
+__global__ __launch_bounds__(NT) void pages_plan_kernel(PlanView p, PagesPlanArgs a)
 {
     constexpr int C = NT == 256 ? 4 : 8, S = NT * C + 1; // requests of a thread; entries of a prefix sum
     __shared__ int px[4 * S];
@@ -347,7 +366,7 @@ __global__ __launch_bounds__(NT) void pages_plan_kernel(Pages p, PagesPlanArgs a
             for (int i = tid; i <= R; i += NT) p.prefix[j * (kPagesMaxRequests + 1) + i] = px[j * S + i];
 }
 
-__global__ __launch_bounds__(256) void pages_lists_kernel(Pages p, PagesPlanArgs a)
+__global__ __launch_bounds__(256) void pages_lists_kernel(PlanView p, PagesPlanArgs a)
 {
     constexpr int S = kPagesMaxRequests + 1;
     __shared__ int px[4 * S];
@@ -363,14 +382,16 @@ hipError_t launch_pages_plan(const Pages &p, const PagesPlanArgs &a, hipStream_t
 {
     if (a.n_requests < 0 || a.n_requests > p.max_requests || a.n_tokens < 0 || a.n_tokens > p.max_tokens)
         return hipErrorInvalidValue;
+    const PlanView v = {p.table, p.length, p.n_free, p.fresh_pages, p.prefix, p.used, p.head, p.req, p.unit, p.item, p.wide, p.angle, p.freqs,
+                        p.mscale, p.page, p.sub, p.sub_shift, p.n_pages, p.max_requests, p.max_context, p.width, p.half, p.group, p.n_kv};
     // what the lists write, in words; an angle counts for several
     const double work = (double)a.n_tokens * (4 + 8.0 * p.half) + (a.table ? (double)a.n_requests * p.width : 0.0);
     const bool lists = work <= 6144, small = a.n_requests <= 256; // a request to a thread, else up to eight
-    if (small && lists) hipLaunchKernelGGL((pages_plan_kernel<256, true>), dim3(1), dim3(256), 0, s, p, a);
-    else if (small) hipLaunchKernelGGL((pages_plan_kernel<256, false>), dim3(1), dim3(256), 0, s, p, a);
-    else if (lists) hipLaunchKernelGGL((pages_plan_kernel<512, true>), dim3(1), dim3(512), 0, s, p, a);
-    else hipLaunchKernelGGL((pages_plan_kernel<512, false>), dim3(1), dim3(512), 0, s, p, a);
-    if (!lists) hipLaunchKernelGGL(pages_lists_kernel, dim3((int)fmin(1024.0, ceil(work / 512))), dim3(256), 0, s, p, a);
+    if (small && lists) hipLaunchKernelGGL((pages_plan_kernel<256, true>), dim3(1), dim3(256), 0, s, v, a);
+    else if (small) hipLaunchKernelGGL((pages_plan_kernel<256, false>), dim3(1), dim3(256), 0, s, v, a);
+    else if (lists) hipLaunchKernelGGL((pages_plan_kernel<512, true>), dim3(1), dim3(512), 0, s, v, a);
+    else hipLaunchKernelGGL((pages_plan_kernel<512, false>), dim3(1), dim3(512), 0, s, v, a);
+    if (!lists) hipLaunchKernelGGL(pages_lists_kernel, dim3((int)fmin(1024.0, ceil(work / 512))), dim3(256), 0, s, v, a);
     return hipGetLastError();
 }
 
@@ -385,7 +406,8 @@ template <int HD>
 struct RowPairs {
     static constexpr int NP = HD / 32;
     int e0[NP], e1[NP];
-    __device__ __forceinline__ RowPairs(const Pages &p, int j)
+    template <typename View>
+    __device__ __forceinline__ RowPairs(const View &p, int j)
     {
 #pragma unroll
         for (int i = 0; i < NP; i++) {
@@ -470,6 +492,22 @@ __device__ __forceinline__ int v_at(int t, int d) { return d * 16 + t; }
 
 } // namespace
 
+namespace {
+struct StoreView {
+    uint8_t *k, *v;
+    float2 *ks;
+    const PagesPlanHead *head;
+    const PagesUnit *unit;
+    const double2 *angle;
+    const float *q, *k_in, *v_in;
+    float *q_out;
+    int64_t q_ld, kv_ld;
+    size_t in_stride;
+    int nin, n_kv, n_heads, group, sub, sub_shift, half, rope_half, orig_ctx;
+    float temp_scale;
+};
+} // namespace
+
 // One workgroup per block that the batch touches and KV head: the block's new
 // tokens' queries (of the head's group) rotated, their keys rotated and stored,
 // their values stored.  Sixteen threads hold a token's row, and keep to one
@@ -480,7 +518,7 @@ __device__ __forceinline__ int v_at(int t, int d) { return d * 16 + t; }
 // already holds are then rounded to the new one.  Bounded by memory: 4 B in per
 // element, 1 B (K, V) or 4 B (q) out.
 template <int HD, bool VEC>
-__global__ __launch_bounds__(256) void pages_store_kernel(Pages p, PagesStoreArgs a)
+__global__ __launch_bounds__(256) void pages_store_kernel(StoreView p)
 {
     constexpr int NP = HD / 32, BYTES = kPageBlock * HD, RING = 2;
     __shared__ __align__(16) uint8_t code[2][BYTES];
@@ -489,17 +527,16 @@ __global__ __launch_bounds__(256) void pages_store_kernel(Pages p, PagesStoreArg
     const PagesUnit un = p.unit[blockIdx.x];
     if ((int)blockIdx.x >= p.head->n_units) return; // (the unit's load does not wait for this)
     const int pos0 = un.pos, n = un.n, row0 = un.row, off = pos0 & (kPageBlock - 1);
-    const bool kv = a.k != nullptr;
+    const bool kv = p.k_in != nullptr;
     const RowPairs<HD> e(p, j);
 
     // this thread's token, and its rows: K (-2), V (-1), then the group's queries
     const int nt = n > 8 ? 16 : n > 4 ? 8 : n > 2 ? 4 : n, step = 16 / nt; // (nt: 1, 2, 4, 8, 16)
-    const int t = (tid >> 4) % nt, row = row0 + t, first = (kv ? -2 : 0) + (tid >> 4) / nt, end = t < n && a.q ? p.group : 0;
+    const int t = (tid >> 4) % nt, row = row0 + t, first = (kv ? -2 : 0) + (tid >> 4) / nt, end = t < n && p.q ? p.group : 0;
     const bool mine = t < n;
 
     // where the block lies
-    const size_t block = ((((size_t)(un.block >> p.sub_shift) * p.n_kv + h) << p.sub_shift) | (un.block & (p.sub - 1))) +
-                         (size_t)a.layer * p.n_blocks();
+    const size_t block = ((((size_t)(un.block >> p.sub_shift) * p.n_kv + h) << p.sub_shift) | (un.block & (p.sub - 1)));
     const bool begun = kv && off > 0;
     float2 s_old = make_float2(0.f, 0.f);
     if (kv) {
@@ -520,13 +557,13 @@ __global__ __launch_bounds__(256) void pages_store_kernel(Pages p, PagesStoreArg
         g[c] = mine && q < p.half ? p.angle[(size_t)row * p.half + q] : make_double2(0.0, 0.0);
     }
     auto load = [&](int which, float2 (&y)[NP]) {
-        const float *src = which == -2 ? a.k + row * a.kv_ld + h * HD
-                           : which == -1 ? a.v + row * a.kv_ld + h * HD
-                                         : a.q + row * a.q_ld + (size_t)(h * p.group + which) * HD;
+        const float *src = which == -2 ? p.k_in + row * p.kv_ld + h * HD
+                           : which == -1 ? p.v_in + row * p.kv_ld + h * HD
+                                         : p.q + row * p.q_ld + (size_t)(h * p.group + which) * HD;
         load_pairs<HD, VEC>(e, src, y);
-        for (int z = 1; z < a.nin; z++) {
+        for (int z = 1; z < p.nin; z++) {
             float2 w[NP];
-            load_pairs<HD, VEC>(e, src + z * a.in_stride, w);
+            load_pairs<HD, VEC>(e, src + z * p.in_stride, w);
 #pragma unroll
             for (int c = 0; c < NP; c++) y[c] = make_float2(y[c].x + w[c].x, y[c].y + w[c].y);
         }
@@ -577,7 +614,7 @@ __global__ __launch_bounds__(256) void pages_store_kernel(Pages p, PagesStoreArg
             for (int i = 0; i < RING; i++)
                 if (w + i * step < end) {
                     rotate(f, y[i]);
-                    store_pairs<HD, VEC>(e, a.q_out + ((size_t)row * p.n_heads + h * p.group + w + i * step) * HD, y[i]);
+                    store_pairs<HD, VEC>(e, p.q_out + ((size_t)row * p.n_heads + h * p.group + w + i * step) * HD, y[i]);
                 }
         }
     }
@@ -650,11 +687,15 @@ hipError_t launch_pages_store(const Pages &p, const PagesStoreArgs &a, hipStream
     // thread with pairs on both sides of the rotated part's end
     const bool v = vec(a.q, a.q_ld) && vec(a.k, a.kv_ld) && vec(a.v, a.kv_ld) && vec(a.q_out, 0) && a.in_stride % np == 0 &&
                    (!p.rope_half || p.half % np == 0);
+    const size_t bytes = (size_t)kPageBlock * p.hd;
+    const StoreView view = {layer_of(p, p.k, a.layer, bytes), layer_of(p, p.v, a.layer, bytes), layer_of(p, p.ks, a.layer, 1), p.head, p.unit,
+                            p.angle, a.q, a.k, a.v, a.q_out, a.q_ld, a.kv_ld, a.in_stride, a.nin, p.n_kv, p.n_heads, p.group,
+                            p.sub, p.sub_shift, p.half, p.rope_half, p.orig_ctx, p.temp_scale};
     const dim3 grid(units, p.n_kv);
-    if (p.hd == 128 && v) hipLaunchKernelGGL((pages_store_kernel<128, true>), grid, dim3(256), 0, s, p, a);
-    else if (p.hd == 128) hipLaunchKernelGGL((pages_store_kernel<128, false>), grid, dim3(256), 0, s, p, a);
-    else if (v) hipLaunchKernelGGL((pages_store_kernel<64, true>), grid, dim3(256), 0, s, p, a);
-    else hipLaunchKernelGGL((pages_store_kernel<64, false>), grid, dim3(256), 0, s, p, a);
+    if (p.hd == 128 && v) hipLaunchKernelGGL((pages_store_kernel<128, true>), grid, dim3(256), 0, s, view);
+    else if (p.hd == 128) hipLaunchKernelGGL((pages_store_kernel<128, false>), grid, dim3(256), 0, s, view);
+    else if (v) hipLaunchKernelGGL((pages_store_kernel<64, true>), grid, dim3(256), 0, s, view);
+    else hipLaunchKernelGGL((pages_store_kernel<64, false>), grid, dim3(256), 0, s, view);
     return hipGetLastError();
 }
 
@@ -769,6 +810,23 @@ __device__ __forceinline__ void merge_parts(At at, int n_parts, float *dst, int 
 
 } // namespace
 
+namespace {
+struct AttendView {
+    const uint8_t *k, *v;
+    const float2 *ks;
+    const int32_t *table;
+    const PagesPlanHead *head;
+    const PagesItem *item, *wide;
+    float *part, *wide_part;
+    int32_t *tickets, *wide_tickets;
+    const float *q;
+    float *out;
+    int n_kv, n_heads, group, sub, sub_shift, width;
+    float scale;
+    int wides, tiles; // workgroups of each kind
+};
+} // namespace
+
 // Sixteen (token, head) rows of a request and KV head over keys [key0, key1) of
 // its pages; the four waves take 64 keys (four blocks) in turn and merge at the
 // end.  S^T = K Q^T: with the rows of the K operand (token i, block b) dealt so
@@ -789,7 +847,7 @@ struct TileLds {
     int last;
 };
 template <int HD>
-__device__ __forceinline__ void attend_tiles(const Pages &p, const PagesAttendArgs &a, TileLds<HD> &lds, int first, int count)
+__device__ __forceinline__ void attend_tiles(const AttendView &p, TileLds<HD> &lds, int first, int count)
 {
     constexpr int NJ = HD / 64, NS = HD / 16, BYTES = kPageBlock * HD, LD = HD + 4;
     auto &lo = lds.lo;
@@ -797,9 +855,9 @@ __device__ __forceinline__ void attend_tiles(const Pages &p, const PagesAttendAr
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, n = lane & 15, h = first % p.n_kv;
     const int n_items = p.head->n_items, stride = count / p.n_kv;
-    const uint8_t *kbase = p.k + (size_t)a.layer * p.n_blocks() * BYTES;
-    const uint8_t *vbase = p.v + (size_t)a.layer * p.n_blocks() * BYTES;
-    const float2 *sbase = p.ks + (size_t)a.layer * p.n_blocks();
+    const uint8_t *kbase = p.k;
+    const uint8_t *vbase = p.v;
+    const float2 *sbase = p.ks;
 
     for (int item = first / p.n_kv; item < n_items; item += stride) {
         const PagesItem it = p.item[item], &r = it;
@@ -847,7 +905,7 @@ __device__ __forceinline__ void attend_tiles(const Pages &p, const PagesAttendAr
         half8_t qh[2 * NJ], ql[2 * NJ];
         float qs;
         {
-            const float *src = a.q + ((size_t)(r.start + token) * p.n_heads + head) * HD + 16 * g;
+            const float *src = p.q + ((size_t)(r.start + token) * p.n_heads + head) * HD + 16 * g;
             float x[2 * NJ][8], m = 0.f;
 #pragma unroll
             for (int c = 0; c < 2 * NJ; c++)
@@ -992,7 +1050,7 @@ __device__ __forceinline__ void attend_tiles(const Pages &p, const PagesAttendAr
             }
             if (it.part < 0) {
                 const int tk = rr / p.group, hd = h * p.group + rr % p.group;
-                float *dst = a.out + ((size_t)(r.start + tk) * p.n_heads + hd) * HD + d;
+                float *dst = p.out + ((size_t)(r.start + tk) * p.n_heads + hd) * HD + d;
                 const float inv = 1.f / sum;
 #pragma unroll
                 for (int k = 0; k < 4; k++) dst[k] = x[k] * inv;
@@ -1011,7 +1069,7 @@ __device__ __forceinline__ void attend_tiles(const Pages &p, const PagesAttendAr
                     const int rr = it.row0 + c, tk = rr / p.group;
                     merge_parts<HD>(
                         [&](int k) { return p.part + (((size_t)(r.part0 + k * tiles + tile) * p.n_kv + h) * kPagesTileRows + c) * LD; },
-                        r.n_parts, a.out + ((size_t)(r.start + tk) * p.n_heads + h * p.group + rr % p.group) * HD, tid & 15);
+                        r.n_parts, p.out + ((size_t)(r.start + tk) * p.n_heads + h * p.group + rr % p.group) * HD, tid & 15);
                 }
         }
         __syncthreads();
@@ -1045,7 +1103,7 @@ struct WideLds {
 
 // A wide tile's end: its outputs, or its part and, from its last part, theirs.
 template <int HD>
-__device__ __forceinline__ void wide_result(const Pages &p, const PagesAttendArgs &a, WideLds<HD> &lds, int item, int h,
+__device__ __forceinline__ void wide_result(const AttendView &p, WideLds<HD> &lds, int item, int h,
                                             const floatx16 (&o)[HD / 32], float up, float m, float l)
 {
     constexpr int ND = HD / 32, LD = HD + 4, kMost = 8;
@@ -1056,7 +1114,7 @@ __device__ __forceinline__ void wide_result(const Pages &p, const PagesAttendArg
     const int n_rows = it.row1 - it.row0; // of the tile
     auto out_of = [&](int c) { // the tile's row c
         const int row = it.row0 + c;
-        return a.out + ((size_t)(r.start + row / p.group) * p.n_heads + h * p.group + row % p.group) * HD;
+        return p.out + ((size_t)(r.start + row / p.group) * p.n_heads + h * p.group + row % p.group) * HD;
     };
     if (it.part < 0) {
         if (wrow >= n_rows) return;
@@ -1129,7 +1187,7 @@ __device__ __forceinline__ void wide_result(const Pages &p, const PagesAttendArg
 }
 
 template <int HD>
-__device__ __forceinline__ void attend_wide(const Pages &p, const PagesAttendArgs &a, WideLds<HD> &lds, int first)
+__device__ __forceinline__ void attend_wide(const AttendView &p, WideLds<HD> &lds, int first)
 {
     constexpr int NC = HD / 16, ND = HD / 32, NL = HD / 64, BYTES = kPageBlock * HD, LD = HD + 4;
     auto &kf = lds.kf;
@@ -1140,9 +1198,9 @@ __device__ __forceinline__ void attend_wide(const Pages &p, const PagesAttendArg
     if (item >= p.head->n_wide) return;
     const PagesItem it = p.wide[item], &r = it;
     const int32_t *table = p.table + (size_t)r.id * p.width;
-    const uint8_t *kbase = p.k + (size_t)a.layer * p.n_blocks() * BYTES;
-    const uint8_t *vbase = p.v + (size_t)a.layer * p.n_blocks() * BYTES;
-    const float2 *sbase = p.ks + (size_t)a.layer * p.n_blocks();
+    const uint8_t *kbase = p.k;
+    const uint8_t *vbase = p.v;
+    const float2 *sbase = p.ks;
 
     const int n_rows = it.row1, wrow = it.row0 + 32 * wave;
     const bool active = wrow < n_rows;
@@ -1196,7 +1254,7 @@ __device__ __forceinline__ void attend_wide(const Pages &p, const PagesAttendArg
     half8_t qh[NC], ql[NC];
     float qs;
     {
-        const float *src = a.q + ((size_t)(r.start + token) * p.n_heads + head) * HD + 8 * hh;
+        const float *src = p.q + ((size_t)(r.start + token) * p.n_heads + head) * HD + 8 * hh;
         float m = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; c++)
@@ -1342,13 +1400,13 @@ __device__ __forceinline__ void attend_wide(const Pages &p, const PagesAttendArg
     }
     l += __shfl_xor(l, 32, 64);
     const float up = ldexpf(1.f, max(ev, -149));
-    wide_result<HD>(p, a, lds, item, h, o, up, m, l);
+    wide_result<HD>(p, lds, item, h, o, up, m, l);
 }
 
 // The attention of a plan in one launch: wide tiles first, then 16-row tiles,
 // `tiles` workgroups of which take turns.
 template <int HD, bool WIDE>
-__global__ __launch_bounds__(256, 2) void pages_attend_kernel(Pages p, PagesAttendArgs a, int wides, int tiles)
+__global__ __launch_bounds__(256, 2) void pages_attend_kernel(AttendView p)
 {
     union Lds {
         TileLds<HD> tile;
@@ -1357,12 +1415,12 @@ __global__ __launch_bounds__(256, 2) void pages_attend_kernel(Pages p, PagesAtte
     __shared__ __align__(16) char mem[sizeof(Lds)];
     Lds &lds = *(Lds *)mem;
     if constexpr (WIDE) {
-        if ((int)blockIdx.x < wides) {
-            attend_wide<HD>(p, a, *(WideLds<HD> *)mem, blockIdx.x);
+        if ((int)blockIdx.x < p.wides) {
+            attend_wide<HD>(p, *(WideLds<HD> *)mem, blockIdx.x);
             return;
         }
     }
-    attend_tiles<HD>(p, a, lds.tile, (int)blockIdx.x - wides, tiles);
+    attend_tiles<HD>(p, lds.tile, (int)blockIdx.x - p.wides, p.tiles);
 }
 
 hipError_t launch_pages_attend(const Pages &p, const PagesAttendArgs &a, hipStream_t s)
@@ -1371,21 +1429,33 @@ hipError_t launch_pages_attend(const Pages &p, const PagesAttendArgs &a, hipStre
     const int64_t most = (int64_t)p.max_parts + (int64_t)a.n_tokens * p.group / kPagesTileRows + a.n_requests;
     const int64_t most_wide = (int64_t)a.n_tokens * p.group / kPagesWideRows + a.n_requests + pages_wide_target(p.n_kv);
     const int wides = a.wide ? (int)(most_wide * p.n_kv) : 0, tiles = (int)(most < 2048 ? most : 2048) * p.n_kv;
-    const dim3 grid(wides + tiles);
-    if (p.hd == 128 && a.wide) hipLaunchKernelGGL((pages_attend_kernel<128, true>), grid, dim3(256), 0, s, p, a, wides, tiles);
-    else if (p.hd == 128) hipLaunchKernelGGL((pages_attend_kernel<128, false>), grid, dim3(256), 0, s, p, a, wides, tiles);
-    else if (a.wide) hipLaunchKernelGGL((pages_attend_kernel<64, true>), grid, dim3(256), 0, s, p, a, wides, tiles);
-    else hipLaunchKernelGGL((pages_attend_kernel<64, false>), grid, dim3(256), 0, s, p, a, wides, tiles);
+    const size_t bytes = (size_t)kPageBlock * p.hd;
+    const AttendView view = {layer_of(p, p.k, a.layer, bytes), layer_of(p, p.v, a.layer, bytes), layer_of(p, p.ks, a.layer, 1), p.table, p.head,
+                             p.item, p.wide, p.part, p.wide_part, p.tickets, p.wide_tickets, a.q, a.out, p.n_kv, p.n_heads, p.group,
+                             p.sub, p.sub_shift, p.width, p.scale, wides, tiles};
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(wides + tiles), dim3(256), 0, s, view); };
+    if (p.hd == 128) launch(a.wide ? pages_attend_kernel<128, true> : pages_attend_kernel<128, false>);
+    else launch(a.wide ? pages_attend_kernel<64, true> : pages_attend_kernel<64, false>);
     return hipGetLastError();
 }
 
 // ------------------------------------------------------------ reading back
 
+namespace {
+struct ReadView {
+    const uint8_t *k, *v;
+    const float2 *ks;
+    const int32_t *slot;
+    float *k_out, *v_out;
+    int n, n_kv, page, sub, n_pages;
+};
+} // namespace
+
 // Sixteen slots and one KV head to a workgroup.  K rows lie in runs of 64
 // dims.  V lies dim by dim, so its bytes are read with the tokens along the
 // lanes (neighbouring slots: one 64-byte run per load) and turned in LDS.
 template <int HD>
-__global__ __launch_bounds__(256) void pages_read_kernel(Pages p, int layer, const int32_t *slot, int n, float *k, float *v)
+__global__ __launch_bounds__(256) void pages_read_kernel(ReadView p)
 {
     constexpr int ND = HD / 16, BYTES = kPageBlock * HD, LD = HD + 4;
     __shared__ __align__(16) float lv[16][LD];
@@ -1397,10 +1467,10 @@ __global__ __launch_bounds__(256) void pages_read_kernel(Pages p, int layer, con
     };
     auto place = [&](int i) { // of the workgroup's slot i
         Place r = {0, 0, make_float2(0.f, 0.f)};
-        const int sl = first + i < n ? slot[first + i] : -1;
+        const int sl = first + i < p.n ? p.slot[first + i] : -1;
         if (sl >= 0 && sl / p.page < p.n_pages) {
             r.token = sl % kPageBlock;
-            r.block = ((size_t)(sl / p.page) * p.n_kv + h) * p.sub + sl % p.page / kPageBlock + (size_t)layer * p.n_blocks();
+            r.block = ((size_t)(sl / p.page) * p.n_kv + h) * p.sub + sl % p.page / kPageBlock ;
             r.s = p.ks[r.block];
         }
         return r; // elsewhere the pool's first block with scales of zero
@@ -1420,20 +1490,23 @@ __global__ __launch_bounds__(256) void pages_read_kernel(Pages p, int layer, con
 #pragma unroll
     for (int c = 0; c < ND / 4; c++) w[c] = *(const uint32_t *)(p.k + r.block * BYTES + k_at<HD>(r.token, ND * j + 4 * c));
     __syncthreads();
-    if (first + i >= n) return;
+    if (first + i >= p.n) return;
     const size_t to = ((size_t)(first + i) * p.n_kv + h) * HD + ND * j;
 #pragma unroll
-    for (int c = 0; c < ND; c++) k[to + c] = (float)((int)((w[c / 4] >> (8 * (c % 4))) & 255u) - 128) * r.s.x;
+    for (int c = 0; c < ND; c++) p.k_out[to + c] = (float)((int)((w[c / 4] >> (8 * (c % 4))) & 255u) - 128) * r.s.x;
 #pragma unroll
-    for (int c = 0; c < ND; c++) v[to + c] = lv[i][ND * j + c];
+    for (int c = 0; c < ND; c++) p.v_out[to + c] = lv[i][ND * j + c];
 }
 
 hipError_t launch_pages_read(const Pages &p, int layer, const int32_t *slot, int n, float *k, float *v, hipStream_t s)
 {
     if (n <= 0) return hipSuccess;
+    const size_t bytes = (size_t)kPageBlock * p.hd;
+    const ReadView view = {layer_of(p, p.k, layer, bytes), layer_of(p, p.v, layer, bytes), layer_of(p, p.ks, layer, 1), slot, k, v,
+                           n, p.n_kv, p.page, p.sub, p.n_pages};
     const dim3 grid((n + 15) / 16, p.n_kv);
-    if (p.hd == 128) hipLaunchKernelGGL(pages_read_kernel<128>, grid, dim3(256), 0, s, p, layer, slot, n, k, v);
-    else hipLaunchKernelGGL(pages_read_kernel<64>, grid, dim3(256), 0, s, p, layer, slot, n, k, v);
+    if (p.hd == 128) hipLaunchKernelGGL(pages_read_kernel<128>, grid, dim3(256), 0, s, view);
+    else hipLaunchKernelGGL(pages_read_kernel<64>, grid, dim3(256), 0, s, view);
     return hipGetLastError();
 }
 
