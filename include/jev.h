@@ -312,7 +312,10 @@ int jev_get_matmul_strategy(void);
  * and jev_pages_attend_device (jev_forward_pages: a whole model step).  The
  * *_device calls only enqueue on the handle's stream and allocate nothing, so a
  * step can be captured into a HIP graph and replayed with other lengths in the
- * same arrays; the lengths and tables stay on the device.  Nothing checks that
+ * same arrays; the lengths and tables stay on the device.  A store or attention
+ * call is for as many requests and tokens as the last plan call named: where a
+ * graph replayed since has planned more, it does nothing, and jev_pages_sync
+ * returns JEV_ESTATE (until the next plan).  Nothing checks that
  * a planned token was stored before it is attended or read: it has whatever its
  * page held.  The stream (jev_pages_stream) orders itself with the device's null
  * stream; a caller on another stream orders the two with events.  A handle's
@@ -384,7 +387,8 @@ int jev_pages_read_device(jev_pages *p, int32_t layer, const int32_t *slot, int3
  * nothing, waited for. */
 int jev_pages_release(jev_pages *p, const int32_t *request, int32_t n);
 
-/* Waits for the handle's stream; JEV_OK, or why the last plan was refused. */
+/* Waits for the handle's stream; JEV_OK, or why the last plan, or a call after
+ * it, was refused. */
 int jev_pages_sync(jev_pages *p);
 /* The handle's HIP stream (hipStream_t). */
 void *jev_pages_stream(jev_pages *p);

@@ -436,19 +436,16 @@ __host__ __device__ inline int pages_part_keys(int len)
 }
 
 struct PagesPlanHead {
-    int32_t status;  // JEV_OK, JEV_EINVAL or JEV_ENOMEM; not OK: everything below is zero
+    int32_t status;  // JEV_OK; JEV_EINVAL or JEV_ENOMEM: everything below is zero; JEV_ESTATE: a call found it too large
     int32_t n_tokens;
     int32_t n_units; // blocks that the batch's tokens go to
     int32_t n_items; // workgroups of attention per KV head, 16-row tiles
     int32_t n_wide;  // the same, wide tiles
-    int32_t n_parts, n_wide_parts; // partial results of split tiles
     int32_t n_requests;
-    int32_t pad;
 };
 struct PagesRequest { // one batch row
     int32_t id, past, len, start; // start: its first token's row in the batch
     int32_t part0, n_parts;       // partial results of its tiles, when split (n_parts > 1)
-    int32_t wide;                 // its tiles are wide ones
 };
 struct PagesUnit { // new tokens of one block: their first row and position, how many, page * blocks of a page + block
     int32_t row, pos, n, block;
@@ -484,8 +481,8 @@ struct Pages {
     PagesItem *item = nullptr, *wide = nullptr;
     double2 *angle = nullptr;               // [max_tokens][half] (cos, sin) * mscale
     const double *freqs = nullptr;
-    float *part = nullptr;                  // [n_parts][kv head][16][hd + 4]: output, max, sum
-    float *wide_part = nullptr;             // [n_wide_parts][kv head][128][hd + 4]
+    float *part = nullptr;                  // [max_parts][kv head][16][hd + 4]: output, max, sum
+    float *wide_part = nullptr;             // [max_wide_parts][kv head][128][hd + 4]
     int32_t *tickets = nullptr, *wide_tickets = nullptr; // [parts][kv head] parts that have arrived, at a tile's first part
     int max_units = 0, max_items = 0, max_wide = 0, max_parts = 0, max_wide_parts = 0;
     __host__ __device__ size_t n_blocks() const { return (size_t)n_pages * n_kv * sub; } // of a layer

@@ -26,6 +26,17 @@ struct PlanView {
 template <typename T>
 T *layer_of(const Pages &p, T *base, int layer, size_t per_block) { return base + layer * p.n_blocks() * per_block; }
 
+// The plan on the device may be a replayed graph's, and larger than the one that
+// this call's grid and its caller's arrays were made for.  Then the call does
+// nothing, and the plan's status says so.
+template <typename View>
+__device__ __forceinline__ bool outgrown(const View &p, const PagesPlanHead &h)
+{
+    if (h.n_tokens <= p.n_tokens && h.n_requests <= p.n_requests && (p.wide || h.n_wide == 0)) return false;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) p.head->status = JEV_ESTATE;
+    return true;
+}
+
 // Exclusive prefix sums over the workgroup's threads of N values at once, in
 // place, and their totals.  `ws`: N words per wave.
 template <int NT, int N, typename T>
@@ -239,7 +250,7 @@ __global__ __launch_bounds__(NT) void pages_plan_kernel(PlanView p, PagesPlanArg
     const long long tokens = all_of[0], more = all_of[1], gone = all_of[2];
     const int status = bad || tokens > a.n_tokens ? JEV_EINVAL : more > n_free + gone ? JEV_ENOMEM : JEV_OK;
     if (status != JEV_OK) {
-        PagesPlanHead h = {status, 0, 0, 0, 0, 0, 0, 0, 0};
+        PagesPlanHead h = {status, 0, 0, 0, 0, 0};
         if (tid == 0) *p.head = h;
         if (LISTS) plan_lists(p, a, h, px, S, tid, NT);
         return;
@@ -256,7 +267,7 @@ __global__ __launch_bounds__(NT) void pages_plan_kernel(PlanView p, PagesPlanArg
         s0 += fresh[i];
         s1 += need[i] - keep[i];
         s2 += own[i] - keep[i];
-        PagesRequest r = {id[i], past[i], past[i] + fresh[i], start[b], 0, 1, 0};
+        PagesRequest r = {id[i], past[i], past[i] + fresh[i], start[b], 0, 1};
         p.req[b] = r;
     }
     if (tid == 0) {
@@ -334,7 +345,7 @@ __global__ __launch_bounds__(NT) void pages_plan_kernel(PlanView p, PagesPlanArg
     block_scan<NT, 5>(n0, all_n, (int *)ws);
     __shared__ PagesPlanHead all;
     if (tid == 0) {
-        PagesPlanHead h = {JEV_OK, (int)tokens, all_n[0], all_n[1], all_n[2], all_n[3], all_n[4], R, 0};
+        PagesPlanHead h = {JEV_OK, (int)tokens, all_n[0], all_n[1], all_n[2], R};
         all = h;
         *p.head = h;
         unit0[R] = h.n_units;
@@ -351,7 +362,6 @@ __global__ __launch_bounds__(NT) void pages_plan_kernel(PlanView p, PagesPlanArg
         wide0[b] = n0[2];
         p.req[b].part0 = c[i].wide ? n0[4] : n0[3];
         p.req[b].n_parts = c[i].n_parts;
-        p.req[b].wide = c[i].wide;
         n0[0] += c[i].units;
         n0[1] += c[i].items;
         n0[2] += c[i].wides;
@@ -496,7 +506,7 @@ namespace {
 struct StoreView {
     uint8_t *k, *v;
     float2 *ks;
-    const PagesPlanHead *head;
+    PagesPlanHead *head;
     const PagesUnit *unit;
     const double2 *angle;
     const float *q, *k_in, *v_in;
@@ -505,6 +515,7 @@ struct StoreView {
     size_t in_stride;
     int nin, n_kv, n_heads, group, sub, sub_shift, half, rope_half, orig_ctx;
     float temp_scale;
+    int n_tokens, n_requests, wide; // of the call's plan
 };
 } // namespace
 
@@ -525,7 +536,8 @@ __global__ __launch_bounds__(256) void pages_store_kernel(StoreView p)
     __shared__ unsigned most[2];
     const int tid = threadIdx.x, j = tid & 15, h = blockIdx.y;
     const PagesUnit un = p.unit[blockIdx.x];
-    if ((int)blockIdx.x >= p.head->n_units) return; // (the unit's load does not wait for this)
+    const PagesPlanHead plan = *p.head; // (the unit's load does not wait for this)
+    if (outgrown(p, plan) || (int)blockIdx.x >= plan.n_units) return;
     const int pos0 = un.pos, n = un.n, row0 = un.row, off = pos0 & (kPageBlock - 1);
     const bool kv = p.k_in != nullptr;
     const RowPairs<HD> e(p, j);
@@ -680,7 +692,6 @@ __global__ __launch_bounds__(256) void pages_store_kernel(StoreView p)
 hipError_t launch_pages_store(const Pages &p, const PagesStoreArgs &a, hipStream_t s)
 {
     const int units = a.n_tokens / kPageBlock + 2 * (a.n_requests < a.n_tokens ? a.n_requests : a.n_tokens);
-    if (units == 0) return hipSuccess;
     const int np = p.hd / 32;
     auto vec = [&](const void *x, int64_t ld) { return !x || ((uintptr_t)x % (4 * np) == 0 && ld % np == 0); };
     // a thread's pairs in vector accesses: rows that start aligned, and no
@@ -690,8 +701,8 @@ hipError_t launch_pages_store(const Pages &p, const PagesStoreArgs &a, hipStream
     const size_t bytes = (size_t)kPageBlock * p.hd;
     const StoreView view = {layer_of(p, p.k, a.layer, bytes), layer_of(p, p.v, a.layer, bytes), layer_of(p, p.ks, a.layer, 1), p.head, p.unit,
                             p.angle, a.q, a.k, a.v, a.q_out, a.q_ld, a.kv_ld, a.in_stride, a.nin, p.n_kv, p.n_heads, p.group,
-                            p.sub, p.sub_shift, p.half, p.rope_half, p.orig_ctx, p.temp_scale};
-    const dim3 grid(units, p.n_kv);
+                            p.sub, p.sub_shift, p.half, p.rope_half, p.orig_ctx, p.temp_scale, a.n_tokens, a.n_requests, 1};
+    const dim3 grid(units > 0 ? units : 1, p.n_kv);
     if (p.hd == 128 && v) hipLaunchKernelGGL((pages_store_kernel<128, true>), grid, dim3(256), 0, s, view);
     else if (p.hd == 128) hipLaunchKernelGGL((pages_store_kernel<128, false>), grid, dim3(256), 0, s, view);
     else if (v) hipLaunchKernelGGL((pages_store_kernel<64, true>), grid, dim3(256), 0, s, view);
@@ -815,15 +826,16 @@ struct AttendView {
     const uint8_t *k, *v;
     const float2 *ks;
     const int32_t *table;
-    const PagesPlanHead *head;
-    const PagesItem *item, *wide;
+    PagesPlanHead *head;
+    const PagesItem *item, *wide_item;
     float *part, *wide_part;
     int32_t *tickets, *wide_tickets;
     const float *q;
     float *out;
     int n_kv, n_heads, group, sub, sub_shift, width;
     float scale;
-    int wides, tiles; // workgroups of each kind
+    int wides, tiles;               // workgroups of each kind
+    int n_tokens, n_requests, wide; // of the call's plan
 };
 } // namespace
 
@@ -847,14 +859,14 @@ struct TileLds {
     int last;
 };
 template <int HD>
-__device__ __forceinline__ void attend_tiles(const AttendView &p, TileLds<HD> &lds, int first, int count)
+__device__ __forceinline__ void attend_tiles(const AttendView &p, TileLds<HD> &lds, int n_items, int first, int count)
 {
     constexpr int NJ = HD / 64, NS = HD / 16, BYTES = kPageBlock * HD, LD = HD + 4;
     auto &lo = lds.lo;
     auto &lm = lds.lm, &ll = lds.ll;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, n = lane & 15, h = first % p.n_kv;
-    const int n_items = p.head->n_items, stride = count / p.n_kv;
+    const int stride = count / p.n_kv;
     const uint8_t *kbase = p.k;
     const uint8_t *vbase = p.v;
     const float2 *sbase = p.ks;
@@ -1109,7 +1121,7 @@ __device__ __forceinline__ void wide_result(const AttendView &p, WideLds<HD> &ld
     constexpr int ND = HD / 32, LD = HD + 4, kMost = 8;
     // read again: nothing of them takes registers during the products
     asm volatile("" : "+s"(item));
-    const PagesItem it = p.wide[item], &r = it;
+    const PagesItem it = p.wide_item[item], &r = it;
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, n = lane & 31, wrow = 32 * (tid >> 6) + n;
     const int n_rows = it.row1 - it.row0; // of the tile
     auto out_of = [&](int c) { // the tile's row c
@@ -1187,16 +1199,16 @@ __device__ __forceinline__ void wide_result(const AttendView &p, WideLds<HD> &ld
 }
 
 template <int HD>
-__device__ __forceinline__ void attend_wide(const AttendView &p, WideLds<HD> &lds, int first)
+__device__ __forceinline__ void attend_wide(const AttendView &p, WideLds<HD> &lds, int n_items, int first)
 {
-    constexpr int NC = HD / 16, ND = HD / 32, NL = HD / 64, BYTES = kPageBlock * HD, LD = HD + 4;
+    constexpr int NC = HD / 16, ND = HD / 32, NL = HD / 64, BYTES = kPageBlock * HD;
     auto &kf = lds.kf;
     auto &vf = lds.vf;
     auto &sc = lds.sc;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hh = lane >> 5, n = lane & 31, h = first % p.n_kv, item = first / p.n_kv;
-    if (item >= p.head->n_wide) return;
-    const PagesItem it = p.wide[item], &r = it;
+    if (item >= n_items) return;
+    const PagesItem it = p.wide_item[item], &r = it;
     const int32_t *table = p.table + (size_t)r.id * p.width;
     const uint8_t *kbase = p.k;
     const uint8_t *vbase = p.v;
@@ -1414,25 +1426,27 @@ __global__ __launch_bounds__(256, 2) void pages_attend_kernel(AttendView p)
     };
     __shared__ __align__(16) char mem[sizeof(Lds)];
     Lds &lds = *(Lds *)mem;
+    const PagesPlanHead plan = *p.head;
+    if (outgrown(p, plan)) return;
     if constexpr (WIDE) {
         if ((int)blockIdx.x < p.wides) {
-            attend_wide<HD>(p, *(WideLds<HD> *)mem, blockIdx.x);
+            attend_wide<HD>(p, *(WideLds<HD> *)mem, plan.n_wide, blockIdx.x);
             return;
         }
     }
-    attend_tiles<HD>(p, lds.tile, (int)blockIdx.x - p.wides, p.tiles);
+    attend_tiles<HD>(p, lds.tile, plan.n_items, (int)blockIdx.x - p.wides, p.tiles);
 }
 
 hipError_t launch_pages_attend(const Pages &p, const PagesAttendArgs &a, hipStream_t s)
 {
-    if (a.n_tokens == 0 || a.n_requests == 0) return hipSuccess;
-    const int64_t most = (int64_t)p.max_parts + (int64_t)a.n_tokens * p.group / kPagesTileRows + a.n_requests;
+    // (no tokens: a workgroup a KV head, for `outgrown`)
+    const int64_t most = a.n_tokens == 0 ? 1 : (int64_t)p.max_parts + (int64_t)a.n_tokens * p.group / kPagesTileRows + a.n_requests;
     const int64_t most_wide = (int64_t)a.n_tokens * p.group / kPagesWideRows + a.n_requests + pages_wide_target(p.n_kv);
     const int wides = a.wide ? (int)(most_wide * p.n_kv) : 0, tiles = (int)(most < 2048 ? most : 2048) * p.n_kv;
     const size_t bytes = (size_t)kPageBlock * p.hd;
     const AttendView view = {layer_of(p, p.k, a.layer, bytes), layer_of(p, p.v, a.layer, bytes), layer_of(p, p.ks, a.layer, 1), p.table, p.head,
                              p.item, p.wide, p.part, p.wide_part, p.tickets, p.wide_tickets, a.q, a.out, p.n_kv, p.n_heads, p.group,
-                             p.sub, p.sub_shift, p.width, p.scale, wides, tiles};
+                             p.sub, p.sub_shift, p.width, p.scale, wides, tiles, a.n_tokens, a.n_requests, a.wide};
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(wides + tiles), dim3(256), 0, s, view); };
     if (p.hd == 128) launch(a.wide ? pages_attend_kernel<128, true> : pages_attend_kernel<128, false>);
     else launch(a.wide ? pages_attend_kernel<64, true> : pages_attend_kernel<64, false>);
@@ -1470,7 +1484,7 @@ __global__ __launch_bounds__(256) void pages_read_kernel(ReadView p)
         const int sl = first + i < p.n ? p.slot[first + i] : -1;
         if (sl >= 0 && sl / p.page < p.n_pages) {
             r.token = sl % kPageBlock;
-            r.block = ((size_t)(sl / p.page) * p.n_kv + h) * p.sub + sl % p.page / kPageBlock ;
+            r.block = ((size_t)(sl / p.page) * p.n_kv + h) * p.sub + sl % p.page / kPageBlock;
             r.s = p.ks[r.block];
         }
         return r; // elsewhere the pool's first block with scales of zero

@@ -2656,6 +2656,8 @@ int pages_status(jev_pages *h, hipStream_t s)
         return fail(JEV_EINVAL, "the plan was refused: a request out of range or named twice, a kept length past what a "
                                 "request has, a context past %d tokens, or more than %d new tokens",
                     h->p.max_context, h->plan.n_tokens);
+    if (head.status == JEV_ESTATE)
+        return fail(JEV_ESTATE, "a store or an attention was called after a smaller plan than the one that a replayed graph has made: it did nothing");
     if (head.status == JEV_ENOMEM)
         return fail(JEV_ENOMEM, "the plan was refused: it needs more pages than are free of the pool's %d", h->p.n_pages);
     return JEV_OK;

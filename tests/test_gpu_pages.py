@@ -499,3 +499,45 @@ def test_many_steps_in_a_row(gpu, rs):
         y = rig.store(rs.randn(n, 4, 64).astype(np.float32), rs.randn(n, 2, 64).astype(np.float32), rs.randn(n, 2, 64).astype(np.float32))
         rig.attend(y.cpu().numpy()[:n])
     rig.check_values()
+
+
+@pytest.mark.parametrize("eager", [([0], [1]), (list(range(12)), [1] * 12), ([0], [40]), ([], [])])
+@pytest.mark.parametrize("replayed", [([1, 2, 0, 3], [1, 1, 1, 1]), ([2, 3], [30, 1]), ([2], [9])])
+def test_calls_for_a_smaller_plan_than_the_replayed_one(gpu, rs, eager, replayed):
+    """A graph's plan, replayed after a plan call of other sizes: the calls after it do all of it or nothing."""
+    hip = ctypes.CDLL("libamdhip64.so.7")
+    rig = Rig(cfg(8, 2, 64, rope=64), 80, 16, 12, 300)
+    rig.fill(rs, list(range(12)), [50, 20, 70, 16] + [5] * 8)
+    t, n, stream = rig.t, sum(replayed[1]), ctypes.c_void_p(rig.p.stream)
+    request, fresh = rig.ints(replayed[0]), rig.ints(replayed[1])
+    graph, ex = ctypes.c_void_p(), ctypes.c_void_p()
+    assert hip.hipStreamBeginCapture(stream, 2) == 0
+    rig.p.plan_device(request.data_ptr(), 0, fresh.data_ptr(), len(replayed[0]), n)
+    assert hip.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(ctypes.byref(ex), graph, None, None, 0) == 0
+    rig.plan(eager[0], eager[1], outputs=False)
+    assert hip.hipGraphLaunch(ex, stream) == 0
+    rig.p.sync()
+    assert rig.table.plan(list(replayed[0]), None, list(replayed[1]), n)[0] == 0
+    # 64 rows are there, so a call that went too far would show and not fault
+    q, k, v = (t.as_tensor(rs.randn(64, h, 64).astype(np.float32), device="cuda") for h in (8, 2, 2))
+    rot, out = t.full((64, 8, 64), -7.0, device="cuda"), t.full((64, 8, 64), -7.0, device="cuda")
+    # requests of more than 16 rows (4 tokens here) get wide tiles, where a plan call has more tokens than requests
+    fits = [n <= sum(eager[1]) and len(replayed[0]) <= len(eager[0])]
+    fits.append(fits[0] and (max(replayed[1]) <= 4 or sum(eager[1]) > len(eager[0])))
+    for ok, got, call in ((fits[0], rot, lambda: rig.p.store_device(0, q.data_ptr(), 512, k.data_ptr(), v.data_ptr(), 128, rot.data_ptr())),
+                          (fits[1], out, lambda: rig.p.attend_device(0, q.data_ptr(), out.data_ptr()))):
+        call()
+        if ok:
+            rig.p.sync()
+        else:
+            with pytest.raises(jev.JevError) as e:
+                rig.p.sync()
+            assert e.value.code == 6
+        y = got.cpu().numpy()
+        assert np.all(y[n if ok else 0:] == -7) and (not ok or not np.any(y[:n] == -7))
+    rig.plan([1], [3], outputs=False)  # and the next plan is as any other
+    xs = [rs.randn(3, h, 64).astype(np.float32) for h in (8, 2, 2)]
+    rig.store(*xs)
+    t.cuda.synchronize()
+    assert hip.hipGraphExecDestroy(ex) == 0 and hip.hipGraphDestroy(graph) == 0
