@@ -207,7 +207,7 @@ int jev_margins(const float *verdicts, int32_t n_options, int32_t n_yes, int32_t
 
 /* ParallelOptions.CancellationToken (MinistralModel.cs:301-304, KernelTests.cs:206-219):
  * cancels the call in flight on ctx -- jev_forward, jev_forward_tree,
- * jev_decode_greedy, jev_capture -- which then returns JEV_ECANCELED with the
+ * jev_decode_greedy, jev_capture, jev_forward_pages -- which then returns JEV_ECANCELED with the
  * cache length unchanged (greedy decoding: advanced by the steps that ran).
  * Those calls keep at most two groups of layers (decode: two steps) enqueued
  * ahead of the device and check between layers, so the work stops within that
@@ -238,9 +238,9 @@ void *jev_stream(jev_ctx *ctx);
  * per-token latency Benchmark.cs:411-422 samples.  Mode 0 turns both off.
  * Enabling clears the counters; reading synchronises the stream. */
 #define JEV_PROF_GEMM 0 /* MFMA prefill GEMM                     */
-#define JEV_PROF_ATTN 1 /* tree attention (prefill); a split pass's merge is a launch of its own */
+#define JEV_PROF_ATTN 1 /* tree attention (prefill); a split pass's merge is a launch of its own.  Paged: prompts */
 #define JEV_PROF_GEMV 2 /* one-token quantized GEMV              */
-#define JEV_PROF_DECODE_ATTN 3 /* decode attention (chunks); their merge where it is a launch of its own */
+#define JEV_PROF_DECODE_ATTN 3 /* decode attention (chunks); their merge where it is a launch of its own.  Paged: one token each */
 #define JEV_PROF_CLASSES 4
 int jev_profile_enable(jev_ctx *ctx, int enable);
 int jev_profile_read(jev_ctx *ctx, int kernel_class, int64_t *launches, double *total_ms, double *flops,

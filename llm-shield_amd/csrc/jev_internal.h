@@ -509,6 +509,7 @@ struct PagesAttendArgs {
     const float *q = nullptr; // [n_tokens][n_heads * hd]
     float *out = nullptr;     // the same
     int n_requests = 0, n_tokens = 0, wide = 0; // of the plan
+    hipEvent_t ev_start = nullptr, ev_stop = nullptr; // optional dispatch-stamped timing
 };
 hipError_t launch_pages_attend(const Pages &p, const PagesAttendArgs &a, hipStream_t s);
 // k, v [n][n_kv][hd] = the values at slots; zeros for slots outside the pool.

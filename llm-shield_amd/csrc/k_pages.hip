@@ -1447,7 +1447,7 @@ hipError_t launch_pages_attend(const Pages &p, const PagesAttendArgs &a, hipStre
     const AttendView view = {layer_of(p, p.k, a.layer, bytes), layer_of(p, p.v, a.layer, bytes), layer_of(p, p.ks, a.layer, 1), p.table, p.head,
                              p.item, p.wide, p.part, p.wide_part, p.tickets, p.wide_tickets, a.q, a.out, p.n_kv, p.n_heads, p.group,
                              p.sub, p.sub_shift, p.width, p.scale, wides, tiles, a.n_tokens, a.n_requests, a.wide};
-    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(wides + tiles), dim3(256), 0, s, view); };
+    auto launch = [&](auto kernel) { launch_stamped(a.ev_start, a.ev_stop, kernel, dim3(wides + tiles), dim3(256), 0, s, view); };
     if (p.hd == 128) launch(a.wide ? pages_attend_kernel<128, true> : pages_attend_kernel<128, false>);
     else launch(a.wide ? pages_attend_kernel<64, true> : pages_attend_kernel<64, false>);
     return hipGetLastError();

@@ -965,7 +965,13 @@ int enqueue_forward(jev_ctx *c, const Plan &p, int mode, int n_rows, float *dout
             pa.n_requests = sa.n_requests;
             pa.n_tokens = T;
             pa.wide = paged->args.wide;
-            HIP_TRY(launch_pages_attend(*paged->pages, pa, s));
+            {
+                ProfScope ps(c, pa.wide ? JEV_PROF_ATTN : JEV_PROF_DECODE_ATTN, 4.0 * f.head_dim * f.n_heads * p.visible_pairs,
+                             2.0 * f.head_dim * f.n_kv_heads * p.kv_rows + 8.0 * T * qdim, true);
+                pa.ev_start = ps.a;
+                pa.ev_stop = ps.z;
+                HIP_TRY(launch_pages_attend(*paged->pages, pa, s));
+            }
             if (T > 1) {
                 HIP_TRY(launch_split(c->y.p, T, qdim, c->xt.p, s));
                 if (L.o.type == kQ5_1) HIP_TRY(launch_block_sums(c->xt.p, T, qdim, c->xsum.p, s));
@@ -2920,9 +2926,14 @@ try {
     if (ids.front() < 0 || ids.back() >= pg.max_requests || std::adjacent_find(ids.begin(), ids.end()) != ids.end())
         return fail(JEV_EINVAL, "requests must be distinct and in [0, %d)", pg.max_requests);
     int64_t total = 0;
+    Plan p;
     for (int b = 0; b < n_requests; b++) {
         if (fresh[b] < 1 || (past && past[b] < 0)) return fail(JEV_EINVAL, "request %d: a negative past or no new token", request[b]);
         total += fresh[b];
+        if (past) { // (else the lengths are the device's, and the profiler's counts are without them)
+            p.visible_pairs += fresh[b] * (past[b] + 0.5 * (fresh[b] + 1));
+            p.kv_rows += past[b] + (double)fresh[b];
+        }
         last[b] = (int32_t)(total - 1);
     }
     if (total != n_tokens) return fail(JEV_EINVAL, "the requests add %lld tokens, and %d came", (long long)total, n_tokens);
@@ -2932,7 +2943,6 @@ try {
     const size_t nf = out_floats(c, mode, n_requests, n_rows);
     if (nf > 0 && (!out || out_len < nf)) return fail(JEV_EINVAL, "the output needs %zu floats", nf);
 
-    Plan p;
     p.T = n_tokens;
     p.n_out = n_requests;
     rc = ensure_workspace(c, n_tokens, n_requests, mode, 1);

@@ -185,3 +185,22 @@ def test_paged_greedy_refuses_what_cannot_fit():
     for prompts, new in (([[1] * 51], 2), ([[1] * 40], 42), ([[]], 2), ([[1]], 0), ([[1]] * 3 + [[1] * 50], 48)):
         with pytest.raises(jev.ArgumentError):
             jev.paged_greedy(m, p, prompts, new)
+
+
+@pytest.mark.parametrize("counts,cls", [([1, 1], "PROF_DECODE_ATTN"), ([3, 1], "PROF_ATTN")])
+def test_attention_over_pages_is_stamped(counts, cls):
+    """The per-kernel profiler times it like every other attention launch (1 ms each there), and counts its work."""
+    log, read = fake_hip.run(f"""
+m = model(heads=4, kv=2)
+p = jev.KvPages(jev.ModelConfig(n_layers=1, n_heads=4, n_kv_heads=2, head_dim=128), 20, 16, 3, 200, 100)
+L = jev.lib()
+jev._lib.check(L.jev_profile_enable(m._h, 1))
+launches()
+m.forward_pages(p, [0, 2], [[1] * n for n in {counts}], past=[20, 0])
+n, ms, flops = ctypes.c_int64(), ctypes.c_double(), ctypes.c_double()
+jev._lib.check(L.jev_profile_read(m._h, jev._lib.{cls}, ctypes.byref(n), ctypes.byref(ms), ctypes.byref(flops), None))
+result = [[(k, a, b) for k, g, a, b in launches() if "pages_attend" in k], [n.value, ms.value, flops.value]]
+""")
+    assert len(log) == 1 and log[0][1] and log[0][2] and log[0][1] != log[0][2]
+    pairs = sum(p + i + 1 for p, n in zip((20, 0), counts) for i in range(n))
+    assert read == [1, 1.0, 4.0 * 128 * 4 * pairs]
