@@ -117,15 +117,16 @@ __device__ __forceinline__ Counts counts(const PlanView &p, int past, int fresh,
 // The lists that follow from a valid plan, by `n` threads of which this is
 // number `i0`: the blocks to store, the attention's workgroups, the angles, and
 // what the caller asked for.  px: tokens, units, items and wide items before
-// each batch row (`stride` apart), R + 1 entries each.
+// each batch row (`stride` apart), R + 1 entries each; req: the batch rows, in
+// LDS or in memory.
 __device__ __forceinline__ void plan_lists(const PlanView &p, const PagesPlanArgs &a, const PagesPlanHead &h, const int *px,
-                                           int stride, int i0, int n)
+                                           int stride, const PagesRequest *req, int i0, int n)
 {
     const int R = h.n_requests;
     const int *start = px, *unit0 = px + stride, *item0 = px + 2 * stride, *wide0 = px + 3 * stride;
     for (int u = i0; u < h.n_units; u += n) {
         const int b = find(unit0, R, u);
-        const PagesRequest r = p.req[b];
+        const PagesRequest r = req[b];
         const int block = r.past / kPageBlock + u - unit0[b], pos = max(r.past, block * kPageBlock);
         const int page = p.table[(size_t)r.id * p.width + (block >> p.sub_shift)];
         const PagesUnit un = {r.start + pos - r.past, pos, min(r.len, (block + 1) * kPageBlock) - pos,
@@ -134,7 +135,7 @@ __device__ __forceinline__ void plan_lists(const PlanView &p, const PagesPlanArg
     }
     for (int i = i0; i < h.n_items; i += n) {
         const int b = find(item0, R, i), k = i - item0[b];
-        const PagesRequest r = p.req[b];
+        const PagesRequest r = req[b];
         const int tiles = (item0[b + 1] - item0[b]) / r.n_parts, t = k % tiles, part = k / tiles;
         const int keys = r.n_parts > 1 ? pages_part_keys(r.len) : r.len;
         const int key0 = part * keys;
@@ -144,7 +145,7 @@ __device__ __forceinline__ void plan_lists(const PlanView &p, const PagesPlanArg
     }
     for (int i = i0; i < h.n_wide; i += n) {
         const int b = find(wide0, R, i), k = i - wide0[b];
-        const PagesRequest r = p.req[b];
+        const PagesRequest r = req[b];
         const int tiles = (wide0[b + 1] - wide0[b]) / r.n_parts, part = k % r.n_parts;
         const int keys = (div_up(r.len, r.n_parts) + 63) & ~63; // parts of a length, in whole blocks of 64
         // a request's tiles take like numbers of rows, whole waves' of 32; the longest come first
@@ -160,7 +161,7 @@ __device__ __forceinline__ void plan_lists(const PlanView &p, const PagesPlanArg
     for (int i = i0; i < h.n_tokens * p.half; i += n) { // (at most 2^22 tokens x 64)
         const int t = i / p.half, j = i - t * p.half, b = find(start, R, t);
         double sn, cs;
-        sincos((double)(p.req[b].past + t - start[b]) * p.freqs[j], &sn, &cs);
+        sincos((double)(req[b].past + t - start[b]) * p.freqs[j], &sn, &cs);
         p.angle[i] = make_double2(cs * p.mscale, sn * p.mscale);
     }
     if (a.slot || a.position || a.row)
@@ -168,7 +169,7 @@ __device__ __forceinline__ void plan_lists(const PlanView &p, const PagesPlanArg
             int b = -1, pos = -1, slot = -1;
             if (t < h.n_tokens) {
                 b = find(start, R, t);
-                const PagesRequest r = p.req[b];
+                const PagesRequest r = req[b];
                 pos = r.past + t - start[b];
                 slot = p.table[(size_t)r.id * p.width + pos / p.page] * p.page + pos % p.page;
             }
@@ -186,7 +187,7 @@ __device__ __forceinline__ void plan_lists(const PlanView &p, const PagesPlanArg
                 for (int u = 0; u < 4; u++) {
                     const int b = b0 + u * (n >> 6);
                     page[u] = -1;
-                    if (b < R && j < div_up(p.req[b].len, p.page)) page[u] = p.table[(size_t)p.req[b].id * p.width + j];
+                    if (b < R && j < div_up(req[b].len, p.page)) page[u] = p.table[(size_t)req[b].id * p.width + j];
                 }
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
@@ -206,7 +207,12 @@ __device__ __forceinline__ void plan_lists(const PlanView &p, const PagesPlanArg
 template <int NT, bool LISTS>
 __global__ __launch_bounds__(NT) void pages_plan_kernel(PlanView p, PagesPlanArgs a)
 {
-    constexpr int C = NT == 256 ? 4 : 8, S = NT * C + 1; // requests of a thread; entries of a prefix sum
+    constexpr int C = NT == 256 ? 1 : 8, S = NT * C + 1; // requests of a thread; entries of a prefix sum
+    constexpr bool FEW = NT == 256;                      // the batch rows fit LDS
+    __shared__ PagesRequest few[FEW ? NT : 1];
+    PagesRequest *req;
+    if constexpr (FEW) req = few;
+    else req = p.req;
     __shared__ int px[4 * S];
     __shared__ unsigned seen[kPagesMaxRequests / 32];
     __shared__ long long ws[5 * NT / 64];
@@ -252,7 +258,7 @@ __global__ __launch_bounds__(NT) void pages_plan_kernel(PlanView p, PagesPlanArg
     if (status != JEV_OK) {
         PagesPlanHead h = {status, 0, 0, 0, 0, 0};
         if (tid == 0) *p.head = h;
-        if (LISTS) plan_lists(p, a, h, px, S, tid, NT);
+        if (LISTS) plan_lists(p, a, h, px, S, req, tid, NT);
         return;
     }
 
@@ -268,7 +274,7 @@ __global__ __launch_bounds__(NT) void pages_plan_kernel(PlanView p, PagesPlanArg
         s1 += need[i] - keep[i];
         s2 += own[i] - keep[i];
         PagesRequest r = {id[i], past[i], past[i] + fresh[i], start[b], 0, 1};
-        p.req[b] = r;
+        req[b] = r;
     }
     if (tid == 0) {
         start[R] = (int)tokens;
@@ -279,7 +285,7 @@ __global__ __launch_bounds__(NT) void pages_plan_kernel(PlanView p, PagesPlanArg
 
     for (int k = tid; k < (int)gone; k += NT) {
         const int b = find(gone0, R, k);
-        const int page = p.table[(size_t)p.req[b].id * p.width + div_up(p.req[b].past, p.page) + k - gone0[b]];
+        const int page = p.table[(size_t)req[b].id * p.width + div_up(req[b].past, p.page) + k - gone0[b]];
         atomicAnd(&p.used[page >> 5], ~(1u << (page & 31)));
     }
     __syncthreads(); // every page is back before the free ones are counted
@@ -305,7 +311,7 @@ __global__ __launch_bounds__(NT) void pages_plan_kernel(PlanView p, PagesPlanArg
         __syncthreads();
         for (int k = tid; k < (int)more; k += NT) {
             const int b = find(need0, R, k);
-            p.table[(size_t)p.req[b].id * p.width + div_up(p.req[b].past, p.page) + k - need0[b]] = p.fresh_pages[k];
+            p.table[(size_t)req[b].id * p.width + div_up(req[b].past, p.page) + k - need0[b]] = p.fresh_pages[k];
         }
     }
     __syncthreads(); // need0 and gone0 are done with
@@ -360,8 +366,8 @@ __global__ __launch_bounds__(NT) void pages_plan_kernel(PlanView p, PagesPlanArg
         unit0[b] = n0[0];
         item0[b] = n0[1];
         wide0[b] = n0[2];
-        p.req[b].part0 = c[i].wide ? n0[4] : n0[3];
-        p.req[b].n_parts = c[i].n_parts;
+        req[b].part0 = c[i].wide ? n0[4] : n0[3];
+        req[b].n_parts = c[i].n_parts;
         n0[0] += c[i].units;
         n0[1] += c[i].items;
         n0[2] += c[i].wides;
@@ -370,10 +376,12 @@ __global__ __launch_bounds__(NT) void pages_plan_kernel(PlanView p, PagesPlanArg
         p.length[id[i]] = past[i] + fresh[i];
     }
     __syncthreads();
-    if (LISTS) plan_lists(p, a, all, px, S, tid, NT);
-    else
+    if (LISTS) plan_lists(p, a, all, px, S, req, tid, NT);
+    else {
         for (int j = 0; j < 4; j++)
             for (int i = tid; i <= R; i += NT) p.prefix[j * (kPagesMaxRequests + 1) + i] = px[j * S + i];
+        if (FEW && tid < R) p.req[tid] = req[tid];
+    }
 }
 
 __global__ __launch_bounds__(256) void pages_lists_kernel(PlanView p, PagesPlanArgs a)
@@ -385,7 +393,7 @@ __global__ __launch_bounds__(256) void pages_lists_kernel(PlanView p, PagesPlanA
         for (int j = 0; j < 4; j++)
             for (int i = threadIdx.x; i <= h.n_requests; i += 256) px[j * S + i] = p.prefix[j * S + i];
     __syncthreads();
-    plan_lists(p, a, h, px, S, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
+    plan_lists(p, a, h, px, S, p.req, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
 hipError_t launch_pages_plan(const Pages &p, const PagesPlanArgs &a, hipStream_t s)
