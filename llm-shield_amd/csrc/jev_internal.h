@@ -429,7 +429,9 @@ __host__ __device__ inline int pages_wide_target(int n_kv) { return n_kv < kPage
 // alone, so that its result does not depend on the other requests.  Fewer keys
 // spread a lone request further, more save each part's start and end (us a pass,
 // 512 / 1024 / 2048 keys: one request of 4000 4.5 / 5.3 / 7.5, of 30000 11.5 / 11.0 /
-// 10.6; 64 of 500 to 12000 91 / 86 / 83, 128 of 2000 106 / 94 / 87).
+// 10.6; 64 of 500 to 12000 91 / 86 / 83, 128 of 2000 106 / 94 / 87; one call after
+// the other in a graph, 512 / 1024: one of 2000 9.5 / 12.2, 16 of 4000 34.8 / 29.7,
+// 700 of 100 to 900 179 / 145).
 __host__ __device__ inline int pages_part_keys(int len)
 {
     return len <= 16384 ? 1024 : len <= 131072 ? 2048 : (len / 64 + 63) & ~63; // at most 65 parts
