@@ -334,7 +334,7 @@ __global__ __launch_bounds__(NT) void pages_plan_kernel(PlanView p, PagesPlanArg
         // at most room + tiles parts, one round; many tiles split only where one
         // is twice as long as their mean
         const long long target = pages_wide_target(p.n_kv), room = max(target - tiles, (target + 1) / 2);
-        wide_keys = (int)max((long long)wide_keys, (keys + room - 1) / room);
+        wide_keys = (int)min((long long)p.max_context, max((long long)wide_keys, (keys + room - 1) / room));
     }
     int n0[5] = {0, 0, 0, 0, 0}; // units, items, wide items, parts, wide parts
     Counts c[C];

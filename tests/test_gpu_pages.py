@@ -541,3 +541,22 @@ def test_calls_for_a_smaller_plan_than_the_replayed_one(gpu, rs, eager, replayed
     rig.store(*xs)
     t.cuda.synchronize()
     assert hip.hipGraphExecDestroy(ex) == 0 and hip.hipGraphDestroy(graph) == 0
+
+
+@pytest.mark.parametrize("fresh", [1, 40])
+def test_pages_past_32_bit_offsets(gpu, rs, fresh):
+    """A pool whose codes lie past 2^32 bytes, after a plan of the most tokens there can be: its tiles' keys
+    are 2^37, and a part's share of them is past 32 bits."""
+    n = 1 << 22
+    rig = Rig(cfg(8, 8, 128), (n >> 8) + 8, 256, 2, n, n)  # 1024 bytes a token: request 0 takes the first 2^32
+    request, count = rig.ints([0]), rig.ints([n])
+    rig.p.plan_device(request.data_ptr(), 0, count.data_ptr(), 1, n)
+    rig.p.sync()
+    rig.table.own[0], rig.table.length[0] = list(range(n >> 8)), n
+    rig.fill(rs, [1], [300], check=True)
+    assert min(rig.table.own[1]) == n >> 8
+    rig.plan([1], [fresh], outputs=False)
+    x = [rs.randn(fresh, 8, 128).astype(np.float32) for _ in "qkv"]
+    rig.store(*x)
+    rig.check_values()
+    rig.attend(x[0])
