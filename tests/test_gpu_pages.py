@@ -560,3 +560,38 @@ def test_pages_past_32_bit_offsets(gpu, rs, fresh):
     rig.store(*x)
     rig.check_values()
     rig.attend(x[0])
+
+
+def test_more_tiles_than_workgroups(gpu, rs):
+    """As many requests as there can be, some in parts: the workgroups of the 16-row tiles take turns."""
+    rig = Rig(cfg(2, 1, 64), 9000, 16, 4096, 3000, 40000)
+    lens = rs.randint(0, 9, 4096)
+    lens[rs.permutation(4096)[:9]] = rs.randint(1024, 2999, 9)
+    for part in np.array_split(np.arange(4096), 2):
+        rig.fill(rs, [int(r) for r in part], [int(x) for x in lens[part]])
+    rig.fill(rs, list(range(4096)), [1] * 4096)
+    rig.attend(rs.randn(4096, 2, 64).astype(np.float32))
+
+
+@pytest.mark.parametrize("fresh", [[1, 1], [70, 3]])
+def test_attention_and_reading_at_any_alignment(gpu, rs, fresh):
+    rig = Rig(cfg(8, 2, 128), 200, 32, 2, 3000)
+    rig.fill(rs, [0, 1], [1500, 40])
+    rig.fill(rs, [0, 1], fresh)
+    t, n = rig.t, sum(fresh)
+    q = rs.randn(n, 8, 128).astype(np.float32)
+    want = rig.attend(q)
+    slots = rig.ints([rig.table.own[0][i // 32] * 32 + i % 32 for i in range(37)])
+    kv = rig.kv[0, 0, "k"].values(37), rig.kv[0, 0, "v"].values(37)
+    for lead in (1, 2, 3):
+        x, out = (t.full((lead + n * 1024 + 4,), -7.0, device="cuda") for _ in "qo")
+        k, v = (t.full((lead + 37 * 256 + 4,), -7.0, device="cuda") for _ in "kv")
+        x[lead:lead + n * 1024] = rig.dev(q).reshape(-1)
+        t.cuda.synchronize()
+        rig.p.attend_device(0, x.data_ptr() + 4 * lead, out.data_ptr() + 4 * lead)
+        rig.p.read_device(0, slots.data_ptr(), 37, k.data_ptr() + 4 * lead, v.data_ptr() + 4 * lead)
+        rig.p.sync()
+        for y, w in ((out, want), (k, kv[0]), (v, kv[1])):
+            y = y.cpu().numpy()
+            np.testing.assert_array_equal(y[lead:-4], np.ravel(w))
+            assert np.all(y[:lead] == -7) and np.all(y[-4:] == -7)
