@@ -595,3 +595,13 @@ def test_attention_and_reading_at_any_alignment(gpu, rs, fresh):
             y = y.cpu().numpy()
             np.testing.assert_array_equal(y[lead:-4], np.ravel(w))
             assert np.all(y[:lead] == -7) and np.all(y[-4:] == -7)
+
+
+def test_parts_of_very_long_contexts(gpu, rs):
+    """Past 131072 tokens a part is a share of the length."""
+    rig = Rig(cfg(2, 1, 64), 9000, 16, 1, 143000, 143000)
+    rig.fill(rs, [0], [142001])
+    rig.fill(rs, [0], [1])
+    rig.attend(rs.randn(1, 2, 64).astype(np.float32))
+    rig.fill(rs, [0], [40])
+    rig.attend(rs.randn(40, 2, 64).astype(np.float32))
