@@ -867,7 +867,7 @@ struct TileLds {
     int last;
 };
 template <int HD>
-__device__ __forceinline__ void attend_tiles(const AttendView &p, TileLds<HD> &lds, int n_items, int first, int count)
+__device__ __forceinline__ void attend_tiles(const AttendView &p, TileLds<HD> &lds, PagesItem it, int n_items, int first, int count)
 {
     constexpr int NJ = HD / 64, NS = HD / 16, BYTES = kPageBlock * HD, LD = HD + 4;
     auto &lo = lds.lo;
@@ -879,8 +879,8 @@ __device__ __forceinline__ void attend_tiles(const AttendView &p, TileLds<HD> &l
     const uint8_t *vbase = p.v;
     const float2 *sbase = p.ks;
 
-    for (int item = first / p.n_kv; item < n_items; item += stride) {
-        const PagesItem it = p.item[item], &r = it;
+    for (int item = first / p.n_kv; item < n_items;) {
+        const PagesItem &r = it;
         const int32_t *table = p.table + (size_t)r.id * p.width;
         // lanes past the request's rows repeat its last one
         const int n_rows = it.row1, row = min(it.row0 + n, n_rows - 1);
@@ -1093,6 +1093,8 @@ __device__ __forceinline__ void attend_tiles(const AttendView &p, TileLds<HD> &l
                 }
         }
         __syncthreads();
+        item += stride;
+        if (item < n_items) it = p.item[item];
     }
 }
 
@@ -1207,7 +1209,7 @@ __device__ __forceinline__ void wide_result(const AttendView &p, WideLds<HD> &ld
 }
 
 template <int HD>
-__device__ __forceinline__ void attend_wide(const AttendView &p, WideLds<HD> &lds, int n_items, int first)
+__device__ __forceinline__ void attend_wide(const AttendView &p, WideLds<HD> &lds, const PagesItem &it, int first)
 {
     constexpr int NC = HD / 16, ND = HD / 32, NL = HD / 64, BYTES = kPageBlock * HD;
     auto &kf = lds.kf;
@@ -1215,8 +1217,7 @@ __device__ __forceinline__ void attend_wide(const AttendView &p, WideLds<HD> &ld
     auto &sc = lds.sc;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hh = lane >> 5, n = lane & 31, h = first % p.n_kv, item = first / p.n_kv;
-    if (item >= n_items) return;
-    const PagesItem it = p.wide_item[item], &r = it;
+    const PagesItem &r = it;
     const int32_t *table = p.table + (size_t)r.id * p.width;
     const uint8_t *kbase = p.k;
     const uint8_t *vbase = p.v;
@@ -1434,15 +1435,19 @@ __global__ __launch_bounds__(256, 2) void pages_attend_kernel(AttendView p)
     };
     __shared__ __align__(16) char mem[sizeof(Lds)];
     Lds &lds = *(Lds *)mem;
+    // (the first item, which is there if not of this plan, does not wait for the head)
+    const bool wide = WIDE && (int)blockIdx.x < p.wides;
+    const int first = wide ? blockIdx.x : (int)blockIdx.x - p.wides, item = first / p.n_kv;
+    const PagesItem it = wide ? p.wide_item[item] : p.item[item];
     const PagesPlanHead plan = *p.head;
-    if (outgrown(p, plan)) return;
+    if (outgrown(p, plan) || item >= (wide ? plan.n_wide : plan.n_items)) return;
     if constexpr (WIDE) {
-        if ((int)blockIdx.x < p.wides) {
-            attend_wide<HD>(p, *(WideLds<HD> *)mem, plan.n_wide, blockIdx.x);
+        if (wide) {
+            attend_wide<HD>(p, *(WideLds<HD> *)mem, it, first);
             return;
         }
     }
-    attend_tiles<HD>(p, lds.tile, plan.n_items, (int)blockIdx.x - p.wides, p.tiles);
+    attend_tiles<HD>(p, lds.tile, it, plan.n_items, first, p.tiles);
 }
 
 hipError_t launch_pages_attend(const Pages &p, const PagesAttendArgs &a, hipStream_t s)
