@@ -1345,7 +1345,6 @@ __device__ __forceinline__ void attend_wide(const AttendView &p, WideLds<HD> &ld
         fetch(kb + 2, next);
         next = page_of(kb + 3);
         const float4 s01 = *(const float4 *)&sc[buf][0], s23 = *(const float4 *)&sc[buf][2];
-        const float vm = fmaxf(fmaxf(s01.y, s01.w), fmaxf(s23.y, s23.w));
         const float2 s0 = hh ? make_float2(s01.z, s01.w) : make_float2(s01.x, s01.y);
         const float2 s1 = hh ? make_float2(s23.z, s23.w) : make_float2(s23.x, s23.y);
         float ks[2] = {s0.x * qs, s1.x * qs}, vs[2] = {s0.y, s1.y};
@@ -1364,7 +1363,7 @@ __device__ __forceinline__ void attend_wide(const AttendView &p, WideLds<HD> &ld
                     if (i > left) s[t][i] = -INFINITY;
             }
         }
-        float mx = -INFINITY;
+        float mx = -INFINITY, vm = fmaxf(vs[0], vs[1]); // (of the visible blocks)
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             float y = -INFINITY;
@@ -1374,6 +1373,8 @@ __device__ __forceinline__ void attend_wide(const AttendView &p, WideLds<HD> &ld
         }
         const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
         mx = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+        const auto scales = __builtin_amdgcn_permlane32_swap(__float_as_uint(vm), __float_as_uint(vm), false, false);
+        vm = fmaxf(__uint_as_float(scales[0]), __uint_as_float(scales[1]));
         const int en = vm > 0.f && vm < INFINITY ? max(ev, __builtin_amdgcn_frexp_expf(vm)) : ev;
         if (__any(mx > m + 6.f || en > ev)) {
             const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2f(m - mn);

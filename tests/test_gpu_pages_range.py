@@ -1,0 +1,78 @@
+"""The paged attention over values whose magnitudes lie far apart, from block to block and
+against fp32's range: keys that a query cannot see, or gives no weight, cost its result nothing.
+
+The bound, per output: with p the exact weights, a weight is off by E relative, of which
+  * its score's error: q within 2^-21 of its fp16 pair, head_dim products summed in fp32
+    (2^-24 each) and a few roundings of scales, all of sum |q| |k|; the exponent's roundings,
+    2^-22 of |score| and 2^-18 (an argument of up to 2^5 beside the score, twice);
+  * 2^-19: the pair's truncation (2^-21), its exponential and the scale on it.
+An error of p_i moves the output by p_i E_i (|v_i| + |out|).  The fp32 sums over n keys are off
+by n 2^-24 sum p |v| (and 2^-20 of it: rescaling and merging).  A weight smaller than the pair's
+last bit, 2^-24 where the heaviest p * (V scale) is at least 2^8, loses at most that bit for
+each of its codes: 2^-32 max(p * scale) sum |code|."""
+import numpy as np
+import pytest
+
+import jev
+import pages_ref as R
+from test_gpu_pages import Rig, cfg
+
+pytestmark = pytest.mark.gpu
+
+
+def attended(rig, r, q, past, layer=0):
+    """Exact attention of q [fresh, heads, dim] over request r's stored values, and its bound."""
+    k, vc = rig.kv[r, layer, "k"], rig.kv[r, layer, "v"]
+    n = past + len(q)
+    heads, d = q.shape[1:]
+    g = heads // k.code.shape[1]
+    keys = k.values(n).astype(np.float64)
+    scale = np.repeat(vc.scale, R.BLOCK, axis=0)[:n].astype(np.float64)
+    code = vc.code[:n]
+    out, off = np.empty(q.shape), np.empty(q.shape)
+    seen = np.arange(n) <= past + np.arange(len(q))[:, None]
+    for h in range(heads):
+        kh, sh, ch = keys[:, h // g], scale[:, h // g], code[:, h // g]
+        x = q[:, h].astype(np.float64)
+        s = np.where(seen, x @ kh.T / np.sqrt(d), -np.inf)
+        p = np.exp(s - s.max(-1, keepdims=True))
+        p /= p.sum(-1, keepdims=True)
+        a = np.abs(x) @ np.abs(kh).T / np.sqrt(d)
+        e = np.expm1(a * (2.0 ** -21 + (d + 4) * 2.0 ** -24) + np.abs(np.where(seen, s, 0)) * 2.0 ** -22 + 2.0 ** -18) + 2.0 ** -19
+        pv, pe = p * sh, p * e
+        out[:, h] = pv @ ch
+        size = pv @ np.abs(ch)
+        moved = ((pe * sh) @ np.abs(ch) + pe.sum(-1, keepdims=True) * np.abs(out[:, h])) / (1 - pe.sum(-1, keepdims=True))
+        off[:, h] = moved + size * (n * 2.0 ** -24 + 2.0 ** -20) + 2.0 ** -32 * pv.max(-1, keepdims=True) * (seen @ np.abs(ch)) + 2.0 ** -140
+    return out, off
+
+
+def check(rig, r, q, got, past):
+    want, off = attended(rig, r, q, past)
+    bad = ~(np.abs(got - want) <= off)
+    worst = np.nanmax(np.abs(got - want) / off)
+    assert not np.count_nonzero(bad), (np.argwhere(bad)[:3].tolist(), worst)
+
+
+@pytest.fixture
+def rs():
+    return np.random.RandomState(17)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("begin", [16, 32, 48])
+@pytest.mark.parametrize("large", [1e6, 1e15, 1e30])
+def test_later_tokens_leave_earlier_ones_alone(gpu, rs, dim, begin, large):
+    """A prompt whose tokens from a block's begin on have far larger values: the ones before have the bits that
+    they have without them."""
+    rig = Rig(cfg(8, 2, dim), 20, 16, 1, 200)
+    q, k, v = (rs.randn(90, h, dim).astype(np.float32) for h in (8, 2, 2))
+    got = []
+    for by in (1.0, large):
+        x = v.copy()
+        x[begin:] *= np.float32(by)
+        rig.plan([0], [90], [0])
+        rig.store(None, k, x)
+        got.append(rig.attend(q, check=False)[:begin])
+        check(rig, 0, q[:begin], got[-1], 0)
+    np.testing.assert_array_equal(got[1], got[0])
