@@ -374,7 +374,10 @@ int jev_pages_store_device(jev_pages *p, int32_t layer, const float *q, int64_t 
 /* out = softmax(q . K / sqrt(head_dim)) . V of every planned token over its
  * request's stored tokens up to and with itself; query head h reads KV head
  * h / (n_heads / n_kv_heads).  q and out are [n_tokens][n_heads * head_dim] and
- * must not overlap; rows past the planned total stay as they were.  A token's
+ * must not overlap; rows past the planned total stay as they were.  Scores,
+ * weights and sums have fp32's accuracy or nearly (weights 2^-21), wherever scales
+ * lie: a key's weight times its V scale loses at most 2^-32 of the largest such
+ * product among the keys that the query sees.  A token's
  * result has the same bits whatever else is in the batch where its request adds
  * one token, or few: fresh * heads per KV head <= 16. */
 int jev_pages_attend_device(jev_pages *p, int32_t layer, const float *q, float *out);

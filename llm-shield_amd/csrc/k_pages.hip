@@ -767,6 +767,32 @@ struct QueryScale {
     }
 };
 
+// A block's weights are 2^(score + log2(V scale) + 9 - e) = 2^(score + c), where e, whole,
+// lies between the row's largest score + log2(V scale) so far, less 6, and that plus 1:
+// a weight falls under fp16's last bit only where it is less than 2^-32 of the heaviest
+// one, however large the scales of blocks without weight are.
+struct ValueScale {
+    int exp;
+    float lg;                                          // log2 of the mantissa; -inf for 0
+    __device__ __forceinline__ ValueScale(float vs)    // vs: the block's V scale, 0 where the row sees none of it
+        : exp(__builtin_amdgcn_frexp_expf(vs)), lg(__builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(vs))) {}
+    __device__ __forceinline__ float top(float mx) const { return mx + ((float)exp + lg); } // mx: the block's largest score
+    // The row's sum takes the block's weights times 2^(-c - mu), so c may be any number where
+    // the outputs do not see them: weights below 2^-31, and a scale of zero's (codes of zero).
+    __device__ __forceinline__ float c(float vs, float mx, float e, float mu) const
+    {
+        if (vs > 0.f && mx > -INFINITY) return fmaxf((float)exp + 9.f - e + lg, -31.f - mx);
+        return vs != vs ? vs : -mu;
+    }
+};
+
+// Outputs held times 2^(9 - e) become relative to 2^m by this factor twice: what it is
+// squared may be outside fp32's range.
+__device__ __forceinline__ float half_scale(float e, float m)
+{
+    return e == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(0.5f * (e - 9.f - m));
+}
+
 // Partial results pass between workgroups inside a launch, which may run on
 // different dies with an L2 each: they are stored and read as agent-scope atomics
 // (written through, and read past, caches that other dies do not see), two floats
@@ -858,10 +884,9 @@ struct AttendView {
 // accumulators are the P^T operand of O^T += V^T P^T as they stand -- no
 // exchange between lanes -- and a lane has one K and one V scale per 64 keys.
 // Codes are exact in fp16; q and p enter as fp16 pairs (hi + lo), ~22 bits, so
-// each product is two matrix instructions.  p carries the V scale, relative to a
-// power of two (2^ev) above the largest so far, through its exponent: one fused
-// multiply-add and one exp2 a score; the maximum moves only when a score passes
-// it by 2^6.  Statistics, scores and outputs are fp32.  The next 64 keys' K is in
+// each product is two matrix instructions.  p carries the V scale through its
+// exponent (ValueScale): one fused multiply-add and one exp2 a score; the maxima move
+// only when a score passes one by 2^6.  Statistics, scores and outputs are fp32.  The next 64 keys' K is in
 // flight during the softmax and V^T P^T, their V during the next scores.
 // Single tokens are bound by HBM: 2 hd bytes a key and KV head (32 heads over 8 x
 // 128: 64 tokens over 500 to 12000 keys 86 us, 5.8 TB/s; one over 120002 41 us, 5.9;
@@ -959,8 +984,7 @@ __device__ __forceinline__ void attend_tiles(const AttendView &p, TileLds<HD> &l
         floatx4 o[NS];
 #pragma unroll
         for (int s = 0; s < NS; s++) o[s] = floatx4{0.f, 0.f, 0.f, 0.f};
-        float m = -INFINITY, l = 0.f;
-        int ev = -200; // outputs are held times 2^(9 - ev); V scales are below 2^ev
+        float m = -INFINITY, l = 0.f, e = -INFINITY; // outputs are held times 2^(9 - e)
 
         for (; kb * 64 < key1; kb += 4) {
             const bool more = (kb + 4) * 64 < key1;
@@ -995,37 +1019,35 @@ __device__ __forceinline__ void attend_tiles(const AttendView &p, TileLds<HD> &l
                     for (int i = 0; i < 4; i++)
                         if (4 * t + i > left) sv[t][i] = -INFINITY;
             }
-            float mx = -INFINITY, vm = vs;
+            float mx = -INFINITY;
 #pragma unroll
             for (int t = 0; t < 4; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) mx = fmaxf(mx, sv[t][i]);
             mx *= ks;
-            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-            vm = fmaxf(vm, __shfl_xor(vm, 16, 64));
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            vm = fmaxf(vm, __shfl_xor(vm, 32, 64));
-            const int en = vm > 0.f && vm < INFINITY ? max(ev, __builtin_amdgcn_frexp_expf(vm)) : ev;
-            if (__any(mx > m + 6.f || en > ev)) {
-                const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2f(m - mn);
-                l *= f;
-                const float up = ldexpf(f, max(ev - en, -400));
+            const ValueScale value(vs);
+            const float mv = value.top(mx);
+            if (__any(mx > m + 6.f || mv > e + 6.f)) {
+                float mn = fmaxf(m, mx), en = fmaxf(e, ceilf(mv));
+                mn = fmaxf(mn, __shfl_xor(mn, 16, 64));
+                en = fmaxf(en, __shfl_xor(en, 16, 64));
+                mn = fmaxf(mn, __shfl_xor(mn, 32, 64));
+                en = fmaxf(en, __shfl_xor(en, 32, 64));
+                l *= m == -INFINITY ? 0.f : exp2f(m - mn);
+                const float up = e == -INFINITY ? 0.f : exp2f(e - en);
 #pragma unroll
                 for (int s = 0; s < NS; s++) o[s] *= up;
                 m = mn;
-                ev = en;
+                e = en;
             }
-            const float mu = m == -INFINITY ? 0.f : m;
-            float lv = vs == 0.f ? 0.f : fmaxf(__builtin_amdgcn_logf(ldexpf(vs, -ev)), -60.f);
-            if (vs != vs) lv = vs;
-            const float c = lv + 9.f - mu;
+            const float mu = m == -INFINITY ? 0.f : m, c = value.c(vs, mx, e, mu);
             float w[16], sum = 0.f;
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 w[i] = __builtin_amdgcn_exp2f(fmaf(sv[i >> 2][i & 3], ks, c));
                 sum += w[i];
             }
-            l += sum * __builtin_amdgcn_exp2f(-9.f - lv);
+            l += sum * __builtin_amdgcn_exp2f(-c - mu);
             uint32_t hi[8], lw[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) split2_mix(w[2 * i], w[2 * i + 1], hi[i], lw[i]);
@@ -1052,9 +1074,9 @@ __device__ __forceinline__ void attend_tiles(const AttendView &p, TileLds<HD> &l
         l += __shfl_xor(l, 32, 64);
 
         // the four waves' results, in wave order
-        const float up = ldexpf(1.f, max(ev, -149));
+        const float up = half_scale(e, m);
 #pragma unroll
-        for (int s = 0; s < NS; s++) *(floatx4 *)&lo[wave][n][16 * s + 4 * g] = o[s] * 0x1p-9f * up;
+        for (int s = 0; s < NS; s++) *(floatx4 *)&lo[wave][n][16 * s + 4 * g] = o[s] * up * up;
         if (g == 0) {
             lm[wave][n] = m;
             ll[wave][n] = l;
@@ -1151,11 +1173,11 @@ __device__ __forceinline__ void wide_result(const AttendView &p, WideLds<HD> &ld
     if (it.part < 0) {
         if (wrow >= n_rows) return;
         float *dst = out_of(wrow);
-        const float f = 0x1p-9f / l;
+        const float f = up / l;
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) dst[32 * d + 8 * (i >> 2) + 4 * hh + (i & 3)] = o[d][i] * f * up;
+            for (int i = 0; i < 16; i++) dst[32 * d + 8 * (i >> 2) + 4 * hh + (i & 3)] = o[d][i] * up * f;
         return;
     }
     // through LDS, where the fragments were: whole runs of a row to a store
@@ -1165,7 +1187,7 @@ __device__ __forceinline__ void wide_result(const AttendView &p, WideLds<HD> &ld
 #pragma unroll
         for (int i = 0; i < 4; i++)
             *(floatx4 *)(mine + 32 * d + 8 * i + 4 * hh) =
-                floatx4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]} * 0x1p-9f * up;
+                floatx4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]} * up * up;
     if (hh == 0) *(float2 *)(mine + HD) = make_float2(m, l);
     __syncthreads();
     float *part = p.wide_part + ((size_t)it.part * p.n_kv + h) * kPagesWideRows * LD;
@@ -1308,8 +1330,7 @@ __device__ __forceinline__ void attend_wide(const AttendView &p, WideLds<HD> &ld
     floatx16 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = floatx16{};
-    float m = -INFINITY, l = 0.f;
-    int ev = -200; // outputs are held times 2^(9 - ev); V scales are below 2^ev
+    float m = -INFINITY, l = 0.f, e = -INFINITY; // outputs are held times 2^(9 - e)
 #pragma unroll
     for (int i = 0; i < 4 * NL; i++) put(0, i);
     fetch(kb + 1, next); // (past the last block: the last again, which nobody reads)
@@ -1363,38 +1384,33 @@ __device__ __forceinline__ void attend_wide(const AttendView &p, WideLds<HD> &ld
                     if (i > left) s[t][i] = -INFINITY;
             }
         }
-        float mx = -INFINITY, vm = fmaxf(vs[0], vs[1]); // (of the visible blocks)
+        float mx[2], mv[2];
+        const ValueScale value[2] = {ValueScale(vs[0]), ValueScale(vs[1])};
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             float y = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 16; i++) y = fmaxf(y, s[t][i]);
-            mx = fmaxf(mx, y * ks[t]);
+            mx[t] = y * ks[t];
+            mv[t] = value[t].top(mx[t]);
         }
-        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-        mx = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
-        const auto scales = __builtin_amdgcn_permlane32_swap(__float_as_uint(vm), __float_as_uint(vm), false, false);
-        vm = fmaxf(__uint_as_float(scales[0]), __uint_as_float(scales[1]));
-        const int en = vm > 0.f && vm < INFINITY ? max(ev, __builtin_amdgcn_frexp_expf(vm)) : ev;
-        if (__any(mx > m + 6.f || en > ev)) {
-            const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2f(m - mn);
-            l *= f;
-            const float g = ldexpf(f, max(ev - en, -400));
+        if (__any(fmaxf(mx[0], mx[1]) > m + 6.f || fmaxf(mv[0], mv[1]) > e + 6.f)) {
+            auto halves = [](float x) { // the larger of the lane's and the other half's
+                const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+                return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+            };
+            const float mn = halves(fmaxf(m, fmaxf(mx[0], mx[1]))), en = halves(fmaxf(e, ceilf(fmaxf(mv[0], mv[1]))));
+            l *= m == -INFINITY ? 0.f : exp2f(m - mn);
+            const float g = e == -INFINITY ? 0.f : exp2f(e - en);
 #pragma unroll
             for (int d = 0; d < ND; d++) o[d] *= g;
             m = mn;
-            ev = en;
+            e = en;
         }
         const float mu = m == -INFINITY ? 0.f : m;
-        // w = 2^(score - m + 9) times the V scale over 2^ev; a scale of zero has codes of zero
-        float lv[2], sum[2] = {0.f, 0.f};
+        const float c0 = value[0].c(vs[0], mx[0], e, mu), c1 = value[1].c(vs[1], mx[1], e, mu);
+        float sum[2] = {0.f, 0.f};
         uint32_t hi[2][8], lw[2][8];
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            lv[t] = vs[t] == 0.f ? 0.f : fmaxf(__builtin_amdgcn_logf(ldexpf(vs[t], -ev)), -60.f);
-            if (vs[t] != vs[t]) lv[t] = vs[t];
-        }
-        const float c0 = lv[0] + 9.f - mu, c1 = lv[1] + 9.f - mu;
         auto weights = [&](int t, int i) { // of tokens 2 i and 2 i + 1 of the lane's block
             const float x = __builtin_amdgcn_exp2f(fmaf(s[t][2 * i], ks[t], t ? c1 : c0));
             const float y = __builtin_amdgcn_exp2f(fmaf(s[t][2 * i + 1], ks[t], t ? c1 : c0));
@@ -1426,13 +1442,12 @@ __device__ __forceinline__ void attend_wide(const AttendView &p, WideLds<HD> &ld
                 v = ahead;
                 __builtin_amdgcn_sched_barrier(0);
             }
-        l += sum[0] * __builtin_amdgcn_exp2f(-9.f - lv[0]);
-        l += sum[1] * __builtin_amdgcn_exp2f(-9.f - lv[1]);
+        l += sum[0] * __builtin_amdgcn_exp2f(-c0 - mu);
+        l += sum[1] * __builtin_amdgcn_exp2f(-c1 - mu);
         __syncthreads();
     }
     l += __shfl_xor(l, 32, 64);
-    const float up = ldexpf(1.f, max(ev, -149));
-    wide_result<HD>(p, lds, item, h, o, up, m, l);
+    wide_result<HD>(p, lds, item, h, o, half_scale(e, m), m, l);
 }
 
 // The attention of a plan in one launch: wide tiles first, then 16-row tiles,

@@ -76,3 +76,82 @@ def test_later_tokens_leave_earlier_ones_alone(gpu, rs, dim, begin, large):
         got.append(rig.attend(q, check=False)[:begin])
         check(rig, 0, q[:begin], got[-1], 0)
     np.testing.assert_array_equal(got[1], got[0])
+
+
+def keys_at(rs, n, heads, dim, score, at):
+    """Keys whose scores with queries of `queries` are about `score` lower at the places `at`."""
+    k = rs.randn(n, heads, dim).astype(np.float32) * np.float32(0.3)
+    k[at, :, 0] = -score * np.sqrt(dim) / 8
+    return k
+
+
+def queries(rs, n, heads, dim):
+    q = rs.randn(n, heads, dim).astype(np.float32) * np.float32(0.5)
+    q[:, :, 0] = 8
+    return q
+
+
+@pytest.mark.parametrize("fresh", [1, 90])
+@pytest.mark.parametrize("where", [(0, 16), (48, 64), (112, 128), (480, 496)])
+@pytest.mark.parametrize("ratio", [2.0 ** 14, 2.0 ** 24, 2.0 ** 34, 2.0 ** 110])
+@pytest.mark.parametrize("score", [0.0, 12.0, 200.0])
+def test_values_far_apart(gpu, rs, fresh, where, ratio, score):
+    """A block of far larger values that the softmax gives little weight, or none, before, among and after the
+    blocks that a query attends."""
+    rig = Rig(cfg(8, 2, 128), 80, 16, 1, 700)
+    n, at = 496 + fresh, slice(*where)
+    k, v = keys_at(rs, n, 2, 128, score, at), rs.randn(n, 2, 128).astype(np.float32)
+    v[at] *= np.float32(ratio)
+    rig.plan([0], [496])
+    rig.store(None, k[:496], v[:496])
+    rig.plan([0], [fresh])
+    rig.store(None, k[496:], v[496:])
+    q = queries(rs, fresh, 8, 128)
+    check(rig, 0, q, rig.attend(q, check=False), 496)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("large", [1e6, 1e15, 1e30])
+def test_values_that_grow_along_a_prompt(gpu, rs, dim, large):
+    """Every row of a prompt whose first tokens, or last ones, have far larger values."""
+    rig = Rig(cfg(8, 2, dim), 20, 16, 1, 200)
+    for at in (slice(0, 16), slice(5, 40), slice(40, 90)):
+        q, k, v = (rs.randn(90, h, dim).astype(np.float32) for h in (8, 2, 2))
+        v[at] *= np.float32(large)
+        rig.plan([0], [90], [0])
+        rig.store(None, k, v)
+        check(rig, 0, q, rig.attend(q, check=False), 0)
+
+
+@pytest.mark.parametrize("dim,fresh", [(64, 1), (128, 1), (64, 70), (128, 70)])
+def test_values_far_apart_in_other_parts(gpu, rs, dim, fresh):
+    """The same where the large values are another part's, and every block's magnitude is its own."""
+    rig = Rig(cfg(4, 1, dim), 400, 16, 1, 5200, 5200)
+    n = 5000 + fresh
+    block = np.arange(n) // 16
+    loud = rs.randint(0, 2, block[-1] + 1)[block] * (np.arange(n) % 1024 < 600)
+    k = keys_at(rs, n, 1, dim, np.where(loud, rs.choice([0, 7, 60, 300], block[-1] + 1)[block], 0)[:, None], slice(None))
+    v = rs.randn(n, 1, dim).astype(np.float32) * np.exp2(np.where(loud, rs.randint(0, 100, block[-1] + 1)[block], -3)).astype(np.float32)[:, None, None]
+    rig.plan([0], [5000])
+    rig.store(None, k[:5000], v[:5000])
+    rig.plan([0], [fresh])
+    rig.store(None, k[5000:], v[5000:])
+    q = queries(rs, fresh, 4, dim)
+    check(rig, 0, q, rig.attend(q, check=False), 5000)
+
+
+@pytest.mark.parametrize("fresh", [1, 90])
+@pytest.mark.parametrize("scale", [2.0 ** -140, 2.0 ** -126, 2.0 ** -100, 0.0])
+def test_the_smallest_values(gpu, rs, fresh, scale):
+    """Values about fp32's smallest numbers, alone and beside ordinary ones of little weight; zeros with all of it."""
+    rig = Rig(cfg(4, 2, 64), 40, 16, 1, 400)
+    n, at = 300 + fresh, slice(64, 96)
+    for large in (scale, 1.0):
+        k, v = keys_at(rs, n, 2, 64, 60.0, at), rs.randn(n, 2, 64).astype(np.float32) * np.float32(scale)
+        v[at] = rs.randn(32, 2, 64) * large
+        rig.plan([0], [300], [0])
+        rig.store(None, k[:300], v[:300])
+        rig.plan([0], [fresh])
+        rig.store(None, k[300:], v[300:])
+        q = queries(rs, fresh, 4, 64)
+        check(rig, 0, q, rig.attend(q, check=False), 300)
