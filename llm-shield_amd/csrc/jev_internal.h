@@ -483,7 +483,7 @@ struct Pages {
     PagesItem *item = nullptr, *wide = nullptr;
     double2 *angle = nullptr;               // [max_tokens][half] (cos, sin) * mscale
     const double *freqs = nullptr;
-    float *part = nullptr;                  // [max_parts][kv head][16][hd + 4]: output, max, sum
+    float *part = nullptr;                  // [max_parts][kv head][16][hd + 4]: mean, max, sum
     float *wide_part = nullptr;             // [max_wide_parts][kv head][128][hd + 4]
     int32_t *tickets = nullptr, *wide_tickets = nullptr; // [parts][kv head] parts that have arrived, at a tile's first part
     int max_units = 0, max_items = 0, max_wide = 0, max_parts = 0, max_wide_parts = 0;

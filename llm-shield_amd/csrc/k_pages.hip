@@ -786,12 +786,15 @@ struct ValueScale {
     }
 };
 
-// Outputs held times 2^(9 - e) become relative to 2^m by this factor twice: what it is
-// squared may be outside fp32's range.
-__device__ __forceinline__ float half_scale(float e, float m)
-{
-    return e == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(0.5f * (e - 9.f - m));
-}
+// Outputs held times 2^(9 - e), weights relative to 2^m and their sum l: a row's mean of
+// its values is (o * f1) * f2.  In two steps, 2^(e - 9 - m) itself may be outside fp32's
+// range.  Means are also what parts of a row pass on: weighted sums of values that fp32
+// holds may be past it.  A part that sees no key (l = 0) has a mean of zeros.
+struct MeanScale {
+    float f1, f2;
+    __device__ __forceinline__ MeanScale(float e, float m, float l)
+        : f1(e == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(0.5f * (e - 9.f - m))), f2(l == 0.f ? 0.f : f1 / l) {}
+};
 
 // Partial results pass between workgroups inside a launch, which may run on
 // different dies with an L2 each: they are stored and read as agent-scope atomics
@@ -825,24 +828,32 @@ __device__ __forceinline__ bool arrives_last(int32_t *ticket, int parts, int &sh
     return shared;
 }
 
-// One row's parts (part k at at(k): HD outputs, maximum, sum) merged in their
-// order by sixteen threads.
+// One row's parts (part k at at(k): HD means, maximum, sum) merged in their order by
+// sixteen threads.
 template <int HD, typename At>
 __device__ __forceinline__ void merge_parts(At at, int n_parts, float *dst, int j)
 {
     constexpr int N = HD / 16;
-    float m = -INFINITY;
-    for (int k = j; k < n_parts; k += 16) m = fmaxf(m, load_shared(at(k) + HD).x);
+    float m = -INFINITY, l = 0.f;
+    auto join = [&](float mk, float lk) {
+        const float mn = fmaxf(m, mk), mu = mn == -INFINITY ? 0.f : mn;
+        l = l * exp2f(m - mu) + lk * exp2f(mk - mu);
+        m = mn;
+    };
+    for (int k = j; k < n_parts; k += 16) {
+        const float2 ml = load_shared(at(k) + HD);
+        join(ml.x, ml.y);
+    }
 #pragma unroll
-    for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    for (int o = 1; o < 16; o <<= 1) join(__shfl_xor(m, o, 64), __shfl_xor(l, o, 64));
     if (m == -INFINITY) m = 0.f;
-    float x[N] = {}, sum = 0.f;
+    const float inv = 1.f / l;
+    float x[N] = {};
 #pragma unroll 4
     for (int k = 0; k < n_parts; k++) {
         const float *src = at(k);
         const float2 ml = load_shared(src + HD);
-        const float f = exp2f(ml.x - m);
-        sum += ml.y * f;
+        const float f = ml.y * exp2f(ml.x - m) * inv;
 #pragma unroll
         for (int i = 0; i < N; i += 2) { // (a row's sixteen threads side by side)
             const float2 y = load_shared(src + 16 * i + 2 * j);
@@ -852,8 +863,8 @@ __device__ __forceinline__ void merge_parts(At at, int n_parts, float *dst, int 
     }
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-        dst[16 * i + 2 * j] = x[i] / sum;
-        dst[16 * i + 2 * j + 1] = x[i + 1] / sum;
+        dst[16 * i + 2 * j] = x[i];
+        dst[16 * i + 2 * j + 1] = x[i + 1];
     }
 }
 
@@ -1074,9 +1085,9 @@ __device__ __forceinline__ void attend_tiles(const AttendView &p, TileLds<HD> &l
         l += __shfl_xor(l, 32, 64);
 
         // the four waves' results, in wave order
-        const float up = half_scale(e, m);
+        const MeanScale mean(e, m, l);
 #pragma unroll
-        for (int s = 0; s < NS; s++) *(floatx4 *)&lo[wave][n][16 * s + 4 * g] = o[s] * up * up;
+        for (int s = 0; s < NS; s++) *(floatx4 *)&lo[wave][n][16 * s + 4 * g] = o[s] * mean.f1 * mean.f2;
         if (g == 0) {
             lm[wave][n] = m;
             ll[wave][n] = l;
@@ -1089,20 +1100,21 @@ __device__ __forceinline__ void attend_tiles(const AttendView &p, TileLds<HD> &l
 #pragma unroll
             for (int w = 1; w < 4; w++) mm = fmaxf(mm, lm[w][c]);
             const float mu = mm == -INFINITY ? 0.f : mm;
-            float sum = 0.f;
+            float sum = 0.f, f[4];
             floatx4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < 4; w++) {
-                const float f = exp2f(lm[w][c] - mu);
-                sum += ll[w][c] * f;
-                x += *(const floatx4 *)&lo[w][c][d] * f;
+                f[w] = ll[w][c] * exp2f(lm[w][c] - mu);
+                sum += f[w];
             }
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+            for (int w = 0; w < 4; w++) x += *(const floatx4 *)&lo[w][c][d] * (f[w] * inv);
             if (it.part < 0) {
                 const int tk = rr / p.group, hd = h * p.group + rr % p.group;
                 float *dst = p.out + ((size_t)(r.start + tk) * p.n_heads + hd) * HD + d;
-                const float inv = 1.f / sum;
 #pragma unroll
-                for (int k = 0; k < 4; k++) dst[k] = x[k] * inv;
+                for (int k = 0; k < 4; k++) dst[k] = x[k];
             } else {
                 float *dst = p.part + (((size_t)it.part * p.n_kv + h) * kPagesTileRows + c) * LD;
                 store_shared(dst + d, x[0], x[1]);
@@ -1149,7 +1161,7 @@ struct WideLds {
             uint4 kf[2][2 * (HD / 16) * 64], vf[2][4 * (HD / 32) * 64];
             float2 sc[2][4];
         };
-        float rows[kPagesWideRows * (HD + 4)]; // a part: outputs, maximum, sum
+        float rows[kPagesWideRows * (HD + 4)]; // a part: means, maximum, sum
         float factor[8][kPagesWideRows];
     };
     int last;
@@ -1158,7 +1170,7 @@ struct WideLds {
 // A wide tile's end: its outputs, or its part and, from its last part, theirs.
 template <int HD>
 __device__ __forceinline__ void wide_result(const AttendView &p, WideLds<HD> &lds, int item, int h,
-                                            const floatx16 (&o)[HD / 32], float up, float m, float l)
+                                            const floatx16 (&o)[HD / 32], const MeanScale &mean, float m, float l)
 {
     constexpr int ND = HD / 32, LD = HD + 4, kMost = 8;
     // read again: nothing of them takes registers during the products
@@ -1173,11 +1185,10 @@ __device__ __forceinline__ void wide_result(const AttendView &p, WideLds<HD> &ld
     if (it.part < 0) {
         if (wrow >= n_rows) return;
         float *dst = out_of(wrow);
-        const float f = up / l;
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) dst[32 * d + 8 * (i >> 2) + 4 * hh + (i & 3)] = o[d][i] * up * f;
+            for (int i = 0; i < 16; i++) dst[32 * d + 8 * (i >> 2) + 4 * hh + (i & 3)] = o[d][i] * mean.f1 * mean.f2;
         return;
     }
     // through LDS, where the fragments were: whole runs of a row to a store
@@ -1187,7 +1198,7 @@ __device__ __forceinline__ void wide_result(const AttendView &p, WideLds<HD> &ld
 #pragma unroll
         for (int i = 0; i < 4; i++)
             *(floatx4 *)(mine + 32 * d + 8 * i + 4 * hh) =
-                floatx4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]} * up * up;
+                floatx4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]} * mean.f1 * mean.f2;
     if (hh == 0) *(float2 *)(mine + HD) = make_float2(m, l);
     __syncthreads();
     float *part = p.wide_part + ((size_t)it.part * p.n_kv + h) * kPagesWideRows * LD;
@@ -1219,7 +1230,7 @@ __device__ __forceinline__ void wide_result(const AttendView &p, WideLds<HD> &ld
             if (k < r.n_parts) sum += ml[k].y * exp2f(ml[k].x - top);
 #pragma unroll
         for (int k = 0; k < kMost; k++)
-            if (k < r.n_parts) lds.factor[k][tid] = exp2f(ml[k].x - top) / sum;
+            if (k < r.n_parts) lds.factor[k][tid] = ml[k].y * exp2f(ml[k].x - top) / sum;
     }
     __syncthreads();
     constexpr int TH = HD / 2, RT = 256 / TH; // threads of a row, rows at once
@@ -1447,7 +1458,7 @@ __device__ __forceinline__ void attend_wide(const AttendView &p, WideLds<HD> &ld
         __syncthreads();
     }
     l += __shfl_xor(l, 32, 64);
-    wide_result<HD>(p, lds, item, h, o, half_scale(e, m), m, l);
+    wide_result<HD>(p, lds, item, h, o, MeanScale(e, m, l), m, l);
 }
 
 // The attention of a plan in one launch: wide tiles first, then 16-row tiles,

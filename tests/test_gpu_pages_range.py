@@ -155,3 +155,20 @@ def test_the_smallest_values(gpu, rs, fresh, scale):
         rig.store(None, k[300:], v[300:])
         q = queries(rs, fresh, 4, 64)
         check(rig, 0, q, rig.attend(q, check=False), 300)
+
+
+@pytest.mark.parametrize("fresh", [1, 90])
+@pytest.mark.parametrize("n", [200, 1900])
+@pytest.mark.parametrize("large", [1e36, 3e38])
+def test_the_largest_values(gpu, rs, fresh, n, large):
+    """Values about fp32's largest numbers: their sum over the keys is past it, their mean is not."""
+    rig = Rig(cfg(8, 2, 128), 140, 16, 1, 2000)
+    n += fresh
+    k, v = (rs.randn(n, 2, 128).astype(np.float32) * np.float32(0.1) for _ in "kv")
+    v = (rs.uniform(0.5, 1, (n, 2, 128)) * large).astype(np.float32)
+    rig.plan([0], [n - fresh])
+    rig.store(None, k[:-fresh], v[:-fresh])
+    rig.plan([0], [fresh])
+    rig.store(None, k[-fresh:], v[-fresh:])
+    q = rs.randn(fresh, 8, 128).astype(np.float32)
+    check(rig, 0, q, rig.attend(q, check=False), n - fresh)
