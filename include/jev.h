@@ -317,7 +317,7 @@ int jev_get_matmul_strategy(void);
  * graph replayed since has planned more, it does nothing, and jev_pages_sync
  * returns JEV_ESTATE (until the next plan).  Nothing checks that
  * a planned token was stored before it is attended or read: it has whatever its
- * page held.  The stream (jev_pages_stream) orders itself with the device's null
+ * page held, zeros in a new pool.  The stream (jev_pages_stream) orders itself with the device's null
  * stream; a caller on another stream orders the two with events.  A handle's
  * calls share its workspaces: one thread at a time, and no two of its graphs at
  * once.  Pointers are device pointers of the handle's device; floats may have

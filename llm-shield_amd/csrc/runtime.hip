@@ -2608,7 +2608,7 @@ double rope_table64(const jev_config &c, std::vector<double> &freqs)
 }
 
 template <typename T>
-int pages_alloc(jev_pages *h, T *&out, size_t n)
+int pages_alloc(jev_pages *h, T *&out, size_t n, int byte = 0)
 {
     void *b = nullptr;
     const size_t bytes = std::max<size_t>(n, 1) * sizeof(T);
@@ -2619,7 +2619,7 @@ int pages_alloc(jev_pages *h, T *&out, size_t n)
     }
     h->blocks.push_back(b);
     out = (T *)b;
-    HIP_TRY(hipMemsetAsync(b, 0, bytes, h->stream));
+    HIP_TRY(hipMemsetAsync(b, byte, bytes, h->stream));
     return JEV_OK;
 }
 
@@ -2752,8 +2752,9 @@ try {
     const size_t codes = p.n_blocks() * p.n_layers * kPageBlock * p.hd;
     const int words = (p.n_pages + 31) / 32;
     double *dfreqs = nullptr;
-    int rc = pages_alloc(h, p.k, codes);
-    if (!rc) rc = pages_alloc(h, p.v, codes);
+    // a scale of zero has codes of zero from the start: the attention relies on it
+    int rc = pages_alloc(h, p.k, codes, 0x80);
+    if (!rc) rc = pages_alloc(h, p.v, codes, 0x80);
     if (!rc) rc = pages_alloc(h, p.ks, p.n_blocks() * p.n_layers);
     if (!rc) rc = pages_alloc(h, p.table, R * p.width);
     if (!rc) rc = pages_alloc(h, p.length, R);

@@ -172,3 +172,21 @@ def test_the_largest_values(gpu, rs, fresh, n, large):
     rig.store(None, k[-fresh:], v[-fresh:])
     q = rs.randn(fresh, 8, 128).astype(np.float32)
     check(rig, 0, q, rig.attend(q, check=False), n - fresh)
+
+
+@pytest.mark.parametrize("fresh", [1, 40])
+def test_tokens_that_were_not_stored_are_zeros_in_a_new_pool(gpu, rs, fresh):
+    """A layer's blocks that nothing was stored into: read and attended as zeros."""
+    rig = Rig(cfg(4, 2, 64), 40, 16, 1, 400)
+    rig.plan([0], [100])
+    for name in "kv":
+        rig.kv[0, 0, name] = R.Cache(2, 64)
+        rig.kv[0, 0, name].store(0, np.zeros((100, 2, 64)))
+    rig.check_values()
+    q = rs.randn(100, 4, 64).astype(np.float32)
+    assert not rig.attend(q).any()
+    rig.plan([0], [fresh])
+    rig.store(None, *(rs.randn(fresh, 2, 64).astype(np.float32) for _ in "kv"))
+    rig.check_values()
+    q = rs.randn(fresh, 4, 64).astype(np.float32)
+    check(rig, 0, q, rig.attend(q, check=False), 100)
