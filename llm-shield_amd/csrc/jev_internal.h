@@ -436,6 +436,11 @@ __host__ __device__ inline int pages_part_keys(int len)
 {
     return len <= 16384 ? 1024 : len <= 131072 ? 2048 : (len / 64 + 63) & ~63; // at most 65 parts
 }
+// The most parts that a request of at most `len` tokens can have.
+inline int pages_most_parts(int len)
+{
+    return len <= 16384 ? (len + 1023) / 1024 : len <= 32768 ? 16 : len <= 131072 ? (len + 2047) / 2048 : 65;
+}
 
 struct PagesPlanHead {
     int32_t status;  // JEV_OK; JEV_EINVAL or JEV_ENOMEM: everything below is zero; JEV_ESTATE: a call found it too large

@@ -1,5 +1,7 @@
 // The 8-bit paged KV cache (Pages in jev_internal.h): a step's plan from the
 // requests' lengths, rotary positions with the store, attention, reading back.
+#include <algorithm>
+
 #include "../../include/jev.h"
 #include "jev_dev.h"
 
@@ -1489,8 +1491,13 @@ __global__ __launch_bounds__(256, 2) void pages_attend_kernel(AttendView p)
 
 hipError_t launch_pages_attend(const Pages &p, const PagesAttendArgs &a, hipStream_t s)
 {
-    // (no tokens: a workgroup a KV head, for `outgrown`)
-    const int64_t most = a.n_tokens == 0 ? 1 : (int64_t)p.max_parts + (int64_t)a.n_tokens * p.group / kPagesTileRows + a.n_requests;
+    // Workgroups for the parts that the call's requests can have, whatever the pool has
+    // room for: one token over 300 keys in a pool of 2^21 tokens and requests of at most
+    // 8192 7.4 us, with a workgroup for every part of the pool (16384 of them) 10.4.
+    // (No tokens: a workgroup a KV head, for `outgrown`.)
+    const int64_t split = (int64_t)((p.group + kPagesTileRows - 1) / kPagesTileRows) * std::min(a.n_requests, a.n_tokens);
+    const int64_t parts = std::min((int64_t)p.max_parts, split * pages_most_parts(p.max_context));
+    const int64_t most = a.n_tokens == 0 ? 1 : parts + (int64_t)a.n_tokens * p.group / kPagesTileRows + a.n_requests;
     const int64_t most_wide = (int64_t)a.n_tokens * p.group / kPagesWideRows + a.n_requests + pages_wide_target(p.n_kv);
     const int wides = a.wide ? (int)(most_wide * p.n_kv) : 0, tiles = (int)(most < 2048 ? most : 2048) * p.n_kv;
     const size_t bytes = (size_t)kPageBlock * p.hd;
