@@ -406,13 +406,21 @@ hipError_t launch_pages_plan(const Pages &p, const PagesPlanArgs &a, hipStream_t
         return hipErrorInvalidValue;
     const PlanView v = {p.table, p.length, p.n_free, p.fresh_pages, p.prefix, p.used, p.head, p.req, p.unit, p.item, p.wide, p.angle, p.freqs,
                         p.mscale, p.page, p.sub, p.sub_shift, p.n_pages, p.max_requests, p.max_context, p.width, p.half, p.group, p.n_kv};
-    // what the lists write, in words; an angle counts for several
+    // What the lists write, in words; an angle counts for several.  Short lists are written
+    // by the plan's own workgroup (in a graph, so / with a launch of their own: 12 requests
+    // of a token and 64 pairs 6.7 / 7.6 us, 16 9.4 / 10.0, 24 10.8 / 9.8, 64 18.6 / 10.2; one
+    // of 20 tokens 8.1 / 9.5, of 60 11.7 / 9.5).
     const double work = (double)a.n_tokens * (4 + 8.0 * p.half) + (a.table ? (double)a.n_requests * p.width : 0.0);
-    const bool lists = work <= 6144, small = a.n_requests <= 256; // a request to a thread, else up to eight
+    const bool lists = work <= 9216;
+    // A request to a thread of 256, or up to eight to one of 512: 200 requests 12.5 / 13.3 us,
+    // 12 6.7 / 9.0.
+    const bool small = a.n_requests <= 256;
     if (small && lists) hipLaunchKernelGGL((pages_plan_kernel<256, true>), dim3(1), dim3(256), 0, s, v, a);
     else if (small) hipLaunchKernelGGL((pages_plan_kernel<256, false>), dim3(1), dim3(256), 0, s, v, a);
     else if (lists) hipLaunchKernelGGL((pages_plan_kernel<512, true>), dim3(1), dim3(512), 0, s, v, a);
     else hipLaunchKernelGGL((pages_plan_kernel<512, false>), dim3(1), dim3(512), 0, s, v, a);
+    // (2048 words to a workgroup of the lists: 64 requests' tables 12.6 us instead of 11.4;
+    // 128: 64 requests of 300 tokens 42.6 instead of 37.9)
     if (!lists) hipLaunchKernelGGL(pages_lists_kernel, dim3((int)fmin(1024.0, ceil(work / 512))), dim3(256), 0, s, v, a);
     return hipGetLastError();
 }

@@ -27,3 +27,16 @@ result = [grids(pages, requests, context) for pages, requests in ((1 << 10, 4), 
         # two requests of 45 tokens: wide tiles over the workgroups there are, and the 16-row form of either
         assert prompts <= kv * (2 * most + 90 * 4 // 16 + 2) + kv * (90 * 4 // 128 + 2 + 512 // kv)
     assert got[4] == got[8]
+
+
+def test_a_decode_step_of_twelve_rows_plans_in_one_launch():
+    """Its angles among the lists: 12 tokens of 64 pairs, as the model has; 24 are quicker with two."""
+    got = fake_hip.run("""
+p = jev.KvPages(jev.ModelConfig(n_layers=1, n_heads=32, n_kv_heads=8, head_dim=128, rope_dim=128), 4096, 16, 64, 1024, 4096)
+result = []
+for n in (1, 12, 16, 24):
+    launches()
+    p.plan_device(64, 64, 64, n, n)
+    result.append(len(launches()))
+""")
+    assert got == [1, 1, 1, 2]
