@@ -758,17 +758,19 @@ __device__ __forceinline__ uint4 codes_f16(uint32_t w0, uint32_t w1)
 
 // A query row as fp16 pairs: scaled by a power of two so that its largest
 // element m lies in [2^13, 2^14); rows of zeros and rows with infinities stay as
-// they are.  `qs` undoes it in the scores, times the softmax scale for exponents
-// of two; f1 f2 is the factor, in two steps that stay inside fp32's range.
+// they are.  `scores` undoes it in a block's K scale (the power alone may be
+// outside fp32's range) and turns scores into exponents of two; f1 f2 is the factor,
+// in two steps that stay inside that range.
 struct QueryScale {
-    float f1, f2, qs;
-    __device__ __forceinline__ QueryScale(float m, float scale)
+    float f1, f2, scale;
+    int ex;
+    QueryScale() = default;
+    __device__ __forceinline__ QueryScale(float m, float softmax)
+        : scale(softmax * 1.44269504088896341f), ex(m > 0.f && m < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(m) : 0)
     {
-        const int ex = m > 0.f && m < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(m) : 0;
-        const int e1 = ex / 2, e2 = ex - e1;
-        f1 = ldexpf(1.f, e1), f2 = ldexpf(1.f, e2);
-        qs = ldexpf(ldexpf(scale * 1.44269504088896341f, -e1), -e2);
+        f1 = ldexpf(1.f, ex / 2), f2 = ldexpf(1.f, ex - ex / 2);
     }
+    __device__ __forceinline__ float scores(float ks) const { return ldexpf(ks, -ex) * scale; }
     __device__ __forceinline__ void split(float x, _Float16 &hi, _Float16 &lo) const
     {
         const float y = x * f1 * f2;
@@ -976,7 +978,7 @@ __device__ __forceinline__ void attend_tiles(const AttendView &p, TileLds<HD> &l
 
         // Q^T fragments: dims 64 j + 16 g + 8 c .. + 7 of row n
         half8_t qh[2 * NJ], ql[2 * NJ];
-        float qs;
+        QueryScale query;
         {
             const float *src = p.q + ((size_t)(r.start + token) * p.n_heads + head) * HD + 16 * g;
             float x[2 * NJ][8], m = 0.f;
@@ -989,14 +991,13 @@ __device__ __forceinline__ void attend_tiles(const AttendView &p, TileLds<HD> &l
                 }
             m = fmaxf(m, __shfl_xor(m, 16, 64));
             m = fmaxf(m, __shfl_xor(m, 32, 64));
-            const QueryScale s(m, p.scale);
-            qs = s.qs;
+            query = QueryScale(m, p.scale);
 #pragma unroll
             for (int c = 0; c < 2 * NJ; c++)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     _Float16 hi, lw;
-                    s.split(x[c][i], hi, lw);
+                    query.split(x[c][i], hi, lw);
                     qh[c][i] = hi;
                     ql[c][i] = lw;
                 }
@@ -1026,7 +1027,7 @@ __device__ __forceinline__ void attend_tiles(const AttendView &p, TileLds<HD> &l
             }
             if (more) fetch_k(kb + 4, pk);
             // a scale of zero has codes of zero: any other does as well
-            float ks = sc.x * qs, vs = sc.y;
+            float ks = query.scores(sc.x), vs = sc.y;
             ks = ks < 1e-37f ? 1e-37f : ks;
             if (kb * 64 + 63 > clear) {
                 const int left = limit - (kb * 64 + 16 * g); // last visible token of the lane's block
@@ -1326,7 +1327,7 @@ __device__ __forceinline__ void attend_wide(const AttendView &p, WideLds<HD> &ld
 
     // Q^T fragments: dims 16 c + 8 hh .. + 7 of row n
     half8_t qh[NC], ql[NC];
-    float qs;
+    QueryScale query;
     {
         const float *src = p.q + ((size_t)(r.start + token) * p.n_heads + head) * HD + 8 * hh;
         float m = 0.f;
@@ -1335,14 +1336,13 @@ __device__ __forceinline__ void attend_wide(const AttendView &p, WideLds<HD> &ld
 #pragma unroll
             for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(src[16 * c + i]));
         m = fmaxf(m, __shfl_xor(m, 32, 64));
-        const QueryScale y(m, p.scale);
-        qs = y.qs;
+        query = QueryScale(m, p.scale);
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 _Float16 hi, lw;
-                y.split(src[16 * c + i], hi, lw);
+                query.split(src[16 * c + i], hi, lw);
                 qh[c][i] = hi;
                 ql[c][i] = lw;
             }
@@ -1389,7 +1389,7 @@ __device__ __forceinline__ void attend_wide(const AttendView &p, WideLds<HD> &ld
         const float4 s01 = *(const float4 *)&sc[buf][0], s23 = *(const float4 *)&sc[buf][2];
         const float2 s0 = hh ? make_float2(s01.z, s01.w) : make_float2(s01.x, s01.y);
         const float2 s1 = hh ? make_float2(s23.z, s23.w) : make_float2(s23.x, s23.y);
-        float ks[2] = {s0.x * qs, s1.x * qs}, vs[2] = {s0.y, s1.y};
+        float ks[2] = {query.scores(s0.x), query.scores(s1.x)}, vs[2] = {s0.y, s1.y};
 #pragma unroll
         for (int t = 0; t < 2; t++) ks[t] = ks[t] < 1e-37f ? 1e-37f : ks[t]; // a scale of zero has codes of zero
         if (kb * 64 + 63 > clear) {

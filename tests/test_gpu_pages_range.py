@@ -190,3 +190,21 @@ def test_tokens_that_were_not_stored_are_zeros_in_a_new_pool(gpu, rs, fresh):
     rig.check_values()
     q = rs.randn(fresh, 4, 64).astype(np.float32)
     check(rig, 0, q, rig.attend(q, check=False), 100)
+
+
+@pytest.mark.parametrize("fresh", [1, 90])
+@pytest.mark.parametrize("large,small", [("k", "q"), ("q", "k")])
+@pytest.mark.parametrize("by", [1e30, 3e37])
+def test_queries_and_keys_at_the_ends_of_the_range(gpu, rs, fresh, large, small, by):
+    """Scores of about one from a factor near fp32's smallest numbers and one near its largest."""
+    rig = Rig(cfg(8, 2, 128), 40, 16, 1, 500)
+    n = 400 + fresh
+    x = {"q": rs.randn(fresh, 8, 128), "k": rs.randn(n, 2, 128), "v": rs.randn(n, 2, 128)}
+    x[large] *= by
+    x[small] /= by
+    x = {name: y.astype(np.float32) for name, y in x.items()}
+    rig.plan([0], [400])
+    rig.store(None, x["k"][:400], x["v"][:400])
+    rig.plan([0], [fresh])
+    rig.store(None, x["k"][400:], x["v"][400:])
+    check(rig, 0, x["q"], rig.attend(x["q"], check=False), 400)
