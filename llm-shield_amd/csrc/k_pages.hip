@@ -1505,7 +1505,7 @@ hipError_t launch_pages_attend(const Pages &p, const PagesAttendArgs &a, hipStre
     // (No tokens: a workgroup a KV head, for `outgrown`.)
     const int64_t split = (int64_t)((p.group + kPagesTileRows - 1) / kPagesTileRows) * std::min(a.n_requests, a.n_tokens);
     const int64_t parts = std::min((int64_t)p.max_parts, split * pages_most_parts(p.max_context));
-    const int64_t most = a.n_tokens == 0 ? 1 : parts + (int64_t)a.n_tokens * p.group / kPagesTileRows + a.n_requests;
+    const int64_t most = a.n_tokens == 0 ? 1 : std::max<int64_t>(1, parts + (int64_t)a.n_tokens * p.group / kPagesTileRows + a.n_requests);
     const int64_t most_wide = (int64_t)a.n_tokens * p.group / kPagesWideRows + a.n_requests + pages_wide_target(p.n_kv);
     const int wides = a.wide ? (int)(most_wide * p.n_kv) : 0, tiles = (int)(most < 2048 ? most : 2048) * p.n_kv;
     const size_t bytes = (size_t)kPageBlock * p.hd;

@@ -40,3 +40,17 @@ for n in (1, 12, 16, 24):
     result.append(len(launches()))
 """)
     assert got == [1, 1, 1, 2]
+
+
+def test_a_batch_of_no_requests_is_launched():
+    """Rows to spare and nothing in them: a grid all the same."""
+    got = fake_hip.run("""
+p = jev.KvPages(jev.ModelConfig(n_layers=1, n_heads=4, n_kv_heads=4, head_dim=64, rope_dim=64), 64, 16, 4, 256, 256)
+result = []
+for t in (0, 1, 5):
+    p.plan_device(0, 0, 0, 0, t)
+    p.store_device(0, 64, 256, 64, 64, 256, 128)
+    p.attend_device(0, 64, 128)
+    result += [min(g) for _, g, _, _ in launches()]
+""")
+    assert min(got) >= 1 and len(got) >= 9
