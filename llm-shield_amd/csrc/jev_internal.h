@@ -419,19 +419,21 @@ constexpr int kPageBlock = 16;         // tokens that share a scale
 constexpr int kPagesMaxRequests = 4096; // a plan's prefix sums live in LDS
 constexpr int kPagesTileRows = 16;     // (token, head) rows of a KV head in one attention tile
 constexpr int kPagesWideRows = 128;    // the same in a wide tile, for requests that add many tokens
-// Wide tiles are split over their keys when there are few: into at most this
-// many workgroups over all KV heads (two fit a compute unit: one round), none of
-// less than kPagesWideKeys keys.
+// Wide tiles are split over their keys when there are few, into no parts of less than
+// kPagesWideKeys keys: fewer tiles than half of this many workgroups over all KV heads (two
+// fit a compute unit: one round) into at most as many, more tiles into half as many on top.
 constexpr int kPagesWideWgs = 512, kPagesWideKeys = 512;
 __host__ __device__ inline int pages_wide_target(int n_kv) { return n_kv < kPagesWideWgs ? kPagesWideWgs / n_kv : 1; }
 
 // Keys per workgroup of a 16-row tile: a function of the request's own length
 // alone, so that its result does not depend on the other requests.  Fewer keys
-// spread a lone request further, more save each part's start and end (us a pass,
-// 512 / 1024 / 2048 keys: one request of 4000 4.5 / 5.3 / 7.5, of 30000 11.5 / 11.0 /
-// 10.6; 64 of 500 to 12000 91 / 86 / 83, 128 of 2000 106 / 94 / 87; one call after
-// the other in a graph, 512 / 1024: one of 2000 9.5 / 12.2, 16 of 4000 34.8 / 29.7,
-// 700 of 100 to 900 179 / 145).
+// spread a lone request further, more save each part's start and end (us, one call after
+// the other in a graph, 512 / 1024 / 2048 keys up to 16384: one request of 2000 9.8 /
+// 12.3 / 15.2, of 4000 10.9 / 13.1 / 18.8; 12 of 500 to 2000 15.0 / 14.5 / 16.0; 16 of
+// 4000 34.7 / 29.5 / 30.0; 64 of 2000 58.9 / 53.4 / 48.4, of 500 to 12000 181 / 162 / 162;
+// 700 of 100 to 900 179 / 143 / 143).  1024 / 2048 / 4096 past 16384: one of 20000 18.1 /
+// 20.9 / 31.1, of 60000 38.4 / 33.4 / 40.2, of 120000 71.2 / 57.7 / 59.0; 4 of 30000 55.0 /
+// 50.5 / 49.1.
 __host__ __device__ inline int pages_part_keys(int len)
 {
     return len <= 16384 ? 1024 : len <= 131072 ? 2048 : (len / 64 + 63) & ~63; // at most 65 parts

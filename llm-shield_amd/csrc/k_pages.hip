@@ -206,7 +206,7 @@ __device__ __forceinline__ void plan_lists(const PlanView &p, const PagesPlanArg
 // launch of its own, over the whole GPU).  Checks first: a plan that does not
 // fit changes nothing and plans no tokens.  Bounded by latency: a few trips to
 // memory, each of which every thread makes at once (12 requests of a token each,
-// lists among it, 8.6 us in a graph; 700 of up to 150 tokens 17 us, their lists 12).
+// every output among it, 8.9 us in a graph; 700 of up to 150 tokens 17 us, their lists 11).
 template <int NT, bool LISTS>
 __global__ __launch_bounds__(NT) void pages_plan_kernel(PlanView p, PagesPlanArgs a)
 {
@@ -547,9 +547,12 @@ struct StoreView {
 // are 64-bit and round to fp32 once, so a stored code does not depend on how
 // they are formed.  A block's scale only grows while the block fills; codes it
 // already holds are then rounded to the new one.  Bounded by memory: 4 B in per
-// element, 1 B (K, V) or 4 B (q) out (queries alone, 8200 tokens x 32 x 128: 54 us,
-// 5.0 TB/s; 9400 tokens of 11 prompts with 8 KV heads 96 us, 4.2 TB/s; with a row of
-// its own for each thread, and its angles, 67 and 198 with the reading back).
+// element, 1 B (K, V) or 4 B (q) out, a begun block's codes both ways (queries alone, 8200 tokens x 32 x 128: 54 us,
+// 5.0 TB/s; 9400 tokens of 11 prompts with 8 KV heads 95 us, 4.2 TB/s; with a row of
+// its own for each thread, and its angles, 67 and 198 with the reading back).  A single
+// token has its whole block read, coded and written again, a chain of trips to memory and
+// barriers in small workgroups: 64 requests 7.5 us, 700 34 (where every scale grows, and
+// every code with it, 3.5 and 14 more).
 template <int HD, bool VEC>
 __global__ __launch_bounds__(256) void pages_store_kernel(StoreView p)
 {
@@ -812,7 +815,7 @@ struct MeanScale {
 // different dies with an L2 each: they are stored and read as agent-scope atomics
 // (written through, and read past, caches that other dies do not see), two floats
 // at a time.  A fence would write back the whole L2 of the die for every part
-// (measured: 64 rows of up to 12000 keys 1090 us instead of 104).
+// (measured: 64 rows of up to 12000 keys 1090 us instead of 104, a launch at a time).
 __device__ __forceinline__ void store_shared(float *p, float x, float y)
 {
     __hip_atomic_store((uint64_t *)p, (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -909,12 +912,13 @@ struct AttendView {
 // Codes are exact in fp16; q and p enter as fp16 pairs (hi + lo), ~22 bits, so
 // each product is two matrix instructions.  p carries the V scale through its
 // exponent (ValueScale): one fused multiply-add and one exp2 a score; the maxima move
-// only when a score passes one by 2^6.  Statistics, scores and outputs are fp32.  The next 64 keys' K is in
-// flight during the softmax and V^T P^T, their V during the next scores.
-// Single tokens are bound by HBM: 2 hd bytes a key and KV head (32 heads over 8 x
-// 128: 64 tokens over 500 to 12000 keys 86 us, 5.8 TB/s; one over 120002 41 us, 5.9;
-// with the next keys asked for after the products 109 and 48).  A lone short request waits for
-// its trips to memory instead: one over 4000 keys 13 us.
+// only when a score passes one by 2^6.  Statistics, scores and outputs are fp32.  The
+// next 64 keys' K is in flight during the softmax and V^T P^T, their V during the next
+// scores.  Many single tokens are bound by HBM: 2 hd bytes a key and KV head (32 heads
+// over 8 x 128, one call after the other over different layers: 64 tokens over 500 to
+// 12000 keys 98 us, 5.1 TB/s; 64 of another draw, 899 MB, 162 us, 5.5).  Few of them wait
+// for their trips to memory instead, and for their parts' merge: one over 300 keys 7.5 us,
+// over 4000 13.3, over 30000 25, over 120002 58 (4.2 TB/s), 12 over 500 to 2000 15.4.
 template <int HD>
 struct TileLds {
     float lo[4][kPagesTileRows][HD + 4];
@@ -1162,9 +1166,12 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 // the maximum moves only when a score passes it by 2^6, so most blocks rescale
 // nothing.  Bound by the matrix cores at two instructions a product, with the
 // exponentials and fp16 pairs of ~9 vector instructions a score beside them: four
-// prompts of 300 to 4000 tokens 320 us, 540 TFLOP/s (a product counted once), the
-// matrix cores 56 % busy and the clock at what the power allows (1.91 GHz).  64 rows
-// to a wave halve the LDS reads and are slower (345 us: one workgroup a compute unit).
+// prompts of 300 to 4000 tokens 312 to 328 us by the card, 530 to 556 TFLOP/s (a product
+// counted once), the matrix cores 56 % busy and the clock at what the power allows
+// (1.91 GHz).  64 rows to a wave halve the LDS reads and are slower (315 -> 345 us: one
+// workgroup a compute unit).  Tens of tokens behind a long cache are bound by what is not
+// split: 9 x 48 over 4096 keys 98 us, of 52, for waves without rows, 80 of 512 places
+// empty, and one workgroup that merges each tile's parts.
 template <int HD>
 struct WideLds {
     union {
@@ -1533,7 +1540,7 @@ struct ReadView {
 // Sixteen slots and one KV head to a workgroup.  K rows lie in runs of 64
 // dims.  V lies dim by dim, so its bytes are read with the tokens along the
 // lanes (neighbouring slots: one 64-byte run per load) and turned in LDS.  Bounded
-// by what it writes (9400 slots of 8 x 128: 26 us, 3.0 TB/s).
+// by what it writes (9400 slots of 8 x 128: 23 us, 3.4 TB/s).
 template <int HD>
 __global__ __launch_bounds__(256) void pages_read_kernel(ReadView p)
 {
