@@ -804,7 +804,8 @@ struct ValueScale {
 // Outputs held times 2^(9 - e), weights relative to 2^m and their sum l: a row's mean of
 // its values is (o * f1) * f2.  In two steps, 2^(e - 9 - m) itself may be outside fp32's
 // range.  Means are also what parts of a row pass on: weighted sums of values that fp32
-// holds may be past it.  A part that sees no key (l = 0) has a mean of zeros.
+// holds may be past it.  A part that sees no key (l = 0) has a mean of zeros; a row that
+// has no weight in any part, all its scores past fp32's range, is NaN.
 struct MeanScale {
     float f1, f2;
     __device__ __forceinline__ MeanScale(float e, float m, float l)
@@ -1122,7 +1123,7 @@ __device__ __forceinline__ void attend_tiles(const AttendView &p, TileLds<HD> &l
                 f[w] = ll[w][c] * exp2f(lm[w][c] - mu);
                 sum += f[w];
             }
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const float inv = sum == 0.f && it.part >= 0 ? 0.f : 1.f / sum;
 #pragma unroll
             for (int w = 0; w < 4; w++) x += *(const floatx4 *)&lo[w][c][d] * (f[w] * inv);
             if (it.part < 0) {
@@ -1203,10 +1204,11 @@ __device__ __forceinline__ void wide_result(const AttendView &p, WideLds<HD> &ld
     if (it.part < 0) {
         if (wrow >= n_rows) return;
         float *dst = out_of(wrow);
+        const float f2 = mean.f1 / l;
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) dst[32 * d + 8 * (i >> 2) + 4 * hh + (i & 3)] = o[d][i] * mean.f1 * mean.f2;
+            for (int i = 0; i < 16; i++) dst[32 * d + 8 * (i >> 2) + 4 * hh + (i & 3)] = o[d][i] * mean.f1 * f2;
         return;
     }
     // through LDS, where the fragments were: whole runs of a row to a store

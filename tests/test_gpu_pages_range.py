@@ -208,3 +208,22 @@ def test_queries_and_keys_at_the_ends_of_the_range(gpu, rs, fresh, large, small,
     rig.plan([0], [fresh])
     rig.store(None, x["k"][400:], x["v"][400:])
     check(rig, 0, x["q"], rig.attend(x["q"], check=False), 400)
+
+
+@pytest.mark.parametrize("fresh", [1, 90])
+@pytest.mark.parametrize("past", [40, 1500])
+def test_scores_past_the_range_are_no_numbers(gpu, rs, fresh, past):
+    """All scores past fp32's least number: NaN, not zeros.  Where one key has a score within the range, its value."""
+    rig = Rig(cfg(4, 2, 64), 140, 16, 1, 2000)
+    n = past + fresh
+    k, v = np.full((n, 2, 64), -1e20, np.float32), rs.randn(n, 2, 64).astype(np.float32)
+    k[16:32, 1] = 0
+    v[16:32, 1] = 127 * 2.0 ** -5
+    rig.plan([0], [past])
+    rig.store(None, k[:past], v[:past])
+    rig.plan([0], [fresh])
+    rig.store(None, k[past:], v[past:])
+    got = rig.attend(np.full((fresh, 4, 64), 1e20, np.float32), check=False)
+    assert np.isnan(got[:, :2]).all()
+    # sixteen equal weights of one value: a rounding each of their sum's parts
+    np.testing.assert_allclose(got[:, 2:], 127 * 2.0 ** -5, rtol=2.0 ** -20)
