@@ -291,12 +291,12 @@ enum { JEV_MATMUL_AUTO = 0, JEV_MATMUL_FLOAT = 1, JEV_MATMUL_INTEGER = 2 };
 int jev_set_matmul_strategy(int strategy);
 int jev_get_matmul_strategy(void);
 
-/* ---- A paged KV cache held in 8 bits, for many requests at once ---- */
+/* ---- A paged KV cache held in 8 or 4 bits, for many requests at once ---- */
 
 /* No counterpart in the reference, whose KvCache belongs to one conversation.
  * A jev_pages is a pool of pages in HBM that requests share: a request is a row
  * of a page table on the device, and grows by whole pages.  K and V take one
- * byte an element.  Sixteen consecutive positions of a request are a block;
+ * byte an element, or four bits (jev_pages_create_bits, below).  Sixteen consecutive positions of a request are a block;
  * per layer, KV head and block K has one scale and V another:
  *
  *   scale = max |x| / 127 (fp32) over the block's values,  code = x / scale
@@ -341,6 +341,25 @@ typedef struct jev_pages_config {
  * with jev_create's meaning (rope_dim 0: no rotation); frequencies, angles and
  * rotations are in 64 bits here, rounded to fp32 once. */
 int jev_pages_create(const jev_config *model, const jev_pages_config *cfg, int device, jev_pages **out);
+
+/* The same with `bits` of 8 or 4 an element; every other call takes either
+ * cache.  In 4 bits a token's row of a KV head, K or V, is held by itself: no
+ * other token changes what it reads as.  The row has a power of two 2^e, and
+ * each 32 elements of it a step u in 1 .. 15 and a zero point z in 0 .. 15; an
+ * element's code n in 0 .. 15 reads as (n - z) u 2^e, exactly.  With hi and lo
+ * the largest of 0 and x, and of 0 and -x, over the 32 elements, and their span
+ * hi + lo in fp32 (as half of it, which stays inside fp32's range):
+ *
+ *   e = the least whole number, at least -126, with every span <= 225 * 2^e
+ *   u = the least one, at least 1, with span <= 15 u 2^e
+ *   z = lo / (u 2^e),  n = x / (u 2^e) + z held to 0 .. 15, each quotient
+ *       rounded to the nearest whole number (a half to the even one),
+ *
+ * so a value is off by at most half a step, and zeros are zeros.  A value that
+ * is not finite, in K or V, makes its token read as NaN there, K and V of that
+ * KV head alone.  A page's bytes, of all layers and KV heads: head_dim (1 + 1 /
+ * 16) + 2 a token, where 8 bits take 2 head_dim + 1 / 2. */
+int jev_pages_create_bits(const jev_config *model, const jev_pages_config *cfg, int32_t bits, int device, jev_pages **out);
 void jev_pages_destroy(jev_pages *p);
 
 /* A step's bookkeeping on the device.  Batch row b < n_requests names request
@@ -376,8 +395,8 @@ int jev_pages_store_device(jev_pages *p, int32_t layer, const float *q, int64_t 
  * h / (n_heads / n_kv_heads).  q and out are [n_tokens][n_heads * head_dim] and
  * must not overlap; rows past the planned total stay as they were.  Scores,
  * weights and sums have fp32's accuracy or nearly (weights 2^-21), wherever scales
- * lie: a key's weight times its V scale loses at most 2^-32 of the largest such
- * product among the keys that the query sees.  A token's
+ * lie: a key's weight times its V scale (4 bits: 2^e) loses at most 2^-32 of the
+ * largest such product among the keys that the query sees.  A token's
  * result has the same bits whatever else is in the batch where its request adds
  * one token, or few: fresh * heads per KV head <= 16. */
 int jev_pages_attend_device(jev_pages *p, int32_t layer, const float *q, float *out);

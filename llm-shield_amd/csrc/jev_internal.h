@@ -469,12 +469,13 @@ struct Pages {
     int n_layers = 0, n_heads = 0, n_kv = 0, hd = 0, group = 1;
     int page = 16, sub = 1, sub_shift = 0;  // tokens and blocks of a page (powers of two)
     int n_pages = 0, max_requests = 0, max_context = 0, max_tokens = 0, width = 0; // width: pages of a table row
+    int bits = 8;                           // of a code: 8 (above) or 4 (Pages4)
     int half = 0, rope_half = 0;            // rotated pairs; 0: (2i, 2i + 1), 1: (i, i + half)
     int orig_ctx = 0;
     float temp_scale = 0.f, scale = 0.f;    // attention temperature; softmax scale
     double mscale = 1.0;
     // pool
-    uint8_t *k = nullptr, *v = nullptr;     // [layer][page][kv head][block][16 * hd]
+    uint8_t *k = nullptr, *v = nullptr;     // [layer][page][kv head][block][16 * hd]; 4 bits: k alone, [pages4_bytes(hd)]
     float2 *ks = nullptr;                   // [layer][page][kv head][block] (K scale, V scale)
     // state
     int32_t *table = nullptr;               // [request][width]
@@ -496,6 +497,19 @@ struct Pages {
     int max_units = 0, max_items = 0, max_wide = 0, max_parts = 0, max_wide_parts = 0;
     __host__ __device__ size_t n_blocks() const { return (size_t)n_pages * n_kv * sub; } // of a layer
 };
+// A block of the 4-bit cache, as the matrix cores take its operands from it: byte offsets of
+//   k   [16 tokens][hd / 2] codes
+//   v   [hd / 32][16 dims][2: dims 16 apart][16 tokens] codes, 8 bytes each
+//   ks  [hd / 32][4] words, K's steps and zero points of tokens r, r + 4, r + 8, r + 12
+//   vs  [hd / 32][4] words, V's steps of tokens 0 - 7, 8 - 15, its zero points of the same
+//   ke, ve  [16 tokens] e + 127; 0: a row of zeros; ve 255: K and V read as NaN
+// and their sum.  Zeroed memory is a block of zeros.
+struct Pages4 {
+    int k, v, ks, vs, ke, ve, bytes;
+    __host__ __device__ constexpr Pages4(int hd)
+        : k(0), v(8 * hd), ks(16 * hd), vs(16 * hd + hd / 2), ke(17 * hd), ve(17 * hd + 16), bytes(17 * hd + 32) {}
+};
+__host__ __device__ constexpr int pages4_bytes(int hd) { return Pages4(hd).bytes; }
 struct PagesPlanArgs {
     const int32_t *request = nullptr, *past = nullptr, *fresh = nullptr; // past may be null: keep everything
     int n_requests = 0, n_tokens = 0;
@@ -513,6 +527,7 @@ struct PagesStoreArgs {
     int n_requests = 0, n_tokens = 0; // of the plan
 };
 hipError_t launch_pages_store(const Pages &p, const PagesStoreArgs &a, hipStream_t s);
+hipError_t launch_pages4_store(const Pages &p, const PagesStoreArgs &a, hipStream_t s);
 struct PagesAttendArgs {
     int layer = 0;
     const float *q = nullptr; // [n_tokens][n_heads * hd]
@@ -521,7 +536,9 @@ struct PagesAttendArgs {
     hipEvent_t ev_start = nullptr, ev_stop = nullptr; // optional dispatch-stamped timing
 };
 hipError_t launch_pages_attend(const Pages &p, const PagesAttendArgs &a, hipStream_t s);
+hipError_t launch_pages4_attend(const Pages &p, const PagesAttendArgs &a, hipStream_t s);
 // k, v [n][n_kv][hd] = the values at slots; zeros for slots outside the pool.
 hipError_t launch_pages_read(const Pages &p, int layer, const int32_t *slot, int n, float *k, float *v, hipStream_t s);
+hipError_t launch_pages4_read(const Pages &p, int layer, const int32_t *slot, int n, float *k, float *v, hipStream_t s);
 
 } // namespace jev

@@ -1,0 +1,743 @@
+// The 4-bit paged KV cache (Pages with bits = 4 in jev_internal.h): rotary positions with
+// the store, attention, reading back.  Plans are the 8-bit cache's (k_pages.hip).
+//
+// A token's row of a KV head (K or V, hd elements) has a power of two 2^e, and each 32
+// elements of it a step u (1 .. 15) and a zero point z (0 .. 15): an element's code n (0 ..
+// 15) stands for (n - z) u 2^e.  (n - z) u is a whole number of at most 225, exact in fp16,
+// so the matrix cores multiply what is stored, and 2^e enters as an exponent.  Rows do not
+// depend on each other: storing a token reads and rounds nothing that is there.
+#include <algorithm>
+
+#include "jev_pages_dev.h"
+
+namespace jev {
+
+namespace {
+
+// A block's bytes (16 tokens of a KV head, Pages4 in jev_internal.h).  A 32-bit word holds
+// eight nibbles, turned two bits to the left so that the second and sixth lie where a
+// masked word is two fp16 numbers 16 + n as it stands: pair p of a word is its nibbles p
+// (low half) and p + 4 (high half).
+constexpr uint32_t kNibble = 0x03c003c0u, kSixteen = 0x4c004c00u;
+
+__device__ __forceinline__ uint32_t turn_left(uint32_t x, int by) { return __builtin_rotateleft32(x, by); }
+
+// Bit of element i (0 .. 7) of a word before the turn: pairs (0, 1), (2, 3), ...
+__host__ __device__ constexpr int nibble_at(int i) { return 4 * ((i >> 1) + 4 * (i & 1)); }
+
+// Pair p of a word as fp16: 16 + n.
+template <int P>
+__device__ __forceinline__ half2_t nibble_pair(uint32_t w)
+{
+    const uint32_t x = P == 0 ? w << 4 : P == 1 ? w : P == 2 ? w >> 4 : turn_left(w, 24);
+    return __builtin_bit_cast(half2_t, (x & kNibble) | kSixteen);
+}
+
+// Steps and zero points turn 16 + n into (n - z) u: (16 + n) u - (16 + z) u, where the
+// second product is a whole number below 2^9.
+struct Steps {
+    half2_t u, m;
+    Steps() = default;
+    __device__ __forceinline__ Steps(half2_t u16, half2_t z16) : u(u16 - half2_t{(_Float16)16.f, (_Float16)16.f}), m(-z16 * u) {}
+    __device__ __forceinline__ uint32_t operator()(half2_t n16) const
+    {
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(n16, u, m));
+    }
+};
+
+// A word's eight elements: with the same step for all, and with one for each pair's halves.
+__device__ __forceinline__ half8_t word_f16(uint32_t w, const Steps &s)
+{
+    return __builtin_bit_cast(half8_t, make_uint4(s(nibble_pair<0>(w)), s(nibble_pair<1>(w)), s(nibble_pair<2>(w)), s(nibble_pair<3>(w))));
+}
+__device__ __forceinline__ half8_t word_f16(uint32_t w, const Steps (&s)[4])
+{
+    return __builtin_bit_cast(half8_t, make_uint4(s[0](nibble_pair<0>(w)), s[1](nibble_pair<1>(w)), s[2](nibble_pair<2>(w)), s[3](nibble_pair<3>(w))));
+}
+
+// Pair t of K's step word (u of token 4 t + r low, its z high), for all of a token's group.
+template <int T>
+__device__ __forceinline__ Steps key_steps(uint32_t w)
+{
+    const half2_t uz = nibble_pair<T>(w);
+    return Steps(half2_t{uz[0], uz[0]}, half2_t{uz[1], uz[1]});
+}
+// V's step and zero words of eight tokens.
+__device__ __forceinline__ void value_steps(uint32_t u, uint32_t z, Steps (&s)[4])
+{
+    s[0] = Steps(nibble_pair<0>(u), nibble_pair<0>(z));
+    s[1] = Steps(nibble_pair<1>(u), nibble_pair<1>(z));
+    s[2] = Steps(nibble_pair<2>(u), nibble_pair<2>(z));
+    s[3] = Steps(nibble_pair<3>(u), nibble_pair<3>(z));
+}
+
+__device__ __forceinline__ uint32_t word_of(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ int byte_of(const uint4 &v, int i) { return (int)((word_of(v, i >> 2) >> (8 * (i & 3))) & 255u); }
+
+__device__ __forceinline__ int most_byte(const uint4 &v)
+{
+    typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
+    ushort2_t m = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t w = word_of(v, i);
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(ushort2_t, w & 0x00ff00ffu));
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(ushort2_t, (w >> 8) & 0x00ff00ffu));
+    }
+    return max((int)m[0], (int)m[1]);
+}
+
+uint8_t *layer4_of(const Pages &p, int layer) { return p.k + (size_t)layer * p.n_blocks() * pages4_bytes(p.hd); }
+
+// y / u to the nearest whole number, a half to the even one; u whole, 1 .. 15, |y| <= 225.
+// The remainder is exact: it is a multiple of y's last bit and not larger than y or u.
+__device__ __forceinline__ float whole_steps(float y, float u, float inv)
+{
+    float q = rintf(y * inv);
+    const float rest = fmaf(-q, u, y), twice = 2.f * fabsf(rest);
+    if (twice > u || (twice == u && ((int)q & 1))) q += rest > 0.f ? 1.f : -1.f;
+    return q;
+}
+
+struct Store4View {
+    uint8_t *pool;
+    PagesPlanHead *head;
+    const PagesUnit *unit;
+    const double2 *angle;
+    const float *q, *k_in, *v_in;
+    float *q_out;
+    int64_t q_ld, kv_ld;
+    size_t in_stride;
+    int nin, n_kv, n_heads, group, sub, sub_shift, half, rope_half, orig_ctx;
+    float temp_scale;
+    int n_tokens, n_requests, wide; // of the call's plan
+};
+
+} // namespace
+
+// One workgroup per block that the batch touches and KV head: the block's new tokens'
+// queries (of the head's group) rotated, their keys rotated, keys and values stored.
+// Sixteen threads hold a token's row; the rotated rows pass through LDS, and a thread
+// takes hd / 16 neighbouring elements of them to steps and codes.  Words that hold other
+// tokens' nibbles (V's, and all steps) are read first and merged.  Rotations are 64-bit
+// and round to fp32 once, quotients are exact: a stored value does not depend on how
+// they are formed.
+template <int HD, bool VEC>
+__global__ __launch_bounds__(256) void pages4_store_kernel(Store4View p)
+{
+    constexpr int NP = HD / 32, NE = HD / 16, NG = HD / 32, TG = 32 / NE, LD = HD + 4, RING = 2;
+    constexpr Pages4 at(HD);
+    __shared__ __align__(16) float xs[2][kPageBlock][LD];
+    __shared__ uint8_t code[kPageBlock][HD];                    // V's
+    __shared__ uint8_t step[2][kPageBlock][NG], zero[2][kPageBlock][NG];
+    const int tid = threadIdx.x, j = tid & 15, h = blockIdx.y;
+    const PagesUnit un = p.unit[blockIdx.x];
+    const PagesPlanHead plan = *p.head; // (the unit's load does not wait for this)
+    if (outgrown(p, plan) || (int)blockIdx.x >= plan.n_units) return;
+    const int pos0 = un.pos, n = un.n, row0 = un.row, off = pos0 & (kPageBlock - 1);
+    const bool kv = p.k_in != nullptr;
+    const RowPairs<HD> e(p, j);
+
+    // this thread's token, and its rows: K (-2), V (-1), then the group's queries
+    const int nt = n > 8 ? 16 : n > 4 ? 8 : n > 2 ? 4 : n, jump = 16 / nt; // (nt: 1, 2, 4, 8, 16)
+    const int t = (tid >> 4) % nt, row = row0 + t, first = (kv ? -2 : 0) + (tid >> 4) / nt, end = t < n && p.q ? p.group : 0;
+    const bool mine = t < n;
+
+    // where the block lies, and the words of it that hold other tokens too
+    uint8_t *block = p.pool + ((((size_t)(un.block >> p.sub_shift) * p.n_kv + h) << p.sub_shift) | (un.block & (p.sub - 1))) * at.bytes;
+    uint32_t *vword = (uint32_t *)(block + at.v) + tid, *sword = (uint32_t *)(block + at.ks) + tid;
+    const bool has_v = kv && tid < 2 * HD, has_s = kv && tid < 8 * NG;
+    uint32_t old_v = 0, old_s = 0;
+    if (off > 0) {
+        if (has_v) old_v = *vword;
+        if (has_s) old_s = *sword;
+    }
+    double2 g[NP];
+#pragma unroll
+    for (int c = 0; c < NP; c++) {
+        const int q = NP * j + c;
+        g[c] = mine && q < p.half ? p.angle[(size_t)row * p.half + q] : make_double2(0.0, 0.0);
+    }
+    auto load = [&](int which, float2 (&y)[NP]) {
+        const float *src = which == -2 ? p.k_in + row * p.kv_ld + h * HD
+                           : which == -1 ? p.v_in + row * p.kv_ld + h * HD
+                                         : p.q + row * p.q_ld + (size_t)(h * p.group + which) * HD;
+        load_pairs<HD, VEC>(e, src, y);
+        for (int i = 1; i < p.nin; i++) {
+            float2 w[NP];
+            load_pairs<HD, VEC>(e, src + i * p.in_stride, w);
+#pragma unroll
+            for (int c = 0; c < NP; c++) y[c] = make_float2(y[c].x + w[c].x, y[c].y + w[c].y);
+        }
+    };
+    auto rotate = [&](double f, float2 (&y)[NP]) {
+#pragma unroll
+        for (int c = 0; c < NP; c++) {
+            const double u = y[c].x, v = y[c].y;
+            const double m0 = u * g[c].x, m1 = v * g[c].y, m2 = u * g[c].y, m3 = v * g[c].x;
+            const bool turned = NP * j + c < p.half;
+            y[c] = make_float2((float)((turned ? m0 - m1 : u) * f), (float)((turned ? m2 + m3 : v) * f));
+        }
+    };
+
+    int w = first;
+    if (kv) {
+        float2 x[2][NP]; // this thread's rows of K and V
+#pragma unroll
+        for (int it = 0; it < 2; it++)
+            if (mine && w + it * jump < 0) load(w + it * jump, x[it]);
+#pragma unroll
+        for (int it = 0; it < 2; it++) {
+            const int which = w + it * jump;
+            if (!mine || which >= 0) continue;
+            if (which == -2) rotate(1.0, x[it]);
+            store_pairs<HD, VEC>(e, xs[which + 2][t], x[it]);
+        }
+        while (w < 0) w += jump;
+    }
+    if (end) {
+        double f = 1.0;
+        const int pos = pos0 + t;
+        if (p.orig_ctx > 0 && p.temp_scale != 0.f && pos >= p.orig_ctx)
+            f = 1.0 + (double)p.temp_scale * log(1.0 + (double)(pos / p.orig_ctx));
+        // RING rows in flight
+        for (; w < end; w += RING * jump) {
+            float2 y[RING][NP];
+#pragma unroll
+            for (int i = 0; i < RING; i++)
+                if (w + i * jump < end) load(w + i * jump, y[i]);
+#pragma unroll
+            for (int i = 0; i < RING; i++)
+                if (w + i * jump < end) {
+                    rotate(f, y[i]);
+                    store_pairs<HD, VEC>(e, p.q_out + ((size_t)row * p.n_heads + h * p.group + w + i * jump) * HD, y[i]);
+                }
+        }
+    }
+    if (!kv) return;
+    __syncthreads();
+
+    // steps and codes of token tid / 16, elements NE j ..
+    const int tk = tid >> 4;
+    if (tk < n) {
+        unsigned bad = 0; // a value that is not finite has the largest bits
+        int power[2];
+#pragma unroll
+        for (int v = 0; v < 2; v++) {
+            float x[NE], hi = 0.f, lo = 0.f;
+            unsigned bits = 0;
+#pragma unroll
+            for (int i = 0; i < NE; i++) {
+                x[i] = xs[v][tk][NE * j + i];
+                hi = fmaxf(hi, x[i]);
+                lo = fmaxf(lo, -x[i]);
+                bits = max(bits, __float_as_uint(fabsf(x[i])));
+            }
+#pragma unroll
+            for (int o = 1; o < TG; o <<= 1) {
+                hi = fmaxf(hi, __shfl_xor(hi, o, 64));
+                lo = fmaxf(lo, __shfl_xor(lo, o, 64));
+            }
+            const float span = 0.5f * hi + 0.5f * lo; // half the group's span: the whole one may be past fp32's range
+            float most = span;
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) {
+                most = fmaxf(most, __shfl_xor(most, o, 64));
+                bits = max(bits, (unsigned)__shfl_xor((int)bits, o, 64));
+            }
+            bad = max(bad, bits);
+            // the least 2^ex with the widest span <= 15 * 15 * 2^ex, 225 = 0.87890625 * 2^8
+            const bool some = most > 0.f && bits < 0x7f800000u;
+            const int ex = max(__builtin_amdgcn_frexp_expf(most) - (__builtin_amdgcn_frexp_mantf(most) <= 0.87890625f ? 7 : 6), -126);
+            const float wide = some ? ldexpf(span, 1 - ex) : 0.f;
+            float u = ceilf(wide * (1.f / 15.f)); // then the least u with span <= 15 u exactly
+            if (15.f * (u - 1.f) >= wide) u -= 1.f;
+            if (15.f * u < wide) u += 1.f;
+            u = fmaxf(u, 1.f);
+            const float inv = __builtin_amdgcn_rcpf(u), z = some ? whole_steps(ldexpf(lo, -ex), u, inv) : 0.f;
+            uint32_t word = 0;
+#pragma unroll
+            for (int i = 0; i < NE; i++) {
+                const float q = some ? whole_steps(ldexpf(x[i], -ex), u, inv) + z : 0.f;
+                const uint32_t c = (uint32_t)(int)fminf(fmaxf(q, 0.f), 15.f);
+                if (v) code[tk][NE * j + i] = (uint8_t)c;
+                else word |= c << nibble_at((NE * j + i) & 7);
+            }
+            if (!v) {
+                if (NE == 4) word |= (uint32_t)__shfl_xor((int)word, 1, 64);
+                if (NE == 8 || !(j & 1)) *(uint32_t *)(block + at.k + (off + tk) * (HD / 2) + 4 * (NE * j / 8)) = turn_left(word, 2);
+            }
+            if (j % TG == 0) {
+                step[v][tk][j / TG] = (uint8_t)(int)u;
+                zero[v][tk][j / TG] = (uint8_t)(int)z;
+            }
+            power[v] = some ? ex + 127 : 0;
+        }
+        // a value that is not finite: the token's V power says so for both
+        if (j < 2) block[(j ? at.ve : at.ke) + off + tk] = (uint8_t)(bad < 0x7f800000u ? power[j] : j ? 255 : 0);
+    }
+    __syncthreads();
+
+    // words over several tokens: the new ones' nibbles among what is there
+    auto merge = [&](uint32_t old, auto token, auto nibble) {
+        uint32_t put = 0, mask = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int tk = token(i) - off;
+            if (tk < 0 || tk >= n) continue;
+            put |= (uint32_t)nibble(i, tk) << nibble_at(i);
+            mask |= 15u << nibble_at(i);
+        }
+        mask = turn_left(mask, 2);
+        return make_uint2((old & ~mask) | turn_left(put, 2), mask);
+    };
+    if (has_v) {
+        const int dim = 32 * (tid >> 6) + 16 * ((tid >> 1) & 1) + ((tid >> 2) & 15), t0 = 8 * (tid & 1);
+        const uint2 r = merge(old_v, [&](int i) { return t0 + i; }, [&](int, int tk) { return code[tk][dim]; });
+        if (r.y) *vword = r.x;
+    }
+    if (has_s) {
+        uint2 r;
+        if (tid < 4 * NG) { // K: tokens r, 4 + r, ..: u the even elements (low half), z the odd ones
+            const int gr = tid >> 2, r0 = tid & 3;
+            r = merge(old_s, [&](int i) { return 4 * (i >> 1) + r0; }, [&](int i, int tk) { return i & 1 ? zero[0][tk][gr] : step[0][tk][gr]; });
+        } else {
+            const int gr = (tid - 4 * NG) >> 2, t0 = 8 * (tid & 1), z = tid & 2;
+            r = merge(old_s, [&](int i) { return t0 + i; }, [&](int, int tk) { return z ? zero[1][tk][gr] : step[1][tk][gr]; });
+        }
+        if (r.y) *sword = r.x;
+    }
+}
+
+hipError_t launch_pages4_store(const Pages &p, const PagesStoreArgs &a, hipStream_t s)
+{
+    const int units = a.n_tokens / kPageBlock + 2 * (a.n_requests < a.n_tokens ? a.n_requests : a.n_tokens);
+    const int np = p.hd / 32;
+    auto vec = [&](const void *x, int64_t ld) { return !x || ((uintptr_t)x % (4 * np) == 0 && ld % np == 0); };
+    // as in the 8-bit store: rows that start aligned, and no thread with pairs on both
+    // sides of the rotated part's end
+    const bool v = vec(a.q, a.q_ld) && vec(a.k, a.kv_ld) && vec(a.v, a.kv_ld) && vec(a.q_out, 0) && a.in_stride % np == 0 &&
+                   (!p.rope_half || p.half % np == 0);
+    const Store4View view = {layer4_of(p, a.layer), p.head, p.unit, p.angle, a.q, a.k, a.v, a.q_out, a.q_ld, a.kv_ld, a.in_stride, a.nin,
+                             p.n_kv, p.n_heads, p.group, p.sub, p.sub_shift, p.half, p.rope_half, p.orig_ctx, p.temp_scale,
+                             a.n_tokens, a.n_requests, 1};
+    const dim3 grid(units > 0 ? units : 1, p.n_kv);
+    if (p.hd == 128 && v) hipLaunchKernelGGL((pages4_store_kernel<128, true>), grid, dim3(256), 0, s, view);
+    else if (p.hd == 128) hipLaunchKernelGGL((pages4_store_kernel<128, false>), grid, dim3(256), 0, s, view);
+    else if (v) hipLaunchKernelGGL((pages4_store_kernel<64, true>), grid, dim3(256), 0, s, view);
+    else hipLaunchKernelGGL((pages4_store_kernel<64, false>), grid, dim3(256), 0, s, view);
+    return hipGetLastError();
+}
+
+// ------------------------------------------------------------ attention
+
+namespace {
+
+struct Attend4View {
+    const uint8_t *pool;
+    const int32_t *table;
+    PagesPlanHead *head;
+    const PagesItem *item, *wide_item;
+    float *part, *wide_part;
+    int32_t *tickets, *wide_tickets;
+    const float *q;
+    float *out;
+    int n_kv, n_heads, group, sub, sub_shift, width;
+    float scale;
+    int wides, tiles;               // workgroups of each kind
+    int n_tokens, n_requests, wide; // of the call's plan
+};
+
+// A query row as fp16 pairs: scaled by a power of two so that its largest element lies in
+// [2^13, 2^14), then by the softmax's scale in powers of two.  A key's 2^e and the row's
+// power meet in a score's exponent, in whole numbers.
+struct Query4 {
+    float f1, f2, scale;
+    int ex;
+    Query4() = default;
+    __device__ __forceinline__ Query4(float m, float softmax)
+        : scale(softmax * 1.44269504088896341f), ex(m > 0.f && m < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(m) : 0)
+    {
+        f1 = ldexpf(1.f, ex / 2), f2 = ldexpf(1.f, ex - ex / 2);
+    }
+    __device__ __forceinline__ int power() const { return -127 - ex; } // with a key's byte
+    __device__ __forceinline__ void split(float x, _Float16 &hi, _Float16 &lo) const
+    {
+        float y = x * f1 * f2 * scale;
+        asm("" : "+v"(y)); // rounded to fp32: hi straight from the product may be another than the one that lo completes
+        hi = (_Float16)y;
+        lo = (_Float16)(y - (float)hi);
+    }
+};
+
+template <int HD>
+struct Tile4Lds {
+    float lo[4][16][HD + 4];
+    float lm[4][kPagesTileRows], ll[4][kPagesTileRows];
+    int last;
+};
+
+// Up to ROWS (token, head) rows of a request and KV head over keys [key0, key1) of its
+// pages; the four waves take 64 keys (four blocks) in turn and merge at the end.
+// S^T = K Q^T with the rows of the K operand dealt so that a lane's sixteen scores are the
+// sixteen tokens of one block, which makes the weights the P^T operand of O^T += V^T P^T
+// as they stand.  q and p enter as fp16 pairs (hi + lo, ~22 bits).  Up to eight rows leave
+// half of the operand's sixteen columns, which take the low parts: one matrix instruction a
+// product instead of two.  A weight is 2^(score - m); the V operand's 2^e and the row's own
+// power are added to its exponent, so that what enters fp16 is relative to the row's
+// heaviest product so far (times 2^9), over the keys that the row sees.
+template <int HD, int ROWS>
+__device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> &lds, const PagesItem &r, int h)
+{
+    constexpr int NC = HD / 32, NS = HD / 16, NI = HD / 32, LD = HD + 4, NQ = ROWS == 8 ? 1 : 2;
+    constexpr Pages4 at(HD);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, n = lane & 15;
+    const int32_t *table = p.table + (size_t)r.id * p.width;
+    // columns past the request's rows repeat its last one
+    const int n_rows = r.row1, row = min(r.row0 + (n & (ROWS - 1)), n_rows - 1);
+    const int token = row / p.group, head = h * p.group + row % p.group;
+    const int limit = r.past + token; // last visible key
+    // the tile's last visible key; keys up to `clear` are seen by every row
+    const int top = r.past + min(n_rows - 1, r.row0 + ROWS - 1) / p.group;
+    const int key1 = min(r.key1, top + 1), clear = r.past + r.row0 / p.group;
+    const int last = (r.len - 1) / kPageBlock; // blocks past it are read as this one, and masked
+
+    // a lane reads K of block n / 4 of the four, V and the powers of block g
+    auto page_of = [&](int kb, int i) { return table[min(4 * kb + i, last) >> p.sub_shift]; };
+    auto block_of = [&](int kb, int i, int page) {
+        return p.pool + ((((size_t)page * p.n_kv + h) << p.sub_shift) + (min(4 * kb + i, last) & (p.sub - 1))) * at.bytes;
+    };
+    uint4 kr[4], vr[NI], vs[NI], ke, ve;
+    uint32_t ks;
+    auto fetch_k = [&](int kb, int page) {
+        const uint8_t *b = block_of(kb, n >> 2, page);
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const uint8_t *src = b + at.k + (4 * t + (n & 3)) * (HD / 2) + 4 * NC * g;
+            if constexpr (NC == 4) kr[t] = *(const uint4 *)src;
+            else {
+                const uint2 x = *(const uint2 *)src;
+                kr[t] = make_uint4(x.x, x.y, 0, 0);
+            }
+        }
+        ks = *(const uint32_t *)(b + at.ks + 4 * (4 * (g * NI / 4) + (n & 3)));
+    };
+    auto fetch_v = [&](int kb, int page) {
+        const uint8_t *b = block_of(kb, g, page);
+        ke = *(const uint4 *)(b + at.ke);
+        ve = *(const uint4 *)(b + at.ve);
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            vr[i] = *(const uint4 *)(b + at.v + 256 * i + 16 * n);
+            vs[i] = *(const uint4 *)(b + at.vs + 16 * i);
+        }
+    };
+    int kb = r.key0 / 64 + wave;
+    int pk = page_of(kb, n >> 2), pv = page_of(kb, g);
+    if (kb * 64 < key1) {
+        fetch_k(kb, pk);
+        fetch_v(kb, pv);
+    }
+    pk = page_of(kb + 4, n >> 2);
+    pv = page_of(kb + 4, g);
+
+    // Q^T fragments: dims 8 NC g + 8 c .. + 7 of column n
+    half8_t qf[NQ][NC];
+    int query;
+    {
+        const float *src = p.q + ((size_t)(r.start + token) * p.n_heads + head) * HD + 8 * NC * g;
+        float x[NC][8], m = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                x[c][i] = src[8 * c + i];
+                m = fmaxf(m, fabsf(x[c][i]));
+            }
+        m = fmaxf(m, __shfl_xor(m, 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        const Query4 scaled(m, p.scale);
+        query = scaled.power();
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                _Float16 hi, lw;
+                scaled.split(x[c][i], hi, lw);
+                if constexpr (NQ == 2) {
+                    qf[0][c][i] = hi;
+                    qf[1][c][i] = lw;
+                } else qf[0][c][i] = n < 8 ? hi : lw;
+            }
+    }
+
+    floatx4 o[NS];
+#pragma unroll
+    for (int s = 0; s < NS; s++) o[s] = floatx4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f, e = -INFINITY; // m and e whole numbers; outputs are held times 2^(9 - e)
+    int value = -127;                            // with a V row's byte: the power from a weight to fp16's
+    const float part = n < 8 ? 0.f : -1.f;       // 8 rows: a column's part of a weight
+
+    for (; kb * 64 < key1; kb += 4) {
+        const bool more = (kb + 4) * 64 < key1;
+        float sv[16];
+        const Steps kst[4] = {key_steps<0>(ks), key_steps<1>(ks), key_steps<2>(ks), key_steps<3>(ks)};
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                const half8_t k = word_f16(word_of(kr[t], c), kst[t]);
+#pragma unroll
+                for (int i = 0; i < NQ; i++) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[i][c], acc, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float x = acc[i];
+                if constexpr (NQ == 1) // the other part's column is eight lanes on
+                    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, true));
+                sv[4 * t + i] = __builtin_amdgcn_ldexpf(x, byte_of(ke, 4 * t + i) + query);
+            }
+        }
+        if (more) fetch_k(kb + 4, pk);
+        if (kb * 64 + 63 > clear) {
+            const int left = limit - (kb * 64 + 16 * g); // last visible token of the lane's block
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                if (i > left) sv[i] = -INFINITY;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; i++) mx = fmaxf(mx, sv[i]);
+        if (__any(mx > m + 6.f)) {
+            float mn = fmaxf(m, ceilf(mx));
+            mn = fmaxf(mn, __shfl_xor(mn, 16, 64));
+            mn = fmaxf(mn, __shfl_xor(mn, 32, 64));
+            l *= m == -INFINITY ? 0.f : exp2f(m - mn);
+            m = mn;
+            value = -127 + (e == -INFINITY ? 0 : (int)(9.f - e + m));
+        }
+        const float mu = m == -INFINITY ? 0.f : m;
+        // the largest score with the largest power bounds what the row's products can be (a
+        // block without visible keys: -inf, or NaN with a token that is not finite)
+        const int mb = most_byte(ve);
+        if (__any(mx + (mb == 255 ? INFINITY : (float)(mb - 127)) > e + 6.f)) {
+            float mv = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int b = byte_of(ve, i);
+                if (b < 255) mv = fmaxf(mv, sv[i] + (float)(b - 127));
+                else if (sv[i] > -INFINITY) l = NAN; // a token that is not finite, seen
+            }
+            float en = fmaxf(e, ceilf(mv));
+            en = fmaxf(en, __shfl_xor(en, 16, 64));
+            en = fmaxf(en, __shfl_xor(en, 32, 64));
+            const float up = e == -INFINITY ? 0.f : exp2f(e - en);
+#pragma unroll
+            for (int s = 0; s < NS; s++) o[s] *= up;
+            e = en;
+            value = -127 + (e == -INFINITY ? 0 : (int)(9.f - e + mu));
+        }
+        float wt[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const float x = __builtin_amdgcn_exp2f(sv[i] - mu);
+            l += x;
+            wt[i] = __builtin_amdgcn_ldexpf(x, byte_of(ve, i) + value);
+        }
+        half8_t pf[NQ][2];
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            uint32_t hi[4], lw[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float x = wt[8 * c + 2 * i], y = wt[8 * c + 2 * i + 1];
+                if constexpr (NQ == 2) split2_mix(x, y, hi[i], lw[i]);
+                else { // the high columns keep x, the low ones what fp16 leaves of it
+                    float r0, r1;
+                    const uint32_t f = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+                    asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(f), "v"(part), "v"(x));
+                    asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(f), "v"(part), "v"(y));
+                    hi[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r0, r1));
+                }
+            }
+            pf[0][c] = __builtin_bit_cast(half8_t, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+            if constexpr (NQ == 2) pf[1][c] = __builtin_bit_cast(half8_t, make_uint4(lw[0], lw[1], lw[2], lw[3]));
+        }
+#pragma unroll
+        for (int i = 0; i < NI; i++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                Steps st[4];
+                value_steps(c ? vs[i].y : vs[i].x, c ? vs[i].w : vs[i].z, st);
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    const half8_t v = word_f16(word_of(vr[i], 2 * b + c), st);
+#pragma unroll
+                    for (int k = 0; k < NQ; k++) o[2 * i + b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf[k][c], o[2 * i + b], 0, 0, 0);
+                }
+            }
+        if (more) {
+            fetch_v(kb + 4, pv);
+            pk = page_of(kb + 8, n >> 2);
+            pv = page_of(kb + 8, g);
+        }
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+
+    // the four waves' results, in wave order
+    const MeanScale mean(e, m, l);
+#pragma unroll
+    for (int s = 0; s < NS; s++) *(floatx4 *)&lds.lo[wave][n][16 * s + 4 * g] = o[s] * mean.f1 * mean.f2;
+    if (g == 0) {
+        lds.lm[wave][n] = m;
+        lds.ll[wave][n] = l;
+    }
+    __syncthreads();
+    for (int i = tid; i < ROWS * (HD / 4); i += 256) {
+        const int c = i / (HD / 4), d = 4 * (i % (HD / 4)), rr = r.row0 + c;
+        if (rr >= n_rows) continue;
+        float mm = lds.lm[0][c];
+#pragma unroll
+        for (int w = 1; w < 4; w++) mm = fmaxf(mm, lds.lm[w][c]);
+        const float mu = mm == -INFINITY ? 0.f : mm;
+        float sum = 0.f, f[4];
+        floatx4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            f[w] = lds.ll[w][c] * exp2f(lds.lm[w][c] - mu);
+            sum += f[w];
+        }
+        const float inv = sum == 0.f && r.part >= 0 ? 0.f : 1.f / sum;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            floatx4 y = *(const floatx4 *)&lds.lo[w][c][d];
+            if constexpr (NQ == 1) y += *(const floatx4 *)&lds.lo[w][c + 8][d];
+            x += y * (f[w] * inv);
+        }
+        if (r.part < 0) {
+            const int tk = rr / p.group, hd = h * p.group + rr % p.group;
+            float *dst = p.out + ((size_t)(r.start + tk) * p.n_heads + hd) * HD + d;
+#pragma unroll
+            for (int k = 0; k < 4; k++) dst[k] = x[k];
+        } else {
+            float *dst = p.part + (((size_t)r.part * p.n_kv + h) * kPagesTileRows + c) * LD;
+            store_shared(dst + d, x[0], x[1]);
+            store_shared(dst + d + 2, x[2], x[3]);
+            if (d == 0) store_shared(dst + HD, mm, sum);
+        }
+    }
+    if (r.part >= 0) {
+        // the tile's last part to arrive merges them all, in their order
+        const int tiles = div_up(n_rows, kPagesTileRows), tile = r.row0 / kPagesTileRows;
+        if (arrives_last(p.tickets + (size_t)(r.part0 + tile) * p.n_kv + h, r.n_parts, lds.last))
+            for (int c = tid >> 4; c < min(ROWS, n_rows - r.row0); c += 16) {
+                const int rr = r.row0 + c, tk = rr / p.group;
+                merge_parts<HD>(
+                    [&](int k) { return p.part + (((size_t)(r.part0 + k * tiles + tile) * p.n_kv + h) * kPagesTileRows + c) * LD; },
+                    r.n_parts, p.out + ((size_t)(r.start + tk) * p.n_heads + h * p.group + rr % p.group) * HD, tid & 15);
+            }
+    }
+    __syncthreads();
+}
+
+} // namespace
+
+// The attention of a plan: its 16-row tiles, workgroups taking turns.
+template <int HD>
+__global__ __launch_bounds__(256, 2) void pages4_attend_kernel(Attend4View p)
+{
+    __shared__ __align__(16) Tile4Lds<HD> lds;
+    const int first = (int)blockIdx.x, h = first % p.n_kv, stride = p.tiles / p.n_kv;
+    int item = first / p.n_kv;
+    PagesItem it = p.item[item]; // (it is there if not of this plan, and does not wait for the head)
+    const PagesPlanHead plan = *p.head;
+    if (outgrown(p, plan)) return;
+    while (item < plan.n_items) {
+        if (it.row1 - it.row0 <= 8) attend4_tile<HD, 8>(p, lds, it, h);
+        else attend4_tile<HD, 16>(p, lds, it, h);
+        item += stride;
+        if (item < plan.n_items) it = p.item[item];
+    }
+}
+
+hipError_t launch_pages4_attend(const Pages &p, const PagesAttendArgs &a, hipStream_t s)
+{
+    // as many workgroups as the call's requests can need (launch_pages_attend)
+    const int64_t split = (int64_t)((p.group + kPagesTileRows - 1) / kPagesTileRows) * std::min(a.n_requests, a.n_tokens);
+    const int64_t parts = std::min((int64_t)p.max_parts, split * pages_most_parts(p.max_context));
+    const int64_t most = a.n_tokens == 0 ? 1 : std::max<int64_t>(1, parts + (int64_t)a.n_tokens * p.group / kPagesTileRows + a.n_requests);
+    const int tiles = (int)(most < 2048 ? most : 2048) * p.n_kv;
+    const Attend4View view = {layer4_of(p, a.layer), p.table, p.head, p.item, p.wide, p.part, p.wide_part, p.tickets, p.wide_tickets,
+                              a.q, a.out, p.n_kv, p.n_heads, p.group, p.sub, p.sub_shift, p.width, p.scale,
+                              0, tiles, a.n_tokens, a.n_requests, 0};
+    auto launch = [&](auto kernel) { launch_stamped(a.ev_start, a.ev_stop, kernel, dim3(tiles), dim3(256), 0, s, view); };
+    launch(p.hd == 128 ? pages4_attend_kernel<128> : pages4_attend_kernel<64>);
+    return hipGetLastError();
+}
+
+// ------------------------------------------------------------ reading back
+
+namespace {
+struct Read4View {
+    const uint8_t *pool;
+    const int32_t *slot;
+    float *k_out, *v_out;
+    int n, n_kv, page, sub, n_pages;
+};
+} // namespace
+
+// Sixteen slots and one KV head to a workgroup, a slot to sixteen threads, hd / 16
+// neighbouring elements to each.
+template <int HD>
+__global__ __launch_bounds__(256) void pages4_read_kernel(Read4View p)
+{
+    constexpr int NE = HD / 16;
+    constexpr Pages4 at(HD);
+    const int tid = threadIdx.x, h = blockIdx.y, i = blockIdx.x * 16 + (tid >> 4), d0 = NE * (tid & 15), gr = d0 / 32;
+    if (i >= p.n) return;
+    const int slot = p.slot[i];
+    float x[2][NE] = {};
+    if (slot >= 0 && slot / p.page < p.n_pages) {
+        const int tk = slot % kPageBlock;
+        const uint8_t *b = p.pool + (((size_t)(slot / p.page) * p.n_kv + h) * p.sub + slot % p.page / kPageBlock) * at.bytes;
+        auto nibble = [](uint32_t w, int i) { return (int)((turn_left(w, 30) >> nibble_at(i)) & 15u); };
+        const uint32_t kw = *(const uint32_t *)(b + at.k + tk * (HD / 2) + 4 * (d0 / 8));
+        const uint32_t ks = *(const uint32_t *)(b + at.ks + 4 * (4 * gr + (tk & 3)));
+        const uint32_t *vs = (const uint32_t *)(b + at.vs) + 4 * gr + (tk >> 3);
+        const uint32_t vu = vs[0], vz = vs[2];
+        const int ke = b[at.ke + tk], ve = b[at.ve + tk];
+        uint32_t vw[NE];
+#pragma unroll
+        for (int k = 0; k < NE; k++) {
+            const int d = d0 + k;
+            vw[k] = *((const uint32_t *)(b + at.v) + 64 * gr + 4 * (d & 15) + 2 * ((d >> 4) & 1) + (tk >> 3));
+        }
+        const int ku = nibble(ks, 2 * (tk >> 2)), kz = nibble(ks, 2 * (tk >> 2) + 1), u = nibble(vu, tk & 7), z = nibble(vz, tk & 7);
+#pragma unroll
+        for (int k = 0; k < NE; k++) {
+            x[0][k] = ve == 255 ? NAN : ldexpf((float)((nibble(kw, (d0 + k) & 7) - kz) * ku), ke - 127);
+            x[1][k] = ve == 255 ? NAN : ldexpf((float)((nibble(vw[k], tk & 7) - z) * u), ve - 127);
+        }
+    }
+    const size_t to = ((size_t)i * p.n_kv + h) * HD + d0;
+#pragma unroll
+    for (int k = 0; k < NE; k++) {
+        p.k_out[to + k] = x[0][k];
+        p.v_out[to + k] = x[1][k];
+    }
+}
+
+hipError_t launch_pages4_read(const Pages &p, int layer, const int32_t *slot, int n, float *k, float *v, hipStream_t s)
+{
+    if (n <= 0) return hipSuccess;
+    const Read4View view = {layer4_of(p, layer), slot, k, v, n, p.n_kv, p.page, p.sub, p.n_pages};
+    const dim3 grid((n + 15) / 16, p.n_kv);
+    if (p.hd == 128) hipLaunchKernelGGL(pages4_read_kernel<128>, grid, dim3(256), 0, s, view);
+    else hipLaunchKernelGGL(pages4_read_kernel<64>, grid, dim3(256), 0, s, view);
+    return hipGetLastError();
+}
+
+} // namespace jev

@@ -2648,7 +2648,7 @@ int pages_plan(jev_pages *h, const PagesPlanArgs &a, hipStream_t s)
     h->plan = a;
     // as many tokens as requests: 16-row tiles serve whatever there is, and the
     // wide tiles' launches are saved
-    h->plan.wide = a.n_tokens > a.n_requests;
+    h->plan.wide = h->p.bits == 8 && a.n_tokens > a.n_requests;
     HIP_TRY(launch_pages_plan(h->p, h->plan, s));
     return JEV_OK;
 }
@@ -2674,10 +2674,16 @@ int pages_status(jev_pages *h, hipStream_t s)
 extern "C" {
 
 int jev_pages_create(const jev_config *model, const jev_pages_config *cfg, int device, jev_pages **out)
+{
+    return jev_pages_create_bits(model, cfg, 8, device, out);
+}
+
+int jev_pages_create_bits(const jev_config *model, const jev_pages_config *cfg, int32_t bits, int device, jev_pages **out)
 try {
     if (!out) return fail(JEV_EINVAL, "out is null");
     *out = nullptr;
     if (!model || !cfg) return fail(JEV_EINVAL, "null argument");
+    if (bits != 8 && bits != 4) return fail(JEV_EINVAL, "%d bits: a paged cache holds 8 or 4", bits);
     const jev_config &f = *model;
     const jev_pages_config &g = *cfg;
     if (f.n_layers <= 0 || f.n_heads <= 0 || f.n_kv_heads <= 0) return fail(JEV_EINVAL, "model dimensions must be positive");
@@ -2719,6 +2725,7 @@ try {
     p.n_heads = f.n_heads;
     p.n_kv = f.n_kv_heads;
     p.hd = f.head_dim;
+    p.bits = bits;
     p.group = f.n_heads / f.n_kv_heads;
     p.page = g.page_tokens;
     p.sub = g.page_tokens / kPageBlock;
@@ -2749,13 +2756,17 @@ try {
     p.max_wide_parts = g.max_context <= kPagesWideKeys
                            ? 0
                            : (int)std::min(2 * target, (T * p.group / kPagesWideRows + R) * ((size_t)g.max_context / kPagesWideKeys + 1));
-    const size_t codes = p.n_blocks() * p.n_layers * kPageBlock * p.hd;
+    const size_t blocks = p.n_blocks() * p.n_layers, codes = blocks * kPageBlock * p.hd;
     const int words = (p.n_pages + 31) / 32;
     double *dfreqs = nullptr;
-    // a scale of zero has codes of zero from the start: the attention relies on it
-    int rc = pages_alloc(h, p.k, codes, 0x80);
-    if (!rc) rc = pages_alloc(h, p.v, codes, 0x80);
-    if (!rc) rc = pages_alloc(h, p.ks, p.n_blocks() * p.n_layers);
+    int rc = JEV_OK;
+    if (bits == 4) rc = pages_alloc(h, p.k, blocks * pages4_bytes(p.hd));
+    else {
+        // a scale of zero has codes of zero from the start: the attention relies on it
+        rc = pages_alloc(h, p.k, codes, 0x80);
+        if (!rc) rc = pages_alloc(h, p.v, codes, 0x80);
+        if (!rc) rc = pages_alloc(h, p.ks, blocks);
+    }
     if (!rc) rc = pages_alloc(h, p.table, R * p.width);
     if (!rc) rc = pages_alloc(h, p.length, R);
     if (!rc) rc = pages_alloc(h, p.used, words);

@@ -140,6 +140,7 @@ def lib():
         "jev_weight_sync": (c_int, [c_void_p]),
         "jev_weight_stream": (c_void_p, [c_void_p]),
         "jev_pages_create": (c_int, [POINTER(Config), POINTER(PagesConfig), c_int, POINTER(c_void_p)]),
+        "jev_pages_create_bits": (c_int, [POINTER(Config), POINTER(PagesConfig), c_int32, c_int, POINTER(c_void_p)]),
         "jev_pages_destroy": (None, [c_void_p]),
         "jev_pages_plan_device": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32] + [c_void_p] * 5),
         "jev_pages_store_device": (c_int, [c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
@@ -182,6 +183,6 @@ EXPORTED = [
     "jev_set_matmul_strategy", "jev_get_matmul_strategy", "jev_quantize_activations", "jev_rope_table",
     "jev_matmul_device_noalloc", "jev_capture", "jev_weight_stream", "jev_kv_snapshot_device",
     "jev_kv_restore_device", "jev_snapshot_length", "jev_snapshot_read", "jev_snapshot_destroy",
-    "jev_pages_create", "jev_pages_destroy", "jev_pages_plan_device", "jev_pages_store_device", "jev_pages_attend_device",
+    "jev_pages_create", "jev_pages_create_bits", "jev_pages_destroy", "jev_pages_plan_device", "jev_pages_store_device", "jev_pages_attend_device",
     "jev_pages_read_device", "jev_pages_release", "jev_pages_sync", "jev_pages_stream", "jev_forward_pages",
 ]

@@ -1,4 +1,4 @@
-"""The paged 8-bit KV cache over libjev's jev_pages_* entry points: one pool of pages
+"""The paged KV cache, held in 8 or 4 bits, over libjev's jev_pages_* entry points: one pool of pages
 in HBM that many requests share, planned on the device (include/jev.h has the rules)."""
 from __future__ import annotations
 
@@ -9,18 +9,20 @@ from .model import ModelConfig, _i32
 
 
 class KvPages:
-    """A pool of `n_pages` pages of `page_tokens` tokens for up to `max_requests` requests.
+    """A pool of `n_pages` pages of `page_tokens` tokens for up to `max_requests` requests, keys and
+    values in `bits` (8 or 4) an element.
 
     The *_device calls take device pointers (integers) and only enqueue on the handle's stream."""
 
     def __init__(self, config: ModelConfig, n_pages: int, page_tokens: int = 16, max_requests: int = 64,
-                 max_context: int = 4096, max_tokens: int = 4096, rope_half: bool = False, device: int = 0):
+                 max_context: int = 4096, max_tokens: int = 4096, rope_half: bool = False, device: int = 0, bits: int = 8):
         self._h = ctypes.c_void_p()
         self._lib = L.lib()
         self.config, self.n_pages, self.page_tokens = config, n_pages, page_tokens
         self.max_requests, self.max_context, self.max_tokens = max_requests, max_context, max_tokens
+        self.bits = bits
         c = L.PagesConfig(n_pages, page_tokens, max_requests, max_context, max_tokens, int(rope_half))
-        L.check(self._lib.jev_pages_create(ctypes.byref(config.to_c()), ctypes.byref(c), device, ctypes.byref(self._h)))
+        L.check(self._lib.jev_pages_create_bits(ctypes.byref(config.to_c()), ctypes.byref(c), bits, device, ctypes.byref(self._h)))
 
     def close(self) -> None:
         if self._h:
