@@ -428,6 +428,50 @@ int jev_forward_pages(jev_ctx *ctx, jev_pages *p, const int32_t *request, const 
                       int32_t n_requests, const int32_t *tokens, int32_t n_tokens, int mode, const int32_t *rows,
                       int32_t n_rows, float *out, size_t out_len);
 
+/* ---- Log probabilities ---- */
+
+/* What the rows of logits of a step answer, without the rows: per row, with T a
+ * temperature (positive),
+ *
+ *   logp(i) = x_i / T - log sum_j exp(x_j / T)      entropy = -sum exp(logp) logp
+ *
+ * of n_given tokens of the row's own, and of its n_top (at most 32) largest
+ * logits in order (jev_decode_greedy's: NaN before all, +0 above -0, the lowest
+ * index first).  One pass; maxima and differences in fp32, sums over a row in 64
+ * bits and without the largest logit's own term, so a probability next to 1 keeps
+ * its logarithm.  Logits of -inf have none.  A row
+ * with a NaN or +inf, or of -inf alone, has NaN in all but its order.
+ *
+ * The *_device call only enqueues on the handle's stream (jev_logprobs_stream,
+ * which orders itself with the device's null stream) and allocates nothing: it
+ * may be captured into a graph.  A handle's calls share its workspace: one
+ * thread at a time, and no two of its graphs at once.  Pointers are device
+ * pointers of the handle's device, of any 4-byte alignment (the result bits are
+ * the same). */
+typedef struct jev_logprobs jev_logprobs;
+/* vocab logits a row, in [1, 2^28]; calls of up to max_rows rows, at most 2^24. */
+int jev_logprobs_create(int32_t vocab, int32_t max_rows, int device, jev_logprobs **out);
+void jev_logprobs_destroy(jev_logprobs *p);
+/* logits [rows][ld >= vocab]; given [rows][n_given] -> logp [rows][n_given] (NaN
+ * for an id outside the vocabulary); entropy [rows]; top, top_logp [rows][n_top].
+ * entropy, top and top_logp may be NULL, and given and logp where n_given is 0;
+ * something must be asked for.  No output may overlap another or the logits. */
+int jev_logprobs_device(jev_logprobs *p, const float *logits, int64_t ld, int32_t rows, const int32_t *given, int32_t n_given,
+                        int32_t n_top, float temperature, float *logp, float *entropy, int32_t *top, float *top_logp);
+int jev_logprobs_sync(jev_logprobs *p);
+void *jev_logprobs_stream(jev_logprobs *p);
+
+/* jev_forward_pages with log probabilities for its logits: at each request's
+ * last token, or with `every` at every token of the step (in the order of
+ * `tokens`), so a prompt scores in one step: row t's given token is the one at
+ * t + 1.  All arrays are host arrays, [rows][..] as above, with n_requests or
+ * n_tokens rows; a given id outside the vocabulary is JEV_EINVAL.  Logits stay
+ * on the device, 256 rows of them at a time. */
+int jev_forward_pages_logprobs(jev_ctx *ctx, jev_pages *p, const int32_t *request, const int32_t *past, const int32_t *fresh,
+                               int32_t n_requests, const int32_t *tokens, int32_t n_tokens, int every, const int32_t *given,
+                               int32_t n_given, int32_t n_top, float temperature, float *logp, float *entropy, int32_t *top,
+                               float *top_logp);
+
 /* ---- Test hooks (no managed counterpart) ---- */
 
 /* The Rope ctor's tables (Rope.cs:33-106): the n = rope_dim / 2 pair

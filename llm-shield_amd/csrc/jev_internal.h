@@ -541,4 +541,26 @@ hipError_t launch_pages4_attend(const Pages &p, const PagesAttendArgs &a, hipStr
 hipError_t launch_pages_read(const Pages &p, int layer, const int32_t *slot, int n, float *k, float *v, hipStream_t s);
 hipError_t launch_pages4_read(const Pages &p, int layer, const int32_t *slot, int n, float *k, float *v, hipStream_t s);
 
+// ---------------------------------------------------------------- log probabilities
+
+constexpr int kLogprobsTop = 32;     // most probable tokens of a row, at most
+constexpr int kLogprobsParts = 2048; // partial results of a call, at most (rows in parts: fewer than half of them)
+struct LogprobsPart {                // of a part of a row: its largest logit, its sums, its largest keys in order
+    double s, t;
+    uint64_t m, key[kLogprobsTop];
+};
+struct LogprobsArgs {
+    const float *logits = nullptr; // [rows][ld]
+    int64_t ld = 0;
+    int rows = 0, vocab = 0, n_given = 0, n_top = 0;
+    const int32_t *given = nullptr;      // [rows][n_given]
+    float temperature = 1.f;
+    float *logp = nullptr, *entropy = nullptr, *top_logp = nullptr; // [rows][n_given], [rows], [rows][n_top]; the last three may be null
+    int32_t *top = nullptr;              // [rows][n_top]
+    LogprobsPart *part = nullptr;        // [kLogprobsParts]
+    int32_t *tickets = nullptr;          // [kLogprobsParts], zeros between calls
+};
+int logprobs_parts(int rows, int vocab);
+hipError_t launch_logprobs(const LogprobsArgs &a, hipStream_t s);
+
 } // namespace jev

@@ -17,6 +17,7 @@
 #include <memory>
 #include <mutex>
 #include <new>
+#include <numeric>
 #include <optional>
 #include <string>
 #include <thread>
@@ -138,6 +139,10 @@ struct jev_ctx {
     DevBuf<AttnTile> tiles;
     DevBuf<float> amax_v;
     DevBuf<int32_t> amax_i;
+    // log probabilities: a step's results, partial results, arrivals (zeros between calls)
+    DevBuf<float> scores;
+    DevBuf<LogprobsPart> lp_part;
+    DevBuf<int32_t> lp_tickets;
     std::vector<int32_t> host_ints;
     std::vector<AttnTile> host_tiles;
     // Pinned staging for the per-call metadata upload; `copied` marks when the
@@ -814,6 +819,89 @@ struct PagedStep {
     PagesPlanArgs args;
 };
 
+#define CAP_TRY(expr)                                                                                           \
+    do {                                                                                                        \
+        if (cap) {                                                                                              \
+            int rc_ = (expr);                                                                                   \
+            if (rc_) return rc_;                                                                                \
+        }                                                                                                       \
+    } while (0)
+
+// The heads of p's output rows, behind the layers.  The last layer's FFN residual
+// is folded into the final norm of the output rows (h itself is not needed after
+// the last layer).
+int enqueue_heads(jev_ctx *c, const Plan &p, int mode, int n_rows, float *dout, Capture *cap = nullptr)
+{
+    const jev_config &f = c->cfg;
+    const int T = p.T, D = f.hidden, s_down = c->split_down(T);
+    const size_t stride_d = (size_t)T * D;
+    hipStream_t s = c->stream;
+    const QWeight &tab = c->table();
+    NormArgs fn;
+    fn.T = p.n_out;
+    fn.D = D;
+    fn.h = c->h.p;
+    fn.add = c->ydown.p;
+    fn.nadd = stored_parts(T, c->layers[f.n_layers - 1].down, s_down);
+    fn.add_stride = stride_d;
+    fn.store_h = false;
+    fn.w = c->out_norm;
+    fn.eps = f.rms_eps;
+    fn.rows = p.d_out;
+    if (mode == JEV_OUT_SELECTED) {
+        fn.out32 = c->xn.p;
+        HIP_TRY(launch_rmsnorm(fn, s));
+        HeadRowsArgs hr;
+        hr.n_out = p.n_out;
+        hr.n_rows = n_rows;
+        hr.D = D;
+        hr.xn = c->xn.p;
+        hr.table = tab;
+        hr.rows = p.d_rows;
+        hr.out = dout;
+        HIP_TRY(launch_head_rows(hr, s));
+        return JEV_OK;
+    }
+    // full vocabulary
+    if (p.n_out == 1) {
+        fn.out32 = c->xn.p;
+        HIP_TRY(launch_rmsnorm(fn, s));
+        CAP_TRY(cap_add(c, cap, "final_norm", c->xn.p, 1, D));
+        GemvArgs g;
+        g.K = D;
+        g.x = c->xn.p;
+        g.nseg = 1;
+        g.seg[0] = tab;
+        g.y = dout;
+        {
+            ProfScope ps(c, JEV_PROF_GEMV, 2.0 * tab.rows * D, weight_bytes(tab) + 4.0 * (D + tab.rows), true);
+            g.ev_start = ps.a;
+            g.ev_stop = ps.z;
+            HIP_TRY(launch_gemv(g, s));
+        }
+        CAP_TRY(cap_add(c, cap, "logits", dout, 1, tab.rows));
+    } else {
+        fn.ot = c->xt.p;
+        fn.xsum = tab.type == kQ5_1 ? c->xsum.p : nullptr;
+        HIP_TRY(launch_rmsnorm(fn, s));
+        GemmArgs g;
+        g.M = p.n_out;
+        g.K = D;
+        g.xt = c->xt.p;
+        g.xsum = c->xsum.p;
+        g.nseg = 1;
+        g.seg[0] = tab;
+        g.ldy = tab.rows;
+        g.y = dout;
+        ProfScope ps(c, JEV_PROF_GEMM, 2.0 * p.n_out * tab.rows * D, weight_bytes(tab) + p.n_out * 4.0 * (D + tab.rows),
+                     true);
+        g.ev_start = ps.a;
+        g.ev_stop = ps.z;
+        HIP_TRY(launch_gemm(g, s));
+    }
+    return JEV_OK;
+}
+
 // `call` (optional) is the cancellable call this pass belongs to: its cancel
 // flag is checked before every layer; with `throttle` the host also waits,
 // before each group of throttle_group layers, until the device has finished
@@ -828,13 +916,6 @@ int enqueue_forward(jev_ctx *c, const Plan &p, int mode, int n_rows, float *dout
                     const CallScope *call = nullptr, bool throttle = false, Capture *cap = nullptr,
                     const PagedStep *paged = nullptr)
 {
-#define CAP_TRY(expr)                                                                                           \
-    do {                                                                                                        \
-        if (cap) {                                                                                              \
-            int rc_ = (expr);                                                                                   \
-            if (rc_) return rc_;                                                                                \
-        }                                                                                                       \
-    } while (0)
     const jev_config &f = c->cfg;
     const int T = p.T, D = f.hidden, qdim = c->qdim(), kvdim = c->kvdim();
     const int group = f.n_heads / f.n_kv_heads;
@@ -1186,75 +1267,9 @@ int enqueue_forward(jev_ctx *c, const Plan &p, int mode, int n_rows, float *dout
             HIP_TRY(hipEventRecord(c->layer_ev[(l / tg) % jev_ctx::kLayerEvents], s));
     }
 
-    // Heads.  The last layer's FFN residual is folded into the final norm of
-    // the output rows (h itself is not needed after the last layer).
-    if (mode == JEV_OUT_NONE) return JEV_OK;
-    const QWeight &tab = c->table();
-    NormArgs fn;
-    fn.T = p.n_out;
-    fn.D = D;
-    fn.h = c->h.p;
-    fn.add = c->ydown.p;
-    fn.nadd = stored_parts(T, c->layers[f.n_layers - 1].down, s_down);
-    fn.add_stride = stride_d;
-    fn.store_h = false;
-    fn.w = c->out_norm;
-    fn.eps = f.rms_eps;
-    fn.rows = p.d_out;
-    if (mode == JEV_OUT_SELECTED) {
-        fn.out32 = c->xn.p;
-        HIP_TRY(launch_rmsnorm(fn, s));
-        HeadRowsArgs hr;
-        hr.n_out = p.n_out;
-        hr.n_rows = n_rows;
-        hr.D = D;
-        hr.xn = c->xn.p;
-        hr.table = tab;
-        hr.rows = p.d_rows;
-        hr.out = dout;
-        HIP_TRY(launch_head_rows(hr, s));
-        return JEV_OK;
-    }
-    // full vocabulary
-    if (p.n_out == 1) {
-        fn.out32 = c->xn.p;
-        HIP_TRY(launch_rmsnorm(fn, s));
-        CAP_TRY(cap_add(c, cap, "final_norm", c->xn.p, 1, D));
-        GemvArgs g;
-        g.K = D;
-        g.x = c->xn.p;
-        g.nseg = 1;
-        g.seg[0] = tab;
-        g.y = dout;
-        {
-            ProfScope ps(c, JEV_PROF_GEMV, 2.0 * tab.rows * D, weight_bytes(tab) + 4.0 * (D + tab.rows), true);
-            g.ev_start = ps.a;
-            g.ev_stop = ps.z;
-            HIP_TRY(launch_gemv(g, s));
-        }
-        CAP_TRY(cap_add(c, cap, "logits", dout, 1, tab.rows));
-    } else {
-        fn.ot = c->xt.p;
-        fn.xsum = tab.type == kQ5_1 ? c->xsum.p : nullptr;
-        HIP_TRY(launch_rmsnorm(fn, s));
-        GemmArgs g;
-        g.M = p.n_out;
-        g.K = D;
-        g.xt = c->xt.p;
-        g.xsum = c->xsum.p;
-        g.nseg = 1;
-        g.seg[0] = tab;
-        g.ldy = tab.rows;
-        g.y = dout;
-        ProfScope ps(c, JEV_PROF_GEMM, 2.0 * p.n_out * tab.rows * D, weight_bytes(tab) + p.n_out * 4.0 * (D + tab.rows),
-                     true);
-        g.ev_start = ps.a;
-        g.ev_stop = ps.z;
-        HIP_TRY(launch_gemm(g, s));
-    }
-    return JEV_OK;
-#undef CAP_TRY
+    return mode == JEV_OUT_NONE ? JEV_OK : enqueue_heads(c, p, mode, n_rows, dout, cap);
 }
+#undef CAP_TRY
 
 size_t out_floats(const jev_ctx *c, int mode, int n_out, int n_rows)
 {
@@ -1277,7 +1292,7 @@ int check_ready(jev_ctx *c)
 
 // Copies n floats of device output to the caller's host buffer through the
 // pinned landing buffer, draining the stream (the call's synchronisation).
-int copy_out(jev_ctx *c, float *host, const float *dev, size_t n)
+int copy_pinned(jev_ctx *c, const float *dev, size_t n)
 {
     if (n > c->pin_out_n) {
         if (c->pin_out) HIP_TRY(hipHostFree(c->pin_out));
@@ -1288,8 +1303,14 @@ int copy_out(jev_ctx *c, float *host, const float *dev, size_t n)
     }
     if (n) HIP_TRY(hipMemcpyAsync(c->pin_out, dev, n * sizeof(float), hipMemcpyDeviceToHost, c->stream));
     HIP_TRY(hipStreamSynchronize(c->stream));
-    if (n) std::memcpy(host, c->pin_out, n * sizeof(float));
     return JEV_OK;
+}
+
+int copy_out(jev_ctx *c, float *host, const float *dev, size_t n)
+{
+    const int rc = copy_pinned(c, dev, n);
+    if (!rc && n) std::memcpy(host, c->pin_out, n * sizeof(float));
+    return rc;
 }
 
 // Common front half of jev_forward / jev_forward_device.
@@ -1409,6 +1430,7 @@ void jev_destroy(jev_ctx *c)
     c->h.release(); c->y.release(); c->yo.release(); c->ydown.release(); c->q.release();
     c->x32.release(); c->f32.release(); c->xn.release(); c->logits.release();
     c->part.release(); c->apart.release(); c->xsum.release(); c->cap32.release(); c->xt.release(); c->ft.release(); c->ints.release(); c->dec_state.release(); c->tiles.release(); c->amax_v.release(); c->amax_i.release();
+    c->scores.release(); c->lp_part.release(); c->lp_tickets.release();
     if (c->pin_ints) (void)hipHostFree(c->pin_ints);
     if (c->pin_tiles) (void)hipHostFree(c->pin_tiles);
     if (c->pin_out) (void)hipHostFree(c->pin_out);
@@ -2904,9 +2926,37 @@ int jev_pages_sync(jev_pages *h)
 
 void *jev_pages_stream(jev_pages *h) { return h ? (void *)h->stream : nullptr; }
 
-int jev_forward_pages(jev_ctx *c, jev_pages *h, const int32_t *request, const int32_t *past, const int32_t *fresh,
-                      int32_t n_requests, const int32_t *tokens, int32_t n_tokens, int mode, const int32_t *rows,
-                      int32_t n_rows, float *out, size_t out_len)
+} // extern "C"
+
+namespace {
+
+// What jev_forward_pages_logprobs asks of a step.
+struct Score {
+    int every, n_given, n_top;
+    const int32_t *given;
+    float temperature;
+    float *logp, *entropy;
+    int32_t *top;
+    float *top_logp;
+};
+constexpr int kScoreRows = 256; // rows of logits at a time: 134 MB of a vocabulary of 131072
+
+int check_logprobs(int n_given, const int32_t *given, const float *logp, int n_top, int vocab, float temperature, bool any)
+{
+    if (n_given < 0 || (n_given > 0 && (!given || !logp))) return fail(JEV_EINVAL, "given tokens need their ids and a place for their log probabilities");
+    if (n_top < 0 || n_top > std::min(kLogprobsTop, vocab))
+        return fail(JEV_EINVAL, "%d most probable tokens: 0 to %d of a vocabulary of %d", n_top, std::min(kLogprobsTop, vocab), vocab);
+    if (!any) return fail(JEV_EINVAL, "nothing is asked for: no given tokens, entropy or most probable ones");
+    const float c = (float)(1.4426950408889634074 / (double)temperature);
+    if (!(temperature > 0.f) || !std::isfinite(temperature) || !std::isfinite(c) || !(c >= 1.1754944e-38f))
+        return fail(JEV_EINVAL, "temperature %g must be positive and finite, and its reciprocal too", (double)temperature);
+    return JEV_OK;
+}
+
+// `score`: instead of logits, log probabilities at each request's last token, or at every token.
+int forward_pages(jev_ctx *c, jev_pages *h, const int32_t *request, const int32_t *past, const int32_t *fresh,
+                  int32_t n_requests, const int32_t *tokens, int32_t n_tokens, int mode, const int32_t *rows,
+                  int32_t n_rows, float *out, size_t out_len, const Score *score = nullptr)
 try {
     int rc = check_ready(c);
     if (rc) return rc;
@@ -2952,13 +3002,34 @@ try {
     for (int t = 0; t < n_tokens; t++)
         if (tokens[t] < 0 || tokens[t] >= c->embd.rows)
             return fail(JEV_EINVAL, "Token id %d is outside the %d-entry embedding table.", tokens[t], c->embd.rows);
-    const size_t nf = out_floats(c, mode, n_requests, n_rows);
+    const size_t nf = score ? 0 : out_floats(c, mode, n_requests, n_rows);
     if (nf > 0 && (!out || out_len < nf)) return fail(JEV_EINVAL, "the output needs %zu floats", nf);
 
     p.T = n_tokens;
     p.n_out = n_requests;
-    rc = ensure_workspace(c, n_tokens, n_requests, mode, 1);
+    if (score && score->every) {
+        p.n_out = n_tokens;
+        last.resize(n_tokens);
+        std::iota(last.begin(), last.end(), 0);
+    }
+    // scored rows' heads go through in like groups, never one row alone among others (its
+    // logits would be the one-token path's)
+    const int groups = score ? (p.n_out + kScoreRows - 1) / kScoreRows : 1, per = (p.n_out + groups - 1) / groups;
+    rc = ensure_workspace(c, n_tokens, per, mode, 1);
     if (rc) return rc;
+    const size_t n_given = score ? (size_t)p.n_out * score->n_given : 0, n_top = score ? (size_t)p.n_out * score->n_top : 0;
+    if (score) {
+        const size_t V = c->table().rows;
+        for (size_t i = 0; i < n_given; i++)
+            if (score->given[i] < 0 || (size_t)score->given[i] >= V)
+                return fail(JEV_EINVAL, "given token %d is outside the %zu-row head", score->given[i], V);
+        HIP_TRY(grow(c, c->scores, n_given + p.n_out + 2 * n_top));
+        HIP_TRY(grow(c, c->lp_part, kLogprobsParts));
+        if (c->lp_tickets.n == 0) {
+            HIP_TRY(grow(c, c->lp_tickets, kLogprobsParts));
+            HIP_TRY(hipMemsetAsync(c->lp_tickets.p, 0, kLogprobsParts * sizeof(int32_t), c->stream));
+        }
+    }
     // tokens, request, past, fresh, last rows, vocabulary rows
     std::vector<int32_t> &H = c->host_ints;
     H.assign(tokens, tokens + n_tokens);
@@ -2972,6 +3043,7 @@ try {
     H.insert(H.end(), last.begin(), last.end());
     const size_t o_rows = H.size();
     if (mode == JEV_OUT_SELECTED) H.insert(H.end(), rows, rows + n_rows);
+    if (n_given) H.insert(H.end(), score->given, score->given + n_given);
     HIP_TRY(grow(c, c->ints, H.size()));
     if (mode == JEV_OUT_SELECTED) HIP_TRY(grow(c, c->logits, nf));
     HIP_TRY(hipStreamSynchronize(h->stream)); // what the handle's own calls do comes first
@@ -2991,8 +3063,44 @@ try {
     CallScope call(c);
     rc = pages_plan(h, step.args, c->stream);
     step.args = h->plan;
-    if (!rc) rc = enqueue_forward(c, p, mode, n_rows, c->logits.p, nullptr, &call, true, nullptr, &step);
-    if (!rc) rc = copy_out(c, out, c->logits.p, nf);
+    if (!rc) rc = enqueue_forward(c, p, score ? JEV_OUT_NONE : mode, n_rows, c->logits.p, nullptr, &call, true, nullptr, &step);
+    float *const d_entropy = c->scores.p + n_given, *const d_top = d_entropy + p.n_out, *const d_top_logp = d_top + n_top;
+    for (int i = 0, r0 = 0; score && !rc && r0 < p.n_out; i++, r0 += per) {
+        if (i >= jev_ctx::kLeadLayers) HIP_TRY(hipEventSynchronize(c->layer_ev[(i - jev_ctx::kLeadLayers) % jev_ctx::kLayerEvents]));
+        if (call.cancelled()) {
+            rc = fail(JEV_ECANCELED, "the forward pass was cancelled at its heads");
+            break;
+        }
+        Plan part = p;
+        part.n_out = std::min(per, p.n_out - r0);
+        part.d_out = p.d_out + r0;
+        rc = enqueue_heads(c, part, JEV_OUT_FULL, 0, c->logits.p);
+        if (rc) break;
+        LogprobsArgs a;
+        a.logits = c->logits.p;
+        a.ld = a.vocab = c->table().rows;
+        a.rows = part.n_out;
+        a.given = n_given ? base + o_rows + (size_t)r0 * score->n_given : nullptr;
+        a.n_given = score->n_given;
+        a.n_top = score->n_top;
+        a.temperature = score->temperature;
+        a.logp = c->scores.p + (size_t)r0 * score->n_given;
+        a.entropy = d_entropy + r0;
+        a.top = (int32_t *)d_top + (size_t)r0 * score->n_top;
+        a.top_logp = d_top_logp + (size_t)r0 * score->n_top;
+        a.part = c->lp_part.p;
+        a.tickets = c->lp_tickets.p;
+        HIP_TRY(launch_logprobs(a, c->stream));
+        HIP_TRY(hipEventRecord(c->layer_ev[i % jev_ctx::kLayerEvents], c->stream));
+    }
+    if (!rc && score) {
+        rc = copy_pinned(c, c->scores.p, n_given + p.n_out + 2 * n_top);
+        const float *from = c->pin_out;
+        if (!rc && n_given) std::memcpy(score->logp, from, n_given * sizeof(float));
+        if (!rc && score->entropy) std::memcpy(score->entropy, from + n_given, p.n_out * sizeof(float));
+        if (!rc && n_top && score->top) std::memcpy(score->top, from + n_given + p.n_out, n_top * sizeof(float));
+        if (!rc && n_top && score->top_logp) std::memcpy(score->top_logp, from + n_given + p.n_out + n_top, n_top * sizeof(float));
+    } else if (!rc) rc = copy_out(c, out, c->logits.p, nf);
     else (void)hipStreamSynchronize(c->stream);
     if (!rc && call.cancelled()) rc = fail(JEV_ECANCELED, "the forward pass was cancelled");
     return rc ? rc : pages_status(h, c->stream);
@@ -3000,5 +3108,123 @@ try {
     if (c) (void)hipStreamSynchronize(c->stream);
     return fail(JEV_ENOMEM, "no host memory for a step over pages");
 }
+
+} // namespace
+
+extern "C" {
+
+int jev_forward_pages(jev_ctx *c, jev_pages *h, const int32_t *request, const int32_t *past, const int32_t *fresh,
+                      int32_t n_requests, const int32_t *tokens, int32_t n_tokens, int mode, const int32_t *rows,
+                      int32_t n_rows, float *out, size_t out_len)
+{
+    return forward_pages(c, h, request, past, fresh, n_requests, tokens, n_tokens, mode, rows, n_rows, out, out_len);
+}
+
+int jev_forward_pages_logprobs(jev_ctx *c, jev_pages *h, const int32_t *request, const int32_t *past, const int32_t *fresh,
+                               int32_t n_requests, const int32_t *tokens, int32_t n_tokens, int every, const int32_t *given,
+                               int32_t n_given, int32_t n_top, float temperature, float *logp, float *entropy, int32_t *top,
+                               float *top_logp)
+{
+    int rc = check_ready(c);
+    if (!rc) rc = check_logprobs(n_given, given, logp, n_top, c->table().rows, temperature, n_given > 0 || entropy || (n_top > 0 && (top || top_logp)));
+    if (rc) return rc;
+    const Score score = {every != 0, n_given, n_top, given, temperature, logp, entropy, top, top_logp};
+    return forward_pages(c, h, request, past, fresh, n_requests, tokens, n_tokens, JEV_OUT_FULL, nullptr, 0, nullptr, 0, &score);
+}
+
+// ---------------------------------------------------------------- log probabilities
+
+} // extern "C"
+
+struct jev_logprobs {
+    int device = 0, vocab = 0, max_rows = 0;
+    hipStream_t stream = nullptr;
+    LogprobsPart *part = nullptr;
+    int32_t *tickets = nullptr;
+};
+
+extern "C" {
+
+int jev_logprobs_create(int32_t vocab, int32_t max_rows, int device, jev_logprobs **out)
+try {
+    if (!out) return fail(JEV_EINVAL, "out is null");
+    *out = nullptr;
+    if (vocab <= 0 || vocab > 1 << 28) return fail(JEV_EINVAL, "vocab %d must be in [1, 2^28]", vocab);
+    if (max_rows <= 0 || max_rows > 1 << 24) return fail(JEV_EINVAL, "max_rows %d must be in [1, 2^24]", max_rows);
+    int ndev = 0;
+    hipError_t e = hipGetDeviceCount(&ndev);
+    if (e != hipSuccess || ndev == 0) return fail(JEV_EDEVICE, "no HIP device: %s", hipGetErrorString(e));
+    if (device < 0 || device >= ndev) return fail(JEV_EINVAL, "device %d of %d", device, ndev);
+    HIP_TRY(hipSetDevice(device));
+    std::unique_ptr<jev_logprobs, decltype(&jev_logprobs_destroy)> own(new jev_logprobs, jev_logprobs_destroy);
+    jev_logprobs *h = own.get();
+    h->device = device;
+    h->vocab = vocab;
+    h->max_rows = max_rows;
+    e = hipStreamCreate(&h->stream);
+    if (e != hipSuccess) return fail(JEV_EDEVICE, "stream: %s", hipGetErrorString(e));
+    e = hipMalloc((void **)&h->part, kLogprobsParts * sizeof(LogprobsPart));
+    if (e == hipSuccess) e = hipMalloc((void **)&h->tickets, kLogprobsParts * sizeof(int32_t));
+    if (e != hipSuccess) {
+        (void)hipGetLastError();
+        return fail(JEV_ENOMEM, "hipMalloc for log probabilities failed: %s", hipGetErrorString(e));
+    }
+    HIP_TRY(hipMemsetAsync(h->tickets, 0, kLogprobsParts * sizeof(int32_t), h->stream));
+    HIP_TRY(hipStreamSynchronize(h->stream));
+    *out = own.release();
+    return JEV_OK;
+} catch (const std::bad_alloc &) {
+    return fail(JEV_ENOMEM, "no host memory for log probabilities");
+}
+
+void jev_logprobs_destroy(jev_logprobs *h)
+{
+    if (!h) return;
+    (void)hipSetDevice(h->device);
+    if (h->stream) (void)hipStreamSynchronize(h->stream);
+    if (h->part) (void)hipFree(h->part);
+    if (h->tickets) (void)hipFree(h->tickets);
+    if (h->stream) (void)hipStreamDestroy(h->stream);
+    delete h;
+}
+
+int jev_logprobs_device(jev_logprobs *h, const float *logits, int64_t ld, int32_t rows, const int32_t *given, int32_t n_given,
+                        int32_t n_top, float temperature, float *logp, float *entropy, int32_t *top, float *top_logp)
+{
+    if (!h) return fail(JEV_EINVAL, "null log-probabilities handle");
+    if (rows < 0 || rows > h->max_rows) return fail(JEV_EINVAL, "%d rows: the handle was made for %d", rows, h->max_rows);
+    if (ld < h->vocab) return fail(JEV_EINVAL, "ld %lld is less than a row of %d", (long long)ld, h->vocab);
+    if (rows > 0 && !logits) return fail(JEV_EINVAL, "logits is null");
+    const int rc = check_logprobs(n_given, given, logp, n_top, h->vocab, temperature, n_given > 0 || entropy || (n_top > 0 && (top || top_logp)));
+    if (rc) return rc;
+    HIP_TRY(hipSetDevice(h->device));
+    LogprobsArgs a;
+    a.logits = logits;
+    a.ld = ld;
+    a.rows = rows;
+    a.vocab = h->vocab;
+    a.n_given = n_given;
+    a.n_top = n_top;
+    a.given = given;
+    a.temperature = temperature;
+    a.logp = logp;
+    a.entropy = entropy;
+    a.top = top;
+    a.top_logp = top_logp;
+    a.part = h->part;
+    a.tickets = h->tickets;
+    HIP_TRY(launch_logprobs(a, h->stream));
+    return JEV_OK;
+}
+
+int jev_logprobs_sync(jev_logprobs *h)
+{
+    if (!h) return fail(JEV_EINVAL, "null log-probabilities handle");
+    HIP_TRY(hipSetDevice(h->device));
+    HIP_TRY(hipStreamSynchronize(h->stream));
+    return JEV_OK;
+}
+
+void *jev_logprobs_stream(jev_logprobs *h) { return h ? (void *)h->stream : nullptr; }
 
 } // extern "C"

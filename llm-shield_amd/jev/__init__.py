@@ -7,9 +7,10 @@ from .gguf import GgufFile, GgufTensorInfo, NotSupportedError, bind_gguf, config
 from .synth import SEED, VERDICT_NO, VERDICT_YES, SynthModel, quantize, random_tokens, synth_tensor
 from .weight import QuantWeight, get_matmul_strategy, quantize_activations, set_matmul_strategy
 from .pages import KvPages
+from .logprobs import LogProbs, TokenLogProbs
 from .prefix_cache import InvalidOperationError, SystemPromptCache
 from .decider import DecisionResult, TreeDecider, common_prefix, temperature_for
-from .reasoning import batched_greedy, decode_batch, index_of_max, paged_greedy, plan_batches, row_bases
+from .reasoning import batched_greedy, decode_batch, index_of_max, paged_greedy, paged_logprobs, plan_batches, row_bases
 
 __all__ = [
     "ArgumentError", "CancelledError", "DeviceSnapshot", "DataError", "GgufFile", "GgufTensorInfo", "JevError", "NotSupportedError",
@@ -18,6 +19,6 @@ __all__ = [
     "TYPE_NAMES", "TYPE_Q4_0", "TYPE_Q5_1", "TYPE_Q8_0", "TokenLayout", "VERDICT_NO", "VERDICT_YES", "lib",
     "margins", "rope_table", "quantize", "random_tokens", "row_bytes", "synth_tensor", "MATMUL_AUTO", "MATMUL_FLOAT",
     "MATMUL_INTEGER", "get_matmul_strategy", "quantize_activations", "set_matmul_strategy",
-    "KvPages", "InvalidOperationError", "SystemPromptCache", "DecisionResult", "TreeDecider", "common_prefix", "temperature_for",
-    "batched_greedy", "decode_batch", "index_of_max", "paged_greedy", "plan_batches", "row_bases",
+    "KvPages", "LogProbs", "TokenLogProbs", "InvalidOperationError", "SystemPromptCache", "DecisionResult", "TreeDecider", "common_prefix", "temperature_for",
+    "batched_greedy", "decode_batch", "index_of_max", "paged_greedy", "paged_logprobs", "plan_batches", "row_bases",
 ]

@@ -151,6 +151,13 @@ def lib():
         "jev_pages_stream": (c_void_p, [c_void_p]),
         "jev_forward_pages": (c_int, [c_void_p, c_void_p, I32P, I32P, I32P, c_int32, I32P, c_int32, c_int, I32P, c_int32,
                                       F32P, c_size_t]),
+        "jev_forward_pages_logprobs": (c_int, [c_void_p, c_void_p, I32P, I32P, I32P, c_int32, I32P, c_int32, c_int, I32P, c_int32,
+                                               c_int32, c_float, F32P, F32P, I32P, F32P]),
+        "jev_logprobs_create": (c_int, [c_int32, c_int32, c_int, POINTER(c_void_p)]),
+        "jev_logprobs_destroy": (None, [c_void_p]),
+        "jev_logprobs_device": (c_int, [c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int32, c_int32, c_float] + [c_void_p] * 4),
+        "jev_logprobs_sync": (c_int, [c_void_p]),
+        "jev_logprobs_stream": (c_void_p, [c_void_p]),
         "jev_rope_table": (c_int, [POINTER(Config), F32P, c_int32, F32P]),
         "jev_dequantize": (c_int, [c_int, c_void_p, c_size_t, F32P, c_int64]),
         "jev_matmul_q": (c_int, [c_int, c_void_p, c_int64, c_int64, F32P, c_int32, F32P]),
@@ -185,4 +192,6 @@ EXPORTED = [
     "jev_kv_restore_device", "jev_snapshot_length", "jev_snapshot_read", "jev_snapshot_destroy",
     "jev_pages_create", "jev_pages_create_bits", "jev_pages_destroy", "jev_pages_plan_device", "jev_pages_store_device", "jev_pages_attend_device",
     "jev_pages_read_device", "jev_pages_release", "jev_pages_sync", "jev_pages_stream", "jev_forward_pages",
+    "jev_forward_pages_logprobs", "jev_logprobs_create", "jev_logprobs_destroy", "jev_logprobs_device", "jev_logprobs_sync",
+    "jev_logprobs_stream",
 ]

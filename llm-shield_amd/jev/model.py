@@ -14,6 +14,7 @@ from typing import Optional, Sequence
 import numpy as np
 
 from . import _lib as L
+from .logprobs import TokenLogProbs
 
 
 @dataclass
@@ -378,16 +379,42 @@ class MinistralModel:
         flat = self.forward_layout(tokens, lay, L.OUT_SELECTED, r).reshape(len(counts), len(r))
         return [flat[i].copy() for i in range(len(counts))]
 
+    @staticmethod
+    def _step(requests, request_tokens, past):
+        """A step's batch as arrays: request ids, token counts, kept lengths, tokens."""
+        ids, counts = _i32(requests), _i32([len(t) for t in request_tokens])
+        kept = _i32(past) if past is not None else None
+        if len(ids) != len(counts) or (kept is not None and len(kept) != len(ids)):
+            raise L.ArgumentError(L.JEV_EINVAL, "requests, request_tokens and past must have one entry per request")
+        return ids, counts, kept, np.concatenate([_i32(t) for t in request_tokens]) if len(counts) else _i32([])
+
+    def forward_pages_logprobs(self, pages, requests, request_tokens, given=None, top: int = 0, temperature: float = 1.0, past=None,
+                               every: bool = False):
+        """forward_pages, answered with log probabilities (TokenLogProbs) in place of logits: at each request's
+        last token, or with `every` at every token of the step.  given[row]: tokens whose log
+        probabilities that row wants, as many for each row; top: how many of its most probable ones."""
+        ids, counts, kept, tok = self._step(requests, request_tokens, past)
+        rows = len(tok) if every else len(ids)
+        want = np.ascontiguousarray(np.zeros((rows, 0)) if given is None else given, np.int32)
+        if want.ndim != 2 or len(want) != rows:
+            raise L.ArgumentError(L.JEV_EINVAL, f"given must have {rows} rows of tokens")
+        n = want.shape[1]
+        # (a count that is refused has no place for its results)
+        out = TokenLogProbs(np.empty((rows, n), np.float32), np.empty(rows, np.float32), np.empty((rows, max(top, 0)), np.int32),
+                            np.empty((rows, max(top, 0)), np.float32))
+        L.check(self._lib.jev_forward_pages_logprobs(
+            self._h, pages.handle, _ptr(ids, ctypes.c_int32), _ptr(kept, ctypes.c_int32), _ptr(counts, ctypes.c_int32), len(ids),
+            _ptr(tok, ctypes.c_int32), len(tok), int(every), _ptr(want, ctypes.c_int32), n, top, temperature,
+            _ptr(out.logp, ctypes.c_float), _ptr(out.entropy, ctypes.c_float), _ptr(out.top, ctypes.c_int32),
+            _ptr(out.top_logp, ctypes.c_float)))
+        return out
+
     def forward_pages(self, pages, requests, request_tokens, past=None, vocab_rows=None, outputs: bool = True):
         """A step over a paged cache (KvPages): requests[b] keeps past[b] tokens (past None: all it
         has) and appends request_tokens[b].  Returns each request's last-token logits (of
         vocab_rows, or the whole vocabulary), or None without `outputs`.  The context's own
         cache is left alone."""
-        ids, counts = _i32(requests), _i32([len(t) for t in request_tokens])
-        kept = _i32(past) if past is not None else None
-        if len(ids) != len(counts) or (kept is not None and len(kept) != len(ids)):
-            raise L.ArgumentError(L.JEV_EINVAL, "requests, request_tokens and past must have one entry per request")
-        tok = np.concatenate([_i32(t) for t in request_tokens]) if len(counts) else _i32([])
+        ids, counts, kept, tok = self._step(requests, request_tokens, past)
         r = _i32(vocab_rows) if vocab_rows is not None else None
         mode = L.OUT_NONE if not outputs else L.OUT_FULL if r is None else L.OUT_SELECTED
         width = 0 if not outputs else self.config.vocab if r is None else len(r)

@@ -15,6 +15,7 @@ from typing import List, Sequence
 import numpy as np
 
 from . import _lib as L
+from .logprobs import TokenLogProbs
 
 MAX_ROWS = 12            # ReasoningDecider.MaxRows (ReasoningDecider.cs:43)
 KV_TOKEN_BUDGET = 24_000  # ReasoningDecider.KvTokenBudget (:46)
@@ -214,4 +215,36 @@ def paged_greedy(model, pages, prompts: Sequence[Sequence[int]], max_new_tokens:
                 del running[i]
             else:
                 running[i] = (request, held + len(fed), [token])
+    return out
+
+
+def paged_logprobs(model, pages, prompts: Sequence[Sequence[int]], top: int = 0, temperature: float = 1.0) -> List[TokenLogProbs]:
+    """How probable the model finds each prompt: per prompt, at every token but its last, the log probability
+    of the token that follows (logp [len - 1][1]), the entropy there and the `top` most probable tokens.
+
+    Prompts that fit the paged cache (KvPages) together share a step.  The requests of `pages` are
+    released first and at the end; what they held before is dropped."""
+    if any(len(p) < 2 for p in prompts):
+        raise L.ArgumentError(L.JEV_EINVAL, "Every prompt needs at least two tokens.")
+    for p in prompts:
+        if len(p) - 1 > min(pages.max_context, pages.max_tokens, pages.n_pages * pages.page_tokens):
+            raise L.ArgumentError(L.JEV_EINVAL, f"a prompt of {len(p)} tokens does not fit the paged cache.")
+    out: List[TokenLogProbs] = []
+    pages.release(range(pages.max_requests))
+    while len(out) < len(prompts):
+        batch, tokens, used = [], 0, 0
+        for p in prompts[len(out):]:
+            n, need = len(p) - 1, -(-(len(p) - 1) // pages.page_tokens)
+            if len(batch) == pages.max_requests or tokens + n > pages.max_tokens or used + need > pages.n_pages:
+                break
+            batch.append(p)
+            tokens, used = tokens + n, used + need
+        requests = list(range(len(batch)))
+        got = model.forward_pages_logprobs(pages, requests, [p[:-1] for p in batch], [[t] for p in batch for t in p[1:]], top, temperature,
+                                           past=[0] * len(batch), every=True)
+        pages.release(requests)
+        at = 0
+        for p in batch:
+            out.append(TokenLogProbs(*(x[at:at + len(p) - 1] for x in got)))
+            at += len(p) - 1
     return out
