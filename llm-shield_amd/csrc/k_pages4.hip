@@ -479,6 +479,10 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
     int value = -127;                            // with a V row's byte: the power from a weight to fp16's
     const float part = n < 8 ? 0.f : -1.f;       // 8 rows: a column's part of a weight
 
+    auto row_max = [](float x) {
+        x = fmaxf(x, __shfl_xor(x, 16, 64));
+        return fmaxf(x, __shfl_xor(x, 32, 64));
+    };
     for (; kb * 64 < key1; kb += 4) {
         const bool more = (kb + 4) * 64 < key1;
         float sv[16];
@@ -510,11 +514,10 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
         float mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 16; i++) mx = fmaxf(mx, sv[i]);
+        // (m and e move by what their own row sees alone, whichever rows the wave looks for)
         if (__any(mx > m + 6.f)) {
-            float mn = fmaxf(m, ceilf(mx));
-            mn = fmaxf(mn, __shfl_xor(mn, 16, 64));
-            mn = fmaxf(mn, __shfl_xor(mn, 32, 64));
-            l *= m == -INFINITY ? 0.f : exp2f(m - mn);
+            const float mr = row_max(mx), mn = mr > m + 6.f ? ceilf(mr) : m;
+            l *= m == mn ? 1.f : exp2f(m - mn);
             m = mn;
             value = -127 + (e == -INFINITY ? 0 : (int)(9.f - e + m));
         }
@@ -530,10 +533,7 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
                 if (b < 255) mv = fmaxf(mv, sv[i] + (float)(b - 127));
                 else if (sv[i] > -INFINITY) l = NAN; // a token that is not finite, seen
             }
-            float en = fmaxf(e, ceilf(mv));
-            en = fmaxf(en, __shfl_xor(en, 16, 64));
-            en = fmaxf(en, __shfl_xor(en, 32, 64));
-            const float up = e == -INFINITY ? 0.f : exp2f(e - en);
+            const float mr = row_max(mv), en = mr > e + 6.f ? ceilf(mr) : e, up = e == en ? 1.f : exp2f(e - en);
 #pragma unroll
             for (int s = 0; s < NS; s++) o[s] *= up;
             e = en;
@@ -643,18 +643,288 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
     __syncthreads();
 }
 
+template <int HD>
+struct Wide4Lds {
+    union {
+        struct {
+            uint4 kf[2][2 * (HD / 16) * 64], vf[2][4 * (HD / 32) * 64];
+            uint4 power[2][2][4]; // of 64 keys: K's, V's bytes
+            int top[2][4];        // a block's largest V byte
+        };
+        float rows[kPagesWideRows * (HD + 4)]; // a part: means, maximum, sum
+        float factor[8][kPagesWideRows];
+    };
+    int last;
+};
+
+// 128 (token, head) rows of a request and KV head, 32 to a wave, over its keys in blocks
+// of 64: as above, with K and V turned into fp16 fragments (codes less zero points times
+// steps) in LDS once for the four waves, double buffered: the next block's codes are in
+// flight during a block's products and become fragments beside its scores' matrix
+// instructions.  v_mfma_f32_32x32x16_f16: S^T is two tiles of 32 keys, their rows dealt so
+// that a lane's sixteen scores are one block's tokens in order.
+template <int HD>
+__device__ __forceinline__ void attend4_wide(const Attend4View &p, Wide4Lds<HD> &lds, const PagesItem &r, int first)
+{
+    constexpr int NC = HD / 16, ND = HD / 32;
+    constexpr Pages4 at(HD);
+    auto &kf = lds.kf;
+    auto &vf = lds.vf;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int hh = lane >> 5, n = lane & 31, h = first % p.n_kv, item = first / p.n_kv;
+    const int32_t *table = p.table + (size_t)r.id * p.width;
+
+    const int n_rows = r.row1, wrow = r.row0 + 32 * wave;
+    const bool active = wrow < n_rows;
+    const int row = min(wrow + n, n_rows - 1), token = row / p.group, head = h * p.group + row % p.group;
+    const int limit = r.past + token; // last visible key
+    const int key1 = min(r.key1, r.past + min(n_rows - 1, r.row0 + kPagesWideRows - 1) / p.group + 1);
+    const int clear = r.past + min(wrow, n_rows - 1) / p.group; // keys up to it are seen by every row of the wave
+    const int last = (r.len - 1) / kPageBlock;
+
+    // A wave stages one of 64 keys' four 16-token blocks.  Buffer loads, as in the 8-bit
+    // cache: their bases are the wave's.
+    const rsrc_t rt = make_rsrc(table, 4 * p.width);
+    auto page_of = [&](int kb) {
+        return __builtin_amdgcn_raw_buffer_load_b32(rt, 0, 4 * (min(4 * kb + wave, last) >> p.sub_shift), 0);
+    };
+    // A lane's share: the codes of a quarter of token lane / 4 (K) and, of all tokens, of
+    // dims 32 i + n and 16 on (V, hd 64: of one), i = lane / 16; their steps.
+    const int vi = lane / (HD == 128 ? 16 : 32), quarter = lane & 3;
+    const int ks_at = at.ks + 4 * (4 * (HD == 128 ? quarter : quarter >> 1) + ((lane >> 2) & 3));
+    uint32_t kr[HD / 32], vr[HD / 32], ks;
+    uint4 vs, er;
+    auto fetch = [&](int kb, int page) {
+        const int c = min(4 * kb + wave, last) & (p.sub - 1);
+        const size_t b = (((size_t)__builtin_amdgcn_readfirstlane(page) * p.n_kv + h) << p.sub_shift) + c;
+        const rsrc_t rb = make_rsrc(p.pool + b * at.bytes, at.bytes);
+        if constexpr (HD == 128) {
+            const uint4 k = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rb, 16 * lane, at.k, 0));
+            const uint4 v = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rb, 16 * lane, at.v, 0));
+            kr[0] = k.x, kr[1] = k.y, kr[2] = k.z, kr[3] = k.w, vr[0] = v.x, vr[1] = v.y, vr[2] = v.z, vr[3] = v.w;
+        } else {
+            const uint2 k = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rb, 8 * lane, at.k, 0));
+            const uint2 v = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rb, 8 * lane, at.v, 0));
+            kr[0] = k.x, kr[1] = k.y, vr[0] = v.x, vr[1] = v.y;
+        }
+        ks = __builtin_amdgcn_raw_buffer_load_b32(rb, ks_at, 0, 0);
+        vs = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rb, 16 * vi, at.vs, 0));
+        er = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rb, 16 * (lane & 1), at.ke, 0));
+    };
+    // K's rows of the tile are dealt by quarter so that neighbouring lanes' writes take all
+    // banks.  NC pieces: a lane's words of K, then of V.
+    const int krow = (8 * (lane >> 4) + 4 * (wave & 1) + ((lane >> 2) & 3)) ^ (quarter << 1);
+    const int vcol = 32 * (wave & 1) + (HD == 128 ? lane & 15 : 16 * (lane & 1) + ((lane >> 1) & 15));
+    Steps kst, vst[4];
+    auto put = [&](int buf, int piece) {
+        if (piece < NC / 2) {
+            if (piece == 0) {
+                const half2_t uz = __builtin_bit_cast(half2_t, (turn_left(ks, (4 - 4 * (lane >> 4)) & 31) & kNibble) | kSixteen);
+                kst = Steps(half2_t{uz[0], uz[0]}, half2_t{uz[1], uz[1]});
+                const int most = most_byte(er);
+                if (lane < 2) lds.power[buf][lane][wave] = er;
+                if (lane == 1) lds.top[buf][wave] = most;
+            }
+            const int c = HD == 128 ? 2 * quarter + (piece >> 1) : quarter;
+            (kf[buf] + ((wave >> 1) * NC + c) * 64 + krow)[32 * (piece & 1)] = __builtin_bit_cast(uint4, word_f16(kr[piece], kst));
+        } else {
+            const int i = piece - NC / 2, j = HD == 128 ? i >> 1 : i, b = HD == 128 ? i & 1 : 0; // tokens 8 j .., dims 16 b ..
+            if (b == 0) value_steps(j ? vs.y : vs.x, j ? vs.w : vs.z, vst);
+            (vf[buf] + ((2 * vi + (wave >> 1)) * 2 + j) * 64 + vcol)[16 * b] = __builtin_bit_cast(uint4, word_f16(vr[HD == 128 ? 2 * b + j : j], vst));
+        }
+    };
+
+    int kb = r.key0 / 64;
+    int next = page_of(kb);
+    fetch(kb, next);
+    next = page_of(kb + 1);
+
+    // Q^T fragments: dims 16 c + 8 hh .. + 7 of row n
+    half8_t qh[NC], ql[NC];
+    int query;
+    {
+        const float *src = p.q + ((size_t)(r.start + token) * p.n_heads + head) * HD + 8 * hh;
+        float m = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(src[16 * c + i]));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        const Query4 scaled(m, p.scale);
+        query = scaled.power();
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                _Float16 hi, lw;
+                scaled.split(src[16 * c + i], hi, lw);
+                qh[c][i] = hi;
+                ql[c][i] = lw;
+            }
+    }
+
+    floatx16 o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; d++) o[d] = floatx16{};
+    float m = -INFINITY, l = 0.f, e = -INFINITY; // m and e whole numbers; outputs are held times 2^(9 - e)
+    int value = -127;                            // with a V row's byte: the power from a weight to fp16's
+#pragma unroll
+    for (int i = 0; i < NC; i++) put(0, i);
+    fetch(kb + 1, next); // (past the last block: the last again, which nobody reads)
+    next = page_of(kb + 2);
+    __syncthreads();
+
+    if (!active) { // no rows of its own: it stages for the others
+        for (int buf = 0; kb * 64 < key1; kb++, buf ^= 1) {
+#pragma unroll
+            for (int i = 0; i < NC; i++) put(buf ^ 1, i);
+            fetch(kb + 2, next);
+            next = page_of(kb + 3);
+            __syncthreads();
+        }
+    }
+    for (int buf = 0; kb * 64 < key1; kb++, buf ^= 1) {
+        floatx16 s[2] = {floatx16{}, floatx16{}};
+        auto kfrag = [&](int t, int c) {
+            return __builtin_bit_cast(half8_t, kf[buf][(t * NC + c) * 64 + (lane ^ (((HD == 128 ? c >> 1 : c) & 3) << 1))]);
+        };
+        half8_t k0 = kfrag(0, 0), k1 = kfrag(1, 0);
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const half8_t n0 = kfrag(0, min(c + 1, NC - 1)), n1 = kfrag(1, min(c + 1, NC - 1));
+            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qh[c], s[0], 0, 0, 0);
+            s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qh[c], s[1], 0, 0, 0);
+            put(buf ^ 1, c);
+            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, ql[c], s[0], 0, 0, 0);
+            s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, ql[c], s[1], 0, 0, 0);
+            k0 = n0, k1 = n1;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        fetch(kb + 2, next);
+        next = page_of(kb + 3);
+        uint4 ve[2];
+        int top[2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const uint4 ke = lds.power[buf][0][2 * t + hh];
+            ve[t] = lds.power[buf][1][2 * t + hh];
+            top[t] = lds.top[buf][2 * t + hh];
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[t][i] = __builtin_amdgcn_ldexpf(s[t][i], byte_of(ke, i) + query);
+        }
+        if (kb * 64 + 63 > clear) {
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const int left = limit - (kb * 64 + 32 * t + 16 * hh); // last visible token of the lane's block
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (i > left) s[t][i] = -INFINITY;
+            }
+        }
+        float mx[2];
+        bool past_e = false;
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            mx[t] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; i++) mx[t] = fmaxf(mx[t], s[t][i]);
+            // (as in attend4_tile: a bound on the row's products, NaN where a block without
+            // visible keys has a token that is not finite)
+            past_e |= mx[t] + (top[t] == 255 ? INFINITY : (float)(top[t] - 127)) > e + 6.f;
+        }
+        auto halves = [](float x) { // the larger of the lane's and the other half's
+            const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+            return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+        };
+        const bool past_m = fmaxf(mx[0], mx[1]) > m + 6.f;
+        if (__any(past_m || past_e)) {
+            if (__any(past_m)) {
+                const float mr = halves(fmaxf(mx[0], mx[1])), mn = mr > m + 6.f ? ceilf(mr) : m;
+                l *= m == mn ? 1.f : exp2f(m - mn);
+                m = mn;
+            }
+            if (__any(past_e)) {
+                float mv = -INFINITY;
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int b = byte_of(ve[t], i);
+                        if (b < 255) mv = fmaxf(mv, s[t][i] + (float)(b - 127));
+                        else if (s[t][i] > -INFINITY) l = NAN; // a token that is not finite, seen
+                    }
+                const float mr = halves(mv), en = mr > e + 6.f ? ceilf(mr) : e, up = e == en ? 1.f : exp2f(e - en);
+#pragma unroll
+                for (int d = 0; d < ND; d++) o[d] *= up;
+                e = en;
+            }
+            value = -127 + (e == -INFINITY ? 0 : (int)(9.f - e + (m == -INFINITY ? 0.f : m)));
+        }
+        const float mu = m == -INFINITY ? 0.f : m;
+        uint32_t hi[2][8], lw[2][8];
+        auto weights = [&](int t, int i) { // of tokens 2 i and 2 i + 1 of the lane's block
+            const float x = __builtin_amdgcn_exp2f(s[t][2 * i] - mu), y = __builtin_amdgcn_exp2f(s[t][2 * i + 1] - mu);
+            l += x;
+            l += y;
+            split2_mix(__builtin_amdgcn_ldexpf(x, byte_of(ve[t], 2 * i) + value),
+                       __builtin_amdgcn_ldexpf(y, byte_of(ve[t], 2 * i + 1) + value), hi[t][i], lw[t][i]);
+        };
+        auto pfrag = [&](const uint32_t (&x)[8], int j) {
+            return __builtin_bit_cast(half8_t, make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]));
+        };
+        auto vfrag = [&](int t, int k) { // k = ND j + d
+            return __builtin_bit_cast(half8_t, vf[buf][(((k % ND) * 2 + t) * 2 + k / ND) * 64 + lane]);
+        };
+        half8_t v = vfrag(0, 0);
+#pragma unroll
+        for (int i = 0; i < 8; i++) weights(0, i);
+        __builtin_amdgcn_sched_barrier(0);
+        // the second tile's exponentials run beside the first's V^T P^T
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int k = 0; k < 2 * ND; k++) {
+                const half8_t ahead = t && k == 2 * ND - 1 ? v : vfrag(k == 2 * ND - 1 ? 1 : t, (k + 1) % (2 * ND));
+                o[k % ND] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pfrag(hi[t], k / ND), o[k % ND], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4 / ND; i++)
+                    if (!t) weights(1, 8 / ND / 2 * k + i);
+                o[k % ND] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pfrag(lw[t], k / ND), o[k % ND], 0, 0, 0);
+                v = ahead;
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        __syncthreads();
+    }
+    l += __shfl_xor(l, 32, 64);
+    wide_result<HD>(p, lds, item, h, o, MeanScale(e, m, l), m, l);
+}
+
 } // namespace
 
-// The attention of a plan: its 16-row tiles, workgroups taking turns.
-template <int HD>
+// The attention of a plan in one launch: wide tiles first, then 16-row tiles, `tiles`
+// workgroups of which take turns.
+template <int HD, bool WIDE>
 __global__ __launch_bounds__(256, 2) void pages4_attend_kernel(Attend4View p)
 {
-    __shared__ __align__(16) Tile4Lds<HD> lds;
-    const int first = (int)blockIdx.x, h = first % p.n_kv, stride = p.tiles / p.n_kv;
+    union Lds {
+        Tile4Lds<HD> tile;
+        Wide4Lds<WIDE ? HD : 32> wide;
+    };
+    __shared__ __align__(16) char mem[sizeof(Lds)];
+    // (the first item, which is there if not of this plan, does not wait for the head)
+    const bool wide = WIDE && (int)blockIdx.x < p.wides;
+    const int first = wide ? blockIdx.x : (int)blockIdx.x - p.wides, h = first % p.n_kv, stride = p.tiles / p.n_kv;
     int item = first / p.n_kv;
-    PagesItem it = p.item[item]; // (it is there if not of this plan, and does not wait for the head)
+    PagesItem it = wide ? p.wide_item[item] : p.item[item];
     const PagesPlanHead plan = *p.head;
-    if (outgrown(p, plan)) return;
+    if (outgrown(p, plan) || item >= (wide ? plan.n_wide : plan.n_items)) return;
+    if constexpr (WIDE) {
+        if (wide) {
+            attend4_wide<HD>(p, *(Wide4Lds<HD> *)mem, it, first);
+            return;
+        }
+    }
+    Tile4Lds<HD> &lds = *(Tile4Lds<HD> *)mem;
     while (item < plan.n_items) {
         if (it.row1 - it.row0 <= 8) attend4_tile<HD, 8>(p, lds, it, h);
         else attend4_tile<HD, 16>(p, lds, it, h);
@@ -669,12 +939,14 @@ hipError_t launch_pages4_attend(const Pages &p, const PagesAttendArgs &a, hipStr
     const int64_t split = (int64_t)((p.group + kPagesTileRows - 1) / kPagesTileRows) * std::min(a.n_requests, a.n_tokens);
     const int64_t parts = std::min((int64_t)p.max_parts, split * pages_most_parts(p.max_context));
     const int64_t most = a.n_tokens == 0 ? 1 : std::max<int64_t>(1, parts + (int64_t)a.n_tokens * p.group / kPagesTileRows + a.n_requests);
-    const int tiles = (int)(most < 2048 ? most : 2048) * p.n_kv;
+    const int64_t most_wide = (int64_t)a.n_tokens * p.group / kPagesWideRows + a.n_requests + pages_wide_target(p.n_kv);
+    const int wides = a.wide ? (int)(most_wide * p.n_kv) : 0, tiles = (int)(most < 2048 ? most : 2048) * p.n_kv;
     const Attend4View view = {layer4_of(p, a.layer), p.table, p.head, p.item, p.wide, p.part, p.wide_part, p.tickets, p.wide_tickets,
                               a.q, a.out, p.n_kv, p.n_heads, p.group, p.sub, p.sub_shift, p.width, p.scale,
-                              0, tiles, a.n_tokens, a.n_requests, 0};
-    auto launch = [&](auto kernel) { launch_stamped(a.ev_start, a.ev_stop, kernel, dim3(tiles), dim3(256), 0, s, view); };
-    launch(p.hd == 128 ? pages4_attend_kernel<128> : pages4_attend_kernel<64>);
+                              wides, tiles, a.n_tokens, a.n_requests, a.wide};
+    auto launch = [&](auto kernel) { launch_stamped(a.ev_start, a.ev_stop, kernel, dim3(wides + tiles), dim3(256), 0, s, view); };
+    if (p.hd == 128) launch(a.wide ? pages4_attend_kernel<128, true> : pages4_attend_kernel<128, false>);
+    else launch(a.wide ? pages4_attend_kernel<64, true> : pages4_attend_kernel<64, false>);
     return hipGetLastError();
 }
 

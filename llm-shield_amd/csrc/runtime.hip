@@ -2670,7 +2670,7 @@ int pages_plan(jev_pages *h, const PagesPlanArgs &a, hipStream_t s)
     h->plan = a;
     // as many tokens as requests: 16-row tiles serve whatever there is, and the
     // wide tiles' launches are saved
-    h->plan.wide = h->p.bits == 8 && a.n_tokens > a.n_requests;
+    h->plan.wide = a.n_tokens > a.n_requests;
     HIP_TRY(launch_pages_plan(h->p, h->plan, s));
     return JEV_OK;
 }
