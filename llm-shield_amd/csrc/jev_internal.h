@@ -544,10 +544,11 @@ hipError_t launch_pages4_read(const Pages &p, int layer, const int32_t *slot, in
 // ---------------------------------------------------------------- log probabilities
 
 constexpr int kLogprobsTop = 32;     // most probable tokens of a row, at most
-constexpr int kLogprobsParts = 2048; // partial results of a call, at most (rows in parts: fewer than half of them)
-struct LogprobsPart {                // of a part of a row: its largest logit, its sums, its largest keys in order
-    double s, t;
-    uint64_t m, key[kLogprobsTop];
+constexpr int kLogprobsParts = 1024; // partial results of a call, at most (rows in parts: a quarter of them)
+constexpr int kLogprobsSplit = 16;   // parts of a row, at most: one wave merges their four waves each
+struct LogprobsPart {                // of a part of a row: its waves' sums, largest logit and how many are it, and its largest keys in order
+    double s[4], t[4];
+    uint64_t m[4], key[kLogprobsTop];
 };
 struct LogprobsArgs {
     const float *logits = nullptr; // [rows][ld]

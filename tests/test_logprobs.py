@@ -73,10 +73,10 @@ for vocab in (100, 50021, 131072, 1 << 28):
 """)
     for vocab, rows, grid in got:
         parts = grid // rows
-        assert grid == rows * parts and parts <= 64 and (parts == 1 or grid <= 2048)
-        assert parts == 1 or (parts - 1) * 4096 < vocab
+        assert grid == rows * parts and parts <= 16 and (parts == 1 or grid <= 1024)
+        assert parts == 1 or (parts - 1) * 8192 < vocab
         if rows == 1 and vocab == 131072:
-            assert parts == 32
+            assert parts == 16
 
 
 def test_scores_refuse_bad_arguments_without_a_step():
