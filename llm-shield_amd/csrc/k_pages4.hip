@@ -25,13 +25,21 @@ __device__ __forceinline__ uint32_t turn_left(uint32_t x, int by) { return __bui
 // Bit of element i (0 .. 7) of a word before the turn: pairs (0, 1), (2, 3), ...
 __host__ __device__ constexpr int nibble_at(int i) { return 4 * ((i >> 1) + 4 * (i & 1)); }
 
-// Pair p of a word as fp16: 16 + n.
-template <int P>
-__device__ __forceinline__ half2_t nibble_pair(uint32_t w)
+// Pair p of a word as fp16: 16 + n.  `k16`: sixteen() in a vector register, so that mask and
+// exponent are one v_and_or (an instruction takes one constant from the scalar side).
+__device__ __forceinline__ uint32_t sixteen()
 {
-    const uint32_t x = P == 0 ? w << 4 : P == 1 ? w : P == 2 ? w >> 4 : turn_left(w, 24);
-    return __builtin_bit_cast(half2_t, (x & kNibble) | kSixteen);
+    uint32_t k = kSixteen;
+    asm("" : "+v"(k));
+    return k;
 }
+__device__ __forceinline__ half2_t masked(uint32_t x, uint32_t k16) { return __builtin_bit_cast(half2_t, (x & kNibble) | k16); }
+template <int P>
+__device__ __forceinline__ half2_t nibble_pair(uint32_t w, uint32_t k16)
+{
+    return masked(P == 0 ? w << 4 : P == 1 ? w : P == 2 ? w >> 4 : turn_left(w, 24), k16);
+}
+__device__ __forceinline__ half2_t nibble_pair(uint32_t w, int p, uint32_t k16) { return masked(turn_left(w, (4 - 4 * p) & 31), k16); }
 
 // Steps and zero points turn 16 + n into (n - z) u: (16 + n) u - (16 + z) u, where the
 // second product is a whole number below 2^9.
@@ -46,29 +54,26 @@ struct Steps {
 };
 
 // A word's eight elements: with the same step for all, and with one for each pair's halves.
-__device__ __forceinline__ half8_t word_f16(uint32_t w, const Steps &s)
+__device__ __forceinline__ half8_t word_f16(uint32_t w, const Steps &s, uint32_t k16)
 {
-    return __builtin_bit_cast(half8_t, make_uint4(s(nibble_pair<0>(w)), s(nibble_pair<1>(w)), s(nibble_pair<2>(w)), s(nibble_pair<3>(w))));
+    return __builtin_bit_cast(half8_t, make_uint4(s(nibble_pair<0>(w, k16)), s(nibble_pair<1>(w, k16)), s(nibble_pair<2>(w, k16)),
+                                                  s(nibble_pair<3>(w, k16))));
 }
-__device__ __forceinline__ half8_t word_f16(uint32_t w, const Steps (&s)[4])
+__device__ __forceinline__ half8_t word_f16(uint32_t w, const Steps (&s)[4], uint32_t k16)
 {
-    return __builtin_bit_cast(half8_t, make_uint4(s[0](nibble_pair<0>(w)), s[1](nibble_pair<1>(w)), s[2](nibble_pair<2>(w)), s[3](nibble_pair<3>(w))));
+    return __builtin_bit_cast(half8_t, make_uint4(s[0](nibble_pair<0>(w, k16)), s[1](nibble_pair<1>(w, k16)), s[2](nibble_pair<2>(w, k16)),
+                                                  s[3](nibble_pair<3>(w, k16))));
 }
 
-// Pair t of K's step word (u of token 4 t + r low, its z high), for all of a token's group.
-template <int T>
-__device__ __forceinline__ Steps key_steps(uint32_t w)
-{
-    const half2_t uz = nibble_pair<T>(w);
-    return Steps(half2_t{uz[0], uz[0]}, half2_t{uz[1], uz[1]});
-}
+// Of a K step word's pair (u of a token's group low, its z high), for all of the group.
+__device__ __forceinline__ Steps key_steps(half2_t uz) { return Steps(half2_t{uz[0], uz[0]}, half2_t{uz[1], uz[1]}); }
 // V's step and zero words of eight tokens.
-__device__ __forceinline__ void value_steps(uint32_t u, uint32_t z, Steps (&s)[4])
+__device__ __forceinline__ void value_steps(uint32_t u, uint32_t z, Steps (&s)[4], uint32_t k16)
 {
-    s[0] = Steps(nibble_pair<0>(u), nibble_pair<0>(z));
-    s[1] = Steps(nibble_pair<1>(u), nibble_pair<1>(z));
-    s[2] = Steps(nibble_pair<2>(u), nibble_pair<2>(z));
-    s[3] = Steps(nibble_pair<3>(u), nibble_pair<3>(z));
+    s[0] = Steps(nibble_pair<0>(u, k16), nibble_pair<0>(z, k16));
+    s[1] = Steps(nibble_pair<1>(u, k16), nibble_pair<1>(z, k16));
+    s[2] = Steps(nibble_pair<2>(u, k16), nibble_pair<2>(z, k16));
+    s[3] = Steps(nibble_pair<3>(u, k16), nibble_pair<3>(z, k16));
 }
 
 __device__ __forceinline__ uint32_t word_of(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
@@ -352,28 +357,60 @@ struct Attend4View {
 // [2^13, 2^14), then by the softmax's scale in powers of two.  A key's 2^e and the row's
 // power meet in a score's exponent, in whole numbers.
 struct Query4 {
-    float f1, f2, scale;
+    float scale;
     int ex;
-    Query4() = default;
     __device__ __forceinline__ Query4(float m, float softmax)
-        : scale(softmax * 1.44269504088896341f), ex(m > 0.f && m < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(m) : 0)
-    {
-        f1 = ldexpf(1.f, ex / 2), f2 = ldexpf(1.f, ex - ex / 2);
-    }
+        : scale(softmax * 1.44269504088896341f), ex(m > 0.f && m < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(m) : 0) {}
     __device__ __forceinline__ int power() const { return -127 - ex; } // with a key's byte
-    __device__ __forceinline__ void split(float x, _Float16 &hi, _Float16 &lo) const
-    {
-        float y = x * f1 * f2 * scale;
-        asm("" : "+v"(y)); // rounded to fp32: hi straight from the product may be another than the one that lo completes
-        hi = (_Float16)y;
-        lo = (_Float16)(y - (float)hi);
-    }
+    __device__ __forceinline__ float scaled(float x) const { return __builtin_amdgcn_ldexpf(x, ex) * scale; }
 };
+
+// Two values as fp16, to nearest, and `part` times that plus the values: with -1 what fp16
+// leaves of them.  (The remainder is taken of the fp32 values: they are rounded to fp32 first.)
+__device__ __forceinline__ uint32_t pair_f16(float x0, float x1)
+{
+    typedef float floatx2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{x0, x1}, half2_t));
+}
+__device__ __forceinline__ void remainders(uint32_t f, float part, float x0, float x1, float &r0, float &r1)
+{
+    asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(f), "v"(part), "v"(x0));
+    asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(f), "v"(part), "v"(x1));
+}
+// Eight elements of a query, rounded to fp32, as a pair of fragments; or the one that `part`
+// (0: high, -1: low) names.
+__device__ __forceinline__ void split_query(const Query4 &q, const float (&x)[8], half8_t &hi, half8_t &lo)
+{
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        float y0 = q.scaled(x[2 * i]), y1 = q.scaled(x[2 * i + 1]), r0, r1;
+        asm("" : "+v"(y0), "+v"(y1)); // hi straight from the product may be another than the one that lo completes
+        h[i] = pair_f16(y0, y1);
+        remainders(h[i], -1.f, y0, y1, r0, r1);
+        l[i] = pair_f16(r0, r1);
+    }
+    hi = __builtin_bit_cast(half8_t, make_uint4(h[0], h[1], h[2], h[3]));
+    lo = __builtin_bit_cast(half8_t, make_uint4(l[0], l[1], l[2], l[3]));
+}
+__device__ __forceinline__ half8_t split_query(const Query4 &q, const float (&x)[8], float part)
+{
+    uint32_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        float y0 = q.scaled(x[2 * i]), y1 = q.scaled(x[2 * i + 1]), r0, r1;
+        asm("" : "+v"(y0), "+v"(y1));
+        remainders(pair_f16(y0, y1), part, y0, y1, r0, r1);
+        h[i] = pair_f16(r0, r1);
+    }
+    return __builtin_bit_cast(half8_t, make_uint4(h[0], h[1], h[2], h[3]));
+}
 
 template <int HD>
 struct Tile4Lds {
     float lo[4][16][HD + 4];
     float lm[4][kPagesTileRows], ll[4][kPagesTileRows];
+    uint2 steps[4][4][HD / 4 + 2]; // a wave's V steps of 64 keys: [block][group of dims][pair of tokens]
     int last;
 };
 
@@ -393,6 +430,7 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
     constexpr Pages4 at(HD);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, n = lane & 15;
+    const uint32_t k16 = sixteen();
     const int32_t *table = p.table + (size_t)r.id * p.width;
     // columns past the request's rows repeat its last one
     const int n_rows = r.row1, row = min(r.row0 + (n & (ROWS - 1)), n_rows - 1);
@@ -403,13 +441,18 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
     const int key1 = min(r.key1, top + 1), clear = r.past + r.row0 / p.group;
     const int last = (r.len - 1) / kPageBlock; // blocks past it are read as this one, and masked
 
+    // V's steps of a block are made by its sixteen lanes, NI / 2 pairs of tokens of a group
+    // each, and shared through LDS
+    const int pair0 = n * (NI / 2), step_at = 16 * (pair0 >> 3) + 4 * ((pair0 >> 2) & 1);
+    auto &steps = lds.steps[wave][g];
+
     // a lane reads K of block n / 4 of the four, V and the powers of block g
     auto page_of = [&](int kb, int i) { return table[min(4 * kb + i, last) >> p.sub_shift]; };
     auto block_of = [&](int kb, int i, int page) {
         return p.pool + ((((size_t)page * p.n_kv + h) << p.sub_shift) + (min(4 * kb + i, last) & (p.sub - 1))) * at.bytes;
     };
-    uint4 kr[4], vr[NI], vs[NI], ke, ve;
-    uint32_t ks;
+    uint4 kr[4], vr[NI], ke, ve;
+    uint32_t ks, vu, vz;
     auto fetch_k = [&](int kb, int page) {
         const uint8_t *b = block_of(kb, n >> 2, page);
 #pragma unroll
@@ -428,10 +471,9 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
         ke = *(const uint4 *)(b + at.ke);
         ve = *(const uint4 *)(b + at.ve);
 #pragma unroll
-        for (int i = 0; i < NI; i++) {
-            vr[i] = *(const uint4 *)(b + at.v + 256 * i + 16 * n);
-            vs[i] = *(const uint4 *)(b + at.vs + 16 * i);
-        }
+        for (int i = 0; i < NI; i++) vr[i] = *(const uint4 *)(b + at.v + 256 * i + 16 * n);
+        vu = *(const uint32_t *)(b + at.vs + step_at);
+        vz = *(const uint32_t *)(b + at.vs + step_at + 8);
     };
     int kb = r.key0 / 64 + wave;
     int pk = page_of(kb, n >> 2), pv = page_of(kb, g);
@@ -445,6 +487,7 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
     // Q^T fragments: dims 8 NC g + 8 c .. + 7 of column n
     half8_t qf[NQ][NC];
     int query;
+    const float part = n < 8 ? 0.f : -1.f; // 8 rows: a column's part of a query or a weight
     {
         const float *src = p.q + ((size_t)(r.start + token) * p.n_heads + head) * HD + 8 * NC * g;
         float x[NC][8], m = 0.f;
@@ -460,16 +503,10 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
         const Query4 scaled(m, p.scale);
         query = scaled.power();
 #pragma unroll
-        for (int c = 0; c < NC; c++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                _Float16 hi, lw;
-                scaled.split(x[c][i], hi, lw);
-                if constexpr (NQ == 2) {
-                    qf[0][c][i] = hi;
-                    qf[1][c][i] = lw;
-                } else qf[0][c][i] = n < 8 ? hi : lw;
-            }
+        for (int c = 0; c < NC; c++) {
+            if constexpr (NQ == 2) split_query(scaled, x[c], qf[0][c], qf[1][c]);
+            else qf[0][c] = split_query(scaled, x[c], part);
+        }
     }
 
     floatx4 o[NS];
@@ -477,7 +514,6 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
     for (int s = 0; s < NS; s++) o[s] = floatx4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f, e = -INFINITY; // m and e whole numbers; outputs are held times 2^(9 - e)
     int value = -127;                            // with a V row's byte: the power from a weight to fp16's
-    const float part = n < 8 ? 0.f : -1.f;       // 8 rows: a column's part of a weight
 
     auto row_max = [](float x) {
         x = fmaxf(x, __shfl_xor(x, 16, 64));
@@ -486,13 +522,14 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
     for (; kb * 64 < key1; kb += 4) {
         const bool more = (kb + 4) * 64 < key1;
         float sv[16];
-        const Steps kst[4] = {key_steps<0>(ks), key_steps<1>(ks), key_steps<2>(ks), key_steps<3>(ks)};
+        const Steps kst[4] = {key_steps(nibble_pair<0>(ks, k16)), key_steps(nibble_pair<1>(ks, k16)), key_steps(nibble_pair<2>(ks, k16)),
+                              key_steps(nibble_pair<3>(ks, k16))};
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             floatx4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < NC; c++) {
-                const half8_t k = word_f16(word_of(kr[t], c), kst[t]);
+                const half8_t k = word_f16(word_of(kr[t], c), kst[t], k16);
 #pragma unroll
                 for (int i = 0; i < NQ; i++) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[i][c], acc, 0, 0, 0);
             }
@@ -500,11 +537,17 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
             for (int i = 0; i < 4; i++) {
                 float x = acc[i];
                 if constexpr (NQ == 1) // the other part's column is eight lanes on
-                    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, true));
+                    x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x128, 0xf, 0xf, true));
                 sv[4 * t + i] = __builtin_amdgcn_ldexpf(x, byte_of(ke, 4 * t + i) + query);
             }
         }
         if (more) fetch_k(kb + 4, pk);
+#pragma unroll
+        for (int i = 0; i < NI / 2; i++) {
+            const int t = (pair0 & 3) + i;
+            const Steps st(nibble_pair(vu, t, k16), nibble_pair(vz, t, k16));
+            steps[pair0 + i] = make_uint2(__builtin_bit_cast(uint32_t, st.u), __builtin_bit_cast(uint32_t, st.m));
+        }
         if (kb * 64 + 63 > clear) {
             const int left = limit - (kb * 64 + 16 * g); // last visible token of the lane's block
 #pragma unroll
@@ -556,9 +599,7 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
                 if constexpr (NQ == 2) split2_mix(x, y, hi[i], lw[i]);
                 else { // the high columns keep x, the low ones what fp16 leaves of it
                     float r0, r1;
-                    const uint32_t f = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
-                    asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(f), "v"(part), "v"(x));
-                    asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(f), "v"(part), "v"(y));
+                    remainders(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y)), part, x, y, r0, r1);
                     hi[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r0, r1));
                 }
             }
@@ -570,10 +611,15 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 Steps st[4];
-                value_steps(c ? vs[i].y : vs[i].x, c ? vs[i].w : vs[i].z, st);
+#pragma unroll
+                for (int k = 0; k < 4; k += 2) {
+                    const uint4 x = *(const uint4 *)&steps[8 * i + 4 * c + k];
+                    st[k].u = __builtin_bit_cast(half2_t, x.x), st[k].m = __builtin_bit_cast(half2_t, x.y);
+                    st[k + 1].u = __builtin_bit_cast(half2_t, x.z), st[k + 1].m = __builtin_bit_cast(half2_t, x.w);
+                }
 #pragma unroll
                 for (int b = 0; b < 2; b++) {
-                    const half8_t v = word_f16(word_of(vr[i], 2 * b + c), st);
+                    const half8_t v = word_f16(word_of(vr[i], 2 * b + c), st, k16);
 #pragma unroll
                     for (int k = 0; k < NQ; k++) o[2 * i + b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf[k][c], o[2 * i + b], 0, 0, 0);
                 }
@@ -715,22 +761,22 @@ __device__ __forceinline__ void attend4_wide(const Attend4View &p, Wide4Lds<HD> 
     // banks.  NC pieces: a lane's words of K, then of V.
     const int krow = (8 * (lane >> 4) + 4 * (wave & 1) + ((lane >> 2) & 3)) ^ (quarter << 1);
     const int vcol = 32 * (wave & 1) + (HD == 128 ? lane & 15 : 16 * (lane & 1) + ((lane >> 1) & 15));
+    const uint32_t k16 = sixteen();
     Steps kst, vst[4];
     auto put = [&](int buf, int piece) {
         if (piece < NC / 2) {
             if (piece == 0) {
-                const half2_t uz = __builtin_bit_cast(half2_t, (turn_left(ks, (4 - 4 * (lane >> 4)) & 31) & kNibble) | kSixteen);
-                kst = Steps(half2_t{uz[0], uz[0]}, half2_t{uz[1], uz[1]});
+                kst = key_steps(nibble_pair(ks, lane >> 4, k16));
                 const int most = most_byte(er);
                 if (lane < 2) lds.power[buf][lane][wave] = er;
                 if (lane == 1) lds.top[buf][wave] = most;
             }
             const int c = HD == 128 ? 2 * quarter + (piece >> 1) : quarter;
-            (kf[buf] + ((wave >> 1) * NC + c) * 64 + krow)[32 * (piece & 1)] = __builtin_bit_cast(uint4, word_f16(kr[piece], kst));
+            (kf[buf] + ((wave >> 1) * NC + c) * 64 + krow)[32 * (piece & 1)] = __builtin_bit_cast(uint4, word_f16(kr[piece], kst, k16));
         } else {
             const int i = piece - NC / 2, j = HD == 128 ? i >> 1 : i, b = HD == 128 ? i & 1 : 0; // tokens 8 j .., dims 16 b ..
-            if (b == 0) value_steps(j ? vs.y : vs.x, j ? vs.w : vs.z, vst);
-            (vf[buf] + ((2 * vi + (wave >> 1)) * 2 + j) * 64 + vcol)[16 * b] = __builtin_bit_cast(uint4, word_f16(vr[HD == 128 ? 2 * b + j : j], vst));
+            if (b == 0) value_steps(j ? vs.y : vs.x, j ? vs.w : vs.z, vst, k16);
+            (vf[buf] + ((2 * vi + (wave >> 1)) * 2 + j) * 64 + vcol)[16 * b] = __builtin_bit_cast(uint4, word_f16(vr[HD == 128 ? 2 * b + j : j], vst, k16));
         }
     };
 
@@ -753,14 +799,12 @@ __device__ __forceinline__ void attend4_wide(const Attend4View &p, Wide4Lds<HD> 
         const Query4 scaled(m, p.scale);
         query = scaled.power();
 #pragma unroll
-        for (int c = 0; c < NC; c++)
+        for (int c = 0; c < NC; c++) {
+            float x[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                _Float16 hi, lw;
-                scaled.split(src[16 * c + i], hi, lw);
-                qh[c][i] = hi;
-                ql[c][i] = lw;
-            }
+            for (int i = 0; i < 8; i++) x[i] = src[16 * c + i];
+            split_query(scaled, x, qh[c], ql[c]);
+        }
     }
 
     floatx16 o[ND];
