@@ -497,17 +497,17 @@ struct Pages {
     int max_units = 0, max_items = 0, max_wide = 0, max_parts = 0, max_wide_parts = 0;
     __host__ __device__ size_t n_blocks() const { return (size_t)n_pages * n_kv * sub; } // of a layer
 };
-// A block of the 4-bit cache, as the matrix cores take its operands from it: byte offsets of
-//   k   [16 tokens][hd / 2] codes
-//   v   [hd / 32][16 dims][2: dims 16 apart][16 tokens] codes, 8 bytes each
-//   ks  [hd / 32][4] words, K's steps and zero points of tokens r, r + 4, r + 8, r + 12
-//   vs  [hd / 32][4] words, V's steps of tokens 0 - 7, 8 - 15, its zero points of the same
-//   ke, ve  [16 tokens] e + 127; 0: a row of zeros; ve 255: K and V read as NaN
+// A block of the 4-bit cache, as a wave loads the matrix cores' operands from it; lane 16 g + n,
+// a quad is four tokens.  Byte offsets of
+//   k   [4 parts of the dims][16 tokens][hd / 8] codes: lane's token n, dims hd / 4 * g on
+//   v   [4 quads][16 dims][hd / 16][2] codes: lane's tokens 4 g .. 4 g + 3 of dims n, 16 + n, ..
+//   ks  [hd / 32][4 quads] words, K's steps and zero points of a group of dims and a quad
+//   vs  [4 quads][hd / 32] words, V's
+//   pw  [4 quads][K, V][4 tokens] e + 127; 0: a row of zeros; V's 255: K and V read as NaN
 // and their sum.  Zeroed memory is a block of zeros.
 struct Pages4 {
-    int k, v, ks, vs, ke, ve, bytes;
-    __host__ __device__ constexpr Pages4(int hd)
-        : k(0), v(8 * hd), ks(16 * hd), vs(16 * hd + hd / 2), ke(17 * hd), ve(17 * hd + 16), bytes(17 * hd + 32) {}
+    int k, v, ks, vs, pw, bytes;
+    __host__ __device__ constexpr Pages4(int hd) : k(0), v(8 * hd), ks(16 * hd), vs(16 * hd + hd / 2), pw(17 * hd), bytes(17 * hd + 32) {}
 };
 __host__ __device__ constexpr int pages4_bytes(int hd) { return Pages4(hd).bytes; }
 struct PagesPlanArgs {

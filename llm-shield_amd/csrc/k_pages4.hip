@@ -53,41 +53,40 @@ struct Steps {
     }
 };
 
-// A word's eight elements: with the same step for all, and with one for each pair's halves.
+// A word's eight elements, with the same step for all.
 __device__ __forceinline__ half8_t word_f16(uint32_t w, const Steps &s, uint32_t k16)
 {
     return __builtin_bit_cast(half8_t, make_uint4(s(nibble_pair<0>(w, k16)), s(nibble_pair<1>(w, k16)), s(nibble_pair<2>(w, k16)),
                                                   s(nibble_pair<3>(w, k16))));
 }
-__device__ __forceinline__ half8_t word_f16(uint32_t w, const Steps (&s)[4], uint32_t k16)
-{
-    return __builtin_bit_cast(half8_t, make_uint4(s[0](nibble_pair<0>(w, k16)), s[1](nibble_pair<1>(w, k16)), s[2](nibble_pair<2>(w, k16)),
-                                                  s[3](nibble_pair<3>(w, k16))));
-}
-
 // Of a K step word's pair (u of a token's group low, its z high), for all of the group.
 __device__ __forceinline__ Steps key_steps(half2_t uz) { return Steps(half2_t{uz[0], uz[0]}, half2_t{uz[1], uz[1]}); }
-// V's step and zero words of eight tokens.
-__device__ __forceinline__ void value_steps(uint32_t u, uint32_t z, Steps (&s)[4], uint32_t k16)
-{
-    s[0] = Steps(nibble_pair<0>(u, k16), nibble_pair<0>(z, k16));
-    s[1] = Steps(nibble_pair<1>(u, k16), nibble_pair<1>(z, k16));
-    s[2] = Steps(nibble_pair<2>(u, k16), nibble_pair<2>(z, k16));
-    s[3] = Steps(nibble_pair<3>(u, k16), nibble_pair<3>(z, k16));
-}
+// V's step word of a quad and group: pairs u of tokens 0 and 1, of 2 and 3, z of the same.
+struct QuadSteps {
+    Steps s[2];
+    QuadSteps() = default;
+    __device__ __forceinline__ QuadSteps(uint32_t w, uint32_t k16)
+        : s{Steps(nibble_pair<0>(w, k16), nibble_pair<2>(w, k16)), Steps(nibble_pair<1>(w, k16), nibble_pair<3>(w, k16))} {}
+    // A V code word: tokens 0 .. 3 of a dim, then of the dim 16 on, two words of fp16 each.
+    __device__ __forceinline__ uint4 operator()(uint32_t w, uint32_t k16) const
+    {
+        return make_uint4(s[0](nibble_pair<0>(w, k16)), s[1](nibble_pair<1>(w, k16)), s[0](nibble_pair<2>(w, k16)), s[1](nibble_pair<3>(w, k16)));
+    }
+};
 
 __device__ __forceinline__ uint32_t word_of(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-__device__ __forceinline__ int byte_of(const uint4 &v, int i) { return (int)((word_of(v, i >> 2) >> (8 * (i & 3))) & 255u); }
+__device__ __forceinline__ int byte_of(uint32_t w, int i) { return (int)((w >> (8 * i)) & 255u); }
 
-__device__ __forceinline__ int most_byte(const uint4 &v)
+// The largest of the words' bytes.
+template <int N>
+__device__ __forceinline__ int most_byte(const uint32_t (&w)[N])
 {
     typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
     ushort2_t m = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t w = word_of(v, i);
-        m = __builtin_elementwise_max(m, __builtin_bit_cast(ushort2_t, w & 0x00ff00ffu));
-        m = __builtin_elementwise_max(m, __builtin_bit_cast(ushort2_t, (w >> 8) & 0x00ff00ffu));
+    for (int i = 0; i < N; i++) {
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(ushort2_t, w[i] & 0x00ff00ffu));
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(ushort2_t, (w[i] >> 8) & 0x00ff00ffu));
     }
     return max((int)m[0], (int)m[1]);
 }
@@ -270,7 +269,8 @@ __global__ __launch_bounds__(256) void pages4_store_kernel(Store4View p)
             }
             if (!v) {
                 if (NE == 4) word |= (uint32_t)__shfl_xor((int)word, 1, 64);
-                if (NE == 8 || !(j & 1)) *(uint32_t *)(block + at.k + (off + tk) * (HD / 2) + 4 * (NE * j / 8)) = turn_left(word, 2);
+                const int w8 = NE * j / 8; // eight dims of them
+                if (NE == 8 || !(j & 1)) *((uint32_t *)(block + at.k) + (w8 / NG * kPageBlock + off + tk) * NG + w8 % NG) = turn_left(word, 2);
             }
             if (j % TG == 0) {
                 step[v][tk][j / TG] = (uint8_t)(int)u;
@@ -279,7 +279,7 @@ __global__ __launch_bounds__(256) void pages4_store_kernel(Store4View p)
             power[v] = some ? ex + 127 : 0;
         }
         // a value that is not finite: the token's V power says so for both
-        if (j < 2) block[(j ? at.ve : at.ke) + off + tk] = (uint8_t)(bad < 0x7f800000u ? power[j] : j ? 255 : 0);
+        if (j < 2) block[at.pw + (off + tk) / 4 * 8 + 4 * j + (off + tk) % 4] = (uint8_t)(bad < 0x7f800000u ? power[j] : j ? 255 : 0);
     }
     __syncthreads();
 
@@ -297,18 +297,18 @@ __global__ __launch_bounds__(256) void pages4_store_kernel(Store4View p)
         return make_uint2((old & ~mask) | turn_left(put, 2), mask);
     };
     if (has_v) {
-        const int dim = 32 * (tid >> 6) + 16 * ((tid >> 1) & 1) + ((tid >> 2) & 15), t0 = 8 * (tid & 1);
-        const uint2 r = merge(old_v, [&](int i) { return t0 + i; }, [&](int, int tk) { return code[tk][dim]; });
+        const int q = tid / (16 * NG), dim = 32 * (tid % NG) + tid / NG % 16;
+        const uint2 r = merge(old_v, [&](int i) { return 4 * q + (i & 3); }, [&](int i, int tk) { return code[tk][dim + 4 * (i & 4)]; });
         if (r.y) *vword = r.x;
     }
     if (has_s) {
         uint2 r;
-        if (tid < 4 * NG) { // K: tokens r, 4 + r, ..: u the even elements (low half), z the odd ones
-            const int gr = tid >> 2, r0 = tid & 3;
-            r = merge(old_s, [&](int i) { return 4 * (i >> 1) + r0; }, [&](int i, int tk) { return i & 1 ? zero[0][tk][gr] : step[0][tk][gr]; });
+        if (tid < 4 * NG) { // K: u of a token, z of it, the quad's next token
+            const int gr = tid >> 2, q = tid & 3;
+            r = merge(old_s, [&](int i) { return 4 * q + (i >> 1); }, [&](int i, int tk) { return i & 1 ? zero[0][tk][gr] : step[0][tk][gr]; });
         } else {
-            const int gr = (tid - 4 * NG) >> 2, t0 = 8 * (tid & 1), z = tid & 2;
-            r = merge(old_s, [&](int i) { return t0 + i; }, [&](int, int tk) { return z ? zero[1][tk][gr] : step[1][tk][gr]; });
+            const int gr = tid % NG, q = (tid - 4 * NG) / NG;
+            r = merge(old_s, [&](int i) { return 4 * q + (i & 3); }, [&](int i, int tk) { return i & 4 ? zero[1][tk][gr] : step[1][tk][gr]; });
         }
         if (r.y) *sword = r.x;
     }
@@ -408,32 +408,40 @@ __device__ __forceinline__ half8_t split_query(const Query4 &q, const float (&x)
 
 template <int HD>
 struct Tile4Lds {
-    float lo[4][16][HD + 4];
-    float lm[4][kPagesTileRows], ll[4][kPagesTileRows];
-    uint2 steps[4][4][HD / 4 + 2]; // a wave's V steps of 64 keys: [block][group of dims][pair of tokens]
+    uint4 q[2][HD / 32][64]; // [part][dims][lane]; eight rows: both parts in [0]
+    struct Wave {
+        union {
+            uint4 steps[4][4][HD / 32]; // V's of 64 keys: [block][quad][group of dims]
+            float rows[16][HD + 4];     // at the end: the means
+        };
+        float m[16], l[16];
+    } wave[4];
     int last;
 };
 
-// Up to ROWS (token, head) rows of a request and KV head over keys [key0, key1) of its
-// pages; the four waves take 64 keys (four blocks) in turn and merge at the end.
-// S^T = K Q^T with the rows of the K operand dealt so that a lane's sixteen scores are the
-// sixteen tokens of one block, which makes the weights the P^T operand of O^T += V^T P^T
-// as they stand.  q and p enter as fp16 pairs (hi + lo, ~22 bits).  Up to eight rows leave
-// half of the operand's sixteen columns, which take the low parts: one matrix instruction a
-// product instead of two.  A weight is 2^(score - m); the V operand's 2^e and the row's own
-// power are added to its exponent, so that what enters fp16 is relative to the row's
-// heaviest product so far (times 2^9), over the keys that the row sees.
-template <int HD, int ROWS>
+// Up to sixteen (token, head) rows of a request and KV head over keys [key0, key1) of its
+// pages; the four waves take 64 keys (four blocks) in turn and merge at the end.  S^T =
+// K Q^T, a block of sixteen keys to a product: a lane's scores are four tokens of each of the
+// four blocks, and its weights the P^T operand of O^T += V^T P^T as they stand.  q and p
+// enter as fp16 pairs (hi + lo, ~22 bits): up to eight rows (!BOTH) as the high and low eight
+// of the operand's sixteen columns, one matrix instruction a product, more (BOTH) as two
+// operands.  A weight is 2^(score - m); the V operand's 2^e and the row's own power are
+// added to its exponent, so that what enters fp16 is relative to the row's heaviest product
+// so far (times 2^9), over the keys that the row sees.
+template <int HD, bool BOTH>
 __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> &lds, const PagesItem &r, int h)
 {
-    constexpr int NC = HD / 32, NS = HD / 16, NI = HD / 32, LD = HD + 4, NQ = ROWS == 8 ? 1 : 2;
+    constexpr int NC = HD / 32, NS = HD / 16, LD = HD + 4, ROWS = BOTH ? 16 : 8;
     constexpr Pages4 at(HD);
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int g = lane >> 4, n = lane & 15;
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid)); // what follows from it is not kept from item to item: registers
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, n = lane & 15;
+    const int n_rows = r.row1;
     const uint32_t k16 = sixteen();
+    auto &own = lds.wave[wave];
     const int32_t *table = p.table + (size_t)r.id * p.width;
     // columns past the request's rows repeat its last one
-    const int n_rows = r.row1, row = min(r.row0 + (n & (ROWS - 1)), n_rows - 1);
+    const int row = min(r.row0 + (n & (ROWS - 1)), n_rows - 1);
     const int token = row / p.group, head = h * p.group + row % p.group;
     const int limit = r.past + token; // last visible key
     // the tile's last visible key; keys up to `clear` are seen by every row
@@ -441,53 +449,55 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
     const int key1 = min(r.key1, top + 1), clear = r.past + r.row0 / p.group;
     const int last = (r.len - 1) / kPageBlock; // blocks past it are read as this one, and masked
 
-    // V's steps of a block are made by its sixteen lanes, NI / 2 pairs of tokens of a group
-    // each, and shared through LDS
-    const int pair0 = n * (NI / 2), step_at = 16 * (pair0 >> 3) + 4 * ((pair0 >> 2) & 1);
-    auto &steps = lds.steps[wave][g];
-
-    // a lane reads K of block n / 4 of the four, V and the powers of block g
-    auto page_of = [&](int kb, int i) { return table[min(4 * kb + i, last) >> p.sub_shift]; };
-    auto block_of = [&](int kb, int i, int page) {
-        return p.pool + ((((size_t)page * p.n_kv + h) << p.sub_shift) + (min(4 * kb + i, last) & (p.sub - 1))) * at.bytes;
+    // the pages of 64 keys' four blocks, a lane each; then the blocks are the wave's, and a
+    // lane's place in all of them is the same
+    auto pages_of = [&](int kb) { return table[min(4 * kb + (lane & 3), last) >> p.sub_shift]; };
+    const uint32_t page_bytes = (uint32_t)(p.n_kv << p.sub_shift) * at.bytes;
+    const uint8_t *const pool = p.pool + (size_t)((h << p.sub_shift) * at.bytes);
+    auto block_of = [&](int kb, int b, int pages) {
+        const uint32_t page = __builtin_amdgcn_readlane(pages, b), sub = min(4 * kb + b, last) & (p.sub - 1);
+        return pool + (uint64_t)page * page_bytes + sub * at.bytes;
     };
-    uint4 kr[4], vr[NI], ke, ve;
-    uint32_t ks, vu, vz;
-    auto fetch_k = [&](int kb, int page) {
-        const uint8_t *b = block_of(kb, n >> 2, page);
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const uint8_t *src = b + at.k + (4 * t + (n & 3)) * (HD / 2) + 4 * NC * g;
-            if constexpr (NC == 4) kr[t] = *(const uint4 *)src;
-            else {
-                const uint2 x = *(const uint2 *)src;
-                kr[t] = make_uint4(x.x, x.y, 0, 0);
-            }
+    const uint32_t codes_at = 4 * NC * lane, ks_at = at.ks + 4 * (4 * (g * NC / 4) + (n >> 2)), vs_at = at.vs + 4 * (lane & (4 * NC - 1));
+    uint32_t kr[4][NC], vr[4][NC], ks[4], vs[4];
+    uint2 power[4]; // K's of the lane's tokens of a block, V's
+    auto load = [&](uint32_t (&to)[NC], const uint8_t *from) {
+        if constexpr (NC == 4) {
+            const uint4 x = *(const uint4 *)from;
+            to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
+        } else {
+            const uint2 x = *(const uint2 *)from;
+            to[0] = x.x, to[1] = x.y;
         }
-        ks = *(const uint32_t *)(b + at.ks + 4 * (4 * (g * NI / 4) + (n & 3)));
     };
-    auto fetch_v = [&](int kb, int page) {
-        const uint8_t *b = block_of(kb, g, page);
-        ke = *(const uint4 *)(b + at.ke);
-        ve = *(const uint4 *)(b + at.ve);
+    auto fetch_k = [&](int kb, int pages) {
 #pragma unroll
-        for (int i = 0; i < NI; i++) vr[i] = *(const uint4 *)(b + at.v + 256 * i + 16 * n);
-        vu = *(const uint32_t *)(b + at.vs + step_at);
-        vz = *(const uint32_t *)(b + at.vs + step_at + 8);
+        for (int b = 0; b < 4; b++) {
+            const uint8_t *block = block_of(kb, b, pages);
+            load(kr[b], block + codes_at);
+            ks[b] = *(const uint32_t *)(block + ks_at);
+        }
+    };
+    auto fetch_v = [&](int kb, int pages) {
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            const uint8_t *block = block_of(kb, b, pages);
+            power[b] = *(const uint2 *)(block + at.pw + 8 * g);
+            load(vr[b], block + at.v + codes_at);
+            vs[b] = *(const uint32_t *)(block + vs_at);
+        }
     };
     int kb = r.key0 / 64 + wave;
-    int pk = page_of(kb, n >> 2), pv = page_of(kb, g);
+    int pages = pages_of(kb);
     if (kb * 64 < key1) {
-        fetch_k(kb, pk);
-        fetch_v(kb, pv);
+        fetch_k(kb, pages);
+        fetch_v(kb, pages);
     }
-    pk = page_of(kb + 4, n >> 2);
-    pv = page_of(kb + 4, g);
+    pages = pages_of(kb + 4);
 
     // Q^T fragments: dims 8 NC g + 8 c .. + 7 of column n
-    half8_t qf[NQ][NC];
     int query;
-    const float part = n < 8 ? 0.f : -1.f; // 8 rows: a column's part of a query or a weight
+    const float part = n < 8 ? 0.f : -1.f; // a column's part of a query or a weight
     {
         const float *src = p.q + ((size_t)(r.start + token) * p.n_heads + head) * HD + 8 * NC * g;
         float x[NC][8], m = 0.f;
@@ -502,12 +512,20 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
         m = fmaxf(m, __shfl_xor(m, 32, 64));
         const Query4 scaled(m, p.scale);
         query = scaled.power();
+        // a wave makes a quarter of the fragments, in LDS for all (and for each 64 keys'
+        // products again: registers)
 #pragma unroll
         for (int c = 0; c < NC; c++) {
-            if constexpr (NQ == 2) split_query(scaled, x[c], qf[0][c], qf[1][c]);
-            else qf[0][c] = split_query(scaled, x[c], part);
+            if (c != wave) continue;
+            if constexpr (BOTH) {
+                half8_t hi, lo;
+                split_query(scaled, x[c], hi, lo);
+                lds.q[0][c][lane] = __builtin_bit_cast(uint4, hi);
+                lds.q[1][c][lane] = __builtin_bit_cast(uint4, lo);
+            } else lds.q[0][c][lane] = __builtin_bit_cast(uint4, split_query(scaled, x[c], part));
         }
     }
+    __syncthreads();
 
     floatx4 o[NS];
 #pragma unroll
@@ -519,40 +537,51 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
         x = fmaxf(x, __shfl_xor(x, 16, 64));
         return fmaxf(x, __shfl_xor(x, 32, 64));
     };
+    auto both = [](float x) { // both parts' sum: the other's column is eight lanes on
+        if constexpr (!BOTH) x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x128, 0xf, 0xf, true));
+        return x;
+    };
     for (; kb * 64 < key1; kb += 4) {
         const bool more = (kb + 4) * 64 < key1;
-        float sv[16];
-        const Steps kst[4] = {key_steps(nibble_pair<0>(ks, k16)), key_steps(nibble_pair<1>(ks, k16)), key_steps(nibble_pair<2>(ks, k16)),
-                              key_steps(nibble_pair<3>(ks, k16))};
+        float sv[16]; // [block][token of the lane's quad]
+        {
+            half8_t qf[1 + BOTH][NC];
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i <= BOTH; i++)
 #pragma unroll
-            for (int c = 0; c < NC; c++) {
-                const half8_t k = word_f16(word_of(kr[t], c), kst[t], k16);
+                for (int c = 0; c < NC; c++) qf[i][c] = __builtin_bit_cast(half8_t, lds.q[i][c][lane]);
 #pragma unroll
-                for (int i = 0; i < NQ; i++) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[i][c], acc, 0, 0, 0);
-            }
+            for (int b = 0; b < 4; b++) {
+                const Steps st = key_steps(nibble_pair(ks[b], n & 3, k16));
+                floatx4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float x = acc[i];
-                if constexpr (NQ == 1) // the other part's column is eight lanes on
-                    x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x128, 0xf, 0xf, true));
-                sv[4 * t + i] = __builtin_amdgcn_ldexpf(x, byte_of(ke, 4 * t + i) + query);
+                for (int c = 0; c < NC; c++) {
+                    const half8_t k = word_f16(kr[b][c], st, k16);
+#pragma unroll
+                    for (int i = 0; i <= BOTH; i++) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[i][c], acc, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) sv[4 * b + i] = __builtin_amdgcn_ldexpf(both(acc[i]), byte_of(power[b].x, i) + query);
             }
         }
-        if (more) fetch_k(kb + 4, pk);
-#pragma unroll
-        for (int i = 0; i < NI / 2; i++) {
-            const int t = (pair0 & 3) + i;
-            const Steps st(nibble_pair(vu, t, k16), nibble_pair(vz, t, k16));
-            steps[pair0 + i] = make_uint2(__builtin_bit_cast(uint32_t, st.u), __builtin_bit_cast(uint32_t, st.m));
+        if (more) fetch_k(kb + 4, pages);
+        // V's steps, a quad's and group's to a lane, for the sixteen lanes that want them
+        {
+            const int b = lane / (4 * NC) & 3;
+            const uint32_t w = b == 0 ? vs[0] : b == 1 ? vs[1] : b == 2 ? vs[2] : vs[3];
+            const QuadSteps st(w, k16);
+            if (NC == 4 || lane < 32)
+                (&own.steps[0][0][0])[lane] = make_uint4(__builtin_bit_cast(uint32_t, st.s[0].u), __builtin_bit_cast(uint32_t, st.s[0].m),
+                                                         __builtin_bit_cast(uint32_t, st.s[1].u), __builtin_bit_cast(uint32_t, st.s[1].m));
         }
         if (kb * 64 + 63 > clear) {
-            const int left = limit - (kb * 64 + 16 * g); // last visible token of the lane's block
 #pragma unroll
-            for (int i = 0; i < 16; i++)
-                if (i > left) sv[i] = -INFINITY;
+            for (int b = 0; b < 4; b++) {
+                const int left = limit - (kb * 64 + 16 * b + 4 * g); // last visible token of the lane's quad
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (i > left) sv[4 * b + i] = -INFINITY;
+            }
         }
         float mx = -INFINITY;
 #pragma unroll
@@ -565,14 +594,15 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
             value = -127 + (e == -INFINITY ? 0 : (int)(9.f - e + m));
         }
         const float mu = m == -INFINITY ? 0.f : m;
-        // the largest score with the largest power bounds what the row's products can be (a
-        // block without visible keys: -inf, or NaN with a token that is not finite)
-        const int mb = most_byte(ve);
+        // the largest score with the largest power bounds what the row's products can be
+        // (without visible keys: -inf, or NaN with a token that is not finite)
+        uint32_t vp[4] = {power[0].y, power[1].y, power[2].y, power[3].y};
+        const int mb = most_byte(vp);
         if (__any(mx + (mb == 255 ? INFINITY : (float)(mb - 127)) > e + 6.f)) {
             float mv = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                const int b = byte_of(ve, i);
+                const int b = byte_of(vp[i >> 2], i & 3);
                 if (b < 255) mv = fmaxf(mv, sv[i] + (float)(b - 127));
                 else if (sv[i] > -INFINITY) l = NAN; // a token that is not finite, seen
             }
@@ -582,87 +612,87 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
             e = en;
             value = -127 + (e == -INFINITY ? 0 : (int)(9.f - e + mu));
         }
-        float wt[16];
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const float x = __builtin_amdgcn_exp2f(sv[i] - mu);
-            l += x;
-            wt[i] = __builtin_amdgcn_ldexpf(x, byte_of(ve, i) + value);
-        }
-        half8_t pf[NQ][2];
+        asm("" : "+v"(vp[0]), "+v"(vp[1]), "+v"(vp[2]), "+v"(vp[3])); // (bytes taken above are not kept: 16 registers)
+        half8_t pf[1 + BOTH][2];
 #pragma unroll
         for (int c = 0; c < 2; c++) {
-            uint32_t hi[4], lw[4];
+            uint32_t w[4], lw[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float x = wt[8 * c + 2 * i], y = wt[8 * c + 2 * i + 1];
-                if constexpr (NQ == 2) split2_mix(x, y, hi[i], lw[i]);
-                else { // the high columns keep x, the low ones what fp16 leaves of it
-                    float r0, r1;
-                    remainders(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y)), part, x, y, r0, r1);
-                    hi[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r0, r1));
+                const int t = 8 * c + 2 * i;
+                float x = __builtin_amdgcn_exp2f(sv[t] - mu), z = __builtin_amdgcn_exp2f(sv[t + 1] - mu), r0, r1;
+                l += x;
+                l += z;
+                x = __builtin_amdgcn_ldexpf(x, byte_of(vp[t >> 2], t & 3) + value);
+                z = __builtin_amdgcn_ldexpf(z, byte_of(vp[t >> 2], (t & 3) + 1) + value);
+                if constexpr (BOTH) split2_mix(x, z, w[i], lw[i]);
+                else { // the high columns keep the weights, the low ones what fp16 leaves of them
+                    remainders(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, z)), part, x, z, r0, r1);
+                    w[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r0, r1));
                 }
             }
-            pf[0][c] = __builtin_bit_cast(half8_t, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-            if constexpr (NQ == 2) pf[1][c] = __builtin_bit_cast(half8_t, make_uint4(lw[0], lw[1], lw[2], lw[3]));
+            pf[0][c] = __builtin_bit_cast(half8_t, make_uint4(w[0], w[1], w[2], w[3]));
+            if constexpr (BOTH) pf[1][c] = __builtin_bit_cast(half8_t, make_uint4(lw[0], lw[1], lw[2], lw[3]));
         }
 #pragma unroll
-        for (int i = 0; i < NI; i++)
+        for (int c = 0; c < 2; c++)
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                Steps st[4];
-#pragma unroll
-                for (int k = 0; k < 4; k += 2) {
-                    const uint4 x = *(const uint4 *)&steps[8 * i + 4 * c + k];
-                    st[k].u = __builtin_bit_cast(half2_t, x.x), st[k].m = __builtin_bit_cast(half2_t, x.y);
-                    st[k + 1].u = __builtin_bit_cast(half2_t, x.z), st[k + 1].m = __builtin_bit_cast(half2_t, x.w);
-                }
+            for (int j = 0; j < NC; j++) { // dims 32 j .., of two blocks
+                uint4 v[2];
 #pragma unroll
                 for (int b = 0; b < 2; b++) {
-                    const half8_t v = word_f16(word_of(vr[i], 2 * b + c), st, k16);
+                    const uint4 x = own.steps[2 * c + b][g][j];
+                    QuadSteps st;
+                    st.s[0].u = __builtin_bit_cast(half2_t, x.x), st.s[0].m = __builtin_bit_cast(half2_t, x.y);
+                    st.s[1].u = __builtin_bit_cast(half2_t, x.z), st.s[1].m = __builtin_bit_cast(half2_t, x.w);
+                    v[b] = st(vr[2 * c + b][j], k16);
+                }
+                const half8_t v0 = __builtin_bit_cast(half8_t, make_uint4(v[0].x, v[0].y, v[1].x, v[1].y)); // dims 32 j + n
+                const half8_t v1 = __builtin_bit_cast(half8_t, make_uint4(v[0].z, v[0].w, v[1].z, v[1].w)); // and 16 on
 #pragma unroll
-                    for (int k = 0; k < NQ; k++) o[2 * i + b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf[k][c], o[2 * i + b], 0, 0, 0);
+                for (int i = 0; i <= BOTH; i++) {
+                    o[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[i][c], o[2 * j], 0, 0, 0);
+                    o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[i][c], o[2 * j + 1], 0, 0, 0);
                 }
             }
         if (more) {
-            fetch_v(kb + 4, pv);
-            pk = page_of(kb + 8, n >> 2);
-            pv = page_of(kb + 8, g);
+            fetch_v(kb + 4, pages);
+            pages = pages_of(kb + 8);
         }
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
 
-    // the four waves' results, in wave order
+    // the waves' results, in wave order
     const MeanScale mean(e, m, l);
 #pragma unroll
-    for (int s = 0; s < NS; s++) *(floatx4 *)&lds.lo[wave][n][16 * s + 4 * g] = o[s] * mean.f1 * mean.f2;
-    if (g == 0) {
-        lds.lm[wave][n] = m;
-        lds.ll[wave][n] = l;
+    for (int s = 0; s < NS; s++) {
+        floatx4 x = o[s] * mean.f1 * mean.f2;
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = both(x[i]);
+        if (n < ROWS) *(floatx4 *)&own.rows[n][16 * s + 4 * g] = x;
+    }
+    if (lane < ROWS) {
+        own.m[lane] = m;
+        own.l[lane] = l;
     }
     __syncthreads();
     for (int i = tid; i < ROWS * (HD / 4); i += 256) {
         const int c = i / (HD / 4), d = 4 * (i % (HD / 4)), rr = r.row0 + c;
         if (rr >= n_rows) continue;
-        float mm = lds.lm[0][c];
-#pragma unroll
-        for (int w = 1; w < 4; w++) mm = fmaxf(mm, lds.lm[w][c]);
+        float mm = -INFINITY;
+        for (int w = 0; w < 4; w++) mm = fmaxf(mm, lds.wave[w].m[c]);
         const float mu = mm == -INFINITY ? 0.f : mm;
         float sum = 0.f, f[4];
         floatx4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-            f[w] = lds.ll[w][c] * exp2f(lds.lm[w][c] - mu);
+            f[w] = lds.wave[w].l[c] * exp2f(lds.wave[w].m[c] - mu);
             sum += f[w];
         }
         const float inv = sum == 0.f && r.part >= 0 ? 0.f : 1.f / sum;
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
-            floatx4 y = *(const floatx4 *)&lds.lo[w][c][d];
-            if constexpr (NQ == 1) y += *(const floatx4 *)&lds.lo[w][c + 8][d];
-            x += y * (f[w] * inv);
-        }
+        for (int w = 0; w < 4; w++) x += *(const floatx4 *)&lds.wave[w].rows[c][d] * (f[w] * inv);
         if (r.part < 0) {
             const int tk = rr / p.group, hd = h * p.group + rr % p.group;
             float *dst = p.out + ((size_t)(r.start + tk) * p.n_heads + hd) * HD + d;
@@ -679,7 +709,7 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
         // the tile's last part to arrive merges them all, in their order
         const int tiles = div_up(n_rows, kPagesTileRows), tile = r.row0 / kPagesTileRows;
         if (arrives_last(p.tickets + (size_t)(r.part0 + tile) * p.n_kv + h, r.n_parts, lds.last))
-            for (int c = tid >> 4; c < min(ROWS, n_rows - r.row0); c += 16) {
+            for (int c = tid >> 4; c < min(kPagesTileRows, n_rows - r.row0); c += 16) {
                 const int rr = r.row0 + c, tk = rr / p.group;
                 merge_parts<HD>(
                     [&](int k) { return p.part + (((size_t)(r.part0 + k * tiles + tile) * p.n_kv + h) * kPagesTileRows + c) * LD; },
@@ -734,12 +764,10 @@ __device__ __forceinline__ void attend4_wide(const Attend4View &p, Wide4Lds<HD> 
     auto page_of = [&](int kb) {
         return __builtin_amdgcn_raw_buffer_load_b32(rt, 0, 4 * (min(4 * kb + wave, last) >> p.sub_shift), 0);
     };
-    // A lane's share: the codes of a quarter of token lane / 4 (K) and, of all tokens, of
-    // dims 32 i + n and 16 on (V, hd 64: of one), i = lane / 16; their steps.
-    const int vi = lane / (HD == 128 ? 16 : 32), quarter = lane & 3;
-    const int ks_at = at.ks + 4 * (4 * (HD == 128 ? quarter : quarter >> 1) + ((lane >> 2) & 3));
-    uint32_t kr[HD / 32], vr[HD / 32], ks;
-    uint4 vs, er;
+    // A lane's share: a part of a token's codes (K), and four tokens' of dims 16 s + t (V)
+    const int t = lane & 15, quad = lane >> 4;
+    const int ks_at = at.ks + 4 * (4 * (quad * ND / 4) + (t >> 2));
+    uint32_t kr[ND], vr[ND], vs[ND], ks, er;
     auto fetch = [&](int kb, int page) {
         const int c = min(4 * kb + wave, last) & (p.sub - 1);
         const size_t b = (((size_t)__builtin_amdgcn_readfirstlane(page) * p.n_kv + h) << p.sub_shift) + c;
@@ -754,29 +782,38 @@ __device__ __forceinline__ void attend4_wide(const Attend4View &p, Wide4Lds<HD> 
             kr[0] = k.x, kr[1] = k.y, vr[0] = v.x, vr[1] = v.y;
         }
         ks = __builtin_amdgcn_raw_buffer_load_b32(rb, ks_at, 0, 0);
-        vs = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rb, 16 * vi, at.vs, 0));
-        er = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rb, 16 * (lane & 1), at.ke, 0));
+        if constexpr (HD == 128) {
+            const uint4 v = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rb, 16 * quad, at.vs, 0));
+            vs[0] = v.x, vs[1] = v.y, vs[2] = v.z, vs[3] = v.w;
+        } else {
+            const uint2 v = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rb, 8 * quad, at.vs, 0));
+            vs[0] = v.x, vs[1] = v.y;
+        }
+        er = __builtin_amdgcn_raw_buffer_load_b32(rb, 4 * (lane & 7), at.pw, 0); // a quad's powers, K's and V's in turn
     };
-    // K's rows of the tile are dealt by quarter so that neighbouring lanes' writes take all
-    // banks.  NC pieces: a lane's words of K, then of V.
-    const int krow = (8 * (lane >> 4) + 4 * (wave & 1) + ((lane >> 2) & 3)) ^ (quarter << 1);
-    const int vcol = 32 * (wave & 1) + (HD == 128 ? lane & 15 : 16 * (lane & 1) + ((lane >> 1) & 15));
+    // NC pieces: a lane's words of K, then of V (four tokens of two dims each).
+    const int krow = 8 * (t >> 2) + 4 * (wave & 1) + (t & 3), vcol = 32 * (wave & 1) + t;
     const uint32_t k16 = sixteen();
-    Steps kst, vst[4];
+    Steps kst;
     auto put = [&](int buf, int piece) {
-        if (piece < NC / 2) {
+        if (piece < ND) {
             if (piece == 0) {
-                kst = key_steps(nibble_pair(ks, lane >> 4, k16));
-                const int most = most_byte(er);
-                if (lane < 2) lds.power[buf][lane][wave] = er;
-                if (lane == 1) lds.top[buf][wave] = most;
+                kst = key_steps(nibble_pair(ks, t & 3, k16));
+                const uint32_t w[1] = {er};
+                const int most = most_byte(w);
+                const int top = max(max(__builtin_amdgcn_readlane(most, 1), __builtin_amdgcn_readlane(most, 3)),
+                                    max(__builtin_amdgcn_readlane(most, 5), __builtin_amdgcn_readlane(most, 7)));
+                if (lane < 8) ((uint32_t *)&lds.power[buf][lane & 1][wave])[lane >> 1] = er;
+                if (lane == 0) lds.top[buf][wave] = top;
             }
-            const int c = HD == 128 ? 2 * quarter + (piece >> 1) : quarter;
+            const int c = HD == 128 ? 2 * quad + (piece >> 1) : quad;
             (kf[buf] + ((wave >> 1) * NC + c) * 64 + krow)[32 * (piece & 1)] = __builtin_bit_cast(uint4, word_f16(kr[piece], kst, k16));
         } else {
-            const int i = piece - NC / 2, j = HD == 128 ? i >> 1 : i, b = HD == 128 ? i & 1 : 0; // tokens 8 j .., dims 16 b ..
-            if (b == 0) value_steps(j ? vs.y : vs.x, j ? vs.w : vs.z, vst, k16);
-            (vf[buf] + ((2 * vi + (wave >> 1)) * 2 + j) * 64 + vcol)[16 * b] = __builtin_bit_cast(uint4, word_f16(vr[HD == 128 ? 2 * b + j : j], vst, k16));
+            const int j = piece - ND;
+            const uint4 v = QuadSteps(vs[j], k16)(vr[j], k16);
+            uint2 *to = (uint2 *)(vf[buf] + ((2 * j + (wave >> 1)) * 2 + (quad >> 1)) * 64 + vcol) + (quad & 1);
+            to[0] = make_uint2(v.x, v.y);
+            to[32] = make_uint2(v.z, v.w);
         }
     };
 
@@ -830,7 +867,7 @@ __device__ __forceinline__ void attend4_wide(const Attend4View &p, Wide4Lds<HD> 
     for (int buf = 0; kb * 64 < key1; kb++, buf ^= 1) {
         floatx16 s[2] = {floatx16{}, floatx16{}};
         auto kfrag = [&](int t, int c) {
-            return __builtin_bit_cast(half8_t, kf[buf][(t * NC + c) * 64 + (lane ^ (((HD == 128 ? c >> 1 : c) & 3) << 1))]);
+            return __builtin_bit_cast(half8_t, kf[buf][(t * NC + c) * 64 + lane]);
         };
         half8_t k0 = kfrag(0, 0), k1 = kfrag(1, 0);
 #pragma unroll
@@ -854,7 +891,7 @@ __device__ __forceinline__ void attend4_wide(const Attend4View &p, Wide4Lds<HD> 
             ve[t] = lds.power[buf][1][2 * t + hh];
             top[t] = lds.top[buf][2 * t + hh];
 #pragma unroll
-            for (int i = 0; i < 16; i++) s[t][i] = __builtin_amdgcn_ldexpf(s[t][i], byte_of(ke, i) + query);
+            for (int i = 0; i < 16; i++) s[t][i] = __builtin_amdgcn_ldexpf(s[t][i], byte_of(word_of(ke, i >> 2), i & 3) + query);
         }
         if (kb * 64 + 63 > clear) {
 #pragma unroll
@@ -893,7 +930,7 @@ __device__ __forceinline__ void attend4_wide(const Attend4View &p, Wide4Lds<HD> 
                 for (int t = 0; t < 2; t++)
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        const int b = byte_of(ve[t], i);
+                        const int b = byte_of(word_of(ve[t], i >> 2), i & 3);
                         if (b < 255) mv = fmaxf(mv, s[t][i] + (float)(b - 127));
                         else if (s[t][i] > -INFINITY) l = NAN; // a token that is not finite, seen
                     }
@@ -910,8 +947,8 @@ __device__ __forceinline__ void attend4_wide(const Attend4View &p, Wide4Lds<HD> 
             const float x = __builtin_amdgcn_exp2f(s[t][2 * i] - mu), y = __builtin_amdgcn_exp2f(s[t][2 * i + 1] - mu);
             l += x;
             l += y;
-            split2_mix(__builtin_amdgcn_ldexpf(x, byte_of(ve[t], 2 * i) + value),
-                       __builtin_amdgcn_ldexpf(y, byte_of(ve[t], 2 * i + 1) + value), hi[t][i], lw[t][i]);
+            split2_mix(__builtin_amdgcn_ldexpf(x, byte_of(word_of(ve[t], i >> 1), 2 * (i & 1)) + value),
+                       __builtin_amdgcn_ldexpf(y, byte_of(word_of(ve[t], i >> 1), 2 * (i & 1) + 1) + value), hi[t][i], lw[t][i]);
         };
         auto pfrag = [&](const uint32_t (&x)[8], int j) {
             return __builtin_bit_cast(half8_t, make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]));
@@ -948,7 +985,7 @@ __device__ __forceinline__ void attend4_wide(const Attend4View &p, Wide4Lds<HD> 
 // The attention of a plan in one launch: wide tiles first, then 16-row tiles, `tiles`
 // workgroups of which take turns.
 template <int HD, bool WIDE>
-__global__ __launch_bounds__(256, 2) void pages4_attend_kernel(Attend4View p)
+__global__ __launch_bounds__(256, WIDE ? 2 : 3) void pages4_attend_kernel(Attend4View p)
 {
     union Lds {
         Tile4Lds<HD> tile;
@@ -969,9 +1006,13 @@ __global__ __launch_bounds__(256, 2) void pages4_attend_kernel(Attend4View p)
         }
     }
     Tile4Lds<HD> &lds = *(Tile4Lds<HD> *)mem;
+    auto scalar = [](int &x) { x = __builtin_amdgcn_readfirstlane(x); };
     while (item < plan.n_items) {
-        if (it.row1 - it.row0 <= 8) attend4_tile<HD, 8>(p, lds, it, h);
-        else attend4_tile<HD, 16>(p, lds, it, h);
+        // the workgroup's, so held in scalar registers
+        scalar(it.id), scalar(it.start), scalar(it.past), scalar(it.len), scalar(it.row0), scalar(it.row1);
+        scalar(it.key0), scalar(it.key1), scalar(it.part), scalar(it.part0), scalar(it.n_parts);
+        if (it.row1 - it.row0 > 8) attend4_tile<HD, true>(p, lds, it, h);
+        else attend4_tile<HD, false>(p, lds, it, h);
         item += stride;
         if (item < plan.n_items) it = p.item[item];
     }
@@ -1020,22 +1061,19 @@ __global__ __launch_bounds__(256) void pages4_read_kernel(Read4View p)
         const int tk = slot % kPageBlock;
         const uint8_t *b = p.pool + (((size_t)(slot / p.page) * p.n_kv + h) * p.sub + slot % p.page / kPageBlock) * at.bytes;
         auto nibble = [](uint32_t w, int i) { return (int)((turn_left(w, 30) >> nibble_at(i)) & 15u); };
-        const uint32_t kw = *(const uint32_t *)(b + at.k + tk * (HD / 2) + 4 * (d0 / 8));
-        const uint32_t ks = *(const uint32_t *)(b + at.ks + 4 * (4 * gr + (tk & 3)));
-        const uint32_t *vs = (const uint32_t *)(b + at.vs) + 4 * gr + (tk >> 3);
-        const uint32_t vu = vs[0], vz = vs[2];
-        const int ke = b[at.ke + tk], ve = b[at.ve + tk];
+        constexpr int NG = HD / 32;
+        const int q = tk / 4, t = tk % 4, w8 = d0 / 8;
+        const uint32_t kw = ((const uint32_t *)(b + at.k))[(w8 / NG * kPageBlock + tk) * NG + w8 % NG];
+        const uint32_t ks = ((const uint32_t *)(b + at.ks))[4 * gr + q], vs = ((const uint32_t *)(b + at.vs))[NG * q + gr];
+        const int ke = b[at.pw + 8 * q + t], ve = b[at.pw + 8 * q + 4 + t];
         uint32_t vw[NE];
 #pragma unroll
-        for (int k = 0; k < NE; k++) {
-            const int d = d0 + k;
-            vw[k] = *((const uint32_t *)(b + at.v) + 64 * gr + 4 * (d & 15) + 2 * ((d >> 4) & 1) + (tk >> 3));
-        }
-        const int ku = nibble(ks, 2 * (tk >> 2)), kz = nibble(ks, 2 * (tk >> 2) + 1), u = nibble(vu, tk & 7), z = nibble(vz, tk & 7);
+        for (int k = 0; k < NE; k++) vw[k] = ((const uint32_t *)(b + at.v))[(16 * q + (d0 + k) % 16) * NG + gr];
+        const int ku = nibble(ks, 2 * t), kz = nibble(ks, 2 * t + 1), u = nibble(vs, t), z = nibble(vs, 4 + t);
 #pragma unroll
         for (int k = 0; k < NE; k++) {
             x[0][k] = ve == 255 ? NAN : ldexpf((float)((nibble(kw, (d0 + k) & 7) - kz) * ku), ke - 127);
-            x[1][k] = ve == 255 ? NAN : ldexpf((float)((nibble(vw[k], tk & 7) - z) * u), ve - 127);
+            x[1][k] = ve == 255 ? NAN : ldexpf((float)((nibble(vw[k], t + ((d0 + k) & 16 ? 4 : 0)) - z) * u), ve - 127);
         }
     }
     const size_t to = ((size_t)i * p.n_kv + h) * HD + d0;
