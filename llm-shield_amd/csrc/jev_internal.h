@@ -425,6 +425,15 @@ constexpr int kPagesWideRows = 128;    // the same in a wide tile, for requests 
 constexpr int kPagesWideWgs = 512, kPagesWideKeys = 512;
 __host__ __device__ inline int pages_wide_target(int n_kv) { return n_kv < kPagesWideWgs ? kPagesWideWgs / n_kv : 1; }
 
+// The 4-bit cache's 16-row tiles also take the rows of drafts, up to kPagesSplit of them a
+// request: their parts spread further than a wide tile of which few rows are there, and are
+// merged by more workgroups (us, with wide tiles: 24 requests of 700 to 3000 tokens that add
+// 5 38 / 43, 8 39 / 46; 64 of 500 to 4000 that add 8 97 / 127, 16 161 / 164); and up to
+// kPagesFew where a step's come to kPagesFewWgs workgroups at most (12 of 500 to 2000 that add
+// 31 39 / 64, one of 20000 56 / 105, 64 there 91 / 140; past it 64 of 500 to 4000 that add
+// 31 300 / 186, 9 of 4096 that add 48 148 / 104).
+constexpr int kPagesSplit = 4, kPagesFew = 16, kPagesFewWgs = 2048;
+
 // Keys per workgroup of a 16-row tile: a function of the request's own length
 // alone, so that its result does not depend on the other requests.  Fewer keys
 // spread a lone request further, more save each part's start and end (us, one call after
@@ -467,6 +476,7 @@ struct PagesItem { // a workgroup's tile and keys, with its request's fields: on
 struct Pages {
     // geometry
     int n_layers = 0, n_heads = 0, n_kv = 0, hd = 0, group = 1;
+    int split = 1, few = 1;                 // 16-row tiles of a request, at most, that are not a wide tile's; the same in a step with few
     int page = 16, sub = 1, sub_shift = 0;  // tokens and blocks of a page (powers of two)
     int n_pages = 0, max_requests = 0, max_context = 0, max_tokens = 0, width = 0; // width: pages of a table row
     int bits = 8;                           // of a code: 8 (above) or 4 (Pages4)

@@ -22,7 +22,7 @@ struct PlanView {
     double2 *angle;
     const double *freqs;
     double mscale;
-    int page, sub, sub_shift, n_pages, max_requests, max_context, width, half, group, n_kv;
+    int page, sub, sub_shift, n_pages, max_requests, max_context, width, half, group, split, few, n_kv;
 };
 // Exclusive prefix sums over the workgroup's threads of N values at once, in
 // place, and their totals.  `ws`: N words per wave.
@@ -75,9 +75,10 @@ __device__ __forceinline__ int find(const int *prefix, int n, int i)
 struct Counts {
     int units, items, wides, parts, wide_parts, n_parts, wide;
 };
+// `wide`: the most 16-row tiles of a request without wide ones, 0: of any.
 __device__ __forceinline__ bool is_wide(const PlanView &p, int fresh, int wide)
 {
-    return wide && div_up(fresh * p.group, kPagesTileRows) > div_up(p.group, kPagesTileRows);
+    return wide && div_up(fresh * p.group, kPagesTileRows) > wide;
 }
 __device__ __forceinline__ Counts counts(const PlanView &p, int past, int fresh, int wide, int wide_keys)
 {
@@ -93,7 +94,7 @@ __device__ __forceinline__ Counts counts(const PlanView &p, int past, int fresh,
         return c;
     }
     const int tiles = div_up(rows, kPagesTileRows);
-    if (tiles <= div_up(p.group, kPagesTileRows)) c.n_parts = div_up(len, pages_part_keys(len));
+    if (tiles <= max(wide, p.split)) c.n_parts = div_up(len, pages_part_keys(len));
     c.items = tiles * c.n_parts;
     c.parts = c.n_parts > 1 ? c.items : 0;
     return c;
@@ -304,12 +305,23 @@ __global__ __launch_bounds__(NT) void pages_plan_kernel(PlanView p, PagesPlanArg
 
     // the lists' prefix sums take their place
     int *unit0 = px + S, *item0 = px + 2 * S, *wide0 = px + 3 * S;
-    int wide_keys = kPagesWideKeys;
+    int wide_keys = kPagesWideKeys, wide = 0;
+    if (a.wide) {
+        wide = p.split;
+        if (p.few > p.split) {
+            long long of[1] = {0}, total[1]; // tiles' parts of the requests between
+#pragma unroll
+            for (int i = 0; i < C; i++)
+                if (is_wide(p, fresh[i], p.split) && !is_wide(p, fresh[i], p.few)) of[0] += counts(p, past[i], fresh[i], p.few, 0).items;
+            block_scan<NT, 1>(of, total, ws);
+            if (total[0] * p.n_kv <= kPagesFewWgs) wide = p.few;
+        }
+    }
     if (a.wide) {
         long long of[2] = {0, 0}, total[2]; // keys over the tiles, tiles
 #pragma unroll
         for (int i = 0; i < C; i++)
-            if (is_wide(p, fresh[i], 1)) {
+            if (is_wide(p, fresh[i], wide)) {
                 const int n = div_up(fresh[i] * p.group, kPagesWideRows);
                 of[0] += (long long)n * (past[i] + fresh[i]);
                 of[1] += n;
@@ -326,7 +338,7 @@ __global__ __launch_bounds__(NT) void pages_plan_kernel(PlanView p, PagesPlanArg
     Counts c[C];
 #pragma unroll
     for (int i = 0; i < C; i++) {
-        c[i] = counts(p, past[i], fresh[i], a.wide, wide_keys);
+        c[i] = counts(p, past[i], fresh[i], wide, wide_keys);
         n0[0] += c[i].units;
         n0[1] += c[i].items;
         n0[2] += c[i].wides;
@@ -388,7 +400,7 @@ hipError_t launch_pages_plan(const Pages &p, const PagesPlanArgs &a, hipStream_t
     if (a.n_requests < 0 || a.n_requests > p.max_requests || a.n_tokens < 0 || a.n_tokens > p.max_tokens)
         return hipErrorInvalidValue;
     const PlanView v = {p.table, p.length, p.n_free, p.fresh_pages, p.prefix, p.used, p.head, p.req, p.unit, p.item, p.wide, p.angle, p.freqs,
-                        p.mscale, p.page, p.sub, p.sub_shift, p.n_pages, p.max_requests, p.max_context, p.width, p.half, p.group, p.n_kv};
+                        p.mscale, p.page, p.sub, p.sub_shift, p.n_pages, p.max_requests, p.max_context, p.width, p.half, p.group, p.split, p.few, p.n_kv};
     // What the lists write, in words; an angle counts for several.  Short lists are written
     // by the plan's own workgroup (in a graph, so / with a launch of their own: 12 requests
     // of a token and 64 pairs 6.7 / 7.6 us, 16 9.4 / 10.0, 24 10.8 / 9.8, 64 18.6 / 10.2; one
@@ -1242,7 +1254,7 @@ hipError_t launch_pages_attend(const Pages &p, const PagesAttendArgs &a, hipStre
     // room for: one token over 300 keys in a pool of 2^21 tokens and requests of at most
     // 8192 7.4 us, with a workgroup for every part of the pool (16384 of them) 10.4.
     // (No tokens: a workgroup a KV head, for `outgrown`.)
-    const int64_t split = (int64_t)((p.group + kPagesTileRows - 1) / kPagesTileRows) * std::min(a.n_requests, a.n_tokens);
+    const int64_t split = (int64_t)p.split * std::min(a.n_requests, a.n_tokens);
     const int64_t parts = std::min((int64_t)p.max_parts, split * pages_most_parts(p.max_context));
     const int64_t most = a.n_tokens == 0 ? 1 : std::max<int64_t>(1, parts + (int64_t)a.n_tokens * p.group / kPagesTileRows + a.n_requests);
     const int64_t most_wide = (int64_t)a.n_tokens * p.group / kPagesWideRows + a.n_requests + pages_wide_target(p.n_kv);

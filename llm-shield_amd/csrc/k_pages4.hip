@@ -1020,9 +1020,12 @@ __global__ __launch_bounds__(256, WIDE ? 2 : 3) void pages4_attend_kernel(Attend
 
 hipError_t launch_pages4_attend(const Pages &p, const PagesAttendArgs &a, hipStream_t s)
 {
-    // as many workgroups as the call's requests can need (launch_pages_attend)
-    const int64_t split = (int64_t)((p.group + kPagesTileRows - 1) / kPagesTileRows) * std::min(a.n_requests, a.n_tokens);
-    const int64_t parts = std::min((int64_t)p.max_parts, split * pages_most_parts(p.max_context));
+    // as many workgroups as the call's requests can need (launch_pages_attend; with a token
+    // each: where one has more, the workgroups take turns)
+    const int64_t each = (int64_t)std::min(a.n_requests, a.n_tokens) * pages_most_parts(p.max_context);
+    const int64_t few = a.wide ? std::min(each * p.few, (int64_t)kPagesFewWgs / p.n_kv) : 0;
+    const int64_t split = a.wide ? p.split : (p.group + kPagesTileRows - 1) / kPagesTileRows;
+    const int64_t parts = std::min((int64_t)p.max_parts, std::max(each * split, few));
     const int64_t most = a.n_tokens == 0 ? 1 : std::max<int64_t>(1, parts + (int64_t)a.n_tokens * p.group / kPagesTileRows + a.n_requests);
     const int64_t most_wide = (int64_t)a.n_tokens * p.group / kPagesWideRows + a.n_requests + pages_wide_target(p.n_kv);
     const int wides = a.wide ? (int)(most_wide * p.n_kv) : 0, tiles = (int)(most < 2048 ? most : 2048) * p.n_kv;

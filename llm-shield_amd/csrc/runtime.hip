@@ -2767,8 +2767,11 @@ try {
 
     // a tile's parts hold pages_part_keys() keys, the smallest where contexts are short
     const size_t R = p.max_requests, T = p.max_tokens, pool = (size_t)p.n_pages * p.page;
-    const size_t split = (p.group + kPagesTileRows - 1) / kPagesTileRows; // tiles of a request that is split
-    p.max_parts = (int)(split * (pool / pages_part_keys(1) + R));
+    p.split = (p.group + kPagesTileRows - 1) / kPagesTileRows;
+    if (p.bits == 4) p.split = std::max(p.split, kPagesSplit);
+    p.few = p.bits == 4 ? std::max(p.split, kPagesFew) : p.split;
+    const size_t split = p.split, few = p.few > p.split ? kPagesFewWgs / p.n_kv : 0;
+    p.max_parts = (int)(split * (pool / pages_part_keys(1) + R) + few);
     p.max_items = (int)(p.max_parts + T * p.group / kPagesTileRows + (split + 1) * R);
     p.max_units = (int)(T / kPageBlock + 2 * R);
     // tiles x parts <= tiles x (keys / keys of a part + 1), and a part is at least the sum over

@@ -187,7 +187,7 @@ def test_prompts(gpu, rs, heads, kv, dim):
 
 @pytest.mark.parametrize("fresh", range(1, 10))
 def test_a_few_tokens(gpu, rs, fresh):
-    """Two to 36 rows of a KV head: columns of eight and of sixteen, and wider tiles."""
+    """Two to 36 rows of a KV head: tiles of eight rows and of sixteen, several of them."""
     for heads, dim in ((8, 128), (4, 64)):
         rig = Rig4(cfg(heads, 2, dim), 300, 32, 3, 1500)
         rig.fill(rs, [0, 1, 2], [1200, 64, 0])
@@ -201,8 +201,9 @@ def test_long_contexts(gpu, rs):
         rig.fill(rs, [0], [past])
         rig.fill(rs, [0], [1])
         rig.attend(rs.randn(1, 4, 64).astype(np.float32))
-        rig.fill(rs, [0], [70])
-        rig.attend(rs.randn(70, 4, 64).astype(np.float32))
+        for fresh in (30, 70):
+            rig.fill(rs, [0], [fresh])
+            rig.attend(rs.randn(fresh, 4, 64).astype(np.float32))
 
 
 def test_parts_of_very_long_contexts(gpu, rs):
@@ -210,11 +211,12 @@ def test_parts_of_very_long_contexts(gpu, rs):
     rig.fill(rs, [0], [142001])
     rig.fill(rs, [0], [1])
     rig.attend(rs.randn(1, 2, 64).astype(np.float32))
-    rig.fill(rs, [0], [40])
-    rig.attend(rs.randn(40, 2, 64).astype(np.float32))
+    for fresh in (40, 200):
+        rig.fill(rs, [0], [fresh])
+        rig.attend(rs.randn(fresh, 2, 64).astype(np.float32))
 
 
-@pytest.mark.parametrize("fresh", [1, 90])
+@pytest.mark.parametrize("fresh", [1, 90, 150])
 def test_scales_far_apart(gpu, rs, fresh):
     """Queries and values far from one: the pairs stay inside fp16's range by powers of two."""
     rig = Rig4(cfg(4, 2, 128), 40, 16, 1, 600)
@@ -230,6 +232,21 @@ def test_scales_far_apart(gpu, rs, fresh):
     rig.attend(np.zeros((fresh, 4, 128), np.float32))
 
 
+@pytest.mark.parametrize("n", [30, 203, 206])
+def test_drafts_of_few_and_of_many_requests(gpu, rs, n):
+    """Five tiles of sixteen rows a request: up to 1024 of them a KV head, and wide tiles where there are more; beside a
+    prompt, a single token, a few, and nothing."""
+    rig = Rig4(cfg(8, 2, 64), 4000, 16, n + 4, 1500, 40000)
+    past = [int(x) for x in rs.randint(0, 200, n + 4)]
+    past[5], past[-1] = 1040, 30  # (in two parts)
+    rig.fill(rs, list(range(n + 4)), past)
+    fresh = [17 + i % 4 for i in range(n)] + [1, 300, 0, 3]
+    rig.plan(list(range(n + 4)), fresh)
+    total = sum(fresh)
+    rig.store(None, *(rs.randn(total, 2, 64).astype(np.float32) for _ in "kv"))
+    rig.attend(rs.randn(total, 8, 64).astype(np.float32))
+
+
 @pytest.mark.parametrize("scale", [1e-37, 1e-25, 1e25])
 def test_queries_and_keys_at_the_ends_of_the_range(gpu, rs, scale):
     """Small queries over large keys and the other way round: their product is what counts."""
@@ -240,7 +257,7 @@ def test_queries_and_keys_at_the_ends_of_the_range(gpu, rs, scale):
     rig.attend(rs.randn(90, 8, 64).astype(np.float32) * np.float32(1.0 / np.float32(scale)))
 
 
-@pytest.mark.parametrize("fresh", [2, 4, 90])
+@pytest.mark.parametrize("fresh", [2, 4, 90, 150])
 def test_masked_places_may_hold_anything(gpu, rs, fresh):
     """NaN past a query's own position leaves it alone; a query that sees one is NaN; one query's NaN stays its own."""
     rig = Rig4(cfg(4, 2, 64), 40, 16, 1, 600)
@@ -290,7 +307,7 @@ def test_single_tokens_do_not_depend_on_the_batch(gpu, rs):
     np.testing.assert_array_equal(rig.attend(x[0])[800], together[3])
 
 
-@pytest.mark.parametrize("fresh", [1, 4, 60])
+@pytest.mark.parametrize("fresh", [1, 4, 60, 80])
 def test_parts_of_an_earlier_call_are_not_seen(gpu, rs, fresh):
     rig = Rig4(cfg(8, 2, 128), 1300, 16, 3, 9100, 20000)
     rig.fill(rs, [0, 1, 2], [9000, 3000, 1030])
@@ -366,7 +383,7 @@ def test_a_step_is_captured_and_replayed(gpu, rs):
     assert hip.hipGraphExecDestroy(ex) == 0 and hip.hipGraphDestroy(graph) == 0
 
 
-@pytest.mark.parametrize("fresh", [[1, 1], [70, 3]])
+@pytest.mark.parametrize("fresh", [[1, 1], [30, 3], [70, 3]])
 def test_attention_and_reading_at_any_alignment(gpu, rs, fresh):
     rig = Rig4(cfg(8, 2, 128), 200, 32, 2, 3000)
     rig.fill(rs, [0, 1], [1500, 40])
@@ -390,7 +407,7 @@ def test_attention_and_reading_at_any_alignment(gpu, rs, fresh):
             assert np.all(y[:lead] == -7) and np.all(y[-4:] == -7)
 
 
-@pytest.mark.parametrize("fresh", [1, 40])
+@pytest.mark.parametrize("fresh", [1, 40, 300])
 def test_pages_past_32_bit_offsets(gpu, rs, fresh):
     """A pool whose codes lie past 2^32 bytes."""
     n = 1 << 22
@@ -419,7 +436,7 @@ def test_more_tiles_than_workgroups(gpu, rs):
 
 
 @pytest.mark.parametrize("heads,kv,dim", [(8, 2, 128), (32, 2, 64), (20, 1, 128)])
-@pytest.mark.parametrize("fresh", [1, 40])
+@pytest.mark.parametrize("fresh", [1, 40, 70])
 def test_queries_keep_their_bits(gpu, rs, heads, kv, dim, fresh):
     """Queries of one element: a score is one product, so its error is the query's alone: its pair (2^-21, lo's own
     rounding among it), the softmax's scale on it (2^-24, and its logarithm's factor), the exponent's rounding."""
@@ -518,7 +535,7 @@ def test_values_far_apart(gpu, rs, fresh, where, ratio, score):
     check(rig, 0, q, rig.attend(q, check=False), 496)
 
 
-@pytest.mark.parametrize("fresh", [1, 40])
+@pytest.mark.parametrize("fresh", [1, 40, 80])
 @pytest.mark.parametrize("ratio", [2.0 ** -60, 2.0 ** -20, 1.0, 2.0 ** 40, 2.0 ** 100])
 def test_any_magnitudes(gpu, rs, fresh, ratio):
     """Every token's key and value row of its own magnitude, zeros among them; attended values at either end of fp32."""
@@ -538,7 +555,7 @@ def test_any_magnitudes(gpu, rs, fresh, ratio):
 
 def test_values_of_zeros_only(gpu, rs):
     rig = Rig4(cfg(4, 1, 64), 20, 16, 1, 100)
-    for fresh in (1, 50):
+    for fresh in (1, 50, 80):
         rig.plan([0], [fresh], [0])
         rig.store(None, rs.randn(fresh, 1, 64).astype(np.float32), np.zeros((fresh, 1, 64), np.float32))
         assert np.all(rig.attend(rs.randn(fresh, 4, 64).astype(np.float32), check=False) == 0)
