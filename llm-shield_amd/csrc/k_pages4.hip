@@ -870,6 +870,7 @@ __device__ __forceinline__ void attend4_wide(const Attend4View &p, Wide4Lds<HD> 
             return __builtin_bit_cast(half8_t, kf[buf][(t * NC + c) * 64 + lane]);
         };
         half8_t k0 = kfrag(0, 0), k1 = kfrag(1, 0);
+        __builtin_amdgcn_s_setprio(1); // of two waves, the one with products to issue goes first (9 prompts of 48 over 4096 keys 104 -> 100 us)
 #pragma unroll
         for (int c = 0; c < NC; c++) {
             const half8_t n0 = kfrag(0, min(c + 1, NC - 1)), n1 = kfrag(1, min(c + 1, NC - 1));
@@ -881,6 +882,7 @@ __device__ __forceinline__ void attend4_wide(const Attend4View &p, Wide4Lds<HD> 
             k0 = n0, k1 = n1;
             __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
         fetch(kb + 2, next);
         next = page_of(kb + 3);
         uint4 ve[2];
@@ -960,6 +962,7 @@ __device__ __forceinline__ void attend4_wide(const Attend4View &p, Wide4Lds<HD> 
 #pragma unroll
         for (int i = 0; i < 8; i++) weights(0, i);
         __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
         // the second tile's exponentials run beside the first's V^T P^T
 #pragma unroll
         for (int t = 0; t < 2; t++)
@@ -974,6 +977,7 @@ __device__ __forceinline__ void attend4_wide(const Attend4View &p, Wide4Lds<HD> 
                 v = ahead;
                 __builtin_amdgcn_sched_barrier(0);
             }
+        __builtin_amdgcn_s_setprio(0);
         __syncthreads();
     }
     l += __shfl_xor(l, 32, 64);
