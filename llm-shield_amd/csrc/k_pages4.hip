@@ -93,14 +93,25 @@ __device__ __forceinline__ int most_byte(const uint32_t (&w)[N])
 
 uint8_t *layer4_of(const Pages &p, int layer) { return p.k + (size_t)layer * p.n_blocks() * pages4_bytes(p.hd); }
 
+// The largest of four, eight or sixteen neighbouring lanes' values (aligned), on all of them.
+template <int N>
+__device__ __forceinline__ unsigned most_of(unsigned x)
+{
+    auto other = [&](auto ctrl) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xf, 0xf, true); };
+    x = max(x, other(std::integral_constant<int, 0xb1>())); // lane ^ 1
+    x = max(x, other(std::integral_constant<int, 0x4e>())); // lane ^ 2
+    if (N >= 8) x = max(x, other(std::integral_constant<int, 0x141>())); // the half row mirrored
+    if (N >= 16) x = max(x, other(std::integral_constant<int, 0x140>())); // the row mirrored
+    return x;
+}
+
 // y / u to the nearest whole number, a half to the even one; u whole, 1 .. 15, |y| <= 225.
 // The remainder is exact: it is a multiple of y's last bit and not larger than y or u.
 __device__ __forceinline__ float whole_steps(float y, float u, float inv)
 {
-    float q = rintf(y * inv);
-    const float rest = fmaf(-q, u, y), twice = 2.f * fabsf(rest);
-    if (twice > u || (twice == u && ((int)q & 1))) q += rest > 0.f ? 1.f : -1.f;
-    return q;
+    const float q = rintf(y * inv), rest = fmaf(-q, u, y), twice = 2.f * fabsf(rest);
+    const bool other = (twice > u) | ((twice == u) & (bool)((int)q & 1));
+    return q + (other ? copysignf(1.f, rest) : 0.f);
 }
 
 struct Store4View {
@@ -134,9 +145,12 @@ __global__ __launch_bounds__(256) void pages4_store_kernel(Store4View p)
     __shared__ __align__(16) float xs[2][kPageBlock][LD];
     __shared__ uint8_t code[kPageBlock][HD];                    // V's
     __shared__ uint8_t step[2][kPageBlock][NG], zero[2][kPageBlock][NG];
+    __shared__ uint16_t power[2][kPageBlock]; // bytes, or kNotFinite
+    constexpr uint16_t kNotFinite = 256;
     const int tid = threadIdx.x, j = tid & 15, h = blockIdx.y;
     const PagesUnit un = p.unit[blockIdx.x];
-    const PagesPlanHead plan = *p.head; // (the unit's load does not wait for this)
+    PagesPlanHead plan = *p.head;
+    asm volatile("" : "+s"(plan.n_tokens), "+s"(plan.n_requests), "+s"(plan.n_units), "+s"(plan.n_wide) : "s"(un.row)); // one wait for all
     if (outgrown(p, plan) || (int)blockIdx.x >= plan.n_units) return;
     const int pos0 = un.pos, n = un.n, row0 = un.row, off = pos0 & (kPageBlock - 1);
     const bool kv = p.k_in != nullptr;
@@ -221,15 +235,14 @@ __global__ __launch_bounds__(256) void pages4_store_kernel(Store4View p)
     if (!kv) return;
     __syncthreads();
 
-    // steps and codes of token tid / 16, elements NE j ..
-    const int tk = tid >> 4;
+    // steps and codes of a token's elements NE j ..: of its key and value, or with up to
+    // eight tokens of one of them
+    const bool apart = n <= 8;
+    const int tk = apart ? tid >> 4 & 7 : tid >> 4, v0 = apart ? tid >> 7 : 0, v1 = apart ? v0 + 1 : 2;
     if (tk < n) {
-        unsigned bad = 0; // a value that is not finite has the largest bits
-        int power[2];
-#pragma unroll
-        for (int v = 0; v < 2; v++) {
+        for (int v = v0; v < v1; v++) {
             float x[NE], hi = 0.f, lo = 0.f;
-            unsigned bits = 0;
+            unsigned bits = 0; // a value that is not finite has the largest
 #pragma unroll
             for (int i = 0; i < NE; i++) {
                 x[i] = xs[v][tk][NE * j + i];
@@ -237,19 +250,12 @@ __global__ __launch_bounds__(256) void pages4_store_kernel(Store4View p)
                 lo = fmaxf(lo, -x[i]);
                 bits = max(bits, __float_as_uint(fabsf(x[i])));
             }
-#pragma unroll
-            for (int o = 1; o < TG; o <<= 1) {
-                hi = fmaxf(hi, __shfl_xor(hi, o, 64));
-                lo = fmaxf(lo, __shfl_xor(lo, o, 64));
-            }
+            // (numbers from zero are ordered as their bits)
+            hi = __uint_as_float(most_of<TG>(__float_as_uint(hi)));
+            lo = __uint_as_float(most_of<TG>(__float_as_uint(lo)));
             const float span = 0.5f * hi + 0.5f * lo; // half the group's span: the whole one may be past fp32's range
-            float most = span;
-#pragma unroll
-            for (int o = 1; o < 16; o <<= 1) {
-                most = fmaxf(most, __shfl_xor(most, o, 64));
-                bits = max(bits, (unsigned)__shfl_xor((int)bits, o, 64));
-            }
-            bad = max(bad, bits);
+            const float most = __uint_as_float(most_of<16>(__float_as_uint(span)));
+            bits = most_of<16>(bits);
             // the least 2^ex with the widest span <= 15 * 15 * 2^ex, 225 = 0.87890625 * 2^8
             const bool some = most > 0.f && bits < 0x7f800000u;
             const int ex = max(__builtin_amdgcn_frexp_expf(most) - (__builtin_amdgcn_frexp_mantf(most) <= 0.87890625f ? 7 : 6), -126);
@@ -262,8 +268,8 @@ __global__ __launch_bounds__(256) void pages4_store_kernel(Store4View p)
             uint32_t word = 0;
 #pragma unroll
             for (int i = 0; i < NE; i++) {
-                const float q = some ? whole_steps(ldexpf(x[i], -ex), u, inv) + z : 0.f;
-                const uint32_t c = (uint32_t)(int)fminf(fmaxf(q, 0.f), 15.f);
+                const float q = whole_steps(ldexpf(x[i], -ex), u, inv) + z;
+                const uint32_t c = some ? (uint32_t)(int)fminf(fmaxf(q, 0.f), 15.f) : 0u;
                 if (v) code[tk][NE * j + i] = (uint8_t)c;
                 else word |= c << nibble_at((NE * j + i) & 7);
             }
@@ -276,22 +282,27 @@ __global__ __launch_bounds__(256) void pages4_store_kernel(Store4View p)
                 step[v][tk][j / TG] = (uint8_t)(int)u;
                 zero[v][tk][j / TG] = (uint8_t)(int)z;
             }
-            power[v] = some ? ex + 127 : 0;
+            if (j == 0) power[v][tk] = (uint16_t)(bits >= 0x7f800000u ? kNotFinite : some ? ex + 127 : 0);
         }
-        // a value that is not finite: the token's V power says so for both
-        if (j < 2) block[at.pw + (off + tk) / 4 * 8 + 4 * j + (off + tk) % 4] = (uint8_t)(bad < 0x7f800000u ? power[j] : j ? 255 : 0);
     }
     __syncthreads();
 
+    // a value that is not finite: the token's V power says so for both
+    if (tid < 2 * n) {
+        const int t = tid >> 1, v = tid & 1;
+        const bool bad = max(power[0][t], power[1][t]) == kNotFinite;
+        block[at.pw + (off + t) / 4 * 8 + 4 * v + (off + t) % 4] = (uint8_t)(bad ? v ? 255 : 0 : power[v][t]);
+    }
     // words over several tokens: the new ones' nibbles among what is there
     auto merge = [&](uint32_t old, auto token, auto nibble) {
         uint32_t put = 0, mask = 0;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int tk = token(i) - off;
-            if (tk < 0 || tk >= n) continue;
-            put |= (uint32_t)nibble(i, tk) << nibble_at(i);
-            mask |= 15u << nibble_at(i);
+            const uint32_t x = nibble(i, tk & 15); // (read whether it is one or not: the reads go out together)
+            const uint32_t m = tk < 0 || tk >= n ? 0u : 15u << nibble_at(i);
+            put |= (x << nibble_at(i)) & m;
+            mask |= m;
         }
         mask = turn_left(mask, 2);
         return make_uint2((old & ~mask) | turn_left(put, 2), mask);
@@ -1053,42 +1064,47 @@ struct Read4View {
 };
 } // namespace
 
-// Sixteen slots and one KV head to a workgroup, a slot to sixteen threads, hd / 16
-// neighbouring elements to each.
+// Sixteen slots and one KV head to a workgroup, a slot to sixteen threads: hd / 16
+// neighbouring elements of K to each, and of V the dims that its words hold, 16 apart.
 template <int HD>
 __global__ __launch_bounds__(256) void pages4_read_kernel(Read4View p)
 {
-    constexpr int NE = HD / 16;
+    constexpr int NE = HD / 16, NG = HD / 32;
     constexpr Pages4 at(HD);
-    const int tid = threadIdx.x, h = blockIdx.y, i = blockIdx.x * 16 + (tid >> 4), d0 = NE * (tid & 15), gr = d0 / 32;
+    typedef float floatx4_any __attribute__((ext_vector_type(4), aligned(4))); // the caller's alignment
+    const int tid = threadIdx.x, h = blockIdx.y, i = blockIdx.x * 16 + (tid >> 4), j = tid & 15, d0 = NE * j, gr = d0 / 32;
     if (i >= p.n) return;
     const int slot = p.slot[i];
     float x[2][NE] = {};
     if (slot >= 0 && slot / p.page < p.n_pages) {
-        const int tk = slot % kPageBlock;
+        const int tk = slot % kPageBlock, q = tk / 4, t = tk % 4, w8 = d0 / 8;
         const uint8_t *b = p.pool + (((size_t)(slot / p.page) * p.n_kv + h) * p.sub + slot % p.page / kPageBlock) * at.bytes;
         auto nibble = [](uint32_t w, int i) { return (int)((turn_left(w, 30) >> nibble_at(i)) & 15u); };
-        constexpr int NG = HD / 32;
-        const int q = tk / 4, t = tk % 4, w8 = d0 / 8;
         const uint32_t kw = ((const uint32_t *)(b + at.k))[(w8 / NG * kPageBlock + tk) * NG + w8 % NG];
-        const uint32_t ks = ((const uint32_t *)(b + at.ks))[4 * gr + q], vs = ((const uint32_t *)(b + at.vs))[NG * q + gr];
+        const uint32_t ks = ((const uint32_t *)(b + at.ks))[4 * gr + q];
         const int ke = b[at.pw + 8 * q + t], ve = b[at.pw + 8 * q + 4 + t];
-        uint32_t vw[NE];
+        uint32_t vw[NG], vs[NG];
 #pragma unroll
-        for (int k = 0; k < NE; k++) vw[k] = ((const uint32_t *)(b + at.v))[(16 * q + (d0 + k) % 16) * NG + gr];
-        const int ku = nibble(ks, 2 * t), kz = nibble(ks, 2 * t + 1), u = nibble(vs, t), z = nibble(vs, 4 + t);
+        for (int g = 0; g < NG; g++) {
+            vw[g] = ((const uint32_t *)(b + at.v))[(16 * q + j) * NG + g];
+            vs[g] = ((const uint32_t *)(b + at.vs))[NG * q + g];
+        }
+        const int ku = nibble(ks, 2 * t), kz = nibble(ks, 2 * t + 1);
 #pragma unroll
         for (int k = 0; k < NE; k++) {
+            const int g = k / 2;
             x[0][k] = ve == 255 ? NAN : ldexpf((float)((nibble(kw, (d0 + k) & 7) - kz) * ku), ke - 127);
-            x[1][k] = ve == 255 ? NAN : ldexpf((float)((nibble(vw[k], t + ((d0 + k) & 16 ? 4 : 0)) - z) * u), ve - 127);
+            x[1][k] = ve == 255 ? NAN : ldexpf((float)((nibble(vw[g], t + 4 * (k & 1)) - nibble(vs[g], 4 + t)) * nibble(vs[g], t)), ve - 127);
         }
     }
-    const size_t to = ((size_t)i * p.n_kv + h) * HD + d0;
+    const size_t to = ((size_t)i * p.n_kv + h) * HD;
 #pragma unroll
-    for (int k = 0; k < NE; k++) {
-        p.k_out[to + k] = x[0][k];
-        p.v_out[to + k] = x[1][k];
+    for (int k = 0; k < NE; k += 4) {
+        const floatx4_any y = {x[0][k], x[0][k + 1], x[0][k + 2], x[0][k + 3]};
+        *(floatx4_any *)(p.k_out + to + d0 + k) = y;
     }
+#pragma unroll
+    for (int k = 0; k < NE; k++) p.v_out[to + 16 * k + j] = x[1][k];
 }
 
 hipError_t launch_pages4_read(const Pages &p, int layer, const int32_t *slot, int n, float *k, float *v, hipStream_t s)
