@@ -417,6 +417,16 @@ __device__ __forceinline__ half8_t split_query(const Query4 &q, const float (&x)
     return __builtin_bit_cast(half8_t, make_uint4(h[0], h[1], h[2], h[3]));
 }
 
+// x of the lanes whose number differs in bits 16 and 32, joined by `op`, on all of them.
+template <typename Op>
+__device__ __forceinline__ float over_quarters(float x, Op op)
+{
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 template <int HD>
 struct Tile4Lds {
     uint4 q[2][HD / 32][64]; // [part][dims][lane]; eight rows: both parts in [0]
@@ -519,9 +529,7 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
                 x[c][i] = src[8 * c + i];
                 m = fmaxf(m, fabsf(x[c][i]));
             }
-        m = fmaxf(m, __shfl_xor(m, 16, 64));
-        m = fmaxf(m, __shfl_xor(m, 32, 64));
-        const Query4 scaled(m, p.scale);
+        const Query4 scaled(over_quarters(m, fmaxf), p.scale);
         query = scaled.power();
         // a wave makes a quarter of the fragments, in LDS for all (and for each 64 keys'
         // products again: registers)
@@ -544,10 +552,7 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
     float m = -INFINITY, l = 0.f, e = -INFINITY; // m and e whole numbers; outputs are held times 2^(9 - e)
     int value = -127;                            // with a V row's byte: the power from a weight to fp16's
 
-    auto row_max = [](float x) {
-        x = fmaxf(x, __shfl_xor(x, 16, 64));
-        return fmaxf(x, __shfl_xor(x, 32, 64));
-    };
+    auto row_max = [](float x) { return over_quarters(x, fmaxf); };
     auto both = [](float x) { // both parts' sum: the other's column is eight lanes on
         if constexpr (!BOTH) x += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x128, 0xf, 0xf, true));
         return x;
@@ -671,8 +676,7 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
             pages = pages_of(kb + 8);
         }
     }
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
+    l = over_quarters(l, [](float a, float b) { return a + b; });
 
     // the waves' results, in wave order
     const MeanScale mean(e, m, l);
