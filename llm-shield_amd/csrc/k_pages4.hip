@@ -475,60 +475,68 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
     auto pages_of = [&](int kb) { return table[min(4 * kb + (lane & 3), last) >> p.sub_shift]; };
     const uint32_t page_bytes = (uint32_t)(p.n_kv << p.sub_shift) * at.bytes;
     const uint8_t *const pool = p.pool + (size_t)((h << p.sub_shift) * at.bytes);
-    auto block_of = [&](int kb, int b, int pages) {
-        const uint32_t page = __builtin_amdgcn_readlane(pages, b), sub = min(4 * kb + b, last) & (p.sub - 1);
-        return pool + (uint64_t)page * page_bytes + sub * at.bytes;
-    };
     const uint32_t codes_at = 4 * NC * lane, ks_at = at.ks + 4 * (4 * (g * NC / 4) + (n >> 2)), vs_at = at.vs + 4 * (lane & (4 * NC - 1));
     uint32_t kr[4][NC], vr[4][NC], ks[4], vs[4];
     uint2 power[4]; // K's of the lane's tokens of a block, V's
-    auto load = [&](uint32_t (&to)[NC], const uint8_t *from) {
+    rsrc_t block[4];
+    // (past the wave's keys buffers without bytes, which cost no traffic: as branches the
+    // loads' waits would be for the worst way through them)
+    auto blocks_of = [&](int kb, int pages) {
+        const int bytes = kb * 64 < key1 ? at.bytes : 0;
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            const uint32_t page = __builtin_amdgcn_readlane(pages, b), sub = min(4 * kb + b, last) & (p.sub - 1);
+            block[b] = make_rsrc(pool + (uint64_t)page * page_bytes + sub * at.bytes, bytes);
+        }
+    };
+    auto load = [&](uint32_t (&to)[NC], const rsrc_t &from, int offset) {
         if constexpr (NC == 4) {
-            const uint4 x = *(const uint4 *)from;
+            const uint4 x = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(from, codes_at, offset, 0));
             to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
         } else {
-            const uint2 x = *(const uint2 *)from;
+            const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(from, codes_at, offset, 0));
             to[0] = x.x, to[1] = x.y;
         }
     };
-    auto fetch_k = [&](int kb, int pages) {
+    auto fetch_k = [&] {
 #pragma unroll
         for (int b = 0; b < 4; b++) {
-            const uint8_t *block = block_of(kb, b, pages);
-            load(kr[b], block + codes_at);
-            ks[b] = *(const uint32_t *)(block + ks_at);
+            load(kr[b], block[b], at.k);
+            ks[b] = __builtin_amdgcn_raw_buffer_load_b32(block[b], ks_at, 0, 0);
         }
     };
-    auto fetch_v = [&](int kb, int pages) {
+    auto fetch_v = [&] {
 #pragma unroll
         for (int b = 0; b < 4; b++) {
-            const uint8_t *block = block_of(kb, b, pages);
-            power[b] = *(const uint2 *)(block + at.pw + 8 * g);
-            load(vr[b], block + at.v + codes_at);
-            vs[b] = *(const uint32_t *)(block + vs_at);
+            power[b] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(block[b], 8 * g, at.pw, 0));
+            load(vr[b], block[b], at.v);
+            vs[b] = __builtin_amdgcn_raw_buffer_load_b32(block[b], vs_at, 0, 0);
         }
     };
     int kb = r.key0 / 64 + wave;
     int pages = pages_of(kb);
-    if (kb * 64 < key1) {
-        fetch_k(kb, pages);
-        fetch_v(kb, pages);
+    float qx[NC][8]; // under way while the page's number is
+    {
+        const float *src = p.q + ((size_t)(r.start + token) * p.n_heads + head) * HD + 8 * NC * g;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) qx[c][i] = src[8 * c + i];
     }
+    blocks_of(kb, pages);
     pages = pages_of(kb + 4);
+    fetch_k();
+    fetch_v();
 
     // Q^T fragments: dims 8 NC g + 8 c .. + 7 of column n
     int query;
     const float part = n < 8 ? 0.f : -1.f; // a column's part of a query or a weight
     {
-        const float *src = p.q + ((size_t)(r.start + token) * p.n_heads + head) * HD + 8 * NC * g;
-        float x[NC][8], m = 0.f;
+        float m = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                x[c][i] = src[8 * c + i];
-                m = fmaxf(m, fabsf(x[c][i]));
-            }
+            for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(qx[c][i]));
         const Query4 scaled(over_quarters(m, fmaxf), p.scale);
         query = scaled.power();
         // a wave makes a quarter of the fragments, in LDS for all (and for each 64 keys'
@@ -538,10 +546,10 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
             if (c != wave) continue;
             if constexpr (BOTH) {
                 half8_t hi, lo;
-                split_query(scaled, x[c], hi, lo);
+                split_query(scaled, qx[c], hi, lo);
                 lds.q[0][c][lane] = __builtin_bit_cast(uint4, hi);
                 lds.q[1][c][lane] = __builtin_bit_cast(uint4, lo);
-            } else lds.q[0][c][lane] = __builtin_bit_cast(uint4, split_query(scaled, x[c], part));
+            } else lds.q[0][c][lane] = __builtin_bit_cast(uint4, split_query(scaled, qx[c], part));
         }
     }
     __syncthreads();
@@ -558,7 +566,6 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
         return x;
     };
     for (; kb * 64 < key1; kb += 4) {
-        const bool more = (kb + 4) * 64 < key1;
         float sv[16]; // [block][token of the lane's quad]
         {
             half8_t qf[1 + BOTH][NC];
@@ -580,7 +587,9 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
                 for (int i = 0; i < 4; i++) sv[4 * b + i] = __builtin_amdgcn_ldexpf(both(acc[i]), byte_of(power[b].x, i) + query);
             }
         }
-        if (more) fetch_k(kb + 4, pages);
+        blocks_of(kb + 4, pages);
+        pages = pages_of(kb + 8);
+        fetch_k();
         // V's steps, a quad's and group's to a lane, for the sixteen lanes that want them
         {
             const int b = lane / (4 * NC) & 3;
@@ -671,10 +680,7 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
                     o[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[i][c], o[2 * j + 1], 0, 0, 0);
                 }
             }
-        if (more) {
-            fetch_v(kb + 4, pages);
-            pages = pages_of(kb + 8);
-        }
+        fetch_v();
     }
     l = over_quarters(l, [](float a, float b) { return a + b; });
 
