@@ -427,6 +427,61 @@ __device__ __forceinline__ float over_quarters(float x, Op op)
     return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
+// x of T neighbouring lanes (16, 32 or 64, aligned) joined by `op`, on all of them.
+template <int T, typename Op>
+__device__ __forceinline__ float over_lanes(float x, Op op)
+{
+    auto other = [&](auto ctrl) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, true)); };
+    x = op(x, other(std::integral_constant<int, 0xb1>()));  // lane ^ 1
+    x = op(x, other(std::integral_constant<int, 0x4e>()));  // lane ^ 2
+    x = op(x, other(std::integral_constant<int, 0x141>())); // the half row mirrored
+    x = op(x, other(std::integral_constant<int, 0x140>())); // the row mirrored
+    if constexpr (T == 64) x = over_quarters(x, op);
+    else if constexpr (T == 32) {
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    }
+    return x;
+}
+
+// One row's parts (merge_parts) by T threads of a wave, at most T of them, their maxima whole
+// numbers or -inf: a part's maximum and sum to a thread, and the first parts' rows under way
+// beside them, so that memory is waited for once.
+template <int HD, int T, typename At>
+__device__ __forceinline__ void merge4_parts(At at, int n_parts, float *dst, int j)
+{
+    constexpr int N = HD / 2 / T, B = 8;
+    const int first = 4 * (threadIdx.x & 63 & ~(T - 1)); // of the row's lanes
+    float2 ml = make_float2(-INFINITY, 0.f), y[B][N];
+    if (j < n_parts) ml = load_shared(at(j) + HD);
+    auto fetch = [&](int k0) {
+#pragma unroll
+        for (int k = 0; k < B; k++)
+            if (k0 + k < n_parts)
+#pragma unroll
+                for (int i = 0; i < N; i++) y[k][i] = load_shared(at(k0 + k) + 2 * (T * i + j));
+    };
+    fetch(0);
+    const float m = over_lanes<T>(ml.x, fmaxf), mu = m == -INFINITY ? 0.f : m;
+    const float w = ldexpf(ml.y, (int)fmaxf(ml.x - mu, -300.f)), f = w * (1.f / over_lanes<T>(w, [](float a, float b) { return a + b; }));
+    float2 x[N] = {};
+    for (int k0 = 0; k0 < n_parts; k0 += B) {
+        if (k0) fetch(k0);
+#pragma unroll
+        for (int k = 0; k < B; k++) {
+            if (k0 + k >= n_parts) break;
+            const float fk = __int_as_float(__builtin_amdgcn_ds_bpermute(first + 4 * (k0 + k), __float_as_int(f)));
+#pragma unroll
+            for (int i = 0; i < N; i++) x[i] = make_float2(x[i].x + y[k][i].x * fk, x[i].y + y[k][i].y * fk);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        dst[2 * (T * i + j)] = x[i].x;
+        dst[2 * (T * i + j) + 1] = x[i].y;
+    }
+}
+
 template <int HD>
 struct Tile4Lds {
     uint4 q[2][HD / 32][64]; // [part][dims][lane]; eight rows: both parts in [0]
@@ -708,7 +763,7 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
         floatx4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-            f[w] = lds.wave[w].l[c] * exp2f(lds.wave[w].m[c] - mu);
+            f[w] = ldexpf(lds.wave[w].l[c], (int)fmaxf(lds.wave[w].m[c] - mu, -300.f)); // (whole numbers)
             sum += f[w];
         }
         const float inv = sum == 0.f && r.part >= 0 ? 0.f : 1.f / sum;
@@ -729,13 +784,21 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
     if (r.part >= 0) {
         // the tile's last part to arrive merges them all, in their order
         const int tiles = div_up(n_rows, kPagesTileRows), tile = r.row0 / kPagesTileRows;
-        if (arrives_last(p.tickets + (size_t)(r.part0 + tile) * p.n_kv + h, r.n_parts, lds.last))
-            for (int c = tid >> 4; c < min(kPagesTileRows, n_rows - r.row0); c += 16) {
-                const int rr = r.row0 + c, tk = rr / p.group;
-                merge_parts<HD>(
-                    [&](int k) { return p.part + (((size_t)(r.part0 + k * tiles + tile) * p.n_kv + h) * kPagesTileRows + c) * LD; },
-                    r.n_parts, p.out + ((size_t)(r.start + tk) * p.n_heads + h * p.group + rr % p.group) * HD, tid & 15);
-            }
+        if (arrives_last(p.tickets + (size_t)(r.part0 + tile) * p.n_kv + h, r.n_parts, lds.last)) {
+            const int rows = min(ROWS, n_rows - r.row0);
+            auto merge = [&](auto threads) { // a row to that many
+                constexpr int T = decltype(threads)::value;
+                const int c = tid / T, rr = r.row0 + c, tk = rr / p.group;
+                if (c >= rows) return;
+                auto at = [&](int k) { return p.part + (((size_t)(r.part0 + k * tiles + tile) * p.n_kv + h) * kPagesTileRows + c) * LD; };
+                float *dst = p.out + ((size_t)(r.start + tk) * p.n_heads + h * p.group + rr % p.group) * HD;
+                if (r.n_parts <= T) merge4_parts<HD, T>(at, r.n_parts, dst, tid % T);
+                else if (tid % T < 16) merge_parts<HD>(at, r.n_parts, dst, tid % T);
+            };
+            if constexpr (BOTH) merge(std::integral_constant<int, 16>());
+            else if (HD == 128 && rows <= 4) merge(std::integral_constant<int, HD == 128 ? 64 : 32>());
+            else merge(std::integral_constant<int, 32>());
+        }
     }
     __syncthreads();
 }
