@@ -404,11 +404,11 @@ hipError_t launch_kv_split(const float *src, uint16_t *dst, int heads_total, int
 hipError_t launch_kv_copy(const float *src, float *dst, int heads_total, int old_cap, int new_cap, int len, int hd,
                           hipStream_t s);
 
-// ---------------------------------------------------------------- 8-bit paged KV cache
+// ---------------------------------------------------------------- paged KV cache, 8 or 4 bits
 //
 // Many requests share one pool of pages of `page` tokens.  Sixteen consecutive
 // positions of a request are a block; per layer, page, KV head and block the
-// pool holds 16 x hd codes of K, as many of V, and their two scales: a value
+// 8-bit pool (the 4-bit one: Pages4) holds 16 x hd codes of K, as many of V, and their two scales: a value
 // is (byte - 128) * scale.  Both orders are the matrix cores' operands as a
 // wave loads them, 16 bytes a lane:
 //   K  [hd / 64][16 tokens][64 dims]: lane 16 g + r of a load reads dims 64 j +

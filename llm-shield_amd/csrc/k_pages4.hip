@@ -136,7 +136,9 @@ struct Store4View {
 // takes hd / 16 neighbouring elements of them to steps and codes.  Words that hold other
 // tokens' nibbles (V's, and all steps) are read first and merged.  Rotations are 64-bit
 // and round to fp32 once, quotients are exact: a stored value does not depend on how
-// they are formed.
+// they are formed.  One token (32 query heads, 8 KV heads of 128) takes 6.3 us, a launch and
+// a chain of trips to memory (arguments, plan and unit, rows and the block's words); 64 7.5;
+// 8000 of a prompt 81, 326 MB at 4.1 TB/s.
 template <int HD, bool VEC>
 __global__ __launch_bounds__(256) void pages4_store_kernel(Store4View p)
 {
@@ -446,7 +448,7 @@ __device__ __forceinline__ float over_lanes(float x, Op op)
 
 // One row's parts (merge_parts) by T threads of a wave, at most T of them, their maxima whole
 // numbers or -inf: a part's maximum and sum to a thread, and the first parts' rows under way
-// beside them, so that memory is waited for once.
+// beside them, so that memory is waited for once (four parts of four rows 10000 -> 2500 cycles).
 template <int HD, int T, typename At>
 __device__ __forceinline__ void merge4_parts(At at, int n_parts, float *dst, int j)
 {
@@ -504,6 +506,14 @@ struct Tile4Lds {
 // operands.  A weight is 2^(score - m); the V operand's 2^e and the row's own power are
 // added to its exponent, so that what enters fp16 is relative to the row's heaviest product
 // so far (times 2^9), over the keys that the row sees.
+// Codes become fp16 by a mask and a fused multiply-add a pair: of 64 keys' ~640 vector
+// instructions (hd 128) 350, and with scores and weights they take longer than the matrix
+// cores' 32 and, below three waves a SIMD, than memory.  So 168 registers: queries
+// in LDS, V's steps made once for sixteen lanes, block addresses the wave's (two waves a SIMD
+// 94 us for 64 tokens over 500 to 12000 keys, three 84; with loads free of branches 80, 285 MB
+// at 3.6 TB/s).  One token over 120000 keys 44 us (133 MB, 3 TB/s and the parts' merge), over
+// 4000 14.3, over 300 8.6: there waves wait for each other's trips to memory, ~1800 cycles an
+// iteration of 2400 of work.  K and V a 64-key block further ahead, in LDS, gained nothing.
 template <int HD, bool BOTH>
 __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> &lds, const PagesItem &r, int h)
 {
@@ -822,7 +832,11 @@ struct Wide4Lds {
 // steps) in LDS once for the four waves, double buffered: the next block's codes are in
 // flight during a block's products and become fragments beside its scores' matrix
 // instructions.  v_mfma_f32_32x32x16_f16: S^T is two tiles of 32 keys, their rows dealt so
-// that a lane's sixteen scores are one block's tokens in order.
+// that a lane's sixteen scores are one block's tokens in order.  Four prompts of 300 to 4000
+// tokens behind 1 to 700 take 330 to 350 us (123 GFLOP, each twice: 740 TFLOP/s) where 16-row
+// tiles took 633.  The matrix cores are busy 47 % of the time at 1.93 GHz: under them the
+// clock falls with the power drawn, and vector work adds to it (without the products' low
+// halves 254 us, without the staging 314, without the weights' exponents 312).
 template <int HD>
 __device__ __forceinline__ void attend4_wide(const Attend4View &p, Wide4Lds<HD> &lds, const PagesItem &r, int first)
 {
@@ -1138,7 +1152,9 @@ struct Read4View {
 } // namespace
 
 // Sixteen slots and one KV head to a workgroup, a slot to sixteen threads: hd / 16
-// neighbouring elements of K to each, and of V the dims that its words hold, 16 apart.
+// neighbouring elements of K to each, and of V the dims that its words hold, 16 apart (V
+// gathered word by word for neighbouring dims: 47 us for 8000 tokens of 8 heads of 128, so
+// 17, 65 MB of values at 4 TB/s).
 template <int HD>
 __global__ __launch_bounds__(256) void pages4_read_kernel(Read4View p)
 {
