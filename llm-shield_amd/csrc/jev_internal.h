@@ -431,7 +431,8 @@ __host__ __device__ inline int pages_wide_target(int n_kv) { return n_kv < kPage
 // 5 38 / 43, 8 39 / 46; 64 of 500 to 4000 that add 8 97 / 127, 16 161 / 164); and up to
 // kPagesFew where a step's come to kPagesFewWgs workgroups at most (12 of 500 to 2000 that add
 // 31 39 / 64, one of 20000 56 / 105, 64 there 91 / 140; past it 64 of 500 to 4000 that add
-// 31 300 / 186, 9 of 4096 that add 48 148 / 104).
+// 31 300 / 186, 9 of 4096 that add 48 148 / 104; since then 16-row tiles have become 5 to 20 %
+// faster, wide ones 4 %).
 constexpr int kPagesSplit = 4, kPagesFew = 16, kPagesFewWgs = 2048;
 
 // Keys per workgroup of a 16-row tile: a function of the request's own length

@@ -254,7 +254,10 @@ __device__ __forceinline__ uint64_t load_shared64(const void *p)
 // maximum (which moves the running sums only where it rises), the exponentials, and, where
 // one of them passes the wave's k-th largest so far, their places in its list.  A wave's
 // maximum, sums and list are its own, so nothing waits inside the pass.  The last part of
-// a row to arrive merges all of them.  Bounded by HBM: each logit is read once.
+// a row to arrive merges all of them.  Bounded by HBM where there are rows enough, each logit
+// being read once: 1000 rows of 131072 (524 MB) 98 us, with the 5 most probable 104, 5.0 to
+// 5.3 TB/s; 64 with the 20 most probable 20 (34 MB: a pass of the lanes, and the lists' merge),
+// one with 5 8.7 (a launch, the pass, two trips to memory and the merge).
 template <bool TOP>
 __global__ __launch_bounds__(256, 4) void logprobs_kernel(LogprobsView p)
 {
