@@ -3068,14 +3068,16 @@ try {
     step.args = h->plan;
     if (!rc) rc = enqueue_forward(c, p, score ? JEV_OUT_NONE : mode, n_rows, c->logits.p, nullptr, &call, true, nullptr, &step);
     float *const d_entropy = c->scores.p + n_given, *const d_top = d_entropy + p.n_out, *const d_top_logp = d_top + n_top;
-    for (int i = 0, r0 = 0; score && !rc && r0 < p.n_out; i++, r0 += per) {
+    for (int i = 0, r0 = 0, n = 0; score && !rc && r0 < p.n_out; i++, r0 += n) {
         if (i >= jev_ctx::kLeadLayers) HIP_TRY(hipEventSynchronize(c->layer_ev[(i - jev_ctx::kLeadLayers) % jev_ctx::kLayerEvents]));
         if (call.cancelled()) {
             rc = fail(JEV_ECANCELED, "the forward pass was cancelled at its heads");
             break;
         }
+        n = std::min(per, p.n_out - r0);
+        if (p.n_out - r0 - n == 1) n--; // (of several groups' rows)
         Plan part = p;
-        part.n_out = std::min(per, p.n_out - r0);
+        part.n_out = n;
         part.d_out = p.d_out + r0;
         rc = enqueue_heads(c, part, JEV_OUT_FULL, 0, c->logits.p);
         if (rc) break;

@@ -75,6 +75,22 @@ def test_every_token_of_a_step(gpu, model, bits):
         np.testing.assert_array_equal(x, y)
 
 
+def test_no_row_is_scored_alone(gpu):
+    """One row more than 255 times the head's 256: the last row has the bits of its request's own step (a head of one
+    row would be the one-token path's)."""
+    rs = np.random.RandomState(12)
+    m = jev.SynthModel(config(n_layers=1), jev.TYPE_Q8_0).open(0)
+    counts = [15] * 255 + [16] * 3841
+    assert sum(counts) == 255 * 256 + 1
+    toks = [rs.randint(0, 3000, n).tolist() for n in counts]
+    pages = jev.KvPages(m.config, 4100, 16, 4096, 16, 66000, bits=4)
+    given = rs.randint(0, 3000, (65281, 20))
+    got = m.forward_pages_logprobs(pages, list(range(4096)), toks, given, 20, past=[0] * 4096, every=True)
+    alone = m.forward_pages_logprobs(pages, [4095], toks[-1:], given[-16:], 20, past=[0], every=True)
+    for x, y in zip(got, alone):
+        np.testing.assert_array_equal(x[-16:], y)
+
+
 @pytest.mark.parametrize("bits", [8, 4])
 def test_prompts_are_scored(gpu, model, bits):
     """paged_logprobs over several steps: each prompt as alone, and its tokens' log probabilities from logits."""
