@@ -307,6 +307,23 @@ def test_single_tokens_do_not_depend_on_the_batch(gpu, rs):
     np.testing.assert_array_equal(rig.attend(x[0])[800], together[3])
 
 
+@pytest.mark.parametrize("fresh", [2, 3, 4])
+def test_a_few_tokens_do_not_depend_on_the_batch(gpu, rs, fresh):
+    """Alone, beside a prompt, beside many drafts: up to sixteen rows of a KV head have the same bits."""
+    for dim in (64, 128):
+        rig = Rig4(cfg(8, 2, dim), 1000, 16, 210, 2500, 8000)
+        rig.fill(rs, [0], [2100])
+        x = [rs.randn(fresh, h, dim).astype(np.float32) for h in (8, 2, 2)]
+        rig.plan([0], [fresh])
+        rig.store(None, *x[1:])
+        alone = rig.attend(x[0])
+        for ids, more in (([1], [800]), (list(range(1, 210)), [17] * 209), ([5], [1])):
+            rig.plan([0] + ids, [fresh] + more, [2100] + [0] * len(ids))
+            y = [np.concatenate([a, rs.randn(sum(more), *a.shape[1:]).astype(np.float32)]) for a in x]
+            rig.store(None, *y[1:])
+            np.testing.assert_array_equal(rig.attend(y[0], check=False)[:fresh], alone)
+
+
 @pytest.mark.parametrize("fresh", [1, 4, 60, 80])
 def test_parts_of_an_earlier_call_are_not_seen(gpu, rs, fresh):
     rig = Rig4(cfg(8, 2, 128), 1300, 16, 3, 9100, 20000)
@@ -379,6 +396,46 @@ def test_a_step_is_captured_and_replayed(gpu, rs):
         assert np.all(got[total:] == -7)
         y = ref.store(*xs)
         np.testing.assert_array_equal(got[:total], ref.attend(y.cpu().numpy()[:total]))
+    rig.t.cuda.synchronize()
+    assert hip.hipGraphExecDestroy(ex) == 0 and hip.hipGraphDestroy(graph) == 0
+
+
+def test_a_graph_replayed_with_few_and_many_drafts(gpu, rs):
+    """A captured plan and attention whose replays have 16-row tiles of all requests, wide ones, none, and both."""
+    hip = ctypes.CDLL("libamdhip64.so.7")
+    R_, n = 220, 5000
+    rig, ref = (Rig4(cfg(8, 2, 64), 1200, 16, R_, 400, n) for _ in range(2))
+    past = [int(x) for x in rs.randint(0, 30, R_)]
+    seed = rs.randint(1 << 30)
+    for r in (rig, ref):
+        r.fill(np.random.RandomState(seed), list(range(R_)), past)
+    t = rig.t
+    request, kept, fresh = rig.ints(list(range(R_))), rig.ints(past), rig.ints([1] * R_)
+    q, out = t.zeros((n, 8, 64), device="cuda"), t.full((n, 8, 64), -7.0, device="cuda")
+    k, v = t.zeros((n, 2, 64), device="cuda"), t.zeros((n, 2, 64), device="cuda")
+    t.cuda.synchronize()
+    stream, graph, ex = ctypes.c_void_p(rig.p.stream), ctypes.c_void_p(), ctypes.c_void_p()
+    assert hip.hipStreamBeginCapture(stream, 2) == 0  # relaxed: other threads' calls are their own
+    rig.p.plan_device(request.data_ptr(), kept.data_ptr(), fresh.data_ptr(), R_, n)
+    rig.p.store_device(0, 0, 0, k.data_ptr(), v.data_ptr(), 128, 0)
+    rig.p.attend_device(0, q.data_ptr(), out.data_ptr())
+    assert hip.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(ctypes.byref(ex), graph, None, None, 0) == 0
+    for more in ([20] * R_, [20] * 30 + [0] * 190, [1] * R_, [0] * R_, [300] + [3] * 100 + [18] * 119, [20] * R_):
+        total = sum(more)
+        xs = [rs.randn(total, h, 64).astype(np.float32) for h in (8, 2, 2)]
+        for dst, x in zip((q, k, v), xs):
+            dst[:total] = rig.dev(x)
+        fresh.copy_(rig.ints(more))
+        out.fill_(-7.0)
+        t.cuda.synchronize()
+        assert hip.hipGraphLaunch(ex, stream) == 0
+        rig.p.sync()
+        ref.plan(list(range(R_)), more, past, outputs=False, pad=n - total)
+        got = out.cpu().numpy()
+        assert np.all(got[total:] == -7)
+        ref.store(None, *xs[1:])
+        np.testing.assert_array_equal(got[:total], ref.attend(xs[0]))
     rig.t.cuda.synchronize()
     assert hip.hipGraphExecDestroy(ex) == 0 and hip.hipGraphDestroy(graph) == 0
 
