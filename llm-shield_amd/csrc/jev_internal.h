@@ -434,6 +434,18 @@ __host__ __device__ inline int pages_wide_target(int n_kv) { return n_kv < kPage
 // 31 300 / 186, 9 of 4096 that add 48 148 / 104; since then 16-row tiles have become 5 to 20 %
 // faster, wide ones 4 %).
 constexpr int kPagesSplit = 4, kPagesFew = 16, kPagesFewWgs = 2048;
+// A call for few rows, over all KV heads at most kPagesSmallRows, and kPagesSmallKeys times a
+// context's tokens, has no wide tiles at all, nor their launch's registers, LDS and empty
+// workgroups (us, without / with them: 12 requests of 500 to 2000 that add 5 15 / 20, 24 of 700
+// to 3000 that add 3 to 5 24 / 25; a prompt of 100 7.7 / 12.8, of 500 20 / 26, of 200 behind
+// 1000 25 / 56; past the bounds, four of 256 29 / 19, 9 of 48 behind 4096 121 / 100, 64 behind
+// 100000 335 / 275, 500 behind 2000 85 / 88, behind 4000 146 / 120).
+constexpr int kPagesSmallRows = 16384;
+constexpr int64_t kPagesSmallKeys = 1 << 25;
+inline bool pages_small(int64_t rows, int n_kv, int max_context)
+{
+    return rows * n_kv <= kPagesSmallRows && rows * n_kv * max_context <= kPagesSmallKeys;
+}
 
 // Keys per workgroup of a 16-row tile: a function of the request's own length
 // alone, so that its result does not depend on the other requests.  Fewer keys
@@ -524,7 +536,8 @@ __host__ __device__ constexpr int pages4_bytes(int hd) { return Pages4(hd).bytes
 struct PagesPlanArgs {
     const int32_t *request = nullptr, *past = nullptr, *fresh = nullptr; // past may be null: keep everything
     int n_requests = 0, n_tokens = 0;
-    int wide = 0; // requests of more rows than a 16-row tile go to the wide list
+    int wide = 0;  // requests of more rows than a 16-row tile go to the wide list
+    int small = 0; // 4 bits, pages_small(): 16-row tiles alone, the keys of all split
     int32_t *table = nullptr, *slot = nullptr, *position = nullptr, *row = nullptr, *start = nullptr; // outputs, or null
 };
 hipError_t launch_pages_plan(const Pages &p, const PagesPlanArgs &a, hipStream_t s);
@@ -543,7 +556,7 @@ struct PagesAttendArgs {
     int layer = 0;
     const float *q = nullptr; // [n_tokens][n_heads * hd]
     float *out = nullptr;     // the same
-    int n_requests = 0, n_tokens = 0, wide = 0; // of the plan
+    int n_requests = 0, n_tokens = 0, wide = 0, small = 0; // of the plan
     hipEvent_t ev_start = nullptr, ev_stop = nullptr; // optional dispatch-stamped timing
 };
 hipError_t launch_pages_attend(const Pages &p, const PagesAttendArgs &a, hipStream_t s);

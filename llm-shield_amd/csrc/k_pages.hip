@@ -80,7 +80,7 @@ __device__ __forceinline__ bool is_wide(const PlanView &p, int fresh, int wide)
 {
     return wide && div_up(fresh * p.group, kPagesTileRows) > wide;
 }
-__device__ __forceinline__ Counts counts(const PlanView &p, int past, int fresh, int wide, int wide_keys)
+__device__ __forceinline__ Counts counts(const PlanView &p, int past, int fresh, int wide, int wide_keys, int small = 0)
 {
     Counts c = {0, 0, 0, 0, 0, 1, 0};
     if (fresh <= 0) return c;
@@ -94,7 +94,7 @@ __device__ __forceinline__ Counts counts(const PlanView &p, int past, int fresh,
         return c;
     }
     const int tiles = div_up(rows, kPagesTileRows);
-    if (tiles <= max(wide, p.split)) c.n_parts = div_up(len, pages_part_keys(len));
+    if (small || tiles <= max(wide, p.split)) c.n_parts = div_up(len, pages_part_keys(len));
     c.items = tiles * c.n_parts;
     c.parts = c.n_parts > 1 ? c.items : 0;
     return c;
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(NT) void pages_plan_kernel(PlanView p, PagesPlanArg
 
     // the lists' prefix sums take their place
     int *unit0 = px + S, *item0 = px + 2 * S, *wide0 = px + 3 * S;
-    int wide_keys = kPagesWideKeys, wide = 0;
+    int wide_keys = kPagesWideKeys, wide = 0; // (a small call's requests are all split)
     if (a.wide) {
         wide = p.split;
         if (p.few > p.split) {
@@ -338,7 +338,7 @@ __global__ __launch_bounds__(NT) void pages_plan_kernel(PlanView p, PagesPlanArg
     Counts c[C];
 #pragma unroll
     for (int i = 0; i < C; i++) {
-        c[i] = counts(p, past[i], fresh[i], wide, wide_keys);
+        c[i] = counts(p, past[i], fresh[i], wide, wide_keys, a.small);
         n0[0] += c[i].units;
         n0[1] += c[i].items;
         n0[2] += c[i].wides;

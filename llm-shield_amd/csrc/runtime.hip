@@ -1046,8 +1046,9 @@ int enqueue_forward(jev_ctx *c, const Plan &p, int mode, int n_rows, float *dout
             pa.n_requests = sa.n_requests;
             pa.n_tokens = T;
             pa.wide = paged->args.wide;
+            pa.small = paged->args.small;
             {
-                ProfScope ps(c, pa.wide ? JEV_PROF_ATTN : JEV_PROF_DECODE_ATTN, 4.0 * f.head_dim * f.n_heads * p.visible_pairs,
+                ProfScope ps(c, pa.wide || pa.small ? JEV_PROF_ATTN : JEV_PROF_DECODE_ATTN, 4.0 * f.head_dim * f.n_heads * p.visible_pairs,
                              2.0 * f.head_dim * f.n_kv_heads * p.kv_rows + 8.0 * T * qdim, true);
                 pa.ev_start = ps.a;
                 pa.ev_stop = ps.z;
@@ -2671,6 +2672,8 @@ int pages_plan(jev_pages *h, const PagesPlanArgs &a, hipStream_t s)
     // as many tokens as requests: 16-row tiles serve whatever there is, and the
     // wide tiles' launches are saved
     h->plan.wide = a.n_tokens > a.n_requests;
+    h->plan.small = h->p.bits == 4 && h->plan.wide && pages_small((int64_t)a.n_tokens * h->p.group, h->p.n_kv, h->p.max_context);
+    if (h->plan.small) h->plan.wide = 0;
     HIP_TRY(launch_pages_plan(h->p, h->plan, s));
     return JEV_OK;
 }
@@ -2770,7 +2773,10 @@ try {
     p.split = (p.group + kPagesTileRows - 1) / kPagesTileRows;
     if (p.bits == 4) p.split = std::max(p.split, kPagesSplit);
     p.few = p.bits == 4 ? std::max(p.split, kPagesFew) : p.split;
-    const size_t split = p.split, few = p.few > p.split ? kPagesFewWgs / p.n_kv : 0;
+    // a small call's requests of more tiles than that have at most so many, each with a last one of fewer rows
+    const size_t split = p.split, rows = std::min<size_t>(kPagesSmallRows, kPagesSmallKeys / p.max_context) / p.n_kv;
+    const size_t small = rows / kPagesTileRows + rows / (split * kPagesTileRows);
+    const size_t few = p.bits == 4 ? std::max<size_t>(kPagesFewWgs / p.n_kv, small * pages_most_parts(p.max_context)) : 0;
     p.max_parts = (int)(split * (pool / pages_part_keys(1) + R) + few);
     p.max_items = (int)(p.max_parts + T * p.group / kPagesTileRows + (split + 1) * R);
     p.max_units = (int)(T / kPageBlock + 2 * R);
@@ -2893,6 +2899,7 @@ int jev_pages_attend_device(jev_pages *h, int32_t layer, const float *q, float *
     a.n_requests = h->plan.n_requests;
     a.n_tokens = h->plan.n_tokens;
     a.wide = h->plan.wide;
+    a.small = h->plan.small;
     HIP_TRY(launch_pages_attend(h->p, a, h->stream));
     return JEV_OK;
 }

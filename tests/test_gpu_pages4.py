@@ -18,6 +18,10 @@ from test_gpu_pages import Rig, cfg
 pytestmark = pytest.mark.gpu
 
 
+# A context of which no call is small enough to go without wide tiles.
+ROOMY = 1 << 20
+
+
 class Rig4(Rig):
     def __init__(self, config, n_pages, page=16, requests=8, context=4096, tokens=4096, half=False):
         import torch
@@ -173,11 +177,12 @@ def test_single_tokens(gpu, rs, heads, kv, dim, page):
 
 
 @pytest.mark.parametrize("heads,kv,dim", [(4, 1, 128), (3, 3, 64), (10, 2, 128), (16, 1, 64), (40, 2, 128), (8, 2, 64)])
-def test_prompts(gpu, rs, heads, kv, dim):
+@pytest.mark.parametrize("context", [500, ROOMY])
+def test_prompts(gpu, rs, heads, kv, dim, context):
     """Ragged batches: nothing, single tokens, a few, more than a tile of any width, behind pasts of any length."""
     past = [0, 5, 0, 63, 300, 129, 0, 17]
     fresh = [1, 130, 0, 2, 33, 64, 301, 4]
-    rig = Rig4(cfg(heads, kv, dim), 200, 16, 8, 500)
+    rig = Rig4(cfg(heads, kv, dim), 200, 16, 8, context)
     rig.fill(rs, list(range(8)), past)
     rig.plan([6, 1, 2, 0, 7, 4, 5, 3], [fresh[i] for i in (6, 1, 2, 0, 7, 4, 5, 3)], pad=5)
     n = sum(fresh)
@@ -195,9 +200,10 @@ def test_a_few_tokens(gpu, rs, fresh):
         rig.attend(rs.randn(3 * fresh, heads, dim).astype(np.float32))
 
 
-def test_long_contexts(gpu, rs):
+@pytest.mark.parametrize("context", [41000, ROOMY])
+def test_long_contexts(gpu, rs, context):
     for past in (5000, 40000):
-        rig = Rig4(cfg(4, 1, 64), 2600, 16, 1, 41000, 41000)
+        rig = Rig4(cfg(4, 1, 64), 2600, 16, 1, context, 41000)
         rig.fill(rs, [0], [past])
         rig.fill(rs, [0], [1])
         rig.attend(rs.randn(1, 4, 64).astype(np.float32))
@@ -206,8 +212,9 @@ def test_long_contexts(gpu, rs):
             rig.attend(rs.randn(fresh, 4, 64).astype(np.float32))
 
 
-def test_parts_of_very_long_contexts(gpu, rs):
-    rig = Rig4(cfg(2, 1, 64), 9000, 16, 1, 143000, 143000)
+@pytest.mark.parametrize("context", [143000, ROOMY])
+def test_parts_of_very_long_contexts(gpu, rs, context):
+    rig = Rig4(cfg(2, 1, 64), 9000, 16, 1, context, 143000)
     rig.fill(rs, [0], [142001])
     rig.fill(rs, [0], [1])
     rig.attend(rs.randn(1, 2, 64).astype(np.float32))
@@ -216,10 +223,10 @@ def test_parts_of_very_long_contexts(gpu, rs):
         rig.attend(rs.randn(fresh, 2, 64).astype(np.float32))
 
 
-@pytest.mark.parametrize("fresh", [1, 90, 150])
-def test_scales_far_apart(gpu, rs, fresh):
+@pytest.mark.parametrize("fresh,context", [(1, 600), (90, 600), (150, 600), (150, ROOMY)])
+def test_scales_far_apart(gpu, rs, fresh, context):
     """Queries and values far from one: the pairs stay inside fp16's range by powers of two."""
-    rig = Rig4(cfg(4, 2, 128), 40, 16, 1, 600)
+    rig = Rig4(cfg(4, 2, 128), 40, 16, 1, context)
     n = 400 + fresh
     k = rs.randn(n, 2, 128).astype(np.float32) * np.float32(1e-18)
     v = rs.randn(n, 2, 128).astype(np.float32) * np.exp2(rs.randint(-100, 100, (n, 1, 1))).astype(np.float32)
@@ -248,19 +255,20 @@ def test_drafts_of_few_and_of_many_requests(gpu, rs, n):
 
 
 @pytest.mark.parametrize("scale", [1e-37, 1e-25, 1e25])
-def test_queries_and_keys_at_the_ends_of_the_range(gpu, rs, scale):
+@pytest.mark.parametrize("context", [200, ROOMY])
+def test_queries_and_keys_at_the_ends_of_the_range(gpu, rs, scale, context):
     """Small queries over large keys and the other way round: their product is what counts."""
-    rig = Rig4(cfg(8, 2, 64), 40, 16, 1, 200)
+    rig = Rig4(cfg(8, 2, 64), 40, 16, 1, context)
     k, v = (rs.randn(90, 2, 64).astype(np.float32) for _ in "kv")
     rig.plan([0], [90])
     rig.store(None, k * np.float32(scale), v)
     rig.attend(rs.randn(90, 8, 64).astype(np.float32) * np.float32(1.0 / np.float32(scale)))
 
 
-@pytest.mark.parametrize("fresh", [2, 4, 90, 150])
-def test_masked_places_may_hold_anything(gpu, rs, fresh):
+@pytest.mark.parametrize("fresh,context", [(2, 600), (4, 600), (90, 600), (150, 600), (150, ROOMY)])
+def test_masked_places_may_hold_anything(gpu, rs, fresh, context):
     """NaN past a query's own position leaves it alone; a query that sees one is NaN; one query's NaN stays its own."""
-    rig = Rig4(cfg(4, 2, 64), 40, 16, 1, 600)
+    rig = Rig4(cfg(4, 2, 64), 40, 16, 1, context)
     rig.fill(rs, [0], [32])
     rig.plan([0], [fresh])
     k, v = (rs.randn(fresh, 2, 64).astype(np.float32) for _ in "kv")
@@ -288,9 +296,10 @@ def test_masked_places_may_hold_anything(gpu, rs, fresh):
         np.testing.assert_array_equal(got[at:, 2:], clean[at:, 2:])
 
 
-def test_single_tokens_do_not_depend_on_the_batch(gpu, rs):
+@pytest.mark.parametrize("context", [2100, ROOMY])
+def test_single_tokens_do_not_depend_on_the_batch(gpu, rs, context):
     past = [3, 700, 64, 2000, 130]
-    rig = Rig4(cfg(8, 2, 128), 300, 16, 6, 2100)
+    rig = Rig4(cfg(8, 2, 128), 300, 16, 6, context)
     rig.fill(rs, [0, 1, 2, 3, 4], past)
     rig.plan([0, 1, 2, 3, 4], [1] * 5)
     q, k, v = (rs.randn(5, h, 128).astype(np.float32) for h in (8, 2, 2))
@@ -308,10 +317,11 @@ def test_single_tokens_do_not_depend_on_the_batch(gpu, rs):
 
 
 @pytest.mark.parametrize("fresh", [2, 3, 4])
-def test_a_few_tokens_do_not_depend_on_the_batch(gpu, rs, fresh):
+@pytest.mark.parametrize("context", [2500, ROOMY])
+def test_a_few_tokens_do_not_depend_on_the_batch(gpu, rs, fresh, context):
     """Alone, beside a prompt, beside many drafts: up to sixteen rows of a KV head have the same bits."""
     for dim in (64, 128):
-        rig = Rig4(cfg(8, 2, dim), 1000, 16, 210, 2500, 8000)
+        rig = Rig4(cfg(8, 2, dim), 1000, 16, 210, context, 8000)
         rig.fill(rs, [0], [2100])
         x = [rs.randn(fresh, h, dim).astype(np.float32) for h in (8, 2, 2)]
         rig.plan([0], [fresh])
@@ -324,9 +334,9 @@ def test_a_few_tokens_do_not_depend_on_the_batch(gpu, rs, fresh):
             np.testing.assert_array_equal(rig.attend(y[0], check=False)[:fresh], alone)
 
 
-@pytest.mark.parametrize("fresh", [1, 4, 60, 80])
-def test_parts_of_an_earlier_call_are_not_seen(gpu, rs, fresh):
-    rig = Rig4(cfg(8, 2, 128), 1300, 16, 3, 9100, 20000)
+@pytest.mark.parametrize("fresh,context", [(1, 9100), (4, 9100), (60, 9100), (80, 9100), (60, ROOMY), (80, ROOMY)])
+def test_parts_of_an_earlier_call_are_not_seen(gpu, rs, fresh, context):
+    rig = Rig4(cfg(8, 2, 128), 1300, 16, 3, context, 20000)
     rig.fill(rs, [0, 1, 2], [9000, 3000, 1030])
     rig.fill(rs, [0, 1, 2], [fresh] * 3)
     q = [rs.randn(3 * fresh, 8, 128).astype(np.float32) * s for s in (1, 3, 0.1)]
@@ -440,9 +450,9 @@ def test_a_graph_replayed_with_few_and_many_drafts(gpu, rs):
     assert hip.hipGraphExecDestroy(ex) == 0 and hip.hipGraphDestroy(graph) == 0
 
 
-@pytest.mark.parametrize("fresh", [[1, 1], [30, 3], [70, 3]])
-def test_attention_and_reading_at_any_alignment(gpu, rs, fresh):
-    rig = Rig4(cfg(8, 2, 128), 200, 32, 2, 3000)
+@pytest.mark.parametrize("fresh,context", [([1, 1], 3000), ([30, 3], 3000), ([70, 3], 3000), ([70, 3], ROOMY)])
+def test_attention_and_reading_at_any_alignment(gpu, rs, fresh, context):
+    rig = Rig4(cfg(8, 2, 128), 200, 32, 2, context)
     rig.fill(rs, [0, 1], [1500, 40])
     rig.fill(rs, [0, 1], fresh)
     t, n = rig.t, sum(fresh)
@@ -493,11 +503,11 @@ def test_more_tiles_than_workgroups(gpu, rs):
 
 
 @pytest.mark.parametrize("heads,kv,dim", [(8, 2, 128), (32, 2, 64), (20, 1, 128)])
-@pytest.mark.parametrize("fresh", [1, 40, 70])
-def test_queries_keep_their_bits(gpu, rs, heads, kv, dim, fresh):
+@pytest.mark.parametrize("fresh,context", [(1, 200), (40, 200), (70, 200), (70, ROOMY)])
+def test_queries_keep_their_bits(gpu, rs, heads, kv, dim, fresh, context):
     """Queries of one element: a score is one product, so its error is the query's alone: its pair (2^-21, lo's own
     rounding among it), the softmax's scale on it (2^-24, and its logarithm's factor), the exponent's rounding."""
-    rig = Rig4(cfg(heads, kv, dim), 100, 16, 40, 200, 3000)
+    rig = Rig4(cfg(heads, kv, dim), 100, 16, 40, context, 3000)
     n = 20 if fresh == 1 else 2
     rig.fill(rs, list(range(n)), [60] * n)
     rig.plan(list(range(n)), [fresh] * n)
@@ -554,10 +564,11 @@ def check(rig, r, q, got, past):
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("begin", [16, 21, 48, 89])
 @pytest.mark.parametrize("large", [1e6, 1e15, 1e30])
-def test_later_tokens_leave_earlier_ones_alone(gpu, rs, dim, begin, large):
+@pytest.mark.parametrize("context", [200, ROOMY])
+def test_later_tokens_leave_earlier_ones_alone(gpu, rs, dim, begin, large, context):
     """A prompt whose tokens from one on, inside a block too, have far larger keys and values: the ones before have
     the bits that they have without them."""
-    rig = Rig4(cfg(8, 2, dim), 20, 16, 1, 200)
+    rig = Rig4(cfg(8, 2, dim), 20, 16, 1, context)
     q, k, v = (rs.randn(90, h, dim).astype(np.float32) for h in (8, 2, 2))
     for side in (1, 0):
         got = []
@@ -571,14 +582,14 @@ def test_later_tokens_leave_earlier_ones_alone(gpu, rs, dim, begin, large):
         np.testing.assert_array_equal(got[1], got[0])
 
 
-@pytest.mark.parametrize("fresh", [1, 3, 90])
+@pytest.mark.parametrize("fresh,context", [(1, 700), (3, 700), (90, 700), (90, ROOMY)])
 @pytest.mark.parametrize("where", [(0, 16), (5, 6), (48, 64), (480, 493)])
 @pytest.mark.parametrize("ratio", [2.0 ** 14, 2.0 ** 24, 2.0 ** 34, 2.0 ** 110])
 @pytest.mark.parametrize("score", [0.0, 12.0, 200.0])
-def test_values_far_apart(gpu, rs, fresh, where, ratio, score):
+def test_values_far_apart(gpu, rs, fresh, context, where, ratio, score):
     """Tokens of far larger values that the softmax gives little weight, or none, before, among and beside those
     that a query attends."""
-    rig = Rig4(cfg(8, 2, 128), 80, 16, 1, 700)
+    rig = Rig4(cfg(8, 2, 128), 80, 16, 1, context)
     n, at = 496 + fresh, slice(*where)
     k, v = rs.randn(n, 2, 128).astype(np.float32) * np.float32(0.3), rs.randn(n, 2, 128).astype(np.float32)
     k[at, :, 0] = -score * np.sqrt(128) / 8
@@ -592,11 +603,11 @@ def test_values_far_apart(gpu, rs, fresh, where, ratio, score):
     check(rig, 0, q, rig.attend(q, check=False), 496)
 
 
-@pytest.mark.parametrize("fresh", [1, 40, 80])
+@pytest.mark.parametrize("fresh,context", [(1, 1200), (40, 1200), (80, 1200), (80, ROOMY)])
 @pytest.mark.parametrize("ratio", [2.0 ** -60, 2.0 ** -20, 1.0, 2.0 ** 40, 2.0 ** 100])
-def test_any_magnitudes(gpu, rs, fresh, ratio):
+def test_any_magnitudes(gpu, rs, fresh, context, ratio):
     """Every token's key and value row of its own magnitude, zeros among them; attended values at either end of fp32."""
-    rig = Rig4(cfg(8, 2, 64), 200, 16, 1, 1200)
+    rig = Rig4(cfg(8, 2, 64), 200, 16, 1, context)
     n = 1000 + fresh
     k = rs.randn(n, 2, 64).astype(np.float32) * np.exp2(rs.uniform(-12, 0.5, (n, 2, 1))).astype(np.float32)
     v = rs.randn(n, 2, 64).astype(np.float32) * np.exp2(rs.uniform(-30, 8, (n, 2, 1))).astype(np.float32) * np.float32(ratio)
@@ -610,8 +621,9 @@ def test_any_magnitudes(gpu, rs, fresh, ratio):
     check(rig, 0, q, rig.attend(q, check=False), 1000)
 
 
-def test_values_of_zeros_only(gpu, rs):
-    rig = Rig4(cfg(4, 1, 64), 20, 16, 1, 100)
+@pytest.mark.parametrize("context", [100, ROOMY])
+def test_values_of_zeros_only(gpu, rs, context):
+    rig = Rig4(cfg(4, 1, 64), 20, 16, 1, context)
     for fresh in (1, 50, 80):
         rig.plan([0], [fresh], [0])
         rig.store(None, rs.randn(fresh, 1, 64).astype(np.float32), np.zeros((fresh, 1, 64), np.float32))
