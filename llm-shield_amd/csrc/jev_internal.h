@@ -422,7 +422,10 @@ constexpr int kPagesWideRows = 128;    // the same in a wide tile, for requests 
 // Wide tiles are split over their keys when there are few, into no parts of less than
 // kPagesWideKeys keys: fewer tiles than half of this many workgroups over all KV heads (two
 // fit a compute unit: one round) into at most as many, more tiles into half as many on top.
-constexpr int kPagesWideWgs = 512, kPagesWideKeys = 512;
+// (The 4-bit cache: of less than kPages4WideKeys, us with 512 / 2048: a prompt of 700 51 / 33,
+// 500 tokens behind 2000 87 / 74, 256 behind 8000 144 / 139, 128 behind 20000 128 / 136; 9 of
+// 48 behind 4096 99 / 100, with 4096 122.)
+constexpr int kPagesWideWgs = 512, kPagesWideKeys = 512, kPages4WideKeys = 2048;
 __host__ __device__ inline int pages_wide_target(int n_kv) { return n_kv < kPagesWideWgs ? kPagesWideWgs / n_kv : 1; }
 
 // The 4-bit cache's 16-row tiles also take the rows of drafts, up to kPagesSplit of them a
@@ -489,6 +492,7 @@ struct PagesItem { // a workgroup's tile and keys, with its request's fields: on
 struct Pages {
     // geometry
     int n_layers = 0, n_heads = 0, n_kv = 0, hd = 0, group = 1;
+    int wide_keys = kPagesWideKeys;         // of a wide tile's part, at least
     int split = 1, few = 1;                 // 16-row tiles of a request, at most, that are not a wide tile's; the same in a step with few
     int page = 16, sub = 1, sub_shift = 0;  // tokens and blocks of a page (powers of two)
     int n_pages = 0, max_requests = 0, max_context = 0, max_tokens = 0, width = 0; // width: pages of a table row

@@ -22,7 +22,7 @@ struct PlanView {
     double2 *angle;
     const double *freqs;
     double mscale;
-    int page, sub, sub_shift, n_pages, max_requests, max_context, width, half, group, split, few, n_kv;
+    int page, sub, sub_shift, n_pages, max_requests, max_context, width, half, group, split, few, wide_keys, n_kv;
 };
 // Exclusive prefix sums over the workgroup's threads of N values at once, in
 // place, and their totals.  `ws`: N words per wave.
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(NT) void pages_plan_kernel(PlanView p, PagesPlanArg
 
     // the lists' prefix sums take their place
     int *unit0 = px + S, *item0 = px + 2 * S, *wide0 = px + 3 * S;
-    int wide_keys = kPagesWideKeys, wide = 0; // (a small call's requests are all split)
+    int wide_keys = p.wide_keys, wide = 0; // (a small call's requests are all split)
     if (a.wide) {
         wide = p.split;
         if (p.few > p.split) {
@@ -400,7 +400,7 @@ hipError_t launch_pages_plan(const Pages &p, const PagesPlanArgs &a, hipStream_t
     if (a.n_requests < 0 || a.n_requests > p.max_requests || a.n_tokens < 0 || a.n_tokens > p.max_tokens)
         return hipErrorInvalidValue;
     const PlanView v = {p.table, p.length, p.n_free, p.fresh_pages, p.prefix, p.used, p.head, p.req, p.unit, p.item, p.wide, p.angle, p.freqs,
-                        p.mscale, p.page, p.sub, p.sub_shift, p.n_pages, p.max_requests, p.max_context, p.width, p.half, p.group, p.split, p.few, p.n_kv};
+                        p.mscale, p.page, p.sub, p.sub_shift, p.n_pages, p.max_requests, p.max_context, p.width, p.half, p.group, p.split, p.few, p.wide_keys, p.n_kv};
     // What the lists write, in words; an angle counts for several.  Short lists are written
     // by the plan's own workgroup (in a graph, so / with a launch of their own: 12 requests
     // of a token and 64 pairs 6.7 / 7.6 us, 16 9.4 / 10.0, 24 10.8 / 9.8, 64 18.6 / 10.2; one

@@ -2773,6 +2773,7 @@ try {
     p.split = (p.group + kPagesTileRows - 1) / kPagesTileRows;
     if (p.bits == 4) p.split = std::max(p.split, kPagesSplit);
     p.few = p.bits == 4 ? std::max(p.split, kPagesFew) : p.split;
+    p.wide_keys = p.bits == 4 ? kPages4WideKeys : kPagesWideKeys;
     // a small call's requests of more tiles than that have at most so many, each with a last one of fewer rows
     const size_t split = p.split, rows = std::min<size_t>(kPagesSmallRows, kPagesSmallKeys / p.max_context) / p.n_kv;
     const size_t small = rows / kPagesTileRows + rows / (split * kPagesTileRows);
