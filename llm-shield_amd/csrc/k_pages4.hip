@@ -1125,7 +1125,7 @@ hipError_t launch_pages4_attend(const Pages &p, const PagesAttendArgs &a, hipStr
     // as many workgroups as the call's requests can need (launch_pages_attend; with a token
     // each: where one has more, the workgroups take turns)
     const int64_t each = (int64_t)std::min(a.n_requests, a.n_tokens) * pages_most_parts(p.max_context);
-    const int64_t few = a.wide || a.small ? std::min(each * p.few, (int64_t)kPagesFewWgs / p.n_kv) : 0;
+    const int64_t few = a.n_tokens > a.n_requests ? std::min(each * p.few, (int64_t)kPagesFewWgs / p.n_kv) : 0;
     const int64_t split = a.wide ? p.split : (p.group + kPagesTileRows - 1) / kPagesTileRows;
     const int64_t parts = std::min((int64_t)p.max_parts, std::max(each * split, few));
     const int64_t most = a.n_tokens == 0 ? 1 : std::max<int64_t>(1, parts + (int64_t)a.n_tokens * p.group / kPagesTileRows + a.n_requests);

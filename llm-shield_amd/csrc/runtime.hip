@@ -1048,7 +1048,7 @@ int enqueue_forward(jev_ctx *c, const Plan &p, int mode, int n_rows, float *dout
             pa.wide = paged->args.wide;
             pa.small = paged->args.small;
             {
-                ProfScope ps(c, pa.wide || pa.small ? JEV_PROF_ATTN : JEV_PROF_DECODE_ATTN, 4.0 * f.head_dim * f.n_heads * p.visible_pairs,
+                ProfScope ps(c, T > sa.n_requests ? JEV_PROF_ATTN : JEV_PROF_DECODE_ATTN, 4.0 * f.head_dim * f.n_heads * p.visible_pairs,
                              2.0 * f.head_dim * f.n_kv_heads * p.kv_rows + 8.0 * T * qdim, true);
                 pa.ev_start = ps.a;
                 pa.ev_stop = ps.z;
@@ -2671,9 +2671,8 @@ int pages_plan(jev_pages *h, const PagesPlanArgs &a, hipStream_t s)
     h->plan = a;
     // as many tokens as requests: 16-row tiles serve whatever there is, and the
     // wide tiles' launches are saved
-    h->plan.wide = a.n_tokens > a.n_requests;
-    h->plan.small = h->p.bits == 4 && h->plan.wide && pages_small((int64_t)a.n_tokens * h->p.group, h->p.n_kv, h->p.max_context);
-    if (h->plan.small) h->plan.wide = 0;
+    h->plan.small = h->p.bits == 4 && pages_small((int64_t)a.n_tokens * h->p.group, h->p.n_kv, h->p.max_context);
+    h->plan.wide = a.n_tokens > a.n_requests && !h->plan.small;
     HIP_TRY(launch_pages_plan(h->p, h->plan, s));
     return JEV_OK;
 }

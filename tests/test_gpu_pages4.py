@@ -239,6 +239,17 @@ def test_scales_far_apart(gpu, rs, fresh, context):
     rig.attend(np.zeros((fresh, 4, 128), np.float32))
 
 
+@pytest.mark.parametrize("context", [3000, ROOMY])
+def test_many_tokens_of_one_among_idle_requests(gpu, rs, context):
+    """No more tokens than requests, nearly all of them one request's: tiles of sixteen rows whose keys are split, or,
+    where the context may be long, are not."""
+    rig = Rig4(cfg(8, 2, 128), 300, 16, 64, context)
+    rig.fill(rs, list(range(64)), [2500] + [16] * 63)
+    rig.plan(list(range(64)), [60] + [0] * 61 + [1, 3])
+    rig.store(None, *(rs.randn(64, 2, 128).astype(np.float32) for _ in "kv"))
+    rig.attend(rs.randn(64, 8, 128).astype(np.float32))
+
+
 @pytest.mark.parametrize("n", [30, 203, 206])
 def test_drafts_of_few_and_of_many_requests(gpu, rs, n):
     """Five tiles of sixteen rows a request: up to 1024 of them a KV head, and wide tiles where there are more; beside a
