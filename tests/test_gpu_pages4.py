@@ -200,16 +200,16 @@ def test_a_few_tokens(gpu, rs, fresh):
         rig.attend(rs.randn(3 * fresh, heads, dim).astype(np.float32))
 
 
+@pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("context", [41000, ROOMY])
-def test_long_contexts(gpu, rs, context):
+def test_long_contexts(gpu, rs, context, dim):
+    """Parts of five lengths and more: rows of one token, two, three, and of several tiles."""
     for past in (5000, 40000):
-        rig = Rig4(cfg(4, 1, 64), 2600, 16, 1, context, 41000)
+        rig = Rig4(cfg(4, 1, dim), 2600, 16, 1, context, 41000)
         rig.fill(rs, [0], [past])
-        rig.fill(rs, [0], [1])
-        rig.attend(rs.randn(1, 4, 64).astype(np.float32))
-        for fresh in (30, 70):
+        for fresh in (1, 2, 3, 30, 70):
             rig.fill(rs, [0], [fresh])
-            rig.attend(rs.randn(fresh, 4, 64).astype(np.float32))
+            rig.attend(rs.randn(fresh, 4, dim).astype(np.float32))
 
 
 @pytest.mark.parametrize("context", [143000, ROOMY])
