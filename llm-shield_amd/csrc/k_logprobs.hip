@@ -22,7 +22,8 @@ struct LogprobsView {
     LogprobsPart *part;
     int32_t *tickets;
     int vocab, n_given, n_top, parts, chunk; // a row's parts, of `chunk` logits each
-    float temperature, c;                    // c = log2(e) / temperature
+    float c;                                 // log2(e) / temperature
+    double inverse;                          // 1 / temperature
 };
 
 typedef float floatx4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -166,7 +167,7 @@ struct Best {
     {
         const int lane = threadIdx.x & 63;
         wave_sync();
-        if (n > 64) { // the k-th largest, bit by bit: the greatest t with k keys at or above it
+        if (n > 128) { // the k-th largest, bit by bit: the greatest t with k keys at or above it
             constexpr int C = (kRoom + 63) / 64;
             uint64_t mine[C], t = 0;
 #pragma unroll
@@ -187,14 +188,22 @@ struct Best {
         }
         if (lane < 8) keys[n + lane] = 0;
         wave_sync();
-        const uint64_t key = lane < n ? keys[lane] : 0;
-        const int above = count_above(keys, n, key);
+        uint64_t key[2];
+        int above[2] = {0, 0};
+        key[0] = lane < n ? keys[lane] : 0;
+        key[1] = 64 + lane < n ? keys[64 + lane] : 0;
+        above[0] = count_above(keys, n, key[0]);
+        if (n > 64) above[1] = count_above(keys, n, key[1]);
         wave_sync();
-        if (lane < n && above < k) keys[above] = key;
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            if (key[i] != 0 && above[i] < k) keys[above[i]] = key[i];
         wave_sync();
         if (n >= k) {
             n = k;
-            at_least(lane_key(key, __ffsll((unsigned long long)__ballot(key != 0 && above == k - 1)) - 1));
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                if (const uint64_t at = __ballot(key[i] != 0 && above[i] == k - 1)) at_least(lane_key(key[i], __ffsll((unsigned long long)at) - 1));
         }
     }
 };
@@ -256,13 +265,14 @@ __device__ __forceinline__ uint64_t load_shared64(const void *p)
 // maximum, sums and list are its own, so nothing waits inside the pass.  The last part of
 // a row to arrive merges all of them.  Bounded by HBM where there are rows enough, each logit
 // being read once: 1000 rows of 131072 (524 MB) 98 us, with the 5 most probable 104, 5.0 to
-// 5.3 TB/s; 64 with the 20 most probable 20 (34 MB: a pass of the lanes, and the lists' merge),
+// 5.3 TB/s; 64 with the 20 most probable 19, 32 20 (34 MB: a pass of the lanes, and the lists' merge),
 // one with 5 8.7 (a launch, the pass, two trips to memory and the merge).
 template <bool TOP>
 __global__ __launch_bounds__(256, 4) void logprobs_kernel(LogprobsView p)
 {
     __shared__ uint64_t keys[4][TOP ? kKeys : 1], least[4];
-    __shared__ Stats stats[4], total;
+    __shared__ Stats stats[4];
+    __shared__ double top_x, log_s; // the row's largest logit, the logarithm of its sum
     __shared__ int count[4], last;
     __shared__ uint32_t first[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -453,19 +463,22 @@ __global__ __launch_bounds__(256, 4) void logprobs_kernel(LogprobsView p)
         const float most = wave_most(st.m);
         if (most > st.m) st.rescale(most, p.c);
         st = wave_total(st);
-        if (lane == 0) total = st;
+        // logp(x) = (x - m) / T - log(1 + s);  H = log(1 + s) - (sum e (x - m) / T) / (1 + s),
+        // where s has all of the sum but one logit that is m
+        const double rest = st.s + (double)(st.ones - 1), log_of = fabsf(st.m) < INFINITY ? log1p(rest) : NAN;
+        if (lane == 0) {
+            top_x = (double)st.m;
+            log_s = log_of;
+            if (p.entropy) p.entropy[row] = (float)(log_of - 0.69314718055994530942 * st.t / (1.0 + rest));
+        }
     }
     __syncthreads();
 
-    // logp(x) = (x - m) / T - log(1 + s);  H = log(1 + s) - (sum e (x - m) / T) / (1 + s),
-    // where s has all of the sum but one logit that is m
-    const Stats r = total;
-    const double rest = r.s + (double)(r.ones - 1), log_s = fabsf(r.m) < INFINITY ? log1p(rest) : NAN;
-    auto logp = [&](float x) { return (float)(((double)x - (double)r.m) / (double)p.temperature - log_s); };
+    const double m = top_x, log_sum = log_s;
+    auto logp = [&](float x) { return (float)(((double)x - m) * p.inverse - log_sum); };
     float *to = p.logp + (size_t)row * p.n_given;
     if (tid < p.n_given) to[tid] = logp(asked);
     for (int i = tid + 256; i < p.n_given; i += 256) to[i] = logp(logit_of(given[i]));
-    if (tid == 0 && p.entropy) p.entropy[row] = (float)(log_s - 0.69314718055994530942 * r.t / (1.0 + rest));
     if constexpr (TOP)
         if (tid < n_top) {
             const uint64_t key = keys[0][tid];
@@ -491,7 +504,7 @@ hipError_t launch_logprobs(const LogprobsArgs &a, hipStream_t s)
     const int parts = logprobs_parts(a.rows, a.vocab);
     const int chunk = ((a.vocab + parts - 1) / parts + 1023) & ~1023;
     const LogprobsView v = {a.logits, a.ld, a.given, a.logp, a.entropy, a.top_logp, a.top, a.part, a.tickets, a.vocab, a.n_given, a.n_top,
-                            parts, chunk, a.temperature, (float)(1.4426950408889634074 / (double)a.temperature)};
+                            parts, chunk, (float)(1.4426950408889634074 / (double)a.temperature), 1.0 / (double)a.temperature};
     const dim3 grid((unsigned)a.rows * parts);
     if (a.n_top > 0) hipLaunchKernelGGL(logprobs_kernel<true>, grid, dim3(256), 0, s, v);
     else hipLaunchKernelGGL(logprobs_kernel<false>, grid, dim3(256), 0, s, v);
