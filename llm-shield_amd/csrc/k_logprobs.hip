@@ -96,12 +96,13 @@ __device__ __forceinline__ int count_above(const T *from, int n, T x)
     return above;
 }
 
-// The `rank`-th largest of the lanes' numbers, or (few wanted) a larger one where some are
-// equal; 0 where fewer are more than 0.  `lds`: 64 of them.
-__device__ __forceinline__ uint32_t rank_of(uint32_t up, int rank, uint32_t *lds)
+// A number that `rank` of the lanes' numbers, or more, are not below; 0 where fewer are more
+// than 0.  The rank-th largest itself or (few wanted, some equal) a larger one; past three its
+// upper half.
+__device__ __forceinline__ uint32_t rank_of(uint32_t up, int rank)
 {
     auto larger = [](uint32_t a, uint32_t b) { return max(a, b); };
-    if (rank <= 3) { // one after the other: 300 cycles each, all at once 1900
+    if (rank <= 3) { // one after the other: 300 cycles each
         uint32_t most = 0;
         for (int n = 0; n < rank;) {
             most = over_wave(up, larger);
@@ -111,12 +112,13 @@ __device__ __forceinline__ uint32_t rank_of(uint32_t up, int rank, uint32_t *lds
         }
         return most;
     }
-    lds[threadIdx.x & 63] = up;
-    wave_sync();
-    const int above = count_above(lds, 64, up);
-    wave_sync();
-    if (__popcll(__ballot(up != 0)) < rank) return 0;
-    return ~over_wave(above < rank ? ~up : 0u, larger);
+    uint32_t t = 0;
+#pragma unroll 4
+    for (int bit = 31; bit >= 16; bit--) {
+        const uint32_t trial = t | 1u << bit;
+        if (__popcll(__ballot(up >= trial)) >= rank) t = trial;
+    }
+    return t;
 }
 
 // A wave's largest keys: `n` of them in LDS, in order except between a push and its cut,
@@ -265,7 +267,7 @@ __device__ __forceinline__ uint64_t load_shared64(const void *p)
 // maximum, sums and list are its own, so nothing waits inside the pass.  The last part of
 // a row to arrive merges all of them.  Bounded by HBM where there are rows enough, each logit
 // being read once: 1000 rows of 131072 (524 MB) 98 us, with the 5 most probable 104, 5.0 to
-// 5.3 TB/s; 64 with the 20 most probable 19, 32 20 (34 MB: a pass of the lanes, and the lists' merge),
+// 5.3 TB/s; 64 with the 20 most probable 18, 32 19 (34 MB: a pass of the lanes, and the lists' merge),
 // one with 5 8.7 (a launch, the pass, two trips to memory and the merge).
 template <bool TOP>
 __global__ __launch_bounds__(256, 4) void logprobs_kernel(LogprobsView p)
@@ -337,7 +339,7 @@ __global__ __launch_bounds__(256, 4) void logprobs_kernel(LogprobsView p)
             const bool has_nan = s != s, some = base + 4 * lane < w1; // (else all of its places are past the end)
             const uint32_t up = some ? (uint32_t)(key_of(m, 0) >> 32) : 0;
             if (base == w0) { // a first bound: as many lanes' largest from each wave as make k of them
-                const uint32_t mine = __any(has_nan) ? 0 : rank_of(up, (n_top + 3) / 4, (uint32_t *)best.keys);
+                const uint32_t mine = __any(has_nan) ? 0 : rank_of(up, (n_top + 3) / 4);
                 if (lane == 0) first[wave] = mine;
                 __syncthreads();
                 best.at_least((uint64_t)min(min(first[0], first[1]), min(first[2], first[3])) << 32);
