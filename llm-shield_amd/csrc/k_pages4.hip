@@ -865,7 +865,7 @@ __device__ __forceinline__ void attend4_wide(const Attend4View &p, Wide4Lds<HD> 
     // A lane's share: a part of a token's codes (K), and four tokens' of dims 16 s + t (V)
     const int t = lane & 15, quad = lane >> 4;
     const int ks_at = at.ks + 4 * (4 * (quad * ND / 4) + (t >> 2));
-    uint32_t kr[ND], vr[ND], vs[ND], ks, er;
+    uint32_t kr[ND], vr[ND], vs, ks, er;
     auto fetch = [&](int kb, int page) {
         const int c = min(4 * kb + wave, last) & (p.sub - 1);
         const size_t b = (((size_t)__builtin_amdgcn_readfirstlane(page) * p.n_kv + h) << p.sub_shift) + c;
@@ -880,19 +880,14 @@ __device__ __forceinline__ void attend4_wide(const Attend4View &p, Wide4Lds<HD> 
             kr[0] = k.x, kr[1] = k.y, vr[0] = v.x, vr[1] = v.y;
         }
         ks = __builtin_amdgcn_raw_buffer_load_b32(rb, ks_at, 0, 0);
-        if constexpr (HD == 128) {
-            const uint4 v = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rb, 16 * quad, at.vs, 0));
-            vs[0] = v.x, vs[1] = v.y, vs[2] = v.z, vs[3] = v.w;
-        } else {
-            const uint2 v = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rb, 8 * quad, at.vs, 0));
-            vs[0] = v.x, vs[1] = v.y;
-        }
+        vs = __builtin_amdgcn_raw_buffer_load_b32(rb, 4 * (ND * quad + t % ND), at.vs, 0);
         er = __builtin_amdgcn_raw_buffer_load_b32(rb, 4 * (lane & 7), at.pw, 0); // a quad's powers, K's and V's in turn
     };
     // NC pieces: a lane's words of K, then of V (four tokens of two dims each).
     const int krow = 8 * (t >> 2) + 4 * (wave & 1) + (t & 3), vcol = 32 * (wave & 1) + t;
     const uint32_t k16 = sixteen();
     Steps kst;
+    uint4 vst; // of group t % ND, for the lanes beside
     auto put = [&](int buf, int piece) {
         if (piece < ND) {
             if (piece == 0) {
@@ -908,7 +903,21 @@ __device__ __forceinline__ void attend4_wide(const Attend4View &p, Wide4Lds<HD> 
             (kf[buf] + ((wave >> 1) * NC + c) * 64 + krow)[32 * (piece & 1)] = __builtin_bit_cast(uint4, word_f16(kr[piece], kst, k16));
         } else {
             const int j = piece - ND;
-            const uint4 v = QuadSteps(vs[j], k16)(vr[j], k16);
+            if (j == 0) {
+                const QuadSteps own(vs, k16);
+                vst = make_uint4(__builtin_bit_cast(uint32_t, own.s[0].u), __builtin_bit_cast(uint32_t, own.s[0].m),
+                                 __builtin_bit_cast(uint32_t, own.s[1].u), __builtin_bit_cast(uint32_t, own.s[1].m));
+            }
+            auto of = [&](uint32_t x) { // lane j's of four
+                const int y = (int)x;
+                return __builtin_bit_cast(half2_t, j == 0   ? __builtin_amdgcn_mov_dpp(y, 0x00, 0xf, 0xf, true)
+                                                   : j == 1 ? __builtin_amdgcn_mov_dpp(y, 0x55, 0xf, 0xf, true)
+                                                   : j == 2 ? __builtin_amdgcn_mov_dpp(y, 0xaa, 0xf, 0xf, true)
+                                                            : __builtin_amdgcn_mov_dpp(y, 0xff, 0xf, 0xf, true));
+            };
+            QuadSteps st;
+            st.s[0].u = of(vst.x), st.s[0].m = of(vst.y), st.s[1].u = of(vst.z), st.s[1].m = of(vst.w);
+            const uint4 v = st(vr[j], k16);
             uint2 *to = (uint2 *)(vf[buf] + ((2 * j + (wave >> 1)) * 2 + (quad >> 1)) * 64 + vcol) + (quad & 1);
             to[0] = make_uint2(v.x, v.y);
             to[32] = make_uint2(v.z, v.w);
