@@ -604,6 +604,7 @@ __device__ __forceinline__ void attend4_tile(const Attend4View &p, Tile4Lds<HD> 
             for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(qx[c][i]));
         const Query4 scaled(over_quarters(m, fmaxf), p.scale);
         query = scaled.power();
+        asm("" : "+v"(query)); // one number: its -127 would be added to each byte by itself
         // a wave makes a quarter of the fragments, in LDS for all (and for each 64 keys'
         // products again: registers)
 #pragma unroll
@@ -942,6 +943,7 @@ __device__ __forceinline__ void attend4_wide(const Attend4View &p, Wide4Lds<HD> 
         m = fmaxf(m, __shfl_xor(m, 32, 64));
         const Query4 scaled(m, p.scale);
         query = scaled.power();
+        asm("" : "+v"(query)); // one number: its -127 would be added to each byte by itself
 #pragma unroll
         for (int c = 0; c < NC; c++) {
             float x[8];
